@@ -108,6 +108,41 @@ for _name in ("dnnopt_cuda_gemm_f32", "dnnopt_cuda_gemm_bf16f32", "dnnopt_cuda_g
     getattr(lib, _name).argtypes = [ctypes.POINTER(GemmDesc), _P, _P, _P, _P]
     getattr(lib, _name).restype = _I
 lib.dnnopt_cuda_gemm_e4m3bf16.argtypes = [ctypes.POINTER(GemmDesc), _P, _P, _P, _P, _P]
+
+
+# ---- decoder-step operators: types and descriptors --------------------------
+TYPE_F32, TYPE_BF16, TYPE_E4M3 = 0, 1, 2
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+
+
+class W4Desc(ctypes.Structure):
+    """dnnopt_w4_desc."""
+    _fields_ = [(n, ctypes.c_int) for n in ("M", "N", "K", "lda", "ldw", "ldc", "group", "lds",
+                                             "io_type", "scale_type")]
+
+
+class PagedAttnDesc(ctypes.Structure):
+    """dnnopt_paged_attn_desc."""
+    _fields_ = ([(n, ctypes.c_int) for n in ("batch", "heads", "kv_heads", "head_dim", "page_size",
+                                              "num_pages", "max_pages", "window", "io_type", "cache_type")]
+                + [(n, ctypes.c_float) for n in ("scale", "softcap", "k_scale", "v_scale")]
+                + [(n, ctypes.c_int64) for n in ("q_batch_stride", "q_head_stride", "out_batch_stride",
+                                                  "out_head_stride", "new_batch_stride", "new_head_stride",
+                                                  "page_stride", "token_stride", "head_stride",
+                                                  "table_stride")])
+
+
+class BlockNormDesc(ctypes.Structure):
+    """dnnopt_block_norm_desc."""
+    _fields_ = ([(n, ctypes.c_int) for n in ("rows", "cols", "post", "pre", "io_type", "weight_type")]
+                + [(n, ctypes.c_float) for n in ("eps", "weight_offset", "residual_scale", "block_scale")]
+                + [(n, ctypes.c_int64) for n in ("ldx", "ldy", "ldh", "ldz", "ldg")]
+                + [("gate_rows", ctypes.c_int)])
+
+
+lib.dnnopt_cuda_gemm_w4.argtypes = [ctypes.POINTER(W4Desc)] + [_P] * 7
+lib.dnnopt_cuda_paged_attention.argtypes = [ctypes.POINTER(PagedAttnDesc)] + [_P] * 10
+lib.dnnopt_cuda_block_norm.argtypes = [ctypes.POINTER(BlockNormDesc)] + [_P] * 10
 lib.dnnopt_has_fp8_support.restype = _I
 lib.dnnopt_gemm_get_num_threads.restype = _I
 lib.dnnopt_gemm_set_num_threads.argtypes = [_I]
@@ -258,6 +293,62 @@ def cuda_conv3d(precision, params, inp, flt, bias, out, post_op=0, stream=None) 
 
 def _stream(stream):
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else ptr(stream)
+
+
+# ---- decoder-step operators (device pointers, asynchronous on `stream`) ------
+def w4_desc(M, N, K, lda, ldw, ldc, group, lds, io_type=TYPE_BF16, scale_type=TYPE_BF16) -> W4Desc:
+    """ldw is in bytes; group 0 = one group per row."""
+    return W4Desc(M, N, K, lda, ldw, ldc, group, lds, io_type, scale_type)
+
+
+def cuda_gemm_w4(d: W4Desc, A, W, scale, zero, bias, C, stream=None) -> int:
+    """C = A * (scale * (codes - zero))^T + bias; zero None = 8, bias None = 0."""
+    return lib.dnnopt_cuda_gemm_w4(ctypes.byref(d), ptr(A), ptr(W), ptr(scale), ptr(zero), ptr(bias),
+                                   ptr(C), _stream(stream))
+
+
+def paged_attn_desc(batch, heads, kv_heads, head_dim, page_size, num_pages, max_pages, *,
+                    io_type=TYPE_BF16, cache_type=TYPE_BF16, page_stride=None, token_stride=None,
+                    head_stride=None, q_strides=None, out_strides=None, new_strides=None,
+                    table_stride=None, scale=None, softcap=0.0, window=0, k_scale=1.0,
+                    v_scale=1.0) -> PagedAttnDesc:
+    """Defaults: dense [batch, heads, head_dim] rows, [page][slot][head][dim] pages, a dense page
+    table and scale = head_dim ** -0.5.  *_strides are (batch, head) pairs, in elements."""
+    qb, qh = q_strides or (heads * head_dim, head_dim)
+    ob, oh = out_strides or (heads * head_dim, head_dim)
+    nb, nh = new_strides or (kv_heads * head_dim, head_dim)
+    ts = kv_heads * head_dim if token_stride is None else token_stride
+    hs = head_dim if head_stride is None else head_stride
+    ps = page_size * kv_heads * head_dim if page_stride is None else page_stride
+    return PagedAttnDesc(batch, heads, kv_heads, head_dim, page_size, num_pages, max_pages, window,
+                         io_type, cache_type, head_dim ** -0.5 if scale is None else scale, softcap,
+                         k_scale, v_scale, qb, qh, ob, oh, nb, nh, ps, ts, hs,
+                         max_pages if table_stride is None else table_stride)
+
+
+def cuda_paged_attention(d: PagedAttnDesc, q, k_cache, v_cache, page_table, seq_lens, out, lse=None,
+                         k_new=None, v_new=None, stream=None) -> int:
+    """One new token's attention; k_new / v_new are stored as token seq_lens[b] - 1 first."""
+    return lib.dnnopt_cuda_paged_attention(ctypes.byref(d), ptr(q), ptr(k_cache), ptr(v_cache),
+                                           ptr(page_table), ptr(seq_lens), ptr(k_new), ptr(v_new),
+                                           ptr(out), ptr(lse), _stream(stream))
+
+
+def block_norm_desc(rows, cols, *, post=NORM_NONE, pre=NORM_RMS, io_type=TYPE_BF16,
+                    weight_type=TYPE_BF16, eps=1e-5, weight_offset=0.0, residual_scale=1.0,
+                    block_scale=1.0, ldx=None, ldy=None, ldh=None, ldz=None, ldg=0,
+                    gate_rows=1) -> BlockNormDesc:
+    """Row pitches default to cols; ldg 0 = one gate row for all rows."""
+    ld = [cols if v is None else v for v in (ldx, ldy, ldh, ldz)]
+    return BlockNormDesc(rows, cols, post, pre, io_type, weight_type, eps, weight_offset,
+                         residual_scale, block_scale, *ld, ldg, gate_rows)
+
+
+def cuda_block_norm(d: BlockNormDesc, x, y, gate, post_w, post_b, pre_w, pre_b, h, z, stream=None) -> int:
+    """h = residual_scale * x + block_scale * gate * post(y); z = pre(h)."""
+    return lib.dnnopt_cuda_block_norm(ctypes.byref(d), ptr(x), ptr(y), ptr(gate), ptr(post_w),
+                                      ptr(post_b), ptr(pre_w), ptr(pre_b), ptr(h), ptr(z),
+                                      _stream(stream))
 
 
 # ---- multi-GPU (one process per GPU) ----------------------------------------

@@ -518,7 +518,7 @@ int host_entry(Kind kind, const dnnopt_gemm_desc* d, const void* A, const void* 
             // Clears the error word and the conv prep's grid-barrier and
             // absmax words (a timed-out barrier may have left them set).
             cudaMemset(it->second.err, 0, 16 * sizeof(uint32_t));
-            return set_status(DNNOPT_STATUS_KERNEL_TIMEOUT);
+            return set_status(kernel_error_status(code));
         }
     }
     return set_status(DNNOPT_STATUS_SUCCESS);
@@ -1207,7 +1207,7 @@ int dnnopt_stream_status(void* stream) {
             // Clears the error word and the conv prep's grid-barrier and
             // absmax words (a timed-out barrier may have left them set).
             cudaMemset(it->second.err, 0, 16 * sizeof(uint32_t));
-            return set_status(DNNOPT_STATUS_KERNEL_TIMEOUT);
+            return set_status(kernel_error_status(code));
         }
     }
     return set_status(DNNOPT_STATUS_SUCCESS);

@@ -22,6 +22,7 @@ enum KernelErrorCode : uint32_t {
     kKerrMbarTimeout = 1,      // an mbarrier wait exceeded its iteration limit
     kKerrTmemAlloc = 2,        // TMEM allocation returned an unusable address
     kKerrPeerTimeout = 3,      // a peer GPU's flag did not arrive within the limit
+    kKerrBadIndex = 4,         // a length or page number in device memory was out of range
 };
 
 __device__ __forceinline__ void record_kernel_error(uint32_t* err, uint32_t code) {

@@ -294,5 +294,73 @@ cudaError_t launch_peer_wait(const uint32_t* flag, int world, uint32_t epoch, ui
 // err: device word that receives a KernelErrorCode when a bounded wait gives up.
 cudaError_t launch_gemm_bf16_tc(const GemmArgs& g, int num_sms, uint32_t* err, cudaStream_t s);
 
+// ---- decoder-step operators --------------------------------------------------
+// Values of the DNNOPT_TYPE_* constants of the C ABI.
+enum class DType : int { F32 = 0, BF16 = 1, E4M3 = 2 };
+
+// C[m,n] = bias[n] + sum_k A[m,k] * scale[n,k/group] * (code[n,k] - zero[n,k/group]).
+struct W4Args {
+    int M, N, K;
+    int group;              // a multiple of 32 (K rounded up to one for "whole row")
+    int groups;             // groups per row
+    DType io, st;           // A and C; scale and zero
+    const void* A;
+    int64_t lda;
+    const uint8_t* W;
+    int64_t ldw;            // bytes
+    const void* scale;
+    const void* zero;       // nullptr: 8
+    int64_t lds;
+    const float* bias;
+    void* C;
+    int64_t ldc;
+};
+cudaError_t launch_gemm_w4(const W4Args& g, cudaStream_t s);
+
+// Attention of one new token per sequence over a paged cache (strides in elements).
+struct PagedAttnArgs {
+    int batch, heads, kv_heads, dim;
+    int page_size, num_pages, max_pages;
+    int window;             // 0: none
+    DType io, ct;           // q, out and new rows; cache
+    float scale, softcap, k_scale, v_scale;
+    const void* q;
+    int64_t q_batch, q_head;
+    void* k;
+    void* v;
+    int64_t page_stride, token_stride, head_stride;
+    const int32_t* table;
+    int64_t table_stride;
+    const int32_t* lens;
+    const void* k_new;      // nullptr: nothing is appended
+    const void* v_new;
+    int64_t new_batch, new_head;
+    void* out;
+    int64_t out_batch, out_head;
+    float* lse;             // nullptr: not written
+    uint32_t* err;          // receives kKerrBadIndex for a length or page out of range
+};
+cudaError_t launch_paged_attention(const PagedAttnArgs& a, cudaStream_t s);
+
+// h = rs * x + bs * gate * post(y), z = pre(h).
+constexpr int kBlockNormMaxCols = 49152;
+struct BlockNormArgs {
+    int rows, cols;
+    int post, pre;          // 0 none, 1 rms, 2 layer
+    DType io, wt;
+    float eps, offset, rs, bs;
+    const void* x;
+    const void* y;          // nullptr: h = rs * x
+    const void* gate;       // nullptr: ones
+    const void* post_w;
+    const void* post_b;
+    const void* pre_w;
+    const void* pre_b;
+    void* h;                // nullptr: not written
+    void* z;                // nullptr: not written
+    int64_t ldx, ldy, ldh, ldz, ldg;
+    int gate_rows;
+};
+cudaError_t launch_block_norm(const BlockNormArgs& a, cudaStream_t s);
 
 }  // namespace dnnopt_b200

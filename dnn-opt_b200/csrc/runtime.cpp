@@ -61,6 +61,11 @@ int cuda_status(cudaError_t e) {
     return set_status(DNNOPT_STATUS_CUDA_ERROR);
 }
 
+int kernel_error_status(uint32_t code) {
+    constexpr uint32_t kBadIndex = 4;   // kKerrBadIndex
+    return code == kBadIndex ? DNNOPT_STATUS_INVALID_VALUE : DNNOPT_STATUS_KERNEL_TIMEOUT;
+}
+
 void note_launch(int n) { g_launches.fetch_add(static_cast<uint64_t>(n), std::memory_order_relaxed); }
 
 int check_injected_fault(int site) {

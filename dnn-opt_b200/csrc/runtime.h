@@ -61,6 +61,8 @@ int set_status(int st);                 // records as the thread's last status
 int cuda_status(cudaError_t e);         // maps a CUDA error to a status (and records it)
 void note_launch(int n = 1);            // library kernel launch counter
 
+int kernel_error_status(uint32_t code); // status of a kernel's error word (nonzero KernelErrorCode)
+
 // Host-side fault injection (tests): returns DNNOPT_STATUS_INJECTED_FAULT
 // while an injected fault of `site` is pending.
 int check_injected_fault(int site);

@@ -229,6 +229,119 @@ int dnnopt_cuda_gemm_f32_noalloc(const dnnopt_gemm_desc* d, const float* A, cons
                                  float* C, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Decoder-step operators (no counterpart in the reference, which stops at the
+ * GEMM).  What a caller of the small-M products runs between them when it
+ * generates one token: products with 4-bit weights, attention of the new
+ * token over a paged key-value cache, and the norms around a block.  Device
+ * pointers only, asynchronous on `stream`, nothing is copied or synchronised.
+ * Inference only (no gradients).  Calls on one stream share its workspace;
+ * a first call with a larger problem may allocate, so make it before a stream
+ * capture.
+ * ---------------------------------------------------------------------- */
+enum { DNNOPT_TYPE_F32 = 0, DNNOPT_TYPE_BF16 = 1, DNNOPT_TYPE_E4M3 = 2 /* OCP E4M3FN */ };
+
+/* Product with 4-bit weights and group scales.
+ *   C[m,n] = bias[n] + sum_k A[m,k] * scale[n,k/group] * (code[n,k] - zero[n,k/group])
+ * W holds N rows of codes 0..15, two per byte, the even k in the low four
+ * bits, rows ldw BYTES apart (ldw >= (K+1)/2; the last byte's high half is
+ * ignored for odd K).  scale and zero hold lds (>= number of groups) values a
+ * row, in scale_type; zero points are in units of codes and need not be whole;
+ * zero == NULL stands for 8 (codes of signed values -8..7).  group is a
+ * multiple of 32, or 0 for one group per row; the last group may be short.
+ * A (M x K, lda) and C (M x N, ldc) are row-major in io_type, bias is FP32 [N]
+ * or NULL.  Products and sums are FP32 or better (bf16 operands are multiplied
+ * exactly, FP32 activations are split into three bf16 parts without loss), C
+ * is rounded once, and results do not depend on the order of execution.
+ * M, N or K == 0 is a no-op.  Fastest with W 16-byte aligned and ldw a
+ * multiple of 16, and M <= 8. */
+typedef struct dnnopt_w4_desc {
+    int M, N, K;
+    int lda, ldw, ldc;
+    int group;
+    int lds;
+    int io_type;      /* A and C: DNNOPT_TYPE_F32 or DNNOPT_TYPE_BF16 */
+    int scale_type;   /* scale and zero: DNNOPT_TYPE_F32 or DNNOPT_TYPE_BF16 */
+} dnnopt_w4_desc;
+int dnnopt_cuda_gemm_w4(const dnnopt_w4_desc* d, const void* A, const uint8_t* W, const void* scale,
+                        const void* zero, const float* bias, void* C, void* stream);
+
+/* Attention of one new token per sequence over a paged key-value cache.
+ * Sequence b has L = seq_lens[b] tokens; token j lives in page
+ * page_table[b * table_stride + j / page_size], slot j % page_size.  Element d
+ * of its key for key-value head h is at
+ *   k_cache[page * page_stride + slot * token_stride + h * head_stride + d]
+ * (strides in elements; the same for values), so both [page][slot][head][d]
+ * and [page][head][slot][d] pages can be passed.  Query head i uses key-value
+ * head i / (heads / kv_heads).  With s_j = scale * k_scale * q.k_j, capped to
+ * softcap * tanh(s_j / softcap) when softcap > 0, over the tokens j < L and,
+ * when window > 0, j >= L - window:
+ *   lse = log sum_j exp(s_j),  out = v_scale * sum_j exp(s_j - lse) v_j.
+ * L == 0 gives out = 0, lse = -inf.  Cache slots and table entries outside
+ * those tokens are never used, whatever they hold.
+ * With k_new and v_new (both or neither; [b][kv head][d] in io_type, rows
+ * new_batch_stride / new_head_stride apart), token L - 1's key and value are
+ * taken from them and stored in the cache: divided by k_scale / v_scale and
+ * rounded to cache_type (E4M3 saturates), and attended to as stored.  Pages
+ * written so must belong to one sequence.
+ * Types: FP32 q / out with an FP32 cache, or BF16 q / out with a BF16 or E4M3
+ * cache; k_scale and v_scale must be 1 unless the cache is E4M3.  Scores,
+ * softmax and sums are FP32.  lse ([b][heads], may be NULL) is FP32 and serves
+ * to join this result with attention over other keys.
+ * head_dim is a multiple of 16 up to 256; cache pointers 16-byte aligned and
+ * strides in multiples of 16 bytes (else DNNOPT_STATUS_NOT_SUPPORTED).  Lengths
+ * and page numbers are read on the device and checked there: a length below 0
+ * or above max_pages * page_size makes its sequence count as empty, a needed
+ * page number outside [0, num_pages) leaves out that page's tokens (nothing is
+ * stored there), and dnnopt_stream_status() then returns
+ * DNNOPT_STATUS_INVALID_VALUE. */
+typedef struct dnnopt_paged_attn_desc {
+    int batch, heads, kv_heads, head_dim;
+    int page_size;                 /* tokens per page, >= 1 */
+    int num_pages;                 /* pages in the cache */
+    int max_pages;                 /* entries per page_table row */
+    int window;                    /* 0: none */
+    int io_type, cache_type;
+    float scale, softcap, k_scale, v_scale;
+    int64_t q_batch_stride, q_head_stride;       /* elements */
+    int64_t out_batch_stride, out_head_stride;
+    int64_t new_batch_stride, new_head_stride;   /* used with k_new / v_new */
+    int64_t page_stride, token_stride, head_stride;
+    int64_t table_stride;
+} dnnopt_paged_attn_desc;
+int dnnopt_cuda_paged_attention(const dnnopt_paged_attn_desc* d, const void* q, void* k_cache,
+                                void* v_cache, const int32_t* page_table, const int32_t* seq_lens,
+                                const void* k_new, const void* v_new, void* out, float* lse,
+                                void* stream);
+
+/* The end of one block and the start of the next, over `rows` rows of `cols`:
+ *   h = residual_scale * x + block_scale * gate * post(y)
+ *   z = pre(h)
+ * post and pre are DNNOPT_NORM_NONE, _RMS: v * rsqrt(mean(v^2) + eps) *
+ * (w + weight_offset) + b, or _LAYER: the same of v - mean(v).  Vectors
+ * post_w, post_b, pre_w, pre_b have `cols` entries in weight_type; a NULL
+ * weight stands for ones (weight_offset is then not added), a NULL bias for
+ * zeros.  x, y, h, z and gate are in io_type, rows ld* elements apart; gate
+ * row r / gate_rows is used for row r (gate_rows >= 1; ldg == 0 uses one gate
+ * row for all).  gate may be NULL (ones); y may be NULL (h = residual_scale *
+ * x; gate and post are then not used); h or z may be NULL (not written; not
+ * both).  Statistics are FP32, of unrounded FP32 values: z is the norm of h before
+ * h is rounded to io_type.  h may be x or y, z may be x or y (the same pointer
+ * and pitch); other overlaps are not allowed.  rows or cols == 0 is a no-op;
+ * cols above 49152 is DNNOPT_STATUS_NOT_SUPPORTED. */
+enum { DNNOPT_NORM_NONE = 0, DNNOPT_NORM_RMS = 1, DNNOPT_NORM_LAYER = 2 };
+typedef struct dnnopt_block_norm_desc {
+    int rows, cols;
+    int post, pre;                 /* DNNOPT_NORM_* */
+    int io_type, weight_type;      /* DNNOPT_TYPE_F32 or DNNOPT_TYPE_BF16 */
+    float eps, weight_offset, residual_scale, block_scale;
+    int64_t ldx, ldy, ldh, ldz, ldg;
+    int gate_rows;                 /* rows that share one row of gate, >= 1 */
+} dnnopt_block_norm_desc;
+int dnnopt_cuda_block_norm(const dnnopt_block_norm_desc* d, const void* x, const void* y,
+                           const void* gate, const void* post_w, const void* post_b,
+                           const void* pre_w, const void* pre_b, void* h, void* z, void* stream);
+
+/* ------------------------------------------------------------------------
  * Multi-GPU (one process per GPU).  No reference counterpart: the reference
  * is single-process CPU code.  Config 5's weight GEMM is N-sharded over the
  * ranks and its output all-gathered inside the GEMM kernel over peer memory.
@@ -277,7 +390,9 @@ int dnnopt_cuda_gemm_e4m3bf16_allgather(const dnnopt_gemm_desc* d, const uint16_
 int dnnopt_cuda_peer_wait(const unsigned int* flags, int world, unsigned int epoch,
                           unsigned int timeout_us, void* stream);
 /* Synchronises `stream` and reports (then clears) a bounded wait that gave up
- * in a kernel this library queued on it. */
+ * in a kernel this library queued on it, or an index in device memory (a
+ * sequence length, a page number) that a kernel refused to follow
+ * (DNNOPT_STATUS_INVALID_VALUE). */
 int dnnopt_stream_status(void* stream);
 
 /* ------------------------------------------------------------------------
