@@ -78,7 +78,9 @@ int dnnopt_cuda_paged_attention(const dnnopt_paged_attn_desc* d, const void* q, 
         return set_status(DNNOPT_STATUS_INVALID_VALUE);
     if ((k_new == nullptr) != (v_new == nullptr)) return set_status(DNNOPT_STATUS_INVALID_VALUE);
     if (d->batch > 1 && d->table_stride < d->max_pages) return set_status(DNNOPT_STATUS_INVALID_VALUE);
-    if (static_cast<int64_t>(d->max_pages) * d->page_size > INT32_MAX) return set_status(DNNOPT_STATUS_INVALID_VALUE);
+    // Positions, rounded up to whole tiles, are 32-bit.
+    if (static_cast<int64_t>(d->max_pages) * d->page_size > INT32_MAX - 65536)
+        return set_status(DNNOPT_STATUS_INVALID_VALUE);
     if (d->batch == 0) return set_status(DNNOPT_STATUS_SUCCESS);
     if (!q || !out || !seq_lens || !element_aligned(lse, DNNOPT_TYPE_F32) ||
         !element_aligned(seq_lens, DNNOPT_TYPE_F32) || !element_aligned(page_table, DNNOPT_TYPE_F32))
@@ -104,11 +106,6 @@ int dnnopt_cuda_paged_attention(const dnnopt_paged_attn_desc* d, const void* q, 
     int st;
     DeviceContext* ctx = current_context(&st);
     if (!ctx) return st;
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    Workspace* w = nullptr;
-    st = ensure_workspace(ctx, s, 0, 0, 0, &w);
-    if (st != DNNOPT_STATUS_SUCCESS) return st;
-    if ((st = inject_launch()) != DNNOPT_STATUS_SUCCESS) return st;
     PagedAttnArgs a;
     a.batch = d->batch; a.heads = d->heads; a.kv_heads = d->kv_heads; a.dim = d->head_dim;
     a.page_size = d->page_size; a.num_pages = d->num_pages; a.max_pages = d->max_pages;
@@ -121,8 +118,17 @@ int dnnopt_cuda_paged_attention(const dnnopt_paged_attn_desc* d, const void* q, 
     a.table = page_table; a.table_stride = d->table_stride; a.lens = seq_lens;
     a.k_new = k_new; a.v_new = v_new; a.new_batch = d->new_batch_stride; a.new_head = d->new_head_stride;
     a.out = out; a.out_batch = d->out_batch_stride; a.out_head = d->out_head_stride;
-    a.lse = lse; a.err = w->err;
-    cudaError_t e = launch_paged_attention(a, s);
+    a.lse = lse; a.err = nullptr;
+    PagedAttnPlan plan;
+    cudaError_t e = paged_attention_plan(a, ctx->num_sms, &plan);
+    if (e != cudaSuccess) return cuda_status(e);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    Workspace* w = nullptr;
+    st = ensure_workspace(ctx, s, plan.ws_floats, plan.tickets, 0, &w);
+    if (st != DNNOPT_STATUS_SUCCESS) return st;
+    if ((st = inject_launch()) != DNNOPT_STATUS_SUCCESS) return st;
+    a.err = w->err;
+    e = launch_paged_attention(a, plan, w->ws, w->counters, s);
     note_launch();
     return cuda_status(e);
 }

@@ -340,7 +340,14 @@ struct PagedAttnArgs {
     float* lse;             // nullptr: not written
     uint32_t* err;          // receives kKerrBadIndex for a length or page out of range
 };
-cudaError_t launch_paged_attention(const PagedAttnArgs& a, cudaStream_t s);
+struct PagedAttnPlan {
+    int ctas;
+    size_t ws_floats;       // partial results
+    size_t tickets;         // zero on entry, left zero
+};
+cudaError_t paged_attention_plan(const PagedAttnArgs& a, int num_sms, PagedAttnPlan* plan);
+cudaError_t launch_paged_attention(const PagedAttnArgs& a, const PagedAttnPlan& plan, float* ws, uint32_t* tickets,
+                                   cudaStream_t s);
 
 // h = rs * x + bs * gate * post(y), z = pre(h).
 constexpr int kBlockNormMaxCols = 49152;
