@@ -121,6 +121,7 @@ int dnnopt_cuda_paged_attention(const dnnopt_paged_attn_desc* d, const void* q, 
     a.lse = lse; a.err = nullptr;
     PagedAttnPlan plan;
     cudaError_t e = paged_attention_plan(a, ctx->num_sms, &plan);
+    if (e == cudaErrorNotSupported) return set_status(DNNOPT_STATUS_NOT_SUPPORTED);
     if (e != cudaSuccess) return cuda_status(e);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     Workspace* w = nullptr;

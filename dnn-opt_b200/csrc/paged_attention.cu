@@ -8,22 +8,28 @@
 // through the workspace.  Scores are kept in units of log 2.
 //
 // What bounds it: each cached element is read once and used by the 1-16 query
-// heads of its group, far below the tensor rate, so HBM.  The group's query
-// heads are the 16 rows of an m16n8k16 product (mma.sync): a 64-token tile
-// costs a warp some 200 instructions per 8 KB, about a seventh of what an SM
-// issues while HBM delivers it, so the 128-row tcgen05 tile (at most 16 rows
-// of which would hold a head) has nothing to win.
+// heads of its group, far below the tensor rate, so HBM.  The products are
+// mma.sync m16n8k16 with the tokens (scores) or the dimensions (output) as the
+// 16 rows and eight heads as the columns, so that one head or eight cost the
+// same and nothing is computed twice; a 128-row tcgen05 tile would have at
+// most 16 of its rows or columns filled.
 //
 // Exactness.  bf16 products are exact and summed in FP32; weights exp(s - m)
 // enter the second product as two bf16 parts (16 bits), so that the output
 // carries one rounding, its own.  E4M3 keys and values are exact in f16: they
 // are multiplied there, the query normalised by a power of two per head and
-// the weights scaled by 2^15 so that neither leaves f16's range.  FP32 operands
+// the weights scaled by 2^7 so that neither leaves f16's range.  FP32 operands
 // are cut into three bf16 parts each (24 bits, no loss); products below 2^-24
-// of the largest are left out.
+// of the largest are left out, and each step's sum starts from zero, because
+// the matrix units truncate what they add to.
+//
+// The reference m of exp(s - m) moves only when a score exceeds it by 2^8:
+// finding a tile's maximum takes six shuffles, asking whether any score
+// exceeds a bound takes one vote.
 #include <cuda_fp8.h>
 
 #include <mutex>
+#include <type_traits>
 #include <unordered_map>
 
 #include "common.cuh"
@@ -32,16 +38,17 @@
 namespace dnnopt_b200 {
 namespace {
 
-constexpr int kTok = 16;            // tokens per warp and tile
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kJoin = 16;           // parts joined by one CTA at a time
+constexpr float kSlack = 8.0f;      // log2 by which a score may exceed the reference
+constexpr float kUp = 7.0f;         // log2 of the scale of f16 weights: 2^(7 + 8) is below f16's 65504
 
 struct Params {
     PagedAttnArgs a;
-    float* ws;                      // partial results: two slots per CTA
-    uint32_t* tickets;              // one per item, then two per CTA
+    float* ws;                      // partial results: two slots per share
+    uint32_t* tickets;              // one per item, then two per share
     int group, hpb, hblocks;        // heads per kv head; per item; items per kv head
+    uint32_t page_mul, page_shift;  // pos / page_size = mulhi(pos, page_mul) >> page_shift (page_size > 1)
 };
 
 template <DType T> struct Io;
@@ -85,6 +92,18 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Transposes an 8 x 8 matrix of 16-bit elements over the warp's lanes.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 __device__ __forceinline__ float hi16(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFF0000u); }
 // The upper halves of two floats (truncation to bf16), x in the low half.
@@ -120,46 +139,61 @@ __device__ __forceinline__ void cut2(float x, float y, uint32_t& h, uint32_t& l)
     }
     l = pack_rn<F16>(x - hx, y - hy);
 }
+// The power of two that brings `top` to [1, 2); 1 for zero, denormal and infinite values.
+__device__ __forceinline__ float to_unit(float top) {
+    uint32_t e = __float_as_uint(top) >> 23;
+    if (e == 0 || e >= 254) e = 127;
+    return __uint_as_float((254 - e) << 23);
+}
 // Four E4M3 bytes as f16, exactly.
 __device__ __forceinline__ void e4m3x4_f16x4(uint32_t four, uint32_t& lo, uint32_t& hi) {
     asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
         : "=r"(lo), "=r"(hi) : "r"(four));
 }
 
-// Tile geometry of one instantiation.  DP: head_dim rounded up to 64, 128 or 256.
-template <DType CT, int DP, bool WIDE>
+// Tile geometry of one instantiation.  DP: head_dim rounded up to 64, 128 or
+// 256; NT: blocks of eight heads per item.
+template <DType CT, int DP, int NT>
 struct Geo {
     static constexpr int EC = CT == DType::F32 ? 4 : (CT == DType::BF16 ? 2 : 1);
-    static constexpr int ROWS = WIDE ? 16 : 8;                     // heads per item
+    static constexpr int HEADS = 8 * NT;                           // heads per item
     static constexpr int PITCH = DP * EC;                          // bytes of a cached row in shared memory
-    static constexpr int KV = kTok * PITCH;                        // one warp's keys (or values) of a tile
-    static constexpr int OUT = ROWS * DP * 4;                      // one warp's O at the end of an item
+    static constexpr int MT = CT == DType::E4M3 && DP <= 128 && NT == 1 ? 2 : 1;   // 16-token blocks per warp and tile
+    static constexpr int TOK = 16 * MT;
+    static constexpr int KV = TOK * PITCH;                         // one warp's keys (or values) of a tile
+    static constexpr int OUT = HEADS * DP * 4;                     // one warp's O at the end of an item
     static constexpr int WS = 2 * KV > OUT ? 2 * KV : OUT;         // one warp's part of a stage
     static constexpr int NW = WS >= 32768 ? 2 : 4;                 // warps
-    static constexpr int TILE = NW * kTok;                         // tokens per tile
-    // Two CTAs per SM where three stages fit twice, so that one streams while the other joins.
-    static constexpr int TWO = 108 * 1024 / (WS * NW), ONE = 216 * 1024 / (WS * NW);
-    static constexpr int STAGES = TWO >= 3 ? (TWO > 6 ? 6 : TWO) : (ONE > 3 ? 3 : ONE);
-    static constexpr int QREGS = CT == DType::F32 ? 6 : (WIDE ? 4 : 2);   // 32-bit words of Q per lane and 16 dims
-    static constexpr int QBYTES = DP / 16 * 32 * QREGS * 4;
+    static constexpr int TILE = NW * TOK;                          // tokens per tile
+    // CTAs per SM: three where two stages fit three times and the registers (168 a thread) suffice.
+    static constexpr int CTAS = WS * NW <= 32768 && DP <= 128 && NT == 1 && !(CT == DType::E4M3) ? 3
+                                : (WS * NW <= 36 * 1024 ? 2 : 1);
+    static constexpr int FIT = (CTAS == 3 ? 70 : (CTAS == 2 ? 108 : 216)) * 1024 / (WS * NW);
+    static constexpr int STAGES = FIT > 4 ? 4 : FIT;
+    static constexpr int QPARTS = CT == DType::F32 ? 3 : 1;
+    static constexpr int QWORDS = 2 * QPARTS * NT;                 // 32-bit words of Q per lane and 16 dims
+    static constexpr int QBYTES = DP / 16 * 32 * QWORDS * 4;
+    static constexpr bool QREG = DP / 16 * QWORDS <= 32;           // queries stay in registers over an item
     static constexpr int SMALL = 2 * NW * 16 * 4 + 16 * 4 + STAGES * NW * 4 + 64;
     static constexpr int SMEM = STAGES * NW * WS + QBYTES + SMALL;
-    static constexpr int PART = ROWS * (DP + 2);                   // floats of one partial result
+    static constexpr int PART = HEADS * (DP + 2);                  // floats of one partial result
     static_assert(STAGES >= 2, "a pipeline needs two stages");
 };
 
-// 16-byte chunk `c` of row `row` in a warp's tile.  bf16 rows are read by
-// ldmatrix, eight rows of one chunk at a time; the others eight chunks at a
-// time from two rows (keys) or four even rows (values): both without bank
-// conflicts.
+// Rotation of a row's 16-byte chunks.  bf16 rows are read by ldmatrix, eight
+// rows of one chunk at a time; the others four chunks from two rows (keys) or
+// two chunks from four even rows (values): all without bank conflicts.
 template <DType CT, int PITCH>
-__device__ __forceinline__ int chunk_at(int row, int c) {
+__device__ __forceinline__ int rotation(int row) {
     int x;
     if constexpr (CT == DType::BF16) x = row & 7;
     else x = ((row & 6) ^ ((row & 1) << 2));
     if constexpr (PITCH == 64) x &= 3;
-    return row * PITCH + ((c ^ x) << 4);
+    return x;
 }
+// 16-byte chunk `c` of row `row` in a warp's tile.
+template <DType CT, int PITCH>
+__device__ __forceinline__ int chunk_at(int row, int c) { return row * PITCH + ((c ^ rotation<CT, PITCH>(row)) << 4); }
 
 // First dimension of the pair that lane t of a quad holds in step s of the
 // score product (the second pair follows at +8 / +2): the order of dimensions
@@ -173,16 +207,18 @@ __device__ __forceinline__ int q_dim(int s, int t) {
 template <DType CT>
 __device__ __forceinline__ int q_second() { return CT == DType::BF16 ? 8 : 2; }
 
-// Where dimension d of an output row lies among the accumulator columns.
+// Dimensions of rows g and g + 8 of output block j.
 template <DType CT>
-__device__ __forceinline__ int o_col(int d) {
-    if constexpr (CT == DType::BF16) return d;
-    else if constexpr (CT == DType::E4M3) return (d & ~63) | ((d & 7) << 3) | ((d >> 3) & 7);
-    else return (d & ~31) | ((d & 3) << 3) | ((d >> 2) & 7);
+__device__ __forceinline__ int o_dim(int j, int g) {
+    if constexpr (CT == DType::BF16) return 16 * j + g;
+    else if constexpr (CT == DType::E4M3) return 64 * (j >> 2) + 8 * g + 2 * (j & 3);
+    else return 32 * (j >> 1) + 4 * g + 2 * (j & 1);
 }
-// Columns of a row are rotated in groups of eight so that the eight rows that
-// a warp stores at once fall into different banks.
-__device__ __forceinline__ int o_at(int row, int col, int pitch) { return row * pitch + (col ^ ((row & 7) << 3)); }
+template <DType CT>
+__device__ __forceinline__ int o_second() { return CT == DType::BF16 ? 8 : 1; }
+// A warp's O in shared memory; the rotation keeps the four heads that it
+// stores at once in different banks.
+__device__ __forceinline__ int o_at(int head, int d, int pitch) { return head * pitch + (d ^ (((head >> 1) & 3) << 3)); }
 
 // A tile's place: sequence, item of the sequence, tile of the item.
 struct Cursor {
@@ -208,13 +244,27 @@ struct Cursor {
     }
 };
 
-template <DType IO, DType CT, int DP, bool WIDE>
-__global__ void __launch_bounds__(Geo<CT, DP, WIDE>::NW * 32) paged_attention_kernel(const Params p) {
-    using G = Geo<CT, DP, WIDE>;
+// Every CTA takes one share of the tiles, equal but for one tile.
+struct Shares {
+    uint32_t total, ctas;
+
+    __device__ Shares(uint32_t tiles, uint32_t grid) : total(tiles), ctas(tiles < grid ? tiles : grid) {}
+    __device__ __forceinline__ uint32_t start(uint32_t c) const {
+        return static_cast<uint32_t>(static_cast<uint64_t>(c) * total / ctas);
+    }
+    // The share that holds tile t: the last one that starts at or before it.
+    __device__ __forceinline__ uint32_t holder(uint32_t t) const {
+        return static_cast<uint32_t>((static_cast<uint64_t>(t + 1) * ctas - 1) / total);
+    }
+};
+
+template <DType IO, DType CT, int DP, int NT>
+__global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTAS) paged_attention_kernel(const Params p) {
+    using G = Geo<CT, DP, NT>;
     using I = Io<IO>;
-    constexpr int NW = G::NW, S = G::STAGES, TILE = G::TILE, ROWS = G::ROWS;
+    constexpr int NW = G::NW, S = G::STAGES, TILE = G::TILE, TOK = G::TOK, MT = G::MT, HEADS = G::HEADS;
     constexpr bool F16 = CT == DType::E4M3;
-    constexpr int KSTEPS = DP / 16, OT = DP / 8;
+    constexpr int KSTEPS = DP / 16, QW = G::QWORDS;
     extern __shared__ __align__(128) unsigned char smem[];
     unsigned char* ring = smem;
     uint32_t* s_q = reinterpret_cast<uint32_t*>(smem + S * NW * G::WS);
@@ -222,80 +272,91 @@ __global__ void __launch_bounds__(Geo<CT, DP, WIDE>::NW * 32) paged_attention_ke
     float* s_l = s_m + NW * 16;
     float* s_f = s_l + NW * 16;                                                  // [16] query scale per head
     uint32_t* s_mask = reinterpret_cast<uint32_t*>(s_f + 16);                    // [S][NW]
-    int* s_find = reinterpret_cast<int*>(s_mask + S * NW);                       // b, ticket
-    long long* s_off = reinterpret_cast<long long*>((reinterpret_cast<uintptr_t>(s_find + 2) + 7) & ~uintptr_t(7));  // sum, offset of b
+    int* s_find = reinterpret_cast<int*>(s_mask + S * NW);                       // [NW], words passed between threads
 
     const PagedAttnArgs& a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     const int items = a.kv_heads * p.hblocks;
     const int dim = a.dim;
 
-    // --- the CTA's share: tiles [lo, hi) of all tiles in (sequence, item, tile) order
-    const int per = (a.batch + NW * 32 - 1) / (NW * 32);
-    long long mine = 0;
-    for (int i = 0; i < per; ++i) {
+    // --- all tiles in (sequence, item, tile) order; a thread (a lane, for up to 32 sequences) knows
+    // the tiles of its own sequences and of those before them
+    const bool few = a.batch <= 32;
+    const int per = few ? 1 : (a.batch + NW * 32 - 1) / (NW * 32);
+    const int b0 = (few ? lane : tid) * per;
+    uint32_t mine = 0;
+    for (int i = 0; i < per && b0 + i < a.batch; ++i) {
         Cursor c;
-        c.b = tid * per + i;
-        if (c.b >= a.batch) break;
+        c.b = b0 + i;
         c.load(p, TILE);
         mine += c.tiles;
     }
-    long long incl = mine;
+    uint32_t incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+        const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
         if (lane >= o) incl += v;
     }
-    long long* s_sum = reinterpret_cast<long long*>(ring);
-    if (lane == 31) s_sum[warp] = incl;
-    __syncthreads();
-    long long before = 0, total = 0;
+    uint32_t total = __shfl_sync(0xFFFFFFFFu, incl, 31);
+    if (!few) {
+        if (lane == 31) s_find[warp] = static_cast<int>(incl);
+        __syncthreads();
+        uint32_t before = 0;
+        total = 0;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-        if (w < warp) before += s_sum[w];
-        total += s_sum[w];
+        for (int w = 0; w < NW; ++w) {
+            if (w < warp) before += s_find[w];
+            total += s_find[w];
+        }
+        incl += before;
+        __syncthreads();
     }
     total *= items;
-    const long long P = total < gridDim.x ? total : gridDim.x;
-    const long long cta = blockIdx.x;
-    if (cta >= P) return;
-    const long long lo = cta * total / P, hi = (cta + 1) * total / P;
-    {
-        const long long start = (before + incl - mine) * items, end = (before + incl) * items;
+    const Shares shares(total, gridDim.x);
+    const uint32_t share = blockIdx.x;
+    if (share >= shares.ctas) return;
+    const uint32_t lo = shares.start(share), hi = shares.start(share + 1);
+    const uint32_t end = incl * items, start = (incl - mine) * items;
+    Cursor cons;
+    uint32_t off0;
+    if (few) {
+        const int owner = __ffs(__ballot_sync(0xFFFFFFFFu, lane < a.batch && lo < end)) - 1;
+        cons.b = owner;
+        off0 = __shfl_sync(0xFFFFFFFFu, start, owner);
+    } else {
         if (lo >= start && lo < end) {
-            long long at = start;
+            uint32_t at = start;
             Cursor c;
-            c.b = tid * per;
+            c.b = b0;
             for (;; ++c.b) {
                 c.load(p, TILE);
-                const long long n = static_cast<long long>(c.tiles) * items;
-                if (lo < at + n) break;
-                at += n;
+                if (lo < at + c.tiles * items) break;
+                at += c.tiles * items;
             }
             s_find[0] = c.b;
-            s_off[0] = at;
+            s_find[1] = static_cast<int>(at);
         }
+        __syncthreads();
+        cons.b = s_find[0];
+        off0 = s_find[1];
+        __syncthreads();
     }
-    __syncthreads();
-    Cursor cons;
-    cons.b = s_find[0];
     cons.load(p, TILE);
-    {
-        const long long in = lo - s_off[0];
-        cons.r = static_cast<int>(in / cons.tiles);
-        cons.t = static_cast<int>(in % cons.tiles);
-    }
-    long long item0 = lo - cons.t;      // first tile of the current item
+    cons.r = static_cast<int>((lo - off0) / cons.tiles);
+    cons.t = static_cast<int>((lo - off0) % cons.tiles);
+    uint32_t item0 = lo - cons.t;       // first tile of the current item
     Cursor prod = cons;
-    __syncthreads();
 
     // --- producer: one warp's tokens of one tile, the page numbers one tile ahead
+    constexpr int LPR = G::PITCH / 16 < 8 ? G::PITCH / 16 : 8;      // lanes per row
+    constexpr int RPP = 32 / LPR;                                   // rows per pass
+    const int nch = dim * G::EC / 16, lrow = lane / LPR, lch = lane % LPR;
     int ent = -1, slot = 0;
     bool want = false, fresh = false;
     auto look = [&]() {
-        const int pos = prod.first + prod.t * TILE + warp * kTok + (lane & 15);
+        const int pos = prod.first + prod.t * TILE + warp * TOK + (lane & (TOK - 1));
         want = pos < prod.len;
-        const int pg = pos / a.page_size;
+        const int pg = a.page_size == 1 ? pos : static_cast<int>(__umulhi(pos, p.page_mul) >> p.page_shift);
         slot = pos - pg * a.page_size;
         ent = want ? __ldg(a.table + prod.b * a.table_stride + pg) : -1;
         fresh = a.k_new != nullptr && pos == prod.len - 1;
@@ -303,36 +364,53 @@ __global__ void __launch_bounds__(Geo<CT, DP, WIDE>::NW * 32) paged_attention_ke
     auto issue = [&](int stage) {
         const bool ok = want && ent >= 0 && ent < a.num_pages;
         if (want && !ok) record_kernel_error(a.err, kKerrBadIndex);
-        const uint32_t valid = __ballot_sync(0xFFFFFFFFu, ok) & 0xFFFFu;
-        const uint32_t real = __ballot_sync(0xFFFFFFFFu, ok && !fresh) & 0xFFFFu;
+        uint32_t valid = __ballot_sync(0xFFFFFFFFu, ok);
+        const uint32_t real = __ballot_sync(0xFFFFFFFFu, ok && !fresh);
+        if constexpr (TOK < 32) valid &= 0xFFFFu;
         if (lane == 0) s_mask[stage * NW + warp] = valid;
         if (valid) {
-            const int kvh = prod.r / p.hblocks;
+            const int kvh = p.hblocks == 1 ? prod.r : prod.r / p.hblocks;
             const long long off = ok ? (ent * a.page_stride + slot * a.token_stride + kvh * a.head_stride) * G::EC : 0;
-            constexpr int LPR = G::PITCH / 16 > 32 ? 32 : G::PITCH / 16;    // lanes per row
-            const uint32_t kbase = smem_u32(ring + (stage * NW + warp) * G::WS);
-            const int nch = dim * G::EC / 16;
+            const uint32_t base = smem_u32(ring + (stage * NW + warp) * G::WS) + lrow * G::PITCH;
 #pragma unroll
-            for (int i = 0; i < kTok * LPR / 32; ++i) {
-                const int row = i * (32 / LPR) + lane / LPR;
-                const long long o = __shfl_sync(0xFFFFFFFFu, off, row);
-                const bool load = (real >> row) & 1u;
+            for (int i = 0; i < TOK / RPP; ++i) {
+                const long long o = __shfl_sync(0xFFFFFFFFu, off, i * RPP + lrow) + lch * 16;
+                const bool load = (real >> (i * RPP + lrow)) & 1u;
+                if (CT != DType::E4M3 && ((valid & ~real) >> (i * RPP + lrow)) & 1u) continue;   // filled below
+                const int x = rotation<CT, G::PITCH>((i * RPP) % 8 + lrow);
+                const uint32_t dst = base + i * RPP * G::PITCH + ((lch ^ x) << 4);
+                const char* ks = static_cast<const char*>(a.k) + o;
+                const char* vs = static_cast<const char*>(a.v) + o;
 #pragma unroll
-                for (int c = lane % LPR; c < G::PITCH / 16; c += LPR) {
-                    if (c < nch) {
-                        const uint32_t dst = kbase + chunk_at<CT, G::PITCH>(row, c);
-                        cp_async16(dst, static_cast<const char*>(a.k) + o + c * 16, load);
-                        cp_async16(dst + G::KV, static_cast<const char*>(a.v) + o + c * 16, load);
+                for (int u = 0; u < G::PITCH / 16 / LPR; ++u) {
+                    // Rows that are not there and dimensions past head_dim become zeros.
+                    const bool in = load && u * LPR + lch < nch;
+                    cp_async16(dst + u * LPR * 16, in ? ks + u * LPR * 16 : static_cast<const char*>(a.k), in);
+                    cp_async16(dst + u * LPR * 16 + G::KV, in ? vs + u * LPR * 16 : static_cast<const char*>(a.v), in);
+                }
+            }
+            if constexpr (CT != DType::E4M3) {
+                if (valid & ~real) {
+                    // The new token's row, from its own tensors.
+                    const int row = __ffs(valid & ~real) - 1;
+                    const int64_t from = prod.b * a.new_batch + kvh * a.new_head;
+                    const uint32_t dst = smem_u32(ring + (stage * NW + warp) * G::WS);
+                    const char* kn = reinterpret_cast<const char*>(static_cast<const typename I::S*>(a.k_new) + from);
+                    const char* vn = reinterpret_cast<const char*>(static_cast<const typename I::S*>(a.v_new) + from);
+                    for (int c = lane; c < G::PITCH / 16; c += 32) {
+                        const bool in = c < nch;
+                        cp_async16(dst + chunk_at<CT, G::PITCH>(row, c), in ? kn + c * 16 : kn, in);
+                        cp_async16(dst + G::KV + chunk_at<CT, G::PITCH>(row, c), in ? vn + c * 16 : vn, in);
                     }
                 }
             }
         }
     };
-    const long long count = hi - lo;
-    long long issued = 0;
+    const int count = static_cast<int>(hi - lo);
+    int issued = 0;
     look();
 #pragma unroll
-    for (int s = 0; s < S - 1; ++s) {
+    for (int s = 0; s < S; ++s) {
         if (issued < count) {
             issue(s);
             if (++issued < count) { prod.next(p, items, TILE); look(); }
@@ -340,384 +418,479 @@ __global__ void __launch_bounds__(Geo<CT, DP, WIDE>::NW * 32) paged_attention_ke
         cp_async_commit();
     }
 
-    float acc[OT][4], m[2], l[2], rowscale[2];
-    int stage = 0;
-    bool begin = true;
-    for (long long i = 0; i < count; ++i) {
-        if (begin) {
-            // --- a new item: its queries in the order of the score product's operand
-            begin = false;
-            const int kvh = cons.r / p.hblocks, h0 = (cons.r - kvh * p.hblocks) * p.hpb;
-            const int nh = p.group - h0 < ROWS ? p.group - h0 : ROWS;
-            const typename I::S* q = static_cast<const typename I::S*>(a.q) + cons.b * a.q_batch +
-                                     (static_cast<int64_t>(kvh) * p.group + h0) * a.q_head;
+    // Lane (g, t) holds heads 2t and 2t + 1 of each block of eight, and of the queries head g.
+    float acc[KSTEPS][NT][4], m[NT][2], l[NT][2], rowscale[NT][2];
+    uint32_t qreg[G::QREG ? KSTEPS : 1][QW];
+    const float cap2 = a.softcap * kLog2e;
+    auto heads_of = [&](const Cursor& c, int64_t& head0) {
+        const int kvh = p.hblocks == 1 ? c.r : c.r / p.hblocks, h0 = (c.r - kvh * p.hblocks) * p.hpb;
+        head0 = static_cast<int64_t>(kvh) * p.group + h0;
+        return p.group - h0 < HEADS ? p.group - h0 : HEADS;
+    };
+    // Two neighbouring query elements, as they lie in memory.
+    using Pair = typename std::conditional<IO == DType::F32, float2, uint32_t>::type;
+    Pair raw[G::QREG ? KSTEPS : 1][NT][2];
+    auto fetch_queries = [&](const Cursor& c) {     // this warp's part of the loads
+        if constexpr (G::QREG) {
+            int64_t head0;
+            const int nh = heads_of(c, head0);
+            const typename I::S* q = static_cast<const typename I::S*>(a.q) + c.b * a.q_batch + head0 * a.q_head;
+#pragma unroll
+            for (int ks = 0; ks < KSTEPS; ++ks)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int d = q_dim<CT>(ks, t4) + e * q_second<CT>(), h = g + 8 * n;
+                        raw[ks][n][e] = Pair{};
+                        if (h < nh && d < dim) raw[ks][n][e] = __ldg(reinterpret_cast<const Pair*>(q + h * a.q_head + d));
+                    }
+        }
+    };
+    auto begin_item = [&](const Cursor& c) {
+        float f8[NT];       // 8-bit caches: power of two that brings head g's largest |q| to [1, 2)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) f8[n] = 1.0f;
+        if constexpr (G::QREG) {
             if constexpr (CT == DType::E4M3) {
-                // Power of two that brings the head's largest |q| to [1, 2).
-                for (int h = warp; h < ROWS; h += NW) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float top = 0.0f;
+#pragma unroll
+                    for (int ks = 0; ks < KSTEPS; ++ks)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            top = fmaxf(top, fmaxf(fabsf(__uint_as_float(raw[ks][n][e] << 16)),
+                                                   fabsf(__uint_as_float(raw[ks][n][e] & 0xFFFF0000u))));
+                    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+                    f8[n] = to_unit(top);
+                }
+            }
+#pragma unroll
+            for (int ks = 0; ks < KSTEPS; ++ks)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        if constexpr (CT == DType::BF16) qreg[ks][2 * n + e] = raw[ks][n][e];
+                        else if constexpr (CT == DType::E4M3)
+                            qreg[ks][2 * n + e] = pack_rn<true>(__uint_as_float(raw[ks][n][e] << 16) * f8[n],
+                                                                __uint_as_float(raw[ks][n][e] & 0xFFFF0000u) * f8[n]);
+                        else cut3(raw[ks][n][e].x, raw[ks][n][e].y, qreg[ks][6 * n + e], qreg[ks][6 * n + 2 + e], qreg[ks][6 * n + 4 + e]);
+                    }
+        } else {
+            // Queries that do not fit the registers: one copy for the CTA, in the order of the operand.
+            int64_t head0;
+            const int nh = heads_of(c, head0);
+            const typename I::S* q = static_cast<const typename I::S*>(a.q) + c.b * a.q_batch + head0 * a.q_head;
+            if constexpr (CT == DType::E4M3) {
+                for (int h = warp; h < HEADS; h += NW) {
                     float top = 0.0f;
                     if (h < nh)
                         for (int d = lane; d < dim; d += 32) top = fmaxf(top, fabsf(I::get(q[h * a.q_head + d])));
 #pragma unroll
                     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-                    uint32_t e = __float_as_uint(top) >> 23;
-                    if (e == 0 || e >= 254) e = 127;
-                    if (lane == 0) s_f[h] = __uint_as_float((254 - e) << 23);
+                    if (lane == 0) s_f[h] = to_unit(top);
                 }
                 __syncthreads();
-            }
-            for (int idx = tid; idx < KSTEPS * 32; idx += NW * 32) {
-                const int ks = idx >> 5, ln = idx & 31, gg = ln >> 2, tt = ln & 3;
-                const int d0 = q_dim<CT>(ks, tt), d1 = d0 + q_second<CT>();
-                float v[ROWS / 8][4];
 #pragma unroll
-                for (int w = 0; w < ROWS / 8; ++w) {
-                    const int h = gg + 8 * w;
+                for (int n = 0; n < NT; ++n) f8[n] = s_f[g + 8 * n];
+            }
+            for (int ks = warp; ks < KSTEPS; ks += NW)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const int d0 = q_dim<CT>(ks, t4), d1 = d0 + q_second<CT>(), h = g + 8 * n;
                     const typename I::S* qh = q + h * a.q_head;
-                    const float f = CT == DType::E4M3 ? s_f[h] : 1.0f;
-                    v[w][0] = h < nh && d0 < dim ? I::get(qh[d0]) * f : 0.0f;
-                    v[w][1] = h < nh && d0 < dim ? I::get(qh[d0 + 1]) * f : 0.0f;
-                    v[w][2] = h < nh && d1 < dim ? I::get(qh[d1]) * f : 0.0f;
-                    v[w][3] = h < nh && d1 < dim ? I::get(qh[d1 + 1]) * f : 0.0f;
+                    uint32_t* dst = s_q + (ks * 32 + lane) * QW;
+                    const float v0 = h < nh && d0 < dim ? I::get(qh[d0]) * f8[n] : 0.0f;
+                    const float v1 = h < nh && d0 < dim ? I::get(qh[d0 + 1]) * f8[n] : 0.0f;
+                    const float v2 = h < nh && d1 < dim ? I::get(qh[d1]) * f8[n] : 0.0f;
+                    const float v3 = h < nh && d1 < dim ? I::get(qh[d1 + 1]) * f8[n] : 0.0f;
+                    if constexpr (CT == DType::F32) {
+                        cut3(v0, v1, dst[6 * n], dst[6 * n + 2], dst[6 * n + 4]);
+                        cut3(v2, v3, dst[6 * n + 1], dst[6 * n + 3], dst[6 * n + 5]);
+                    } else {
+                        dst[2 * n] = pack_rn<F16>(v0, v1);
+                        dst[2 * n + 1] = pack_rn<F16>(v2, v3);
+                    }
                 }
-                uint32_t* dst = s_q + idx * G::QREGS;
-                if constexpr (CT == DType::F32) {
-                    // rows 0-7 the first part, rows 8-15 the second; then the third
-                    cut3(v[0][0], v[0][1], dst[0], dst[1], dst[4]);
-                    cut3(v[0][2], v[0][3], dst[2], dst[3], dst[5]);
-                } else if constexpr (WIDE) {
-                    dst[0] = pack_rn<F16>(v[0][0], v[0][1]);
-                    dst[1] = pack_rn<F16>(v[1][0], v[1][1]);
-                    dst[2] = pack_rn<F16>(v[0][2], v[0][3]);
-                    dst[3] = pack_rn<F16>(v[1][2], v[1][3]);
-                } else {
-                    dst[0] = pack_rn<F16>(v[0][0], v[0][1]);
-                    dst[1] = pack_rn<F16>(v[0][2], v[0][3]);
-                }
-            }
             __syncthreads();
+        }
 #pragma unroll
-            for (int w = 0; w < ROWS / 8; ++w) {
-                m[w] = -INFINITY;
-                l[w] = 0.0f;
-                rowscale[w] = a.scale * a.k_scale;
-                if constexpr (CT == DType::E4M3) rowscale[w] /= s_f[g + 8 * w];     // exact: a power of two
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                m[n][e] = -INFINITY;
+                l[n][e] = 0.0f;
+                float f = a.scale * a.k_scale;
+                if constexpr (CT == DType::E4M3) f /= __shfl_sync(0xFFFFFFFFu, f8[n], 4 * (2 * t4 + e));    // exact
+                rowscale[n][e] = a.softcap > 0.0f ? f / a.softcap : f * kLog2e;
             }
 #pragma unroll
-            for (int j = 0; j < OT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+            for (int j = 0; j < KSTEPS; ++j) acc[j][n][0] = acc[j][n][1] = acc[j][n][2] = acc[j][n][3] = 0.0f;
         }
+    };
 
-        cp_async_wait<S - 2>();
+    // Where an item's parts are: its shares, and the slots of their partial results.
+    struct Parts {
+        uint32_t first, last, tail;     // an item that begins inside its first share is that share's last one
+    };
+    auto parts_of = [&](uint32_t item0, int tiles) {
+        Parts r;
+        r.first = shares.holder(item0);
+        r.last = shares.holder(item0 + tiles - 1);
+        r.tail = shares.start(r.first) < item0 ? 1 : 0;
+        return r;
+    };
+    auto slot_of = [&](const Parts& r, uint32_t c) { return 2 * c + (c == r.first ? r.tail : 0); };
+    // The parts that one CTA joins at a time, and the ticket that says who is the last of them: with
+    // up to 16 parts all, else groups of neighbours, and then the groups.
+    auto near_of = [](uint32_t n) { return n <= 16 ? n : (n <= 256 ? 16u : 32u); };
+    auto first_ticket = [&](const Parts& r, const Cursor& c) {
+        const uint32_t n = r.last - r.first + 1, near = near_of(n);
+        return n <= near ? p.tickets + static_cast<int64_t>(c.b) * items + c.r
+                         : p.tickets + static_cast<int64_t>(a.batch) * items + slot_of(r, r.first + (share - r.first) / near * near);
+    };
+    auto finish = [&](const Cursor& c, int row, int v, float4 sum, float M, float L) {
+        int64_t head0;
+        heads_of(c, head0);
+        const float f = L == 0.0f ? 0.0f : __fdiv_rn(a.v_scale, L);
+        typename I::S* dst = static_cast<typename I::S*>(a.out) + c.b * a.out_batch + (head0 + row) * a.out_head + 4 * v;
+        typename I::S r[4] = {I::put(sum.x * f), I::put(sum.y * f), I::put(sum.z * f), I::put(sum.w * f)};
+        if constexpr (sizeof(typename I::S) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(r);
+        else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(r);
+        if (v == 0 && a.lse)
+            a.lse[static_cast<int64_t>(c.b) * a.heads + head0 + row] =
+                L == 0.0f ? -INFINITY : (M + log2f(L) - (F16 ? kUp : 0.0f)) * kLn2;
+    };
+    constexpr int VPR = DP / 4, RPT = NW * 32 / VPR;        // threads per output row, rows at a time
+    const int orow = tid / VPR, ov = tid % VPR;
+
+    const Cursor head = cons;           // the first item: it may have begun in another share
+    const uint32_t head_item0 = item0;
+    uint32_t ticket0 = 0, ticket1 = 0;  // of the first and the last item, thread 0's
+    bool partial0 = false, partial1 = false;
+    int stage = 0;
+    fetch_queries(cons);
+    begin_item(cons);
+    for (int i = 0; i < count; ++i) {
+        cp_async_wait<S - 1>();
         __syncwarp();
-        // The next tile goes where the previous one was.
-        if (issued < count) {
-            issue(stage == 0 ? S - 1 : stage - 1);
-            if (++issued < count) { prod.next(p, items, TILE); look(); }
-        }
-        cp_async_commit();
-
         const uint32_t mask = s_mask[stage * NW + warp];
         unsigned char* kt = ring + (stage * NW + warp) * G::WS;
         if (mask) {
             if (a.k_new) {
-                // --- the new token's row: into the tile and into the cache
-                const int row = cons.len - 1 - (cons.first + cons.t * TILE + warp * kTok);
-                if (row >= 0 && row < kTok && ((mask >> row) & 1u)) {
+                // --- the new token's row goes into the cache (8-bit caches: and into the tile, rounded)
+                const int row = cons.len - 1 - (cons.first + cons.t * TILE + warp * TOK);
+                if (row >= 0 && row < TOK && ((mask >> row) & 1u)) {
                     const int pos = cons.len - 1, pg = pos / a.page_size, kvh = cons.r / p.hblocks;
                     const long long off = __ldg(a.table + cons.b * a.table_stride + pg) * a.page_stride +
                                           (pos - pg * a.page_size) * a.token_stride + kvh * a.head_stride;
                     const bool keep = cons.r == kvh * p.hblocks;    // one item of the head stores it
-                    const int64_t from = cons.b * a.new_batch + kvh * a.new_head;
+                    for (int c = lane; c < 2 * nch; c += 32) {
+                        const int which = c >= nch, ch = which ? c - nch : c;
+                        uint4* tile = reinterpret_cast<uint4*>(kt + which * G::KV + chunk_at<CT, G::PITCH>(row, ch));
+                        if constexpr (CT == DType::E4M3) {
+                            const uint4* src = reinterpret_cast<const uint4*>(
+                                static_cast<const typename I::S*>(which ? a.v_new : a.k_new) + cons.b * a.new_batch +
+                                kvh * a.new_head + ch * 16);
+                            const float div = which ? a.v_scale : a.k_scale;
+                            const uint4 x = src[0], y = src[1];
+                            const uint32_t in[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                            uint32_t o[4];
 #pragma unroll
-                    for (int which = 0; which < 2; ++which) {
-                        const typename I::S* src = static_cast<const typename I::S*>(which ? a.v_new : a.k_new) + from;
-                        char* dst = static_cast<char*>(which ? a.v : a.k) + off * G::EC;
-                        unsigned char* tile = kt + which * G::KV;
-                        constexpr int N = 16 / G::EC;       // elements of a chunk
-                        for (int c = lane; c * N < dim; c += 32) {
-                            uint4 w;
-                            if constexpr (CT == DType::E4M3) {
-                                const float div = which ? a.v_scale : a.k_scale;
-                                uint32_t* o = reinterpret_cast<uint32_t*>(&w);
+                            for (int e = 0; e < 4; ++e) {
+                                o[e] = 0;
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    o[e] = 0;
-#pragma unroll
-                                    for (int f = 0; f < 4; ++f)
-                                        o[e] |= static_cast<uint32_t>(__nv_cvt_float_to_fp8(
-                                                    __fdiv_rn(I::get(src[c * 16 + e * 4 + f]), div), __NV_SATFINITE, __NV_E4M3))
-                                                << (8 * f);
+                                for (int f = 0; f < 2; ++f) {
+                                    const float2 v = make_float2(__fdiv_rn(__uint_as_float(in[2 * e + f] << 16), div),
+                                                                 __fdiv_rn(__uint_as_float(in[2 * e + f] & 0xFFFF0000u), div));
+                                    o[e] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3)) << (16 * f);
                                 }
-                            } else {
-                                w = *reinterpret_cast<const uint4*>(src + c * N);
                             }
-                            *reinterpret_cast<uint4*>(tile + chunk_at<CT, G::PITCH>(row, c)) = w;
-                            if (keep) *reinterpret_cast<uint4*>(dst + c * 16) = w;
+                            *tile = make_uint4(o[0], o[1], o[2], o[3]);
                         }
+                        if (keep) *reinterpret_cast<uint4*>(static_cast<char*>(which ? a.v : a.k) + off * G::EC + ch * 16) = *tile;
                     }
                     __syncwarp();
                 }
             }
 
-            // --- scores of 16 tokens: two products of 8
-            float s[2][4] = {};
+            // --- scores: 16 tokens x 8 heads per block, four to a lane
+            float s[MT][NT][4];
+#pragma unroll
+            for (int b = 0; b < MT; ++b)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) s[b][n][0] = s[b][n][1] = s[b][n][2] = s[b][n][3] = 0.0f;
             const uint32_t k32 = smem_u32(kt);
+            auto query = [&](int ks, uint32_t (&q)[QW]) {
+                if constexpr (G::QREG) {
+#pragma unroll
+                    for (int w = 0; w < QW; ++w) q[w] = qreg[ks][w];
+                } else {
+#pragma unroll
+                    for (int w = 0; w < QW; w += 2) {
+                        const uint2 v = *reinterpret_cast<const uint2*>(s_q + (ks * 32 + lane) * QW + w);
+                        q[w] = v.x;
+                        q[w + 1] = v.y;
+                    }
+                }
+            };
             if constexpr (CT == DType::BF16) {
-                // ldmatrix: lanes 0-7 tokens 0-7 first half of the step, 8-15 second half, 16-31 tokens 8-15
-                const int row = (lane & 7) + ((lane >> 4) << 3);
+                const int row = lane & 15;      // ldmatrix: lanes 0-15 the step's first half, 16-31 its second
 #pragma unroll
                 for (int ks = 0; ks < KSTEPS; ++ks) {
-                    if (ks * 16 < dim) {
-                        uint32_t b[4], q[4];
-                        ldsm_x4(k32 + chunk_at<CT, G::PITCH>(row, 2 * ks + ((lane >> 3) & 1)), b);
-                        if constexpr (WIDE) {
-                            const uint4 v = reinterpret_cast<const uint4*>(s_q)[ks * 32 + lane];
-                            q[0] = v.x; q[1] = v.y; q[2] = v.z; q[3] = v.w;
-                        } else {
-                            const uint2 v = reinterpret_cast<const uint2*>(s_q)[ks * 32 + lane];
-                            q[0] = v.x; q[1] = 0u; q[2] = v.y; q[3] = 0u;
-                        }
-                        mma<false>(s[0], q, b[0], b[1]);
-                        mma<false>(s[1], q, b[2], b[3]);
+                    uint32_t q[QW];
+                    query(ks, q);
+#pragma unroll
+                    for (int b = 0; b < MT; ++b) {
+                        uint32_t k[4];
+                        ldsm_x4(k32 + b * 16 * G::PITCH + chunk_at<CT, G::PITCH>(row, 2 * ks + (lane >> 4)), k);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma<false>(s[b][n], k, q[2 * n], q[2 * n + 1]);
                     }
                 }
             } else if constexpr (CT == DType::E4M3) {
 #pragma unroll
-                for (int c = 0; c < DP / 64; ++c) {
-                    if (c * 64 < dim) {
-                        uint32_t w[2][4];
+                for (int c = 0; c < DP / 64; ++c)
 #pragma unroll
-                        for (int n = 0; n < 2; ++n) {
-                            // Past head_dim the tile holds whatever was there before: no NaN may meet the query's zero.
-                            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                            if (64 * c + 16 * t4 < dim)
-                                v = *reinterpret_cast<const uint4*>(kt + chunk_at<CT, G::PITCH>(g + 8 * n, 4 * c + t4));
-                            w[n][0] = v.x; w[n][1] = v.y; w[n][2] = v.z; w[n][3] = v.w;
-                        }
+                    for (int b = 0; b < MT; ++b) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(kt + chunk_at<CT, G::PITCH>(16 * b + g, 4 * c + t4));
+                        const uint4 y = *reinterpret_cast<const uint4*>(kt + chunk_at<CT, G::PITCH>(16 * b + g + 8, 4 * c + t4));
+                        const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            uint32_t q[4];
-                            if constexpr (WIDE) {
-                                const uint4 v = reinterpret_cast<const uint4*>(s_q)[(4 * c + j) * 32 + lane];
-                                q[0] = v.x; q[1] = v.y; q[2] = v.z; q[3] = v.w;
-                            } else {
-                                const uint2 v = reinterpret_cast<const uint2*>(s_q)[(4 * c + j) * 32 + lane];
-                                q[0] = v.x; q[1] = 0u; q[2] = v.y; q[3] = 0u;
-                            }
+                            uint32_t q[QW], k[4];
+                            query(4 * c + j, q);
+                            e4m3x4_f16x4(xw[j], k[0], k[2]);
+                            e4m3x4_f16x4(yw[j], k[1], k[3]);
 #pragma unroll
-                            for (int n = 0; n < 2; ++n) {
-                                uint32_t b0, b1;
-                                e4m3x4_f16x4(w[n][j], b0, b1);
-                                mma<true>(s[n], q, b0, b1);
-                            }
+                            for (int n = 0; n < NT; ++n) mma<true>(s[b][n], k, q[2 * n], q[2 * n + 1]);
                         }
                     }
-                }
             } else {
 #pragma unroll
                 for (int ks = 0; ks < KSTEPS; ++ks) {
-                    if (ks * 16 < dim) {
-                        const uint2* qs = reinterpret_cast<const uint2*>(s_q + (ks * 32 + lane) * 6);
-                        const uint2 q01 = qs[0], q23 = qs[1], q45 = qs[2];
-                        const uint32_t qa[4] = {q01.x, q01.y, q23.x, q23.y}, qb[4] = {q45.x, 0u, q45.y, 0u};
+                    uint32_t q[QW];
+                    query(ks, q);
 #pragma unroll
-                        for (int n = 0; n < 2; ++n) {
-                            const float4 v = *reinterpret_cast<const float4*>(kt + chunk_at<CT, G::PITCH>(g + 8 * n, 4 * ks + t4));
-                            uint32_t h0, m0, l0, h1, m1, l1;
-                            cut3(v.x, v.y, h0, m0, l0);
-                            cut3(v.z, v.w, h1, m1, l1);
-                            mma<false>(s[n], qa, l0, l1);
-                            mma<false>(s[n], qb, h0, h1);
-                            mma<false>(s[n], qa, m0, m1);
-                            mma<false>(s[n], qa, h0, h1);
+                    for (int b = 0; b < MT; ++b) {
+                        const float4 x = *reinterpret_cast<const float4*>(kt + chunk_at<CT, G::PITCH>(16 * b + g, 4 * ks + t4));
+                        const float4 y = *reinterpret_cast<const float4*>(kt + chunk_at<CT, G::PITCH>(16 * b + g + 8, 4 * ks + t4));
+                        uint32_t kh[4], km[4], kl[4];
+                        cut3(x.x, x.y, kh[0], km[0], kl[0]);
+                        cut3(y.x, y.y, kh[1], km[1], kl[1]);
+                        cut3(x.z, x.w, kh[2], km[2], kl[2]);
+                        cut3(y.z, y.w, kh[3], km[3], kl[3]);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            const uint32_t* qn = q + 6 * n;
+                            float c[4] = {};
+                            mma<false>(c, kl, qn[0], qn[1]);
+                            mma<false>(c, km, qn[2], qn[3]);
+                            mma<false>(c, kh, qn[4], qn[5]);
+                            mma<false>(c, km, qn[0], qn[1]);
+                            mma<false>(c, kh, qn[2], qn[3]);
+                            mma<false>(c, kh, qn[0], qn[1]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[b][n][e] += c[e];
                         }
                     }
                 }
+            }
+
+            // --- softmax
+            bool over = false;
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {       // rows 8-15 hold the second part's share
-                    s[n][0] += s[n][2];
-                    s[n][1] += s[n][3];
+            for (int b = 0; b < MT; ++b) {
+                const bool in0 = (mask >> (16 * b + g)) & 1u, in1 = (mask >> (16 * b + g + 8)) & 1u;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float& x = s[b][n][e];
+                        x *= rowscale[n][e & 1];
+                        if (a.softcap > 0.0f) x = cap2 * tanhf(x);
+                        x = (e < 2 ? in0 : in1) ? x : -INFINITY;
+                        over = over || x > m[n][e & 1] + kSlack;
+                    }
+            }
+            if (__any_sync(0xFFFFFFFFu, over)) {
+                // The reference moves to the largest score so far.
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float top = m[n][e];
+#pragma unroll
+                        for (int b = 0; b < MT; ++b) top = fmaxf(top, fmaxf(s[b][n][e], s[b][n][e + 2]));
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
+                        const float alpha = m[n][e] == -INFINITY ? 0.0f : ex2(m[n][e] - top);
+                        m[n][e] = top;
+                        l[n][e] *= alpha;
+#pragma unroll
+                        for (int j = 0; j < KSTEPS; ++j) {
+                            acc[j][n][e] *= alpha;
+                            acc[j][n][e + 2] *= alpha;
+                        }
+                    }
+            }
+
+            // --- weights, transposed into the second product's operand: tokens by pairs, a head to each g
+            constexpr int PP = CT == DType::F32 ? 3 : 2;        // parts of a weight
+            uint32_t w[MT][NT][PP][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float up[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) up[e] = m[n][e] == -INFINITY ? 0.0f : (F16 ? kUp - m[n][e] : -m[n][e]);
+#pragma unroll
+                for (int b = 0; b < MT; ++b) {
+                    float (&x)[4] = s[b][n];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        x[e] = ex2(x[e] + up[e & 1]);
+                        l[n][e & 1] += x[e];
+                    }
+                    uint32_t c[PP][2];
+                    if constexpr (CT == DType::F32) {
+                        cut3(x[0], x[1], c[0][0], c[1][0], c[PP - 1][0]);
+                        cut3(x[2], x[3], c[0][1], c[1][1], c[PP - 1][1]);
+                    } else {
+                        cut2<F16>(x[0], x[1], c[0][0], c[1][0]);
+                        cut2<F16>(x[2], x[3], c[0][1], c[1][1]);
+                    }
+#pragma unroll
+                    for (int q = 0; q < PP; ++q) {
+                        w[b][n][q][0] = transpose8x8(c[q][0]);
+                        w[b][n][q][1] = transpose8x8(c[q][1]);
+                    }
                 }
             }
 
-            // --- softmax over the tile's tokens: each lane has two of every eight
-            float alpha[2];
-#pragma unroll
-            for (int w = 0; w < ROWS / 8; ++w) {
-                float top = -INFINITY;
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float& x = s[n][2 * w + e];
-                        x *= rowscale[w];
-                        if (a.softcap > 0.0f) x = a.softcap * tanhf(__fdividef(x, a.softcap));
-                        x = (mask >> (8 * n + 2 * t4 + e)) & 1u ? x * kLog2e : -INFINITY;
-                        top = fmaxf(top, x);
-                    }
-                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                top = fmaxf(top, m[w]);
-                const float ref = top == -INFINITY ? 0.0f : top;
-                alpha[w] = exp2f(m[w] - ref);
-                m[w] = top;
-                l[w] *= alpha[w];
-                const float up = F16 ? 15.0f - ref : -ref;
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float& x = s[n][2 * w + e];
-                        x = exp2f(x + up);
-                        l[w] += x;
-                    }
-            }
-            const bool moved = WIDE ? (alpha[0] != 1.0f || alpha[ROWS / 8 - 1] != 1.0f) : alpha[0] != 1.0f;
-            if (__any_sync(0xFFFFFFFFu, moved)) {
-#pragma unroll
-                for (int j = 0; j < OT; ++j) {
-                    acc[j][0] *= alpha[0];
-                    acc[j][1] *= alpha[0];
-                    acc[j][2] *= alpha[WIDE ? ROWS / 8 - 1 : 0];
-                    acc[j][3] *= alpha[WIDE ? ROWS / 8 - 1 : 0];
-                }
-            }
-
-            // --- weights as operand parts; narrow items carry the second part in rows 8-15
-            uint32_t pa[4], pb[4];
-            if constexpr (CT == DType::F32) {
-                pb[1] = pb[3] = 0u;
-                cut3(s[0][0], s[0][1], pa[0], pa[1], pb[0]);
-                cut3(s[1][0], s[1][1], pa[2], pa[3], pb[2]);
-            } else if constexpr (WIDE) {
-                cut2<F16>(s[0][0], s[0][1], pa[0], pb[0]);
-                cut2<F16>(s[0][2], s[0][3], pa[1], pb[1]);
-                cut2<F16>(s[1][0], s[1][1], pa[2], pb[2]);
-                cut2<F16>(s[1][2], s[1][3], pa[3], pb[3]);
-            } else {
-                cut2<F16>(s[0][0], s[0][1], pa[0], pa[1]);
-                cut2<F16>(s[1][0], s[1][1], pa[2], pa[3]);
-            }
-
-            // --- weights times values
+            // --- values times weights: 16 dimensions x 8 heads per block
             const unsigned char* vt = kt + G::KV;
             if constexpr (CT == DType::BF16) {
-                const int row = lane & 15;
+                const int row = (lane & 7) + ((lane >> 4) << 3);    // lanes 8-15, 24-31 the block's second half
 #pragma unroll
-                for (int j = 0; j < DP / 16; ++j) {
-                    if (j * 16 < dim) {
-                        uint32_t b[4];
-                        ldsm_x4_t(k32 + G::KV + chunk_at<CT, G::PITCH>(row, 2 * j + (lane >> 4)), b);
-                        mma<false>(acc[2 * j], pa, b[0], b[1]);
-                        mma<false>(acc[2 * j + 1], pa, b[2], b[3]);
-                        if constexpr (WIDE) {
-                            mma<false>(acc[2 * j], pb, b[0], b[1]);
-                            mma<false>(acc[2 * j + 1], pb, b[2], b[3]);
+                for (int j = 0; j < KSTEPS; ++j)
+#pragma unroll
+                    for (int b = 0; b < MT; ++b) {
+                        uint32_t v[4];
+                        ldsm_x4_t(k32 + G::KV + b * 16 * G::PITCH + chunk_at<CT, G::PITCH>(row, 2 * j + ((lane >> 3) & 1)), v);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            mma<false>(acc[j][n], v, w[b][n][1][0], w[b][n][1][1]);
+                            mma<false>(acc[j][n], v, w[b][n][0][0], w[b][n][0][1]);
                         }
                     }
-                }
             } else if constexpr (CT == DType::E4M3) {
 #pragma unroll
-                for (int c = 0; c < DP / 64; ++c) {
-                    if (c * 64 < dim) {
+                for (int c = 0; c < DP / 64; ++c)
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {      // four dims of the lane's eight
+                    for (int b = 0; b < MT; ++b) {
+                        uint2 x[4];     // eight dimensions of the lane's four tokens
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            x[k] = *reinterpret_cast<const uint2*>(
+                                vt + chunk_at<CT, G::PITCH>(16 * b + 2 * t4 + (k & 1) + 8 * (k >> 1), 4 * c + (g >> 1)) + (g & 1) * 8);
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
                             uint32_t f[4][2];
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const int row = 2 * t4 + (k & 1) + 8 * (k >> 1);
-                                const uint32_t w = *reinterpret_cast<const uint32_t*>(
-                                    vt + chunk_at<CT, G::PITCH>(row, 4 * c + (g >> 1)) + (g & 1) * 8 + half * 4);
-                                e4m3x4_f16x4(w, f[k][0], f[k][1]);
-                            }
+                            for (int k = 0; k < 4; ++k) e4m3x4_f16x4(half ? x[k].y : x[k].x, f[k][0], f[k][1]);
 #pragma unroll
                             for (int pr = 0; pr < 2; ++pr) {
-                                const int j = 8 * c + half * 4 + pr * 2;
-                                const uint32_t x0 = prmt(f[0][pr], f[1][pr], 0x5410), x1 = prmt(f[2][pr], f[3][pr], 0x5410);
-                                const uint32_t y0 = prmt(f[0][pr], f[1][pr], 0x7632), y1 = prmt(f[2][pr], f[3][pr], 0x7632);
-                                mma<true>(acc[j], pa, x0, x1);
-                                mma<true>(acc[j + 1], pa, y0, y1);
-                                if constexpr (WIDE) {
-                                    mma<true>(acc[j], pb, x0, x1);
-                                    mma<true>(acc[j + 1], pb, y0, y1);
+                                const int j = 4 * c + 2 * half + pr;
+                                const uint32_t v[4] = {prmt(f[0][pr], f[1][pr], 0x5410), prmt(f[0][pr], f[1][pr], 0x7632),
+                                                       prmt(f[2][pr], f[3][pr], 0x5410), prmt(f[2][pr], f[3][pr], 0x7632)};
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) {
+                                    mma<true>(acc[j][n], v, w[b][n][1][0], w[b][n][1][1]);
+                                    mma<true>(acc[j][n], v, w[b][n][0][0], w[b][n][0][1]);
                                 }
                             }
                         }
                     }
-                }
             } else {
 #pragma unroll
-                for (int c = 0; c < DP / 32; ++c) {
-                    if (c * 32 < dim) {
-                        float4 v[4];
+                for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+                    for (int b = 0; b < MT; ++b) {
+                        float4 x[4];
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            v[k] = *reinterpret_cast<const float4*>(vt + chunk_at<CT, G::PITCH>(2 * t4 + (k & 1) + 8 * (k >> 1), 8 * c + g));
+                            x[k] = *reinterpret_cast<const float4*>(
+                                vt + chunk_at<CT, G::PITCH>(16 * b + 2 * t4 + (k & 1) + 8 * (k >> 1), 8 * c + g));
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float x[4] = {(&v[0].x)[j], (&v[1].x)[j], (&v[2].x)[j], (&v[3].x)[j]};
-                            uint32_t h0, m0, l0, h1, m1, l1;
-                            cut3(x[0], x[1], h0, m0, l0);
-                            cut3(x[2], x[3], h1, m1, l1);
-                            mma<false>(acc[4 * c + j], pa, l0, l1);
-                            mma<false>(acc[4 * c + j], pb, h0, h1);
-                            mma<false>(acc[4 * c + j], pa, m0, m1);
-                            mma<false>(acc[4 * c + j], pa, h0, h1);
+                        for (int jj = 0; jj < 2; ++jj) {
+                            uint32_t vh[4], vm[4], vl[4];
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                cut3((&x[0].x)[2 * jj + e], (&x[1].x)[2 * jj + e], vh[e], vm[e], vl[e]);
+                                cut3((&x[2].x)[2 * jj + e], (&x[3].x)[2 * jj + e], vh[e + 2], vm[e + 2], vl[e + 2]);
+                            }
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                const auto& wn = w[b][n];
+                                float o[4] = {};
+                                mma<false>(o, vl, wn[0][0], wn[0][1]);
+                                mma<false>(o, vm, wn[1][0], wn[1][1]);
+                                mma<false>(o, vh, wn[PP - 1][0], wn[PP - 1][1]);
+                                mma<false>(o, vm, wn[0][0], wn[0][1]);
+                                mma<false>(o, vh, wn[1][0], wn[1][1]);
+                                mma<false>(o, vh, wn[0][0], wn[0][1]);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) acc[2 * c + jj][n][e] += o[e];
+                            }
                         }
                     }
-                }
             }
         }
 
-        const bool last = cons.t == cons.tiles - 1 || i + 1 == count;
-        if (last) {
-            // --- the item's end in this CTA: join the warps; the stage just used holds their sums
-            begin = true;
+        const bool ends = cons.t == cons.tiles - 1 || i + 1 == count;
+        if (ends) {
+            // --- the item's end in this share: join the warps; the stage just used holds their sums
             __syncwarp();
             float* o = reinterpret_cast<float*>(kt);
 #pragma unroll
-            for (int w = 0; w < ROWS / 8; ++w) {
-                l[w] += __shfl_xor_sync(0xFFFFFFFFu, l[w], 1);
-                l[w] += __shfl_xor_sync(0xFFFFFFFFu, l[w], 2);
-                if (t4 == 0) {
-                    s_m[warp * 16 + g + 8 * w] = m[w];
-                    s_l[warp * 16 + g + 8 * w] = l[w];
-                }
-            }
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int j = 0; j < OT; ++j) {
-                if constexpr (WIDE) {
-                    *reinterpret_cast<float2*>(o + o_at(g, 8 * j + 2 * t4, DP)) = make_float2(acc[j][0], acc[j][1]);
-                    *reinterpret_cast<float2*>(o + o_at(g + 8, 8 * j + 2 * t4, DP)) = make_float2(acc[j][2], acc[j][3]);
-                } else {
-                    *reinterpret_cast<float2*>(o + o_at(g, 8 * j + 2 * t4, DP)) =
-                        make_float2(acc[j][0] + acc[j][2], acc[j][1] + acc[j][3]);
+                for (int e = 0; e < 2; ++e) {
+                    const int h = 8 * n + 2 * t4 + e;
+                    float sum = l[n][e];
+                    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 4);
+                    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 8);
+                    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 16);
+                    if (g == 0) {
+                        s_m[warp * 16 + h] = m[n][e];
+                        s_l[warp * 16 + h] = sum;
+                    }
+#pragma unroll
+                    for (int j = 0; j < KSTEPS; ++j) {
+                        const int d = o_dim<CT>(j, g);
+                        o[o_at(h, d, DP)] = acc[j][n][e];
+                        o[o_at(h, d + o_second<CT>(), DP)] = acc[j][n][e + 2];
+                    }
                 }
-            }
+            const Cursor done = cons;
+            cons.next(p, items, TILE);
+            if (i + 1 < count) fetch_queries(cons);     // under way while the warps join
             __syncthreads();
-            const int kvh = cons.r / p.hblocks, h0 = (cons.r - kvh * p.hblocks) * p.hpb;
-            const int nh = p.group - h0 < ROWS ? p.group - h0 : ROWS;
-            const int64_t head0 = static_cast<int64_t>(kvh) * p.group + h0;
-            typename I::S* out = static_cast<typename I::S*>(a.out) + cons.b * a.out_batch + head0 * a.out_head;
-            float* lse = a.lse ? a.lse + static_cast<int64_t>(cons.b) * a.heads + head0 : nullptr;
-            const bool whole = item0 >= lo && item0 + cons.tiles <= hi;
-            auto slot_of = [&](long long c, long long first_c) {
-                // An item that begins inside its first CTA's share is that CTA's last one.
-                const bool tail = c == first_c && c * total / P < item0;
-                return p.ws + (2 * c + (tail ? 1 : 0)) * G::PART;
-            };
-            const int vecs = dim / 4;
-            auto finish = [&](int row, int v, float4 sum, float M, float L) {
-                const float f = L == 0.0f ? 0.0f : __fdiv_rn(a.v_scale, L);
-                typename I::S* dst = out + row * a.out_head + 4 * v;
-                typename I::S r[4] = {I::put(sum.x * f), I::put(sum.y * f), I::put(sum.z * f), I::put(sum.w * f)};
-                if constexpr (sizeof(typename I::S) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(r);
-                else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(r);
-                if (v == 0 && lse) lse[row] = L == 0.0f ? -INFINITY : (M + log2f(L) - (F16 ? 15.0f : 0.0f)) * kLn2;
-            };
-            const long long c_first = ((item0 + 1) * P - 1) / total, c_last = ((item0 + cons.tiles) * P - 1) / total;
-            float* part = whole ? nullptr : slot_of(cta, c_first);
-            for (int idx = tid; idx < nh * vecs; idx += NW * 32) {
-                const int row = idx / vecs, v = idx - row * vecs;
+            int64_t head0;
+            const int nh = heads_of(done, head0);
+            const bool whole = item0 >= lo && item0 + done.tiles <= hi;
+            Parts at = {};
+            float* part = nullptr;
+            if (!whole) {
+                at = parts_of(item0, done.tiles);
+                part = p.ws + static_cast<size_t>(slot_of(at, share)) * G::PART;
+            }
+            for (int row = orow; row < nh; row += RPT) {
+                if (4 * ov >= dim) break;
                 float M = -INFINITY, L = 0.0f;
 #pragma unroll
                 for (int w = 0; w < NW; ++w) M = fmaxf(M, s_m[w * 16 + row]);
@@ -725,86 +898,126 @@ __global__ void __launch_bounds__(Geo<CT, DP, WIDE>::NW * 32) paged_attention_ke
                 float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                 for (int w = 0; w < NW; ++w) {
-                    const float f = exp2f(s_m[w * 16 + row] - ref);
-                    const float* ow = reinterpret_cast<const float*>(ring + (stage * NW + w) * G::WS);
+                    const float f = ex2(s_m[w * 16 + row] - ref);
+                    const float4 x = *reinterpret_cast<const float4*>(
+                        reinterpret_cast<const float*>(ring + (stage * NW + w) * G::WS) + o_at(row, 4 * ov, DP));
                     L = fmaf(f, s_l[w * 16 + row], L);
-                    sum.x = fmaf(f, ow[o_at(row, o_col<CT>(4 * v), DP)], sum.x);
-                    sum.y = fmaf(f, ow[o_at(row, o_col<CT>(4 * v + 1), DP)], sum.y);
-                    sum.z = fmaf(f, ow[o_at(row, o_col<CT>(4 * v + 2), DP)], sum.z);
-                    sum.w = fmaf(f, ow[o_at(row, o_col<CT>(4 * v + 3), DP)], sum.w);
+                    sum.x = fmaf(f, x.x, sum.x);
+                    sum.y = fmaf(f, x.y, sum.y);
+                    sum.z = fmaf(f, x.z, sum.z);
+                    sum.w = fmaf(f, x.w, sum.w);
                 }
                 if (whole) {
-                    finish(row, v, sum, M, L);
+                    finish(done, row, ov, sum, M, L);
                 } else {
-                    *reinterpret_cast<float4*>(part + row * DP + 4 * v) = sum;
-                    if (v == 0) {
-                        part[ROWS * DP + row] = M;
-                        part[ROWS * DP + ROWS + row] = L;
-                    }
-                }
-            }
-            if (!whole) {
-                // --- join the CTAs of the item: the last of every kJoin neighbours to arrive joins
-                // theirs, in order, and the last of those joins the joined ones.
-                const long long parts = c_last - c_first + 1;
-                const long long mine_g = (cta - c_first) / kJoin, groups = (parts + kJoin - 1) / kJoin;
-                long long c0 = c_first + mine_g * kJoin, step = 1;
-                long long n = c_last - c0 + 1 < kJoin ? c_last - c0 + 1 : kJoin;
-                uint32_t* ticket = p.tickets + static_cast<int64_t>(a.batch) * items + (slot_of(c0, c_first) - p.ws) / G::PART;
-                for (int level = groups > 1 ? 0 : 1;; ++level) {
-                    if (level == 1) {
-                        ticket = p.tickets + static_cast<int64_t>(cons.b) * items + cons.r;
-                        if (groups > 1) { c0 = c_first; step = kJoin; n = groups; }
-                    }
-                    __syncthreads();
-                    if (tid == 0) s_find[1] = static_cast<int>(atom_add_acq_rel_gpu_u32(ticket, 1u));
-                    __syncthreads();
-                    if (s_find[1] != static_cast<int>(n) - 1) break;
-                    __threadfence();
-                    if (tid == 0) *ticket = 0u;
-                    float* dst0 = slot_of(c0, c_first);
-                    for (int idx = tid; idx < nh * vecs; idx += NW * 32) {
-                        const int row = idx / vecs, v = idx - row * vecs;
-                        float M = -INFINITY, L = 0.0f;
-                        for (long long k = 0; k < n; ++k)
-                            M = fmaxf(M, __ldcg(slot_of(c0 + k * step, c_first) + ROWS * DP + row));
-                        const float ref = M == -INFINITY ? 0.0f : M;
-                        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-                        for (long long k = 0; k < n; ++k) {
-                            const float* from = slot_of(c0 + k * step, c_first);
-                            const float f = exp2f(__ldcg(from + ROWS * DP + row) - ref);
-                            const float4 x = __ldcg(reinterpret_cast<const float4*>(from + row * DP + 4 * v));
-                            L = fmaf(f, __ldcg(from + ROWS * DP + ROWS + row), L);
-                            sum.x = fmaf(f, x.x, sum.x);
-                            sum.y = fmaf(f, x.y, sum.y);
-                            sum.z = fmaf(f, x.z, sum.z);
-                            sum.w = fmaf(f, x.w, sum.w);
-                        }
-                        if (level == 1) {
-                            finish(row, v, sum, M, L);
-                        } else {
-                            // Each thread replaces only elements that it alone reads, the maxima and
-                            // sums after the barrier below.
-                            *reinterpret_cast<float4*>(dst0 + row * DP + 4 * v) = sum;
-                            if (v == 0) { s_m[row] = M; s_l[row] = L; }
-                        }
-                    }
-                    if (level == 1) break;
-                    __syncthreads();
-                    if (tid < nh) {
-                        dst0[ROWS * DP + tid] = s_m[tid];
-                        dst0[ROWS * DP + ROWS + tid] = s_l[tid];
-                    }
+                    *reinterpret_cast<float4*>(part + row * DP + 4 * ov) = sum;
+                    if (ov == 0) *reinterpret_cast<float2*>(part + HEADS * DP + 2 * row) = make_float2(M, L);
                 }
             }
             __syncthreads();
-            item0 += cons.tiles;
+            if (!whole) {
+                // Whether this share is the last of its item is asked now and looked at when the share is done.
+                uint32_t got = 0;
+                if (tid == 0) got = atom_add_acq_rel_gpu_u32(first_ticket(at, done), 1u);
+                if (item0 == head_item0) { partial0 = true; ticket0 = got; }
+                else { partial1 = true; ticket1 = got; }
+            }
+            item0 += done.tiles;
+            if (i + 1 < count) begin_item(cons);
+            else cons = done;
+        } else {
+            cons.next(p, items, TILE);
         }
-        cons.next(p, items, TILE);
+        // The stage is free: every stage's loads but this one's are under way while the next is awaited.
+        __syncwarp();
+        if (issued < count) {
+            issue(stage);
+            if (++issued < count) { prod.next(p, items, TILE); look(); }
+        }
+        cp_async_commit();
         stage = stage + 1 == S ? 0 : stage + 1;
     }
     cp_async_wait<0>();
+
+    // --- join the shares of the first and the last item, if this one was the last to arrive: the
+    // parts in their order, so that results do not depend on which share that is
+    if (tid == 0) {
+        s_find[0] = static_cast<int>(ticket0);
+        s_find[1] = static_cast<int>(ticket1);
+    }
+    __syncthreads();
+    for (int which = 0; which < 2; ++which) {
+        if (!(which == 0 ? partial0 : partial1)) continue;
+        const Cursor c = which == 0 ? head : cons;
+        const Parts at = parts_of(which == 0 ? head_item0 : item0 - cons.tiles, c.tiles);
+        const uint32_t all = at.last - at.first + 1, near = near_of(all), group = (share - at.first) / near;
+        int64_t head0;
+        const int nh = heads_of(c, head0);
+        uint32_t c0 = at.first + group * near, step = 1, n = all - group * near < near ? all - group * near : near;
+        uint32_t got = static_cast<uint32_t>(s_find[which]);
+        uint32_t* ticket = first_ticket(at, c);
+        for (bool top = all <= near;; top = true) {
+            if (got != n - 1) break;
+            if (tid == 0) *ticket = 0u;
+            float* dst = p.ws + static_cast<size_t>(slot_of(at, c0)) * G::PART;
+            for (int row = orow; row < nh; row += RPT) {
+                if (4 * ov >= dim) break;
+                float M = -INFINITY, L = 0.0f;
+                float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                constexpr uint32_t B = 16;      // parts whose loads are under way together
+                for (uint32_t k0 = 0; k0 < n; k0 += B) {
+                    float2 ml[B];
+                    float4 x[B];
+#pragma unroll
+                    for (uint32_t k = 0; k < B; ++k) {
+                        ml[k] = make_float2(-INFINITY, 0.0f);
+                        x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (k0 + k < n) {
+                            const float* from = p.ws + static_cast<size_t>(slot_of(at, c0 + (k0 + k) * step)) * G::PART;
+                            ml[k] = __ldcg(reinterpret_cast<const float2*>(from + HEADS * DP + 2 * row));
+                            x[k] = __ldcg(reinterpret_cast<const float4*>(from + row * DP + 4 * ov));
+                        }
+                    }
+                    float most = M;
+#pragma unroll
+                    for (uint32_t k = 0; k < B; ++k) most = fmaxf(most, ml[k].x);
+                    const float ref = most == -INFINITY ? 0.0f : most, f0 = ex2(M - ref);
+                    L *= f0;
+                    sum.x *= f0; sum.y *= f0; sum.z *= f0; sum.w *= f0;
+                    M = most;
+#pragma unroll
+                    for (uint32_t k = 0; k < B; ++k) {
+                        const float f = ex2(ml[k].x - ref);
+                        L = fmaf(f, ml[k].y, L);
+                        sum.x = fmaf(f, x[k].x, sum.x);
+                        sum.y = fmaf(f, x[k].y, sum.y);
+                        sum.z = fmaf(f, x[k].z, sum.z);
+                        sum.w = fmaf(f, x[k].w, sum.w);
+                    }
+                }
+                if (top) {
+                    finish(c, row, ov, sum, M, L);
+                } else {
+                    // Each thread replaces only elements that it alone reads, the maxima and sums after
+                    // the barrier below.
+                    *reinterpret_cast<float4*>(dst + row * DP + 4 * ov) = sum;
+                    if (ov == 0) { s_m[row] = M; s_l[row] = L; }
+                }
+            }
+            if (top) break;
+            __syncthreads();
+            if (tid < nh) *reinterpret_cast<float2*>(dst + HEADS * DP + 2 * tid) = make_float2(s_m[tid], s_l[tid]);
+            __syncthreads();
+            ticket = p.tickets + static_cast<int64_t>(c.b) * items + c.r;
+            if (tid == 0) s_find[2] = static_cast<int>(atom_add_acq_rel_gpu_u32(ticket, 1u));
+            __syncthreads();
+            got = static_cast<uint32_t>(s_find[2]);
+            c0 = at.first;
+            step = near;
+            n = (all + near - 1) / near;
+        }
+        __syncthreads();
+    }
 }
 
 struct Kernel {
@@ -812,25 +1025,27 @@ struct Kernel {
     int threads, smem, rows, part_floats, tile;
 };
 
-template <DType IO, DType CT, int DP, bool WIDE>
+template <DType IO, DType CT, int DP, int NT>
 Kernel kernel_of() {
-    using G = Geo<CT, DP, WIDE>;
-    return {reinterpret_cast<const void*>(&paged_attention_kernel<IO, CT, DP, WIDE>), G::NW * 32, G::SMEM, G::ROWS, G::PART, G::TILE};
+    using G = Geo<CT, DP, NT>;
+    return {reinterpret_cast<const void*>(&paged_attention_kernel<IO, CT, DP, NT>), G::NW * 32, G::SMEM, G::HEADS, G::PART, G::TILE};
 }
 
-template <DType IO, DType CT, bool WIDE>
+template <DType IO, DType CT, int NT>
 Kernel kernel_for_dim(int dim) {
-    if (dim <= 64) return kernel_of<IO, CT, 64, WIDE>();
-    if (dim <= 128) return kernel_of<IO, CT, 128, WIDE>();
-    return kernel_of<IO, CT, 256, WIDE>();
+    if (dim <= 64) return kernel_of<IO, CT, 64, NT>();
+    if (dim <= 128) return kernel_of<IO, CT, 128, NT>();
+    return kernel_of<IO, CT, 256, NT>();
 }
 
 Kernel select(const PagedAttnArgs& a) {
-    const bool wide = a.heads / a.kv_heads > 8;
-    if (a.ct == DType::F32) return kernel_for_dim<DType::F32, DType::F32, false>(a.dim);
+    // Up to eight heads of a group are one block of columns, more are blocks of 16 (two at a time).
+    const bool two = a.heads / a.kv_heads > 8;
+    if (a.ct == DType::F32)
+        return two ? kernel_for_dim<DType::F32, DType::F32, 2>(a.dim) : kernel_for_dim<DType::F32, DType::F32, 1>(a.dim);
     if (a.ct == DType::BF16)
-        return wide ? kernel_for_dim<DType::BF16, DType::BF16, true>(a.dim) : kernel_for_dim<DType::BF16, DType::BF16, false>(a.dim);
-    return wide ? kernel_for_dim<DType::BF16, DType::E4M3, true>(a.dim) : kernel_for_dim<DType::BF16, DType::E4M3, false>(a.dim);
+        return two ? kernel_for_dim<DType::BF16, DType::BF16, 2>(a.dim) : kernel_for_dim<DType::BF16, DType::BF16, 1>(a.dim);
+    return two ? kernel_for_dim<DType::BF16, DType::E4M3, 2>(a.dim) : kernel_for_dim<DType::BF16, DType::E4M3, 1>(a.dim);
 }
 
 // Resident CTAs per SM, asked once per kernel and device.
@@ -874,6 +1089,8 @@ cudaError_t paged_attention_plan(const PagedAttnArgs& a, int num_sms, PagedAttnP
     int64_t ctas = static_cast<int64_t>(num_sms) * per_sm;
     if (tiles * items < ctas) ctas = tiles * items;
     plan->ctas = static_cast<int>(ctas);
+    // Tiles are counted in 32 bits.
+    if (tiles * items > INT32_MAX) return cudaErrorNotSupported;
     plan->ws_floats = static_cast<size_t>(2 * ctas) * k.part_floats;
     plan->tickets = static_cast<size_t>(items + 2 * ctas);
     return cudaSuccess;
@@ -889,6 +1106,11 @@ cudaError_t launch_paged_attention(const PagedAttnArgs& a, const PagedAttnPlan& 
     p.group = a.heads / a.kv_heads;
     p.hpb = k.rows;
     p.hblocks = (p.group + k.rows - 1) / k.rows;
+    // Exact for every position below 2^31: mul = ceil(2^(31 + ceil(log2 size)) / size).
+    int log = 0;
+    while (log < 31 && (int64_t(1) << log) < a.page_size) ++log;
+    p.page_mul = static_cast<uint32_t>(((uint64_t(1) << (31 + log)) + a.page_size - 1) / a.page_size);
+    p.page_shift = log > 0 ? log - 1 : 0;
     void* args[] = {&p};
     return cudaLaunchKernel(k.fn, dim3(plan.ctas), dim3(k.threads), args, static_cast<size_t>(k.smem), s);
 }
