@@ -48,7 +48,6 @@ int dnnopt_cuda_gemm_w4(const dnnopt_w4_desc* d, const void* A, const uint8_t* W
     int st;
     DeviceContext* ctx = current_context(&st);
     if (!ctx) return st;
-    if ((st = inject_launch()) != DNNOPT_STATUS_SUCCESS) return st;
     W4Args g;
     g.M = d->M; g.N = d->N; g.K = d->K;
     g.groups = groups;
@@ -60,7 +59,14 @@ int dnnopt_cuda_gemm_w4(const dnnopt_w4_desc* d, const void* A, const uint8_t* W
     g.scale = scale; g.zero = zero; g.lds = d->lds;
     g.bias = bias;
     g.C = C; g.ldc = d->ldc;
-    cudaError_t e = launch_gemm_w4(g, static_cast<cudaStream_t>(stream));
+    W4Plan plan;
+    if (!gemm_w4_plan(g, ctx->num_sms, &plan)) return set_status(DNNOPT_STATUS_NOT_SUPPORTED);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    Workspace* w = nullptr;
+    st = ensure_workspace(ctx, s, plan.ws_floats, plan.tickets, 0, &w);
+    if (st != DNNOPT_STATUS_SUCCESS) return st;
+    if ((st = inject_launch()) != DNNOPT_STATUS_SUCCESS) return st;
+    cudaError_t e = launch_gemm_w4(g, plan, w->ws, w->counters, s);
     note_launch();
     return cuda_status(e);
 }
