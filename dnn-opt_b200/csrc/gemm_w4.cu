@@ -114,7 +114,6 @@ struct Cursor {
         q = q0 + warp;
         settle(per_tile, warp);
     }
-    __device__ __forceinline__ bool valid() const { return q < end; }
     __device__ __forceinline__ void settle(uint32_t per_tile, int warp) {
         while (q >= end && left > 0) {
             ++tile;
@@ -122,10 +121,6 @@ struct Cursor {
             left -= end;
             q = warp;
         }
-    }
-    __device__ __forceinline__ void next(uint32_t per_tile, int warp) {
-        q += kWarps;
-        settle(per_tile, warp);
     }
 };
 
@@ -173,49 +168,61 @@ __global__ void __launch_bounds__(kTeams * kTeamThreads, 1) gemm_w4_kernel(const
         const int gi = p.gmul ? static_cast<int>(__umulhi(chunk, p.gmul) >> p.gshift) : static_cast<int>(chunk);
         return gi < g.groups ? gi : g.groups - 1;
     };
-    auto issue = [&](const Cursor& c, int slot) {
-        const uint32_t dst = smem_u32(ring + slot * p.slot_bytes) + lane * 16;
-        const uint32_t chunk = (k_step0 + c.q) * 4 + t4;
-        const int at = static_cast<int>(chunk) * 16;
-        const int here = row_bytes - at < 0 ? 0 : (row_bytes - at > 16 ? 16 : row_bytes - at);
-        const int gi = group_of(chunk);
+    const int es = f32s ? 2 : 1;            // log2 of a scale's bytes
+    const int64_t to_zero = reinterpret_cast<intptr_t>(g.zero) - reinterpret_cast<intptr_t>(g.scale);
+    const uint8_t* wrow[2];                 // the lane's two rows of the tile being requested
+    uintptr_t srow[2];
+    auto open = [&](uint32_t t) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            int64_t n = static_cast<int64_t>(c.tile) * 16 + gr + 8 * h;
+            int64_t n = static_cast<int64_t>(t) * 16 + gr + 8 * h;
             if (n >= g.N) n = g.N - 1;
-            const uint8_t* w = g.W + n * g.ldw;
+            wrow[h] = g.W + n * g.ldw;
+            srow[h] = reinterpret_cast<uintptr_t>(g.scale) + ((n * g.lds) << es);
+        }
+    };
+    const uint32_t mine = smem_u32(ring) + lane * 16;
+    auto issue = [&](uint32_t q, uint32_t slot_off) {
+        const uint32_t dst = mine + slot_off, sdst = dst - lane * 12 + 1024;
+        const uint32_t chunk = (k_step0 + q) * 4 + t4;
+        const int at = static_cast<int>(chunk) * 16, here = max(0, min(16, row_bytes - at));
+        const uint32_t gi = static_cast<uint32_t>(group_of(chunk)) << es;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
             if (aligned) {
-                cp_async16(dst + h * 512, here > 0 ? w + at : w, here);
+                cp_async16(dst + h * 512, here > 0 ? wrow[h] + at : wrow[h], here);
             } else {
                 // Rows that start anywhere: whole 4-byte words that hold at least one byte of the row.
-                const uintptr_t from = reinterpret_cast<uintptr_t>(w) + at, end = reinterpret_cast<uintptr_t>(w) + row_bytes;
+                const uintptr_t row = reinterpret_cast<uintptr_t>(wrow[h]), from = row + at, end = row + row_bytes;
                 const uint32_t* a4 = reinterpret_cast<const uint32_t*>(from & ~uintptr_t(3));
                 uint32_t x[5];
 #pragma unroll
                 for (int i = 0; i < 5; ++i) x[i] = here > 0 && reinterpret_cast<uintptr_t>(a4 + i) < end ? __ldg(a4 + i) : 0u;
                 const uint32_t sh = static_cast<uint32_t>(from & 3) * 8;
-                *reinterpret_cast<uint4*>(ring + slot * p.slot_bytes + lane * 16 + h * 512) =
+                *reinterpret_cast<uint4*>(ring + slot_off + lane * 16 + h * 512) =
                     make_uint4(__funnelshift_r(x[0], x[1], sh), __funnelshift_r(x[1], x[2], sh),
                                __funnelshift_r(x[2], x[3], sh), __funnelshift_r(x[3], x[4], sh));
             }
             // The 4-byte word that holds the scale (bf16: its half is told apart when it is read).
-            const uintptr_t s = reinterpret_cast<uintptr_t>(g.scale) + (n * g.lds + gi) * (f32s ? 4 : 2);
-            cp_async4(smem_u32(ring + slot * p.slot_bytes) + 1024 + h * 128 + lane * 4, reinterpret_cast<const void*>(s & ~uintptr_t(3)));
-            if (zeros) {
-                const uintptr_t z = reinterpret_cast<uintptr_t>(g.zero) + (n * g.lds + gi) * (f32s ? 4 : 2);
-                cp_async4(smem_u32(ring + slot * p.slot_bytes) + 1280 + h * 128 + lane * 4, reinterpret_cast<const void*>(z & ~uintptr_t(3)));
-            }
+            cp_async4(sdst + h * 128, reinterpret_cast<const void*>((srow[h] + gi) & ~uintptr_t(3)));
+            if (zeros) cp_async4(sdst + 256 + h * 128, reinterpret_cast<const void*>((srow[h] + to_zero + gi) & ~uintptr_t(3)));
         }
     };
     Cursor prod(lo, hi, nq, warp);
-#pragma unroll
-    for (int s = 0; s < kSlots; ++s) {
-        if (prod.valid()) {
-            issue(prod, s);
-            prod.next(nq, warp);
+    open(prod.tile);
+    auto request = [&](uint32_t slot_off) {     // the warp's next step
+        if (prod.q < prod.end) {
+            issue(prod.q, slot_off);
+            prod.q += kWarps;
+            if (prod.q >= prod.end && prod.left > 0) {
+                prod.settle(nq, warp);
+                open(prod.tile);
+            }
         }
         cp_async_commit();
-    }
+    };
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) request(s * p.slot_bytes);
 
     // --- the K-range's activations, eight to a thread: as bf16 in the operand's order, and their
     // sums over each stretch of F chunks
@@ -292,40 +299,42 @@ __global__ void __launch_bounds__(kTeams * kTeamThreads, 1) gemm_w4_kernel(const
         return f32s ? __uint_as_float(word) : __uint_as_float((index & 1u) ? word & 0xFFFF0000u : word << 16);
     };
     const uint32_t sbase = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(g.scale) >> 1);
-    const uint32_t zbase = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(g.zero) >> 1);
+    const uint32_t zflip = static_cast<uint32_t>(to_zero >> 1);
+    const uint32_t ring_end = kSlots * p.slot_bytes;
+    const unsigned char* act_lane = act + gr * 64 + t4 * 16;
+    const uint32_t act_word = p.cols * 64;
     // The slots of K-range y.
     auto range_slots = [&](uint32_t y) {
         return p.ws + (static_cast<size_t>(blockIdx.z) * gridDim.y + y) * (p.tiles + gridDim.x * kTeams) * (16 * ROWS);
     };
     uint32_t tile = lo / nq, q0 = lo - tile * nq, done = lo;
-    int slot = 0;
+    uint32_t slot = 0;      // byte offset in the ring
     while (done < hi) {
         const uint32_t n = hi - done < nq - q0 ? hi - done : nq - q0, q1 = q0 + n;
         float tot[NT][4] = {};
+        uint32_t half[2];       // which half of its word a bf16 scale of group 0 is
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t row = tile * 16 + gr + 8 * h;
+            half[h] = (row < static_cast<uint32_t>(g.N) ? row : g.N - 1) * static_cast<uint32_t>(g.lds) + sbase;
+        }
         for (uint32_t q = q0 + warp; q < q1; q += kWarps) {
             cp_async_wait<kSlots - 1>();
-            const unsigned char* src = ring + slot * p.slot_bytes;
-            const uint4 x0 = *reinterpret_cast<const uint4*>(src + lane * 16);
-            const uint4 x1 = *reinterpret_cast<const uint4*>(src + lane * 16 + 512);
+            const unsigned char* src = ring + slot + lane * 16;
+            const uint4 x0 = *reinterpret_cast<const uint4*>(src);
+            const uint4 x1 = *reinterpret_cast<const uint4*>(src + 512);
             uint32_t w[2][4] = {{x0.x, x0.y, x0.z, x0.w}, {x1.x, x1.y, x1.z, x1.w}};
-            const uint32_t chunk = (k_step0 + q) * 4 + t4;
-            const int gi = group_of(chunk);
+            const uint32_t gi = group_of((k_step0 + q) * 4 + t4);
             float sc[2], zr[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                int64_t row = static_cast<int64_t>(tile) * 16 + gr + 8 * h;
-                if (row >= g.N) row = g.N - 1;
-                const uint32_t e = static_cast<uint32_t>(row * g.lds) + gi;
-                sc[h] = to_float(*reinterpret_cast<const uint32_t*>(src + 1024 + h * 128 + lane * 4), e + sbase);
-                zr[h] = zeros ? to_float(*reinterpret_cast<const uint32_t*>(src + 1280 + h * 128 + lane * 4), e + zbase) : 8.0f;
+                const uint32_t* words = reinterpret_cast<const uint32_t*>(src - lane * 12 + 1024 + h * 128);
+                sc[h] = to_float(words[0], half[h] + gi);
+                zr[h] = zeros ? to_float(words[64], half[h] + gi + zflip) : 8.0f;
             }
             // The slot is free: its next step is requested before this one is worked on.
-            if (prod.valid()) {
-                issue(prod, slot);
-                prod.next(nq, warp);
-            }
-            cp_async_commit();
-            slot = slot + 1 == kSlots ? 0 : slot + 1;
+            request(slot);
+            slot = slot + p.slot_bytes == ring_end ? 0 : slot + p.slot_bytes;
 
             // A product takes a word from each lane of a quad.  Lane t holds the four words of chunk t:
             // scales shared by fewer chunks want the words of one chunk (or two) on all four lanes.
@@ -362,8 +371,7 @@ __global__ void __launch_bounds__(kTeams * kTeamThreads, 1) gemm_w4_kernel(const
 #pragma unroll
                     for (int b = 0; b < NT; ++b) {
                         uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                        if (8 * b + gr < cols)
-                            x = *reinterpret_cast<const uint4*>(act + (static_cast<size_t>(q * 4 + wi) * p.cols + 8 * b + gr) * 64 + t4 * 16);
+                        if (8 * b + gr < cols) x = *reinterpret_cast<const uint4*>(act_lane + (q * 4 + wi) * act_word + b * 512);
                         mma_bf16(c[b], a0, x.x, x.y);
                         mma_bf16(c[b], a1, x.z, x.w);
                     }
@@ -405,7 +413,7 @@ __global__ void __launch_bounds__(kTeams * kTeamThreads, 1) gemm_w4_kernel(const
             for (int e = 0; e < 4; ++e) red[(warp * NT * 4 + b * 4 + e) * 32 + lane] = tot[b][e];
         sync();
         const bool whole = n == nq && gridDim.y == 1;
-        float* part_sums = range_slots(blockIdx.y) + part_slot(shares, share, tile, nq, p.tiles) * (16 * ROWS);
+        float* part_sums = whole ? nullptr : range_slots(blockIdx.y) + part_slot(shares, share, tile, nq, p.tiles) * (16 * ROWS);
         for (int idx = tt; idx < 16 * mt; idx += kTeamThreads) {
             const int r = idx & 15, m = idx >> 4;
             const int64_t row = static_cast<int64_t>(tile) * 16 + r;
