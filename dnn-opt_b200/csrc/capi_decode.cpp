@@ -66,7 +66,7 @@ int dnnopt_cuda_gemm_w4(const dnnopt_w4_desc* d, const void* A, const uint8_t* W
     st = ensure_workspace(ctx, s, plan.ws_floats, plan.tickets, 0, &w);
     if (st != DNNOPT_STATUS_SUCCESS) return st;
     if ((st = inject_launch()) != DNNOPT_STATUS_SUCCESS) return st;
-    cudaError_t e = launch_gemm_w4(g, plan, w->ws, w->counters, s);
+    cudaError_t e = launch_gemm_w4(g, plan, w->ws, w->counters, w->err, s);
     note_launch();
     return cuda_status(e);
 }

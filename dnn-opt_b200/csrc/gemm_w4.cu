@@ -19,13 +19,17 @@
 // Activations that are infinite or NaN stay out of the products (they would
 // meet the zero points' sums) and are added for their own row at the end.
 //
-// Work.  128 weights of 16 rows (1 KB) are a step.  All steps, tile after tile
+// Work.  128 weights of 16 rows (1 KB) are a step, one TMA box into the ring of the
+// warp that works on it (16-byte cp.async of the same rows cost 23 shared-memory
+// cycles an instruction and held the kernel at 1.6 TB/s).  All steps, tile after tile
 // of 16 rows, are cut into equal shares, one for each team of eight warps, two
 // teams to an SM; a team's warps take the steps of a tile in turn and add up
 // in shared memory.  A tile cut by a share's end, or by the ends of a K-range, is
 // finished by the last of its shares to arrive, adding the parts in order.  The
 // activations of the K-range sit in shared memory in the order in which the
 // operand reads them.
+#include <cuda.h>
+
 #include <mutex>
 #include <type_traits>
 #include <unordered_set>
@@ -39,8 +43,10 @@ namespace {
 constexpr int kTeams = 2;           // per CTA
 constexpr int kTeamThreads = 256;
 constexpr int kWarps = 8;           // per team
-constexpr int kSlots = 4;           // steps under way per warp
+constexpr int kMaxSlots = 8;        // steps under way per warp, where the activations leave room
+constexpr int kMinSlots = 4;
 constexpr int kStepK = 128;
+constexpr int kStepBytes = 1024;
 constexpr int kMaxSmem = 227 * 1024;
 
 struct Params {
@@ -48,22 +54,14 @@ struct Params {
     int tiles;                      // of 16 rows of W
     int steps;                      // ceil(K / 128)
     int split_steps;                // steps of one K-range (gridDim.y of them)
-    int slot_bytes;
+    int slots;                      // of a warp's ring
+    int aligned;                    // rows of W start at multiples of 16 bytes: the map below holds
     int cols;                       // columns of activations: rows of A, or three parts of each
     uint32_t gmul, gshift;          // chunk of 32 weights -> group
     float* ws;                      // partial tiles, see part_slot
     uint32_t* tickets;              // one per tile and block of rows of A
+    uint32_t* err;                  // receives kKerrMbarTimeout
 };
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int n) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -133,10 +131,12 @@ __device__ __forceinline__ size_t part_slot(const Shares& s, uint32_t share, uin
 // F: chunks of 32 weights that share their scales for sure (4, 2 or 1); sums
 // are scaled every F chunks.  NT: blocks of eight columns.
 template <DType IO, int NT, int F>
-__global__ void __launch_bounds__(kTeams * kTeamThreads, 1) gemm_w4_kernel(const Params p) {
+__global__ void __launch_bounds__(kTeams * kTeamThreads, 1)
+gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     using T = typename std::conditional<IO == DType::F32, float, __nv_bfloat16>::type;
     constexpr bool PARTS = IO == DType::F32;
     constexpr int ROWS = PARTS ? NT * 8 / 3 : NT * 8;       // rows of A per pass
+    constexpr int RED = NT * 128;                           // floats of a warp's sums of a tile
     extern __shared__ __align__(128) unsigned char smem[];
     const W4Args& g = p.g;
     const int tid = threadIdx.x, lane = tid & 31, team = tid / kTeamThreads, tt = tid % kTeamThreads, warp = tt >> 5;
@@ -147,12 +147,14 @@ __global__ void __launch_bounds__(kTeams * kTeamThreads, 1) gemm_w4_kernel(const
     const uint32_t nq = p.steps - k_step0 < p.split_steps ? p.steps - k_step0 : p.split_steps;
     const uint32_t per = static_cast<uint32_t>(p.split_steps);
 
-    unsigned char* ring = smem + (team * kWarps + warp) * kSlots * p.slot_bytes;
-    unsigned char* act = smem + kTeams * kWarps * kSlots * p.slot_bytes;
+    unsigned char* ring = smem + (team * kWarps + warp) * p.slots * kStepBytes;
+    unsigned char* act = smem + kTeams * kWarps * p.slots * kStepBytes;
     float* asum = reinterpret_cast<float*>(act + static_cast<size_t>(per) * p.cols * 256);   // [step][flush][col]
-    float* red = asum + per * (4 / F) * p.cols + team * kWarps * NT * 128;                   // [warp][4 NT][lane]
-    // Rows of A with an infinity or NaN.
-    uint32_t* odd = reinterpret_cast<uint32_t*>(asum + per * (4 / F) * p.cols + kTeams * kWarps * NT * 128);
+    float* red = asum + per * (4 / F) * p.cols + team * 2 * kWarps * RED;                    // [2][warp][4 NT][lane]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(
+        (reinterpret_cast<uintptr_t>(asum + per * (4 / F) * p.cols + kTeams * 2 * kWarps * RED) + 7) & ~uintptr_t(7));
+    uint32_t* odd = reinterpret_cast<uint32_t*>(bars + kTeams * kWarps * kMaxSlots);    // rows of A with an infinity or NaN
+    bars += (team * kWarps + warp) * kMaxSlots;
     const bool zeros = g.zero != nullptr;
     const bool f32s = g.st == DType::F32;
     const int row_bytes = (g.K + 1) / 2;
@@ -162,179 +164,194 @@ __global__ void __launch_bounds__(kTeams * kTeamThreads, 1) gemm_w4_kernel(const
     const bool busy = share < shares.n;
     const uint32_t lo = busy ? shares.start(share) : 0, hi = busy ? shares.start(share + 1) : 0;
 
-    // --- producer: a step's weights (two rows of the tile to a lane, 32 weights each) and their scales
-    const bool aligned = g.ldw % 16 == 0 && reinterpret_cast<uintptr_t>(g.W) % 16 == 0;
-    auto group_of = [&](uint32_t chunk) {
-        const int gi = p.gmul ? static_cast<int>(__umulhi(chunk, p.gmul) >> p.gshift) : static_cast<int>(chunk);
-        return gi < g.groups ? gi : g.groups - 1;
-    };
-    const int es = f32s ? 2 : 1;            // log2 of a scale's bytes
-    const int64_t to_zero = reinterpret_cast<intptr_t>(g.zero) - reinterpret_cast<intptr_t>(g.scale);
-    const uint8_t* wrow[2];                 // the lane's two rows of the tile being requested
-    uintptr_t srow[2];
-    auto open = [&](uint32_t t) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            int64_t n = static_cast<int64_t>(t) * 16 + gr + 8 * h;
-            if (n >= g.N) n = g.N - 1;
-            wrow[h] = g.W + n * g.ldw;
-            srow[h] = reinterpret_cast<uintptr_t>(g.scale) + ((n * g.lds) << es);
-        }
-    };
-    const uint32_t mine = smem_u32(ring) + lane * 16;
-    auto issue = [&](uint32_t q, uint32_t slot_off) {
-        const uint32_t dst = mine + slot_off, sdst = dst - lane * 12 + 1024;
-        const uint32_t chunk = (k_step0 + q) * 4 + t4;
-        const int at = static_cast<int>(chunk) * 16, here = max(0, min(16, row_bytes - at));
-        const uint32_t gi = static_cast<uint32_t>(group_of(chunk)) << es;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (aligned) {
-                cp_async16(dst + h * 512, here > 0 ? wrow[h] + at : wrow[h], here);
+    // --- producer: one step's weights, lane (g, t) two rows of the tile and 32 weights of each
+    if (lane == 0)
+        for (int i = 0; i < p.slots; ++i) mbar_init(bars + i, 1);
+    if (tid == 0) *odd = 0u;
+    fence_mbar_init();
+    __syncwarp();
+    Cursor prod(lo, hi, nq, warp);
+    auto request = [&](int slot) {      // the warp's next step, into a slot that it is done with
+        if (prod.q < prod.end) {
+            if (p.aligned) {
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(bars + slot, kStepBytes);
+                    tma_load_2d(ring + slot * kStepBytes, &map, bars + slot, static_cast<int>((k_step0 + prod.q) * 64),
+                                static_cast<int>(prod.tile * 16));
+                }
             } else {
                 // Rows that start anywhere: whole 4-byte words that hold at least one byte of the row.
-                const uintptr_t row = reinterpret_cast<uintptr_t>(wrow[h]), from = row + at, end = row + row_bytes;
-                const uint32_t* a4 = reinterpret_cast<const uint32_t*>(from & ~uintptr_t(3));
-                uint32_t x[5];
+                const uint32_t at = ((k_step0 + prod.q) * 4 + t4) * 16;
 #pragma unroll
-                for (int i = 0; i < 5; ++i) x[i] = here > 0 && reinterpret_cast<uintptr_t>(a4 + i) < end ? __ldg(a4 + i) : 0u;
-                const uint32_t sh = static_cast<uint32_t>(from & 3) * 8;
-                *reinterpret_cast<uint4*>(ring + slot_off + lane * 16 + h * 512) =
-                    make_uint4(__funnelshift_r(x[0], x[1], sh), __funnelshift_r(x[1], x[2], sh),
-                               __funnelshift_r(x[2], x[3], sh), __funnelshift_r(x[3], x[4], sh));
+                for (int h = 0; h < 2; ++h) {
+                    int64_t n = static_cast<int64_t>(prod.tile) * 16 + gr + 8 * h;
+                    if (n >= g.N) n = g.N - 1;
+                    const uintptr_t row = reinterpret_cast<uintptr_t>(g.W) + n * g.ldw, from = row + at, end = row + row_bytes;
+                    const uint32_t* a4 = reinterpret_cast<const uint32_t*>(from & ~uintptr_t(3));
+                    uint32_t x[5];
+#pragma unroll
+                    for (int i = 0; i < 5; ++i)
+                        x[i] = from < end && reinterpret_cast<uintptr_t>(a4 + i) < end ? __ldg(a4 + i) : 0u;
+                    const uint32_t sh = static_cast<uint32_t>(from & 3) * 8;
+                    *reinterpret_cast<uint4*>(ring + slot * kStepBytes + lane * 16 + h * 512) =
+                        make_uint4(__funnelshift_r(x[0], x[1], sh), __funnelshift_r(x[1], x[2], sh),
+                                   __funnelshift_r(x[2], x[3], sh), __funnelshift_r(x[3], x[4], sh));
+                }
             }
-            // The 4-byte word that holds the scale (bf16: its half is told apart when it is read).
-            cp_async4(sdst + h * 128, reinterpret_cast<const void*>((srow[h] + gi) & ~uintptr_t(3)));
-            if (zeros) cp_async4(sdst + 256 + h * 128, reinterpret_cast<const void*>((srow[h] + to_zero + gi) & ~uintptr_t(3)));
-        }
-    };
-    Cursor prod(lo, hi, nq, warp);
-    open(prod.tile);
-    auto request = [&](uint32_t slot_off) {     // the warp's next step
-        if (prod.q < prod.end) {
-            issue(prod.q, slot_off);
             prod.q += kWarps;
-            if (prod.q >= prod.end && prod.left > 0) {
-                prod.settle(nq, warp);
-                open(prod.tile);
-            }
+            if (prod.q >= prod.end) prod.settle(nq, warp);
         }
-        cp_async_commit();
     };
-#pragma unroll
-    for (int s = 0; s < kSlots; ++s) request(s * p.slot_bytes);
+    for (int s = 0; s < p.slots; ++s) request(s);
 
-    // --- the K-range's activations, eight to a thread: as bf16 in the operand's order, and their
-    // sums over each stretch of F chunks
-    if (tid == 0) *odd = 0u;
+    // --- the K-range's activations: as bf16 in the operand's order, and their sums over each stretch
+    // of F chunks.  Half a warp takes 128 activations of a row, eight to a lane.
     __syncthreads();
     {
-        const uint32_t blocks = nq * 16;
         const bool vec = g.lda % (16 / sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(g.A) % 16 == 0;
-        for (uint32_t idx = tid; idx < blocks * mt; idx += kTeams * kTeamThreads) {
-            const uint32_t m = idx / blocks, j = idx - m * blocks, q = j >> 4, r = j & 15;
-            const int64_t k = static_cast<int64_t>(k_step0) * kStepK + j * 8;
-            const T* a = static_cast<const T*>(g.A) + (m0 + m) * g.lda + k;
-            float v[8];
-            if (vec && k + 8 <= g.K) {
-                if constexpr (PARTS) {
-                    const float4 x = __ldg(reinterpret_cast<const float4*>(a)), y = __ldg(reinterpret_cast<const float4*>(a) + 1);
-                    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-                    v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
-                } else {
-                    const uint4 x = __ldg(reinterpret_cast<const uint4*>(a));
-                    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        const uint32_t units = mt * nq, r = tid & 15;
+        // Which word of which lane these eight weights are, after the exchanges below.
+        const uint32_t w = F == 4 ? (r & 3) : (F == 1 ? (r >> 2) : ((r >> 3) * 2 + (r & 1)));
+        const uint32_t t = F == 4 ? (r >> 2) : (F == 1 ? (r & 3) : (((r >> 2) & 1) + (r & 2)));
+        uint32_t u = tid >> 4, m = u / nq, q = u - m * nq;
+        const uint32_t dm = (kTeams * kTeamThreads / 16) / nq, dq = (kTeams * kTeamThreads / 16) - dm * nq;
+        for (uint32_t u0 = u & ~1u; u0 < units; u0 += kTeams * kTeamThreads / 16) {     // the same count for a whole warp
+            const bool in = u < units;
+            const int64_t k = static_cast<int64_t>(k_step0 + q) * kStepK + r * 8;
+            const T* a = static_cast<const T*>(g.A) + static_cast<int64_t>(m0 + m) * g.lda + k;
+            const uint32_t col = PARTS ? 3 * m : m;
+            unsigned char* dst = act + ((q * 4 + w) * p.cols + col) * 64 + t * 16;
+            float* sums = asum + (q * (4 / F) + r / (4 * F)) * p.cols + col;
+            if constexpr (PARTS) {
+                float v[8] = {};
+                if (in) {
+                    if (vec && k + 8 <= g.K) {
+                        const float4 x = __ldg(reinterpret_cast<const float4*>(a)), y = __ldg(reinterpret_cast<const float4*>(a) + 1);
+                        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+                        v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = k + i < g.K ? a[i] : 0.0f;
+                    }
+                }
+                bool bad = false;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (!(fabsf(v[i]) <= 3.402823466e38f)) { v[i] = 0.0f; bad = true; }
+                if (bad) atomicOr(odd, 1u << m);
+#pragma unroll
+                for (int part = 0; part < 3; ++part) {
+                    uint32_t o[4];
+                    float sum = 0.0f;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        v[2 * i] = __uint_as_float(w[i] << 16);
-                        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+                        o[i] = __byte_perm(__float_as_uint(v[i]), __float_as_uint(v[i + 4]), 0x7632);
+                        const float hx = __uint_as_float(o[i] << 16), hy = __uint_as_float(o[i] & 0xFFFF0000u);
+                        sum += hx + hy;
+                        v[i] -= hx;
+                        v[i + 4] -= hy;
                     }
+                    if (in) *reinterpret_cast<uint4*>(dst + part * 64) = make_uint4(o[0], o[1], o[2], o[3]);
+#pragma unroll
+                    for (int s = 1; s < 4 * F; s <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, s);
+                    if (in && (r & (4 * F - 1)) == 0) sums[part] = sum;
                 }
             } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = k + i < g.K ? static_cast<float>(a[i]) : 0.0f;
-            }
-            bool bad = false;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (!(fabsf(v[i]) <= 3.402823466e38f)) { v[i] = 0.0f; bad = true; }
-            if (bad) atomicOr(odd, 1u << m);
-            // Which word of which lane these eight weights are, after the exchanges below.
-            const uint32_t w = F == 4 ? (r & 3) : (F == 1 ? (r >> 2) : ((r >> 3) * 2 + (r & 1)));
-            const uint32_t t = F == 4 ? (r >> 2) : (F == 1 ? (r & 3) : (((r >> 2) & 1) + (r & 2)));
-            const uint32_t col = PARTS ? 3 * m : m;
-            unsigned char* dst = act + (static_cast<size_t>(q * 4 + w) * p.cols + col) * 64 + t * 16;
-#pragma unroll
-            for (int part = 0; part < (PARTS ? 3 : 1); ++part) {
-                uint32_t o[4];
-                float sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float x = v[i], y = v[i + 4];
-                    o[i] = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
-                    if constexpr (PARTS) {
-                        const float hx = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
-                        const float hy = __uint_as_float(__float_as_uint(y) & 0xFFFF0000u);
-                        sum += hx + hy;
-                        v[i] = x - hx;
-                        v[i + 4] = y - hy;
+                uint32_t x[4] = {};
+                if (in) {
+                    if (vec && k + 8 <= g.K) {
+                        const uint4 y = __ldg(reinterpret_cast<const uint4*>(a));
+                        x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
                     } else {
-                        sum += x + y;
+                        const uint16_t* b = reinterpret_cast<const uint16_t*>(a);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (k + i < g.K) x[i >> 1] |= static_cast<uint32_t>(b[i]) << (16 * (i & 1));
                     }
                 }
-                *reinterpret_cast<uint4*>(dst + part * 64) = make_uint4(o[0], o[1], o[2], o[3]);
-                // There is a multiple of 16 of blocks, so the lanes of a stretch are all here or all gone.
-                const uint32_t here = blocks * mt - (idx - lane) >= 32 ? 0xFFFFFFFFu : 0xFFFFu;
+                float sum = 0.0f;
 #pragma unroll
-                for (int s = 1; s < 4 * F; s <<= 1) sum += __shfl_xor_sync(here, sum, s);
-                if ((r & (4 * F - 1)) == 0) asum[(q * (4 / F) + r / (4 * F)) * p.cols + col + part] = sum;
+                for (int i = 0; i < 4; ++i) sum += __uint_as_float(x[i] << 16) + __uint_as_float(x[i] & 0xFFFF0000u);
+                if (!(fabsf(sum) <= 3.402823466e38f)) {
+                    // An infinity or NaN among them, or finite values whose sum is none: all go the long way.
+                    atomicOr(odd, 1u << m);
+                    sum = 0.0f;
+                    x[0] = x[1] = x[2] = x[3] = 0u;
+                }
+                if (in)
+                    *reinterpret_cast<uint4*>(dst) = make_uint4(__byte_perm(x[0], x[2], 0x5410), __byte_perm(x[0], x[2], 0x7632),
+                                                                __byte_perm(x[1], x[3], 0x5410), __byte_perm(x[1], x[3], 0x7632));
+#pragma unroll
+                for (int s = 1; s < 4 * F; s <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, s);
+                if (in && (r & (4 * F - 1)) == 0) sums[0] = sum;
             }
+            u += kTeams * kTeamThreads / 16;
+            m += dm;
+            q += dq;
+            if (q >= nq) { q -= nq; ++m; }
         }
     }
     __syncthreads();
     if (!busy) return;
 
     auto sync = [&]() { named_barrier_sync(1 + team, kTeamThreads); };
-    auto to_float = [&](uint32_t word, uint32_t index) {    // index: the element's, counted from its 4-byte word
-        return f32s ? __uint_as_float(word) : __uint_as_float((index & 1u) ? word & 0xFFFF0000u : word << 16);
+    // A scale or zero point as it lies in memory (bf16: in the low half), and its value.
+    const int up = f32s ? 0 : 16;
+    auto fetch = [&](const void* base, int64_t e) -> uint32_t {
+        return f32s ? __ldg(static_cast<const uint32_t*>(base) + e) : __ldg(static_cast<const uint16_t*>(base) + e);
     };
-    const uint32_t sbase = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(g.scale) >> 1);
-    const uint32_t zflip = static_cast<uint32_t>(to_zero >> 1);
-    const uint32_t ring_end = kSlots * p.slot_bytes;
-    const unsigned char* act_lane = act + gr * 64 + t4 * 16;
-    const uint32_t act_word = p.cols * 64;
+    auto value = [&](uint32_t raw) { return __uint_as_float(raw << up); };
+    auto group_of = [&](uint32_t chunk) {
+        const int gi = p.gmul ? static_cast<int>(__umulhi(chunk, p.gmul) >> p.gshift) : static_cast<int>(chunk);
+        return gi < g.groups ? gi : g.groups - 1;
+    };
     // The slots of K-range y.
     auto range_slots = [&](uint32_t y) {
         return p.ws + (static_cast<size_t>(blockIdx.z) * gridDim.y + y) * (p.tiles + gridDim.x * kTeams) * (16 * ROWS);
     };
+
+    const unsigned char* act_lane = act + gr * 64 + t4 * 16;
+    const uint32_t act_word = p.cols * 64;
     uint32_t tile = lo / nq, q0 = lo - tile * nq, done = lo;
-    uint32_t slot = 0;      // byte offset in the ring
+    uint32_t phase = 0, buffer = 0;
+    int slot = 0;
+    bool dead = false;
     while (done < hi) {
         const uint32_t n = hi - done < nq - q0 ? hi - done : nq - q0, q1 = q0 + n;
-        float tot[NT][4] = {};
-        uint32_t half[2];       // which half of its word a bf16 scale of group 0 is
+        int64_t srow[2];        // the lane's two rows' first scales
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint32_t row = tile * 16 + gr + 8 * h;
-            half[h] = (row < static_cast<uint32_t>(g.N) ? row : g.N - 1) * static_cast<uint32_t>(g.lds) + sbase;
+            const int64_t row = static_cast<int64_t>(tile) * 16 + gr + 8 * h;
+            srow[h] = (row < g.N ? row : g.N - 1) * g.lds;
         }
+        // A step's scales are read one step ahead; here the tile's come into L2.
+        uint32_t raw[2] = {0, 0}, rawz[2] = {0, 0};
+        auto scales_of = [&](uint32_t q) {
+            const int gi = group_of((k_step0 + q) * 4 + t4);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                raw[h] = fetch(g.scale, srow[h] + gi);
+                if (zeros) rawz[h] = fetch(g.zero, srow[h] + gi);
+            }
+        };
+        if (q0 + warp < q1) scales_of(q0 + warp);
+        float tot[NT][4] = {};
         for (uint32_t q = q0 + warp; q < q1; q += kWarps) {
-            cp_async_wait<kSlots - 1>();
-            const unsigned char* src = ring + slot + lane * 16;
-            const uint4 x0 = *reinterpret_cast<const uint4*>(src);
-            const uint4 x1 = *reinterpret_cast<const uint4*>(src + 512);
-            uint32_t w[2][4] = {{x0.x, x0.y, x0.z, x0.w}, {x1.x, x1.y, x1.z, x1.w}};
-            const uint32_t gi = group_of((k_step0 + q) * 4 + t4);
             float sc[2], zr[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint32_t* words = reinterpret_cast<const uint32_t*>(src - lane * 12 + 1024 + h * 128);
-                sc[h] = to_float(words[0], half[h] + gi);
-                zr[h] = zeros ? to_float(words[64], half[h] + gi + zflip) : 8.0f;
+                sc[h] = value(raw[h]);
+                zr[h] = zeros ? value(rawz[h]) : 8.0f;
             }
-            // The slot is free: its next step is requested before this one is worked on.
-            request(slot);
-            slot = slot + p.slot_bytes == ring_end ? 0 : slot + p.slot_bytes;
+            if (q + kWarps < q1) scales_of(q + kWarps);
+            if (p.aligned && !mbar_try_wait(bars + slot, phase) && !dead) dead = !mbar_wait(bars + slot, phase, nullptr, p.err);
+            const unsigned char* src = ring + slot * kStepBytes + lane * 16;
+            const uint4 x0 = *reinterpret_cast<const uint4*>(src);
+            const uint4 x1 = *reinterpret_cast<const uint4*>(src + 512);
+            uint32_t w[2][4] = {{x0.x, x0.y, x0.z, x0.w}, {x1.x, x1.y, x1.z, x1.w}};
+            __syncwarp();
+            request(slot);      // every lane has read it
+            if (++slot == p.slots) { slot = 0; phase ^= 1u; }
 
             // A product takes a word from each lane of a quad.  Lane t holds the four words of chunk t:
             // scales shared by fewer chunks want the words of one chunk (or two) on all four lanes.
@@ -358,6 +375,7 @@ __global__ void __launch_bounds__(kTeams * kTeamThreads, 1) gemm_w4_kernel(const
                         if (t4 & 1) w[h][i] = have; else w[h][i + 1] = have;
                     }
             }
+            const unsigned char* act_q = act_lane + q * 4 * act_word;
 #pragma unroll
             for (int f = 0; f < 4 / F; ++f) {
                 float c[NT][4] = {};
@@ -371,7 +389,7 @@ __global__ void __launch_bounds__(kTeams * kTeamThreads, 1) gemm_w4_kernel(const
 #pragma unroll
                     for (int b = 0; b < NT; ++b) {
                         uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                        if (8 * b + gr < cols) x = *reinterpret_cast<const uint4*>(act_lane + (q * 4 + wi) * act_word + b * 512);
+                        if (8 * b + gr < cols) x = *reinterpret_cast<const uint4*>(act_q + wi * act_word + b * 512);
                         mma_bf16(c[b], a0, x.x, x.y);
                         mma_bf16(c[b], a1, x.z, x.w);
                     }
@@ -406,11 +424,14 @@ __global__ void __launch_bounds__(kTeams * kTeamThreads, 1) gemm_w4_kernel(const
             }
         }
 
-        // --- the tile's end in this share: add up the warps
+        // --- the tile's end in this share: add up the warps.  Two buffers in turn: whoever writes one
+        // again has passed the barrier that follows its last reading.
+        float* sums = red + buffer * kWarps * RED;
+        buffer ^= 1u;
 #pragma unroll
         for (int b = 0; b < NT; ++b)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) red[(warp * NT * 4 + b * 4 + e) * 32 + lane] = tot[b][e];
+            for (int e = 0; e < 4; ++e) sums[(warp * NT * 4 + b * 4 + e) * 32 + lane] = tot[b][e];
         sync();
         const bool whole = n == nq && gridDim.y == 1;
         float* part_sums = whole ? nullptr : range_slots(blockIdx.y) + part_slot(shares, share, tile, nq, p.tiles) * (16 * ROWS);
@@ -425,34 +446,38 @@ __global__ void __launch_bounds__(kTeams * kTeamThreads, 1) gemm_w4_kernel(const
                 const int col = PARTS ? 3 * m + 2 - part : m, b = col >> 3, e = (col & 1) + 2 * (r >> 3);
                 const int ln = (r & 7) * 4 + ((col & 7) >> 1);
 #pragma unroll
-                for (int wv = 0; wv < kWarps; ++wv) sum += red[(wv * NT * 4 + b * 4 + e) * 32 + ln];
+                for (int wv = 0; wv < kWarps; ++wv) sum += sums[(wv * NT * 4 + b * 4 + e) * 32 + ln];
             }
             if ((*odd >> m) & 1u) {
-                const T* a = static_cast<const T*>(g.A) + (m0 + m) * g.lda;
+                // The activations that stayed out: each stretch of eight that is not finite as a whole.
+                const T* a = static_cast<const T*>(g.A) + static_cast<int64_t>(m0 + m) * g.lda;
                 const int64_t k1 = static_cast<int64_t>(k_step0 + q1) * kStepK < g.K ? static_cast<int64_t>(k_step0 + q1) * kStepK : g.K;
                 for (int64_t k = static_cast<int64_t>(k_step0 + q0) * kStepK; k < k1; ++k) {
                     const float v = static_cast<float>(a[k]);
-                    if (fabsf(v) <= 3.402823466e38f) continue;
+                    bool out = !(fabsf(v) <= 3.402823466e38f);
+                    if (!PARTS) {
+                        float eight[8], s8 = 0.0f;
+                        for (int i = 0; i < 8; ++i) eight[i] = (k & ~7) + i < g.K ? static_cast<float>(a[(k & ~7) + i]) : 0.0f;
+                        for (int i = 0; i < 8; i += 2) s8 += eight[i] + eight[i + 1];
+                        out = !(fabsf(s8) <= 3.402823466e38f);
+                    }
+                    if (!out) continue;
                     const uint32_t code = (g.W[row * g.ldw + k / 2] >> (4 * (k & 1))) & 15u;
                     const int64_t e = row * g.lds + k / g.group;
-                    auto value = [&](const void* s) {
-                        return f32s ? static_cast<const float*>(s)[e] : __bfloat162float(static_cast<const __nv_bfloat16*>(s)[e]);
-                    };
-                    sum += v * (value(g.scale) * (static_cast<float>(code) - (zeros ? value(g.zero) : 8.0f)));
+                    sum += v * (value(fetch(g.scale, e)) * (static_cast<float>(code) - (zeros ? value(fetch(g.zero, e)) : 8.0f)));
                 }
             }
             if (whole) {
                 const float out = sum + (g.bias ? g.bias[row] : 0.0f);
-                static_cast<T*>(g.C)[(m0 + m) * g.ldc + row] = static_cast<T>(out);
+                static_cast<T*>(g.C)[static_cast<int64_t>(m0 + m) * g.ldc + row] = static_cast<T>(out);
             } else {
                 part_sums[idx] = sum;
             }
         }
-        sync();
         done += n;
         if (done < hi) { ++tile; q0 = 0; }
     }
-    cp_async_wait<0>();
+    sync();
 
     // --- tiles that other shares worked on too: the last to arrive adds the parts, K-range after
     // K-range and share after share, so that the sum does not depend on who that is
@@ -492,7 +517,7 @@ __global__ void __launch_bounds__(kTeams * kTeamThreads, 1) gemm_w4_kernel(const
                     for (uint32_t s = s0; s <= s1; ++s)
                         sum += __ldcg(base + (s == s0 ? at : p.tiles + s) * static_cast<size_t>(16 * ROWS));
                 }
-                static_cast<T*>(g.C)[(m0 + m) * g.ldc + row] = static_cast<T>(sum + (g.bias ? g.bias[row] : 0.0f));
+                static_cast<T*>(g.C)[static_cast<int64_t>(m0 + m) * g.ldc + row] = static_cast<T>(sum + (g.bias ? g.bias[row] : 0.0f));
             }
         }
         sync();
@@ -523,6 +548,34 @@ Kernel select(const W4Args& g) {
            : g.M <= 16 ? kernel_for_flush<DType::BF16, 2>(f) : kernel_for_flush<DType::BF16, 4>(f);
 }
 
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+    static EncodeTiled fn = [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            return static_cast<EncodeTiled>(nullptr);
+        return reinterpret_cast<EncodeTiled>(ptr);
+    }();
+    return fn;
+}
+
+// W as bytes [N][(K+1)/2], read in boxes of 64 bytes x 16 rows; bytes and rows past the ends read as zeros.
+bool encode_weights(const W4Args& g, CUtensorMap* map) {
+    EncodeTiled fn = encode_tiled();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>((static_cast<int64_t>(g.K) + 1) / 2), static_cast<cuuint64_t>(g.N)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(g.ldw)};
+    const cuuint32_t box[2] = {64, 16}, one[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(g.W), dims, strides, box, one,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace
 
 bool gemm_w4_plan(const W4Args& g, int num_sms, W4Plan* plan) {
@@ -530,15 +583,18 @@ bool gemm_w4_plan(const W4Args& g, int num_sms, W4Plan* plan) {
     const int rows = g.M < k.rows ? g.M : k.rows;
     const int64_t steps = (static_cast<int64_t>(g.K) + kStepK - 1) / kStepK, tiles = (static_cast<int64_t>(g.N) + 15) / 16;
     plan->cols = g.io == DType::F32 ? 3 * rows : rows;
-    plan->slot_bytes = 1024 + 256 + (g.zero ? 256 : 0);
-    // As much of K at a time as the activations leave room for beside the rings.
-    const int fixed = kTeams * kWarps * (kSlots * plan->slot_bytes + k.nt * 512) + 64;
+    // As much of K at a time as the activations leave room for beside the smallest rings; the rings
+    // take what is left.
+    const int warps = kTeams * kWarps;
+    const int fixed = warps * (2 * k.nt * 512 + kMaxSlots * 8) + 64;
     const int per_step = plan->cols * (256 + 4 * (4 / k.flush));
-    const int64_t most = (kMaxSmem - fixed) / per_step;
+    const int64_t most = (kMaxSmem - fixed - warps * kMinSlots * kStepBytes) / per_step;
     const int64_t splits = (steps + most - 1) / most;
     plan->split_steps = static_cast<int>((steps + splits - 1) / splits);
     plan->splits = static_cast<int>((steps + plan->split_steps - 1) / plan->split_steps);
-    plan->smem = fixed + per_step * plan->split_steps;
+    const int rest = (kMaxSmem - fixed - per_step * plan->split_steps) / (warps * kStepBytes);
+    plan->slots = rest < kMaxSlots ? rest : kMaxSlots;
+    plan->smem = fixed + per_step * plan->split_steps + warps * plan->slots * kStepBytes;
     plan->blocks = (g.M + k.rows - 1) / k.rows;
     // Every SM a CTA, shared among the K-ranges; no more than there are shares of eight steps.
     int64_t ctas = (num_sms + plan->splits - 1) / plan->splits;
@@ -552,7 +608,8 @@ bool gemm_w4_plan(const W4Args& g, int num_sms, W4Plan* plan) {
     return true;
 }
 
-cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint32_t* tickets, cudaStream_t s) {
+cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint32_t* tickets, uint32_t* err,
+                           cudaStream_t s) {
     const Kernel k = select(g);
     static std::mutex mu;
     static std::unordered_set<const void*> known[64];
@@ -573,7 +630,7 @@ cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint3
     p.tiles = (g.N + 15) / 16;
     p.steps = static_cast<int>((static_cast<int64_t>(g.K) + kStepK - 1) / kStepK);
     p.split_steps = plan.split_steps;
-    p.slot_bytes = plan.slot_bytes;
+    p.slots = plan.slots;
     p.cols = plan.cols;
     // chunk / (group / 32) for chunks below 2^31: mul = ceil(2^(31 + ceil(log2 d)) / d).
     const int64_t d = g.groups > 1 ? g.group / 32 : int64_t(1) << 30;
@@ -583,7 +640,10 @@ cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint3
     p.gshift = log > 0 ? log - 1 : 0;
     p.ws = ws;
     p.tickets = tickets;
-    void* args[] = {&p};
+    p.err = err;
+    CUtensorMap map = {};
+    p.aligned = g.ldw % 16 == 0 && reinterpret_cast<uintptr_t>(g.W) % 16 == 0 && encode_weights(g, &map);
+    void* args[] = {&p, &map};
     return cudaLaunchKernel(k.fn, dim3(plan.ctas, plan.splits, plan.blocks), dim3(kTeams * kTeamThreads), args,
                             static_cast<size_t>(plan.smem), s);
 }
