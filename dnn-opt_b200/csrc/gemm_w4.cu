@@ -2,32 +2,37 @@
 //   C[m,n] = bias[n] + sum_k A[m,k] * scale[n,k/g] * (code[n,k] - zero[n,k/g]).
 //
 // What bounds it: a weight is half a byte and used M times, so HBM up to
-// M of about 64; below that, turning codes into operands is the work.  The
-// products are mma.sync m16n8k16 with 16 rows of W and eight columns of
-// activations: a code becomes a bf16 number by placing its four bits in the
-// mantissa of 16.0 (16 + code, one shift and one three-input logic operation
-// for two codes), and the 16 and the zero point are taken off once a group:
-//   sum (code - zero) a = sum (16 + code) a - (16 + zero) sum a.
-// A tcgen05 tile would need the decoded weights in shared memory first, four
-// times the bytes that arrive, for 8 of its at least 64 columns.
+// M of about 64; below that, turning codes into operands is the work, on the
+// pipe that shifts and masks 16 lanes a cycle.  The products are therefore
+// integer ones, mma.sync m16n8k32 of unsigned by signed bytes: the eight codes
+// of a word become two operand registers in three operations (a code to bf16
+// takes one for each and held this kernel at 2.1 TB/s).  16 rows of W are the
+// rows, digits of the activations the columns; a tcgen05 tile would need the
+// decoded weights in shared memory first, four times the bytes that arrive,
+// for at most 24 of its at least 64 columns.
 //
-// Exactness.  16 + code and bf16 activations multiply exactly; sums are FP32
-// and start from zero every 128 (64, 32) weights, because the matrix units
-// truncate what they add to.  FP32 activations are cut into three bf16 parts
-// (24 bits, no loss) that take a column each; there the codes have 8 taken off
-// before the product, since (16 + zero) sum a would cost five bits.
-// Activations that are infinite or NaN stay out of the products (they would
-// meet the zero points' sums) and are added for their own row at the end.
+// Mathematics.  Within 128 consecutive k, a row of A is a power of two times
+// whole numbers |i| < 2^22 (bf16) or 2^30 (FP32), the power chosen by the
+// largest of the 128, and i = sum_d 256^d i_d with signed bytes i_d.  The sums
+// sum_k (code - 8) i_d are exact in 32-bit integers: they start from -8 sum i_d
+// and the bits of 1.5 * 2^23, so that they come out as FP32 numbers.  Then, in
+// FP32, once for every group or 128 weights:
+//   sum (code - zero) a = 2^e (sum_d 256^d sum (code - 8) i_d - (zero - 8) sum i).
+// What is rounded are activations below 2^-14 (bf16; 2^-6, FP32) of the largest
+// of their 128, to 2^-23 (2^-31) of it: less than FP32 sums round.
+// Activations that are infinite or NaN stay out of the products and are added
+// for their own row at the end.
 //
 // Work.  128 weights of 16 rows (1 KB) are a step, one TMA box into the ring of the
 // warp that works on it (16-byte cp.async of the same rows cost 23 shared-memory
-// cycles an instruction and held the kernel at 1.6 TB/s).  All steps, tile after tile
-// of 16 rows, are cut into equal shares, one for each team of eight warps, two
+// cycles an instruction and held the kernel at 1.6 TB/s).  All steps, tile after
+// tile of 16 rows, are cut into equal shares, one for each team of eight warps, two
 // teams to an SM; a team's warps take the steps of a tile in turn and add up
 // in shared memory.  A tile cut by a share's end, or by the ends of a K-range, is
 // finished by the last of its shares to arrive, adding the parts in order.  The
-// activations of the K-range sit in shared memory in the order in which the
-// operand reads them.
+// digits of the K-range sit in shared memory in the order in which the operand
+// reads them.  Rows of W that do not start at multiples of 16 bytes are first
+// copied to a workspace where they do.
 #include <cuda.h>
 
 #include <mutex>
@@ -55,32 +60,26 @@ struct Params {
     int steps;                      // ceil(K / 128)
     int split_steps;                // steps of one K-range (gridDim.y of them)
     int slots;                      // of a warp's ring
-    int aligned;                    // rows of W start at multiples of 16 bytes: the map below holds
-    int cols;                       // columns of activations: rows of A, or three parts of each
+    int rows, cols;                 // rows of A at a time, and columns: a digit of each
+    int bars_at;                    // of the barriers, in shared memory
     uint32_t gmul, gshift;          // chunk of 32 weights -> group
     float* ws;                      // partial tiles, see part_slot
     uint32_t* tickets;              // one per tile and block of rows of A
     uint32_t* err;                  // receives kKerrMbarTimeout
 };
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+__device__ __forceinline__ void mma_u8s8(uint32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-
-// Codes I and I + 4 of a word as two bf16 numbers: 16 + code, or (MINUS8) code - 8.
-template <int I, bool MINUS8>
-__device__ __forceinline__ uint32_t decode(uint32_t w) {
-    const uint32_t s = I == 0 ? w << 3 : w >> (4 * I - 3);
-    uint32_t r = (s & 0x00780078u) | 0x41804180u;
-    if constexpr (MINUS8) {
-        const __nv_bfloat162 off = __floats2bfloat162_rn(24.0f, 24.0f);
-        __nv_bfloat162 v = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&r), off);
-        r = *reinterpret_cast<uint32_t*>(&v);
-    }
-    return r;
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
 }
+constexpr float kMagic = 12582912.0f;           // 1.5 * 2^23: whole numbers below 2^22 added to it keep their bits
+constexpr uint32_t kMagicBits = 0x4B400000u;
 
 // Equal shares of `total` steps, at least eight (one for each warp of a team).
 struct Shares {
@@ -128,36 +127,42 @@ __device__ __forceinline__ size_t part_slot(const Shares& s, uint32_t share, uin
     return s.start(share) <= tile * per_tile ? tile : tiles + share;
 }
 
-// F: chunks of 32 weights that share their scales for sure (4, 2 or 1); sums
-// are scaled every F chunks.  NT: blocks of eight columns.
-template <DType IO, int NT, int F>
+// D digits of an activation: three of bf16, four of FP32.  MI = 0: the digits of
+// up to 8 / D rows of A share one block of eight columns; else MI blocks of
+// eight rows for each digit.  F: chunks of 32 weights that share their scales
+// for sure (4, 2 or 1); sums are scaled every F chunks.
+template <DType IO, int MI, int F>
 __global__ void __launch_bounds__(kTeams * kTeamThreads, 1)
 gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     using T = typename std::conditional<IO == DType::F32, float, __nv_bfloat16>::type;
-    constexpr bool PARTS = IO == DType::F32;
-    constexpr int ROWS = PARTS ? NT * 8 / 3 : NT * 8;       // rows of A per pass
-    constexpr int RED = NT * 128;                           // floats of a warp's sums of a tile
+    constexpr bool PARTS = IO == DType::F32, PACKED = MI == 0;
+    constexpr int D = PARTS ? 4 : 3, BITS = PARTS ? 30 : 22;
+    constexpr int NT = PACKED ? 1 : D * MI;                 // blocks of eight columns
+    constexpr int NB = PACKED ? 1 : MI;                     // blocks of sums, after the digits are put together
+    constexpr int ROWS = PACKED ? 8 / D : 8 * MI;           // rows of A per pass
+    constexpr int RED = NB * 128;                           // floats of a warp's sums of a tile
     extern __shared__ __align__(128) unsigned char smem[];
     const W4Args& g = p.g;
     const int tid = threadIdx.x, lane = tid & 31, team = tid / kTeamThreads, tt = tid % kTeamThreads, warp = tt >> 5;
     const int gr = lane >> 2, t4 = lane & 3;
     const int m0 = blockIdx.z * ROWS, mt = g.M - m0 < ROWS ? g.M - m0 : ROWS;
-    const int cols = PARTS ? 3 * mt : mt;
+    const int tcols = PACKED ? p.cols : p.rows;             // columns of the two tables below
     const int k_step0 = blockIdx.y * p.split_steps;
     const uint32_t nq = p.steps - k_step0 < p.split_steps ? p.steps - k_step0 : p.split_steps;
     const uint32_t per = static_cast<uint32_t>(p.split_steps);
 
     unsigned char* ring = smem + (team * kWarps + warp) * p.slots * kStepBytes;
-    unsigned char* act = smem + kTeams * kWarps * p.slots * kStepBytes;
-    float* asum = reinterpret_cast<float*>(act + static_cast<size_t>(per) * p.cols * 256);   // [step][flush][col]
-    float* red = asum + per * (4 / F) * p.cols + team * 2 * kWarps * RED;                    // [2][warp][4 NT][lane]
+    unsigned char* act = smem + kTeams * kWarps * p.slots * kStepBytes;                      // [step][2][col][t] 16 bytes
+    float* unit = reinterpret_cast<float*>(act + static_cast<size_t>(per) * p.cols * 128);   // [step][tcol]
+    uint32_t* base = reinterpret_cast<uint32_t*>(unit + per * tcols);                        // [step][flush][col]
+    float* isum = reinterpret_cast<float*>(base + per * (4 / F) * p.cols);                   // [step][flush][tcol]
+    float* red = isum + per * (4 / F) * tcols + team * 2 * kWarps * RED;                     // [2][warp][4 NB][lane]
     uint64_t* bars = reinterpret_cast<uint64_t*>(
-        (reinterpret_cast<uintptr_t>(asum + per * (4 / F) * p.cols + kTeams * 2 * kWarps * RED) + 7) & ~uintptr_t(7));
+        smem + p.bars_at);
     uint32_t* odd = reinterpret_cast<uint32_t*>(bars + kTeams * kWarps * kMaxSlots);    // rows of A with an infinity or NaN
     bars += (team * kWarps + warp) * kMaxSlots;
     const bool zeros = g.zero != nullptr;
     const bool f32s = g.st == DType::F32;
-    const int row_bytes = (g.K + 1) / 2;
 
     const Shares shares(p.tiles * nq, gridDim.x * kTeams);
     const uint32_t share = team * gridDim.x + blockIdx.x;
@@ -173,30 +178,10 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     Cursor prod(lo, hi, nq, warp);
     auto request = [&](int slot) {      // the warp's next step, into a slot that it is done with
         if (prod.q < prod.end) {
-            if (p.aligned) {
-                if (lane == 0) {
-                    mbar_arrive_expect_tx(bars + slot, kStepBytes);
-                    tma_load_2d(ring + slot * kStepBytes, &map, bars + slot, static_cast<int>((k_step0 + prod.q) * 64),
-                                static_cast<int>(prod.tile * 16));
-                }
-            } else {
-                // Rows that start anywhere: whole 4-byte words that hold at least one byte of the row.
-                const uint32_t at = ((k_step0 + prod.q) * 4 + t4) * 16;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    int64_t n = static_cast<int64_t>(prod.tile) * 16 + gr + 8 * h;
-                    if (n >= g.N) n = g.N - 1;
-                    const uintptr_t row = reinterpret_cast<uintptr_t>(g.W) + n * g.ldw, from = row + at, end = row + row_bytes;
-                    const uint32_t* a4 = reinterpret_cast<const uint32_t*>(from & ~uintptr_t(3));
-                    uint32_t x[5];
-#pragma unroll
-                    for (int i = 0; i < 5; ++i)
-                        x[i] = from < end && reinterpret_cast<uintptr_t>(a4 + i) < end ? __ldg(a4 + i) : 0u;
-                    const uint32_t sh = static_cast<uint32_t>(from & 3) * 8;
-                    *reinterpret_cast<uint4*>(ring + slot * kStepBytes + lane * 16 + h * 512) =
-                        make_uint4(__funnelshift_r(x[0], x[1], sh), __funnelshift_r(x[1], x[2], sh),
-                                   __funnelshift_r(x[2], x[3], sh), __funnelshift_r(x[3], x[4], sh));
-                }
+            if (lane == 0) {
+                mbar_arrive_expect_tx(bars + slot, kStepBytes);
+                tma_load_2d(ring + slot * kStepBytes, &map, bars + slot, static_cast<int>((k_step0 + prod.q) * 64),
+                            static_cast<int>(prod.tile * 16));
             }
             prod.q += kWarps;
             if (prod.q >= prod.end) prod.settle(nq, warp);
@@ -204,8 +189,9 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     };
     for (int s = 0; s < p.slots; ++s) request(s);
 
-    // --- the K-range's activations: as bf16 in the operand's order, and their sums over each stretch
-    // of F chunks.  Half a warp takes 128 activations of a row, eight to a lane.
+    // --- the K-range's activations as digits in the operand's order, the unit of each 128, and the
+    // sums of whole numbers over each stretch of F chunks.  Half a warp takes 128 activations of a
+    // row, eight to a lane: a word's worth.
     __syncthreads();
     {
         const bool vec = g.lda % (16 / sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(g.A) % 16 == 0;
@@ -219,71 +205,104 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
             const bool in = u < units;
             const int64_t k = static_cast<int64_t>(k_step0 + q) * kStepK + r * 8;
             const T* a = static_cast<const T*>(g.A) + static_cast<int64_t>(m0 + m) * g.lda + k;
-            const uint32_t col = PARTS ? 3 * m : m;
-            unsigned char* dst = act + ((q * 4 + w) * p.cols + col) * 64 + t * 16;
-            float* sums = asum + (q * (4 / F) + r / (4 * F)) * p.cols + col;
-            if constexpr (PARTS) {
-                float v[8] = {};
-                if (in) {
-                    if (vec && k + 8 <= g.K) {
+            float v[8] = {};
+            if (in) {
+                if (vec && k + 8 <= g.K) {
+                    if constexpr (PARTS) {
                         const float4 x = __ldg(reinterpret_cast<const float4*>(a)), y = __ldg(reinterpret_cast<const float4*>(a) + 1);
                         v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
                         v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
                     } else {
+                        const uint4 y = __ldg(reinterpret_cast<const uint4*>(a));
+                        const uint32_t x[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = k + i < g.K ? a[i] : 0.0f;
+                        for (int i = 0; i < 4; ++i) {
+                            v[2 * i] = __uint_as_float(x[i] << 16);
+                            v[2 * i + 1] = __uint_as_float(x[i] & 0xFFFF0000u);
+                        }
                     }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = k + i < g.K ? static_cast<float>(a[i]) : 0.0f;
                 }
-                bool bad = false;
+            }
+            float top = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (!(fabsf(v[i]) <= 3.402823466e38f)) { v[i] = 0.0f; bad = true; }
-                if (bad) atomicOr(odd, 1u << m);
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+            bool bad = top > 3.402823466e38f;
 #pragma unroll
-                for (int part = 0; part < 3; ++part) {
-                    uint32_t o[4];
+            for (int i = 0; i < 8; ++i) bad = bad || v[i] != v[i];
+            if (bad) {
+                atomicOr(odd, 1u << m);
+                top = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (!(fabsf(v[i]) <= 3.402823466e38f)) v[i] = 0.0f;
+                    top = fmaxf(top, fabsf(v[i]));
+                }
+            }
+#pragma unroll
+            for (int s = 1; s < 16; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s));
+            // 2^e is above every |v|; the unit 2^(e - BITS) stays a normal number.
+            int e = static_cast<int>(__float_as_uint(top) >> 23) - 126;
+            e = max(e, BITS - 126);
+            const float scale = __uint_as_float(static_cast<uint32_t>(127 + BITS - e) << 23);
+            uint32_t x[8];
+            if constexpr (PARTS) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = static_cast<uint32_t>(__float2int_rn(v[i] * scale)) + 0x80808080u;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)     // every digit plus 128
+                    x[i] = __float_as_uint(fmaf(v[i], scale, kMagic)) - kMagicBits + 0x00808080u;
+            }
+            // Even k are the low nibbles, the first operand register; odd k the second.
+            uint2 o[4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t p0 = __byte_perm(x[h], x[h + 2], 0x5140), p1 = __byte_perm(x[h + 4], x[h + 6], 0x5140);
+                const uint32_t p2 = __byte_perm(x[h], x[h + 2], 0x7362), p3 = __byte_perm(x[h + 4], x[h + 6], 0x7362);
+                const uint32_t d0 = __byte_perm(p0, p1, 0x5410) ^ 0x80808080u, d1 = __byte_perm(p0, p1, 0x7632) ^ 0x80808080u;
+                const uint32_t d2 = __byte_perm(p2, p3, 0x5410) ^ 0x80808080u, d3 = __byte_perm(p2, p3, 0x7632) ^ 0x80808080u;
+                (h ? o[0].y : o[0].x) = d0;
+                (h ? o[1].y : o[1].x) = d1;
+                (h ? o[2].y : o[2].x) = d2;
+                (h ? o[3].y : o[3].x) = d3;
+            }
+            // Sums of the digits, two to a word: each stays within 16 bits.
+            int pair[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int lo = __dp4a(static_cast<int>(o[2 * h].x), 0x01010101, __dp4a(static_cast<int>(o[2 * h].y), 0x01010101, 0));
+                const int up = __dp4a(static_cast<int>(o[2 * h + 1].x), 0x01010101, __dp4a(static_cast<int>(o[2 * h + 1].y), 0x01010101, 0));
+                pair[h] = lo + up * 65536;
+                if (2 * h + 1 >= D) pair[h] = lo;
+#pragma unroll
+                for (int s = 1; s < 4 * F; s <<= 1) pair[h] += __shfl_xor_sync(0xFFFFFFFFu, pair[h], s);
+            }
+            if (in) {
+                unsigned char* dst = act + ((q * 2 + (w >> 1)) * p.cols + m) * 64 + t * 16 + (w & 1) * 8;
+#pragma unroll
+                for (int d = 0; d < D; ++d) *reinterpret_cast<uint2*>(dst + d * p.rows * 64) = o[d];
+                const float u1 = __uint_as_float(static_cast<uint32_t>(127 + e - BITS) << 23);
+                if (r == 0) {
+#pragma unroll
+                    for (int d = 0; d < (PACKED ? D : 1); ++d)      // packed: digit d has a column of its own, worth 256^d
+                        unit[q * tcols + d * p.rows + m] = u1 * static_cast<float>(1u << (8 * d));
+                }
+                if ((r & (4 * F - 1)) == 0) {
+                    const uint32_t at = q * (4 / F) + r / (4 * F);
                     float sum = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        o[i] = __byte_perm(__float_as_uint(v[i]), __float_as_uint(v[i + 4]), 0x7632);
-                        const float hx = __uint_as_float(o[i] << 16), hy = __uint_as_float(o[i] & 0xFFFF0000u);
-                        sum += hx + hy;
-                        v[i] -= hx;
-                        v[i + 4] -= hy;
+                    for (int d = D - 1; d >= 0; --d) {
+                        const int lo = static_cast<int16_t>(pair[d / 2] & 0xFFFF);
+                        const int digits = d % 2 ? (pair[d / 2] - lo) >> 16 : (d == 2 && D == 3 ? pair[1] : lo);
+                        base[at * p.cols + d * p.rows + m] = kMagicBits - static_cast<uint32_t>(8 * digits);
+                        if constexpr (PACKED) isum[at * tcols + d * p.rows + m] = static_cast<float>(digits);
+                        sum = fmaf(sum, 256.0f, static_cast<float>(digits));
                     }
-                    if (in) *reinterpret_cast<uint4*>(dst + part * 64) = make_uint4(o[0], o[1], o[2], o[3]);
-#pragma unroll
-                    for (int s = 1; s < 4 * F; s <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, s);
-                    if (in && (r & (4 * F - 1)) == 0) sums[part] = sum;
+                    if constexpr (!PACKED) isum[at * tcols + m] = sum;
                 }
-            } else {
-                uint32_t x[4] = {};
-                if (in) {
-                    if (vec && k + 8 <= g.K) {
-                        const uint4 y = __ldg(reinterpret_cast<const uint4*>(a));
-                        x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
-                    } else {
-                        const uint16_t* b = reinterpret_cast<const uint16_t*>(a);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (k + i < g.K) x[i >> 1] |= static_cast<uint32_t>(b[i]) << (16 * (i & 1));
-                    }
-                }
-                float sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sum += __uint_as_float(x[i] << 16) + __uint_as_float(x[i] & 0xFFFF0000u);
-                if (!(fabsf(sum) <= 3.402823466e38f)) {
-                    // An infinity or NaN among them, or finite values whose sum is none: all go the long way.
-                    atomicOr(odd, 1u << m);
-                    sum = 0.0f;
-                    x[0] = x[1] = x[2] = x[3] = 0u;
-                }
-                if (in)
-                    *reinterpret_cast<uint4*>(dst) = make_uint4(__byte_perm(x[0], x[2], 0x5410), __byte_perm(x[0], x[2], 0x7632),
-                                                                __byte_perm(x[1], x[3], 0x5410), __byte_perm(x[1], x[3], 0x7632));
-#pragma unroll
-                for (int s = 1; s < 4 * F; s <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, s);
-                if (in && (r & (4 * F - 1)) == 0) sums[0] = sum;
             }
             u += kTeams * kTeamThreads / 16;
             m += dm;
@@ -310,8 +329,22 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
         return p.ws + (static_cast<size_t>(blockIdx.z) * gridDim.y + y) * (p.tiles + gridDim.x * kTeams) * (16 * ROWS);
     };
 
-    const unsigned char* act_lane = act + gr * 64 + t4 * 16;
-    const uint32_t act_word = p.cols * 64;
+    // Shared-memory addresses of the lane's operand columns (those that are not there repeat the last)
+    // and of its columns' tables.
+    uint32_t act_at[NT], base_at[NT][2], tab[NB][2];
+    const uint32_t ring_at = smem_u32(ring) + lane * 16, act_step = p.cols * 128;
+#pragma unroll
+    for (int b = 0; b < NT; ++b) {
+        const int col = PACKED ? min(gr, p.cols - 1) : (b % D) * p.rows + min(8 * (b / D) + gr, mt - 1);
+        act_at[b] = smem_u32(act) + col * 64 + t4 * 16;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            base_at[b][e] = PACKED ? min(2 * t4 + e, p.cols - 1) : (b % D) * p.rows + min(8 * (b / D) + 2 * t4 + e, mt - 1);
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) tab[b][e] = min(8 * b + 2 * t4 + e, tcols - 1);
     uint32_t tile = lo / nq, q0 = lo - tile * nq, done = lo;
     uint32_t phase = 0, buffer = 0;
     int slot = 0;
@@ -335,7 +368,7 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
             }
         };
         if (q0 + warp < q1) scales_of(q0 + warp);
-        float tot[NT][4] = {};
+        float tot[NB][4] = {};
         for (uint32_t q = q0 + warp; q < q1; q += kWarps) {
             float sc[2], zr[2];
 #pragma unroll
@@ -344,10 +377,8 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
                 zr[h] = zeros ? value(rawz[h]) : 8.0f;
             }
             if (q + kWarps < q1) scales_of(q + kWarps);
-            if (p.aligned && !mbar_try_wait(bars + slot, phase) && !dead) dead = !mbar_wait(bars + slot, phase, nullptr, p.err);
-            const unsigned char* src = ring + slot * kStepBytes + lane * 16;
-            const uint4 x0 = *reinterpret_cast<const uint4*>(src);
-            const uint4 x1 = *reinterpret_cast<const uint4*>(src + 512);
+            if (!mbar_try_wait(bars + slot, phase) && !dead) dead = !mbar_wait(bars + slot, phase, nullptr, p.err);
+            const uint4 x0 = lds128(ring_at + slot * kStepBytes), x1 = lds128(ring_at + slot * kStepBytes + 512);
             uint32_t w[2][4] = {{x0.x, x0.y, x0.z, x0.w}, {x1.x, x1.y, x1.z, x1.w}};
             __syncwarp();
             request(slot);      // every lane has read it
@@ -375,25 +406,31 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
                         if (t4 & 1) w[h][i] = have; else w[h][i + 1] = have;
                     }
             }
-            const unsigned char* act_q = act_lane + q * 4 * act_word;
+            float un[NB][2];
 #pragma unroll
-            for (int f = 0; f < 4 / F; ++f) {
-                float c[NT][4] = {};
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int i = 0; i < F; ++i) {
-                    const int wi = f * F + i;
-                    const uint32_t a0[4] = {decode<0, PARTS>(w[0][wi]), decode<0, PARTS>(w[1][wi]),
-                                            decode<1, PARTS>(w[0][wi]), decode<1, PARTS>(w[1][wi])};
-                    const uint32_t a1[4] = {decode<2, PARTS>(w[0][wi]), decode<2, PARTS>(w[1][wi]),
-                                            decode<3, PARTS>(w[0][wi]), decode<3, PARTS>(w[1][wi])};
+                for (int e = 0; e < 2; ++e) un[b][e] = unit[q * tcols + tab[b][e]];
+            uint4 x[NT];        // the operand columns of two words
+            uint32_t c[NT][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (i % F == 0) {
 #pragma unroll
                     for (int b = 0; b < NT; ++b) {
-                        uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                        if (8 * b + gr < cols) x = *reinterpret_cast<const uint4*>(act_q + wi * act_word + b * 512);
-                        mma_bf16(c[b], a0, x.x, x.y);
-                        mma_bf16(c[b], a1, x.z, x.w);
+                        c[b][0] = c[b][2] = base[(q * (4 / F) + i / F) * p.cols + base_at[b][0]];
+                        c[b][1] = c[b][3] = base[(q * (4 / F) + i / F) * p.cols + base_at[b][1]];
                     }
                 }
+                const uint32_t av[4] = {w[0][i] & 0x0F0F0F0Fu, w[1][i] & 0x0F0F0F0Fu, (w[0][i] >> 4) & 0x0F0F0F0Fu,
+                                        (w[1][i] >> 4) & 0x0F0F0F0Fu};
+#pragma unroll
+                for (int b = 0; b < NT; ++b) {
+                    if (i % 2 == 0) x[b] = lds128(act_at[b] + (q * 2 + i / 2) * (act_step / 2));
+                    mma_u8s8(c[b], av, i % 2 ? x[b].z : x[b].x, i % 2 ? x[b].w : x[b].y);
+                }
+                if ((i + 1) % F != 0) continue;
+                const int f = i / F;
                 float s0 = sc[0], s1 = sc[1], z0 = zr[0], z1 = zr[1];
                 if constexpr (F < 4) {
                     const int from = (lane & 28) | (f * F);
@@ -404,23 +441,21 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
                         z1 = __shfl_sync(0xFFFFFFFFu, z1, from);
                     }
                 }
-                const float off0 = PARTS ? z0 - 8.0f : z0 + 16.0f, off1 = PARTS ? z1 - 8.0f : z1 + 16.0f;
 #pragma unroll
-                for (int b = 0; b < NT; ++b) {
-                    if (!PARTS || zeros) {
-                        const int col = 8 * b + 2 * t4;
-                        const float* as = asum + (q * (4 / F) + f) * p.cols + col;
-                        const float u0 = col < cols ? as[0] : 0.0f, u1 = col + 1 < cols ? as[1] : 0.0f;
-                        c[b][0] = fmaf(-off0, u0, c[b][0]);
-                        c[b][1] = fmaf(-off0, u1, c[b][1]);
-                        c[b][2] = fmaf(-off1, u0, c[b][2]);
-                        c[b][3] = fmaf(-off1, u1, c[b][3]);
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float y;
+                        if constexpr (PACKED) {
+                            y = __uint_as_float(c[0][e]) - kMagic;
+                        } else {
+                            y = __uint_as_float(c[b * D + D - 1][e]) - kMagic;
+#pragma unroll
+                            for (int d = D - 2; d >= 0; --d) y = fmaf(y, 256.0f, __uint_as_float(c[b * D + d][e]) - kMagic);
+                        }
+                        if (zeros) y = fmaf(8.0f - (e < 2 ? z0 : z1), isum[(q * (4 / F) + f) * tcols + tab[b][e & 1]], y);
+                        tot[b][e] = fmaf((e < 2 ? s0 : s1) * un[b][e & 1], y, tot[b][e]);
                     }
-                    tot[b][0] = fmaf(s0, c[b][0], tot[b][0]);
-                    tot[b][1] = fmaf(s0, c[b][1], tot[b][1]);
-                    tot[b][2] = fmaf(s1, c[b][2], tot[b][2]);
-                    tot[b][3] = fmaf(s1, c[b][3], tot[b][3]);
-                }
             }
         }
 
@@ -429,9 +464,9 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
         float* sums = red + buffer * kWarps * RED;
         buffer ^= 1u;
 #pragma unroll
-        for (int b = 0; b < NT; ++b)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sums[(warp * NT * 4 + b * 4 + e) * 32 + lane] = tot[b][e];
+            for (int e = 0; e < 4; ++e) sums[(warp * NB * 4 + b * 4 + e) * 32 + lane] = tot[b][e];
         sync();
         const bool whole = n == nq && gridDim.y == 1;
         float* part_sums = whole ? nullptr : range_slots(blockIdx.y) + part_slot(shares, share, tile, nq, p.tiles) * (16 * ROWS);
@@ -441,27 +476,19 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
             if (row >= g.N) continue;
             float sum = 0.0f;
 #pragma unroll
-            for (int part = 0; part < (PARTS ? 3 : 1); ++part) {
-                // The smallest parts first.
-                const int col = PARTS ? 3 * m + 2 - part : m, b = col >> 3, e = (col & 1) + 2 * (r >> 3);
+            for (int d = 0; d < (PACKED ? D : 1); ++d) {
+                const int col = d * p.rows + m, b = col >> 3, e = (col & 1) + 2 * (r >> 3);
                 const int ln = (r & 7) * 4 + ((col & 7) >> 1);
 #pragma unroll
-                for (int wv = 0; wv < kWarps; ++wv) sum += sums[(wv * NT * 4 + b * 4 + e) * 32 + ln];
+                for (int wv = 0; wv < kWarps; ++wv) sum += sums[(wv * NB * 4 + b * 4 + e) * 32 + ln];
             }
             if ((*odd >> m) & 1u) {
-                // The activations that stayed out: each stretch of eight that is not finite as a whole.
+                // The activations that stayed out.
                 const T* a = static_cast<const T*>(g.A) + static_cast<int64_t>(m0 + m) * g.lda;
                 const int64_t k1 = static_cast<int64_t>(k_step0 + q1) * kStepK < g.K ? static_cast<int64_t>(k_step0 + q1) * kStepK : g.K;
                 for (int64_t k = static_cast<int64_t>(k_step0 + q0) * kStepK; k < k1; ++k) {
                     const float v = static_cast<float>(a[k]);
-                    bool out = !(fabsf(v) <= 3.402823466e38f);
-                    if (!PARTS) {
-                        float eight[8], s8 = 0.0f;
-                        for (int i = 0; i < 8; ++i) eight[i] = (k & ~7) + i < g.K ? static_cast<float>(a[(k & ~7) + i]) : 0.0f;
-                        for (int i = 0; i < 8; i += 2) s8 += eight[i] + eight[i + 1];
-                        out = !(fabsf(s8) <= 3.402823466e38f);
-                    }
-                    if (!out) continue;
+                    if (fabsf(v) <= 3.402823466e38f) continue;
                     const uint32_t code = (g.W[row * g.ldw + k / 2] >> (4 * (k & 1))) & 15u;
                     const int64_t e = row * g.lds + k / g.group;
                     sum += v * (value(fetch(g.scale, e)) * (static_cast<float>(code) - (zeros ? value(fetch(g.zero, e)) : 8.0f)));
@@ -524,29 +551,47 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     }
 }
 
+// Rows of W at multiples of 16 bytes: a warp copies a row's words of four bytes, each cut from the two
+// aligned words that hold it.
+__global__ void __launch_bounds__(256) repack_rows_kernel(const uint8_t* w, int64_t ldw, int rows, int row_bytes, uint8_t* out,
+                                                          int64_t pitch) {
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    if (n >= rows) return;
+    const uintptr_t row = reinterpret_cast<uintptr_t>(w) + n * ldw, end = row + row_bytes;
+    const uint32_t* from = reinterpret_cast<const uint32_t*>(row & ~uintptr_t(3));
+    const uint32_t shift = static_cast<uint32_t>(row & 3) * 8;
+    for (int i = threadIdx.x & 31; i < (row_bytes + 3) / 4; i += 32) {
+        const uint32_t lo = __ldg(from + i);
+        const uint32_t hi = shift && reinterpret_cast<uintptr_t>(from + i + 1) < end ? __ldg(from + i + 1) : 0u;
+        *reinterpret_cast<uint32_t*>(out + n * pitch + i * 4) = __funnelshift_r(lo, hi, shift);
+    }
+}
+
 struct Kernel {
     const void* fn;
-    int nt, rows, flush;
+    int rows, digits, blocks, flush, packed;
 };
 
-template <DType IO, int NT>
+template <DType IO, int MI>
 Kernel kernel_for_flush(int f) {
-    const int rows = IO == DType::F32 ? NT * 8 / 3 : NT * 8;
-    const void* fn = f == 4 ? reinterpret_cast<const void*>(&gemm_w4_kernel<IO, NT, 4>)
-                     : f == 2 ? reinterpret_cast<const void*>(&gemm_w4_kernel<IO, NT, 2>)
-                              : reinterpret_cast<const void*>(&gemm_w4_kernel<IO, NT, 1>);
-    return {fn, NT, rows, f};
+    constexpr int D = IO == DType::F32 ? 4 : 3;
+    const void* fn = f == 4 ? reinterpret_cast<const void*>(&gemm_w4_kernel<IO, MI, 4>)
+                     : f == 2 ? reinterpret_cast<const void*>(&gemm_w4_kernel<IO, MI, 2>)
+                              : reinterpret_cast<const void*>(&gemm_w4_kernel<IO, MI, 1>);
+    return {fn, MI ? 8 * MI : 8 / D, D, MI ? MI : 1, f, MI == 0};
 }
 
 Kernel select(const W4Args& g) {
     // How many chunks of 32 weights share their scales for sure, up to the four of a step.
     const int f = g.groups == 1 || g.group % 128 == 0 ? 4 : (g.group % 64 == 0 ? 2 : 1);
-    if (g.io == DType::F32)
-        return g.M <= 2 ? kernel_for_flush<DType::F32, 1>(f)
-               : g.M <= 5 ? kernel_for_flush<DType::F32, 2>(f) : kernel_for_flush<DType::F32, 3>(f);
-    return g.M <= 8 ? kernel_for_flush<DType::BF16, 1>(f)
-           : g.M <= 16 ? kernel_for_flush<DType::BF16, 2>(f) : kernel_for_flush<DType::BF16, 4>(f);
+    if (g.io == DType::F32) return g.M <= 2 ? kernel_for_flush<DType::F32, 0>(f) : kernel_for_flush<DType::F32, 1>(f);
+    return g.M <= 2 ? kernel_for_flush<DType::BF16, 0>(f)
+           : g.M <= 8 ? kernel_for_flush<DType::BF16, 1>(f) : kernel_for_flush<DType::BF16, 2>(f);
 }
+
+bool aligned_rows(const W4Args& g) { return g.ldw % 16 == 0 && reinterpret_cast<uintptr_t>(g.W) % 16 == 0; }
+
+int64_t row_bytes_of(const W4Args& g) { return (static_cast<int64_t>(g.K) + 1) / 2; }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -565,13 +610,13 @@ EncodeTiled encode_tiled() {
 }
 
 // W as bytes [N][(K+1)/2], read in boxes of 64 bytes x 16 rows; bytes and rows past the ends read as zeros.
-bool encode_weights(const W4Args& g, CUtensorMap* map) {
+bool encode_weights(const W4Args& g, const uint8_t* w, int64_t pitch, CUtensorMap* map) {
     EncodeTiled fn = encode_tiled();
     if (!fn) return false;
-    const cuuint64_t dims[2] = {static_cast<cuuint64_t>((static_cast<int64_t>(g.K) + 1) / 2), static_cast<cuuint64_t>(g.N)};
-    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(g.ldw)};
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(row_bytes_of(g)), static_cast<cuuint64_t>(g.N)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
     const cuuint32_t box[2] = {64, 16}, one[2] = {1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(g.W), dims, strides, box, one,
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(w), dims, strides, box, one,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -580,14 +625,14 @@ bool encode_weights(const W4Args& g, CUtensorMap* map) {
 
 bool gemm_w4_plan(const W4Args& g, int num_sms, W4Plan* plan) {
     const Kernel k = select(g);
-    const int rows = g.M < k.rows ? g.M : k.rows;
+    plan->rows = g.M < k.rows ? g.M : k.rows;
     const int64_t steps = (static_cast<int64_t>(g.K) + kStepK - 1) / kStepK, tiles = (static_cast<int64_t>(g.N) + 15) / 16;
-    plan->cols = g.io == DType::F32 ? 3 * rows : rows;
-    // As much of K at a time as the activations leave room for beside the smallest rings; the rings
-    // take what is left.
+    plan->cols = k.digits * plan->rows;
+    // As much of K at a time as the digits leave room for beside the smallest rings; the rings take
+    // what is left.
     const int warps = kTeams * kWarps;
-    const int fixed = warps * (2 * k.nt * 512 + kMaxSlots * 8) + 64;
-    const int per_step = plan->cols * (256 + 4 * (4 / k.flush));
+    const int fixed = warps * (2 * k.blocks * 512 + kMaxSlots * 8) + 64;
+    const int per_step = plan->cols * (128 + 4 * (4 / k.flush)) + 4 * (k.packed ? plan->cols : plan->rows) * (1 + 4 / k.flush);
     const int64_t most = (kMaxSmem - fixed - warps * kMinSlots * kStepBytes) / per_step;
     const int64_t splits = (steps + most - 1) / most;
     plan->split_steps = static_cast<int>((steps + splits - 1) / splits);
@@ -595,6 +640,9 @@ bool gemm_w4_plan(const W4Args& g, int num_sms, W4Plan* plan) {
     const int rest = (kMaxSmem - fixed - per_step * plan->split_steps) / (warps * kStepBytes);
     plan->slots = rest < kMaxSlots ? rest : kMaxSlots;
     plan->smem = fixed + per_step * plan->split_steps + warps * plan->slots * kStepBytes;
+    plan->bars_at = (plan->smem - warps * kMaxSlots * 8 - 16) & ~7;
+    plan->pitch = aligned_rows(g) ? 0 : (row_bytes_of(g) + 15) / 16 * 16;
+    plan->copy_bytes = static_cast<size_t>(plan->pitch) * g.N;
     plan->blocks = (g.M + k.rows - 1) / k.rows;
     // Every SM a CTA, shared among the K-ranges; no more than there are shares of eight steps.
     int64_t ctas = (num_sms + plan->splits - 1) / plan->splits;
@@ -608,8 +656,8 @@ bool gemm_w4_plan(const W4Args& g, int num_sms, W4Plan* plan) {
     return true;
 }
 
-cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint32_t* tickets, uint32_t* err,
-                           cudaStream_t s) {
+cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint32_t* tickets, void* copy,
+                           uint32_t* err, cudaStream_t s) {
     const Kernel k = select(g);
     static std::mutex mu;
     static std::unordered_set<const void*> known[64];
@@ -632,6 +680,8 @@ cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint3
     p.split_steps = plan.split_steps;
     p.slots = plan.slots;
     p.cols = plan.cols;
+    p.rows = plan.rows;
+    p.bars_at = plan.bars_at;
     // chunk / (group / 32) for chunks below 2^31: mul = ceil(2^(31 + ceil(log2 d)) / d).
     const int64_t d = g.groups > 1 ? g.group / 32 : int64_t(1) << 30;
     int log = 0;
@@ -641,8 +691,17 @@ cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint3
     p.ws = ws;
     p.tickets = tickets;
     p.err = err;
-    CUtensorMap map = {};
-    p.aligned = g.ldw % 16 == 0 && reinterpret_cast<uintptr_t>(g.W) % 16 == 0 && encode_weights(g, &map);
+    const uint8_t* w = g.W;
+    int64_t pitch = g.ldw;
+    if (plan.pitch) {
+        w = static_cast<const uint8_t*>(copy);
+        pitch = plan.pitch;
+        repack_rows_kernel<<<(static_cast<unsigned>(g.N) + 7) / 8, 256, 0, s>>>(g.W, g.ldw, g.N, static_cast<int>(row_bytes_of(g)),
+                                                                              static_cast<uint8_t*>(copy), pitch);
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    }
+    CUtensorMap map;
+    if (!encode_weights(g, w, pitch, &map)) return cudaErrorNotSupported;
     void* args[] = {&p, &map};
     return cudaLaunchKernel(k.fn, dim3(plan.ctas, plan.splits, plan.blocks), dim3(kTeams * kTeamThreads), args,
                             static_cast<size_t>(plan.smem), s);
