@@ -23,10 +23,10 @@
 // Activations that are infinite or NaN stay out of the products and are added
 // for their own row at the end.
 //
-// Work.  128 weights of 16 rows (1 KB) are a step, one TMA box into the ring of the
+// Work.  256 weights of 16 rows (2 KB) are a step, two TMA boxes into the ring of the
 // warp that works on it (16-byte cp.async of the same rows cost 23 shared-memory
 // cycles an instruction and held the kernel at 1.6 TB/s).  All steps, tile after
-// tile of 16 rows, are cut into equal shares, one for each team of eight warps, two
+// tile of 16 rows, are cut into equal shares, one for each team of four warps, four
 // teams to an SM; a team's warps take the steps of a tile in turn and add up
 // in shared memory.  A tile cut by a share's end, or by the ends of a K-range, is
 // finished by the last of its shares to arrive, adding the parts in order.  The
@@ -45,25 +45,27 @@
 namespace dnnopt_b200 {
 namespace {
 
-constexpr int kTeams = 2;           // per CTA
-constexpr int kTeamThreads = 256;
-constexpr int kWarps = 8;           // per team
-constexpr int kMaxSlots = 8;        // steps under way per warp, where the activations leave room
-constexpr int kMinSlots = 4;
-constexpr int kStepK = 128;
-constexpr int kStepBytes = 1024;
+constexpr int kTeams = 4;           // per CTA
+constexpr int kTeamThreads = 128;
+constexpr int kWarps = 4;           // per team
+constexpr int kMaxSlots = 4;        // steps under way per warp, where the activations leave room
+constexpr int kMinSlots = 2;
+constexpr int kStepK = 256;
+constexpr int kStepBytes = 2048;
+constexpr int kBoxBytes = 1024;     // 128 weights of 16 rows
 constexpr int kMaxSmem = 227 * 1024;
 
 struct Params {
     W4Args g;
     int tiles;                      // of 16 rows of W
-    int steps;                      // ceil(K / 128)
+    int steps;                      // ceil(K / 256)
     int split_steps;                // steps of one K-range (gridDim.y of them)
     int slots;                      // of a warp's ring
     int rows, cols;                 // rows of A at a time, and columns: a digit of each
     int bars_at;                    // of the barriers, in shared memory
     uint32_t gmul, gshift;          // chunk of 32 weights -> group
-    float* ws;                      // partial tiles, see part_slot
+    float* ws;                      // partial tiles of a K-range: the part with a tile's first step by
+                                    // tile, then the parts that begin a share by share
     uint32_t* tickets;              // one per tile and block of rows of A
     uint32_t* err;                  // receives kKerrMbarTimeout
 };
@@ -81,7 +83,7 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
 constexpr float kMagic = 12582912.0f;           // 1.5 * 2^23: whole numbers below 2^22 added to it keep their bits
 constexpr uint32_t kMagicBits = 0x4B400000u;
 
-// Equal shares of `total` steps, at least eight (one for each warp of a team).
+// Equal shares of `total` steps, at least one for each warp of a team.
 struct Shares {
     uint32_t total, n;
 
@@ -98,7 +100,7 @@ struct Shares {
     }
 };
 
-// One warp's steps of a share: every eighth of each tile's.
+// One warp's steps of a share: every fourth of each tile's.
 struct Cursor {
     uint32_t tile, q, end, left;    // step q of [.., end) of the tile; steps of the share after it
 
@@ -120,12 +122,6 @@ struct Cursor {
         }
     }
 };
-
-// Slot of a partial tile within its K-range: the part with the tile's first
-// step goes by the tile, a later part begins its share and goes by the share.
-__device__ __forceinline__ size_t part_slot(const Shares& s, uint32_t share, uint32_t tile, uint32_t per_tile, int tiles) {
-    return s.start(share) <= tile * per_tile ? tile : tiles + share;
-}
 
 // D digits of an activation: three of bf16, four of FP32.  MI = 0: the digits of
 // up to 8 / D rows of A share one block of eight columns; else MI blocks of
@@ -152,11 +148,11 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     const uint32_t per = static_cast<uint32_t>(p.split_steps);
 
     unsigned char* ring = smem + (team * kWarps + warp) * p.slots * kStepBytes;
-    unsigned char* act = smem + kTeams * kWarps * p.slots * kStepBytes;                      // [step][2][col][t] 16 bytes
-    float* unit = reinterpret_cast<float*>(act + static_cast<size_t>(per) * p.cols * 128);   // [step][tcol]
-    uint32_t* base = reinterpret_cast<uint32_t*>(unit + per * tcols);                        // [step][flush][col]
-    float* isum = reinterpret_cast<float*>(base + per * (4 / F) * p.cols);                   // [step][flush][tcol]
-    float* red = isum + per * (4 / F) * tcols + team * 2 * kWarps * RED;                     // [2][warp][4 NB][lane]
+    unsigned char* act = smem + kTeams * kWarps * p.slots * kStepBytes;                      // [128][2][col][t] 16 bytes
+    float* unit = reinterpret_cast<float*>(act + static_cast<size_t>(per) * p.cols * 256);   // [128][tcol]
+    uint32_t* base = reinterpret_cast<uint32_t*>(unit + per * 2 * tcols);                    // [128][flush][col]
+    float* isum = reinterpret_cast<float*>(base + per * 2 * (4 / F) * p.cols);               // [128][flush][tcol]
+    float* red = isum + per * 2 * (4 / F) * tcols + team * 2 * kWarps * RED;                     // [2][warp][4 NB][lane]
     uint64_t* bars = reinterpret_cast<uint64_t*>(
         smem + p.bars_at);
     uint32_t* odd = reinterpret_cast<uint32_t*>(bars + kTeams * kWarps * kMaxSlots);    // rows of A with an infinity or NaN
@@ -179,9 +175,11 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     auto request = [&](int slot) {      // the warp's next step, into a slot that it is done with
         if (prod.q < prod.end) {
             if (lane == 0) {
+                const int x = static_cast<int>((k_step0 + prod.q) * (kStepK / 2)), y = static_cast<int>(prod.tile * 16);
+                unsigned char* dst = ring + slot * kStepBytes;
                 mbar_arrive_expect_tx(bars + slot, kStepBytes);
-                tma_load_2d(ring + slot * kStepBytes, &map, bars + slot, static_cast<int>((k_step0 + prod.q) * 64),
-                            static_cast<int>(prod.tile * 16));
+                tma_load_2d(dst, &map, bars + slot, x, y);
+                tma_load_2d(dst + kBoxBytes, &map, bars + slot, x + 64, y);
             }
             prod.q += kWarps;
             if (prod.q >= prod.end) prod.settle(nq, warp);
@@ -195,15 +193,15 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     __syncthreads();
     {
         const bool vec = g.lda % (16 / sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(g.A) % 16 == 0;
-        const uint32_t units = mt * nq, r = tid & 15;
+        const uint32_t nh = nq * 2, units = mt * nh, r = tid & 15;
         // Which word of which lane these eight weights are, after the exchanges below.
         const uint32_t w = F == 4 ? (r & 3) : (F == 1 ? (r >> 2) : ((r >> 3) * 2 + (r & 1)));
         const uint32_t t = F == 4 ? (r >> 2) : (F == 1 ? (r & 3) : (((r >> 2) & 1) + (r & 2)));
-        uint32_t u = tid >> 4, m = u / nq, q = u - m * nq;
-        const uint32_t dm = (kTeams * kTeamThreads / 16) / nq, dq = (kTeams * kTeamThreads / 16) - dm * nq;
+        uint32_t u = tid >> 4, m = u / nh, q = u - m * nh;       // q: stretch of 128
+        const uint32_t dm = (kTeams * kTeamThreads / 16) / nh, dq = (kTeams * kTeamThreads / 16) - dm * nh;
         for (uint32_t u0 = u & ~1u; u0 < units; u0 += kTeams * kTeamThreads / 16) {     // the same count for a whole warp
             const bool in = u < units;
-            const int64_t k = static_cast<int64_t>(k_step0 + q) * kStepK + r * 8;
+            const int64_t k = static_cast<int64_t>(k_step0) * kStepK + q * 128 + r * 8;
             const T* a = static_cast<const T*>(g.A) + static_cast<int64_t>(m0 + m) * g.lda + k;
             float v[8] = {};
             if (in) {
@@ -307,7 +305,7 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
             u += kTeams * kTeamThreads / 16;
             m += dm;
             q += dq;
-            if (q >= nq) { q -= nq; ++m; }
+            if (q >= nh) { q -= nh; ++m; }
         }
     }
     __syncthreads();
@@ -332,7 +330,7 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     // Shared-memory addresses of the lane's operand columns (those that are not there repeat the last)
     // and of its columns' tables.
     uint32_t act_at[NT], base_at[NT][2], tab[NB][2];
-    const uint32_t ring_at = smem_u32(ring) + lane * 16, act_step = p.cols * 128;
+    const uint32_t ring_at = smem_u32(ring) + lane * 16, act_half = p.cols * 64;
 #pragma unroll
     for (int b = 0; b < NT; ++b) {
         const int col = PACKED ? min(gr, p.cols - 1) : (b % D) * p.rows + min(8 * (b / D) + gr, mt - 1);
@@ -345,117 +343,144 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int e = 0; e < 2; ++e) tab[b][e] = min(8 * b + 2 * t4 + e, tcols - 1);
+    // Scales are read one step ahead of their products, across the ends of tiles.
+    Cursor ahead(lo, hi, nq, warp);
+    int64_t srow[2];        // the lane's two rows' first scales
+    uint32_t raw[2][2] = {}, rawz[2][2] = {};       // [half][row]
+    auto open = [&](uint32_t t) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t row = static_cast<int64_t>(t) * 16 + gr + 8 * h;
+            srow[h] = (row < g.N ? row : g.N - 1) * g.lds;
+        }
+    };
+    auto fetch_scales = [&]() {
+        if (ahead.q >= ahead.end) return;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int gi = group_of((k_step0 + ahead.q) * 8 + half * 4 + t4);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                raw[half][h] = fetch(g.scale, srow[h] + gi);
+                if (zeros) rawz[half][h] = fetch(g.zero, srow[h] + gi);
+            }
+        }
+        ahead.q += kWarps;
+        if (ahead.q >= ahead.end && ahead.left > 0) {
+            ahead.settle(nq, warp);
+            open(ahead.tile);
+        }
+    };
+    open(ahead.tile);
+    fetch_scales();
+
     uint32_t tile = lo / nq, q0 = lo - tile * nq, done = lo;
     uint32_t phase = 0, buffer = 0;
     int slot = 0;
     bool dead = false;
     while (done < hi) {
         const uint32_t n = hi - done < nq - q0 ? hi - done : nq - q0, q1 = q0 + n;
-        int64_t srow[2];        // the lane's two rows' first scales
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int64_t row = static_cast<int64_t>(tile) * 16 + gr + 8 * h;
-            srow[h] = (row < g.N ? row : g.N - 1) * g.lds;
-        }
-        // A step's scales are read one step ahead; here the tile's come into L2.
-        uint32_t raw[2] = {0, 0}, rawz[2] = {0, 0};
-        auto scales_of = [&](uint32_t q) {
-            const int gi = group_of((k_step0 + q) * 4 + t4);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                raw[h] = fetch(g.scale, srow[h] + gi);
-                if (zeros) rawz[h] = fetch(g.zero, srow[h] + gi);
-            }
-        };
-        if (q0 + warp < q1) scales_of(q0 + warp);
         float tot[NB][4] = {};
         for (uint32_t q = q0 + warp; q < q1; q += kWarps) {
-            float sc[2], zr[2];
+            float sc[2][2], zr[2][2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                sc[h] = value(raw[h]);
-                zr[h] = zeros ? value(rawz[h]) : 8.0f;
-            }
-            if (q + kWarps < q1) scales_of(q + kWarps);
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    sc[half][h] = value(raw[half][h]);
+                    zr[half][h] = 8.0f - (zeros ? value(rawz[half][h]) : 8.0f);
+                }
+            fetch_scales();
             if (!mbar_try_wait(bars + slot, phase) && !dead) dead = !mbar_wait(bars + slot, phase, nullptr, p.err);
-            const uint4 x0 = lds128(ring_at + slot * kStepBytes), x1 = lds128(ring_at + slot * kStepBytes + 512);
-            uint32_t w[2][4] = {{x0.x, x0.y, x0.z, x0.w}, {x1.x, x1.y, x1.z, x1.w}};
+            uint32_t w[2][2][4];        // [half][row][word]
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint4 v = lds128(ring_at + slot * kStepBytes + half * kBoxBytes + h * 512);
+                    w[half][h][0] = v.x; w[half][h][1] = v.y; w[half][h][2] = v.z; w[half][h][3] = v.w;
+                }
             __syncwarp();
             request(slot);      // every lane has read it
             if (++slot == p.slots) { slot = 0; phase ^= 1u; }
 
-            // A product takes a word from each lane of a quad.  Lane t holds the four words of chunk t:
-            // scales shared by fewer chunks want the words of one chunk (or two) on all four lanes.
-            if constexpr (F <= 2) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t qh = q * 2 + half;
+                uint32_t (&wh)[2][4] = w[half];
+                // A product takes a word from each lane of a quad.  Lane t holds the four words of chunk t:
+                // scales shared by fewer chunks want the words of one chunk (or two) on all four lanes.
+                if constexpr (F <= 2) {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {       // words 2, 3 of lanes 0, 1 for words 0, 1 of lanes 2, 3
-                        const uint32_t give = (t4 & 2) ? w[h][i] : w[h][i + 2];
-                        const uint32_t have = __shfl_xor_sync(0xFFFFFFFFu, give, 2);
-                        if (t4 & 2) w[h][i] = have; else w[h][i + 2] = have;
-                    }
-            }
-            if constexpr (F == 1) {
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < 4; i += 2) {    // odd words of even lanes for even words of odd lanes
-                        const uint32_t give = (t4 & 1) ? w[h][i] : w[h][i + 1];
-                        const uint32_t have = __shfl_xor_sync(0xFFFFFFFFu, give, 1);
-                        if (t4 & 1) w[h][i] = have; else w[h][i + 1] = have;
-                    }
-            }
-            float un[NB][2];
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) un[b][e] = unit[q * tcols + tab[b][e]];
-            uint4 x[NT];        // the operand columns of two words
-            uint32_t c[NT][4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (i % F == 0) {
-#pragma unroll
-                    for (int b = 0; b < NT; ++b) {
-                        c[b][0] = c[b][2] = base[(q * (4 / F) + i / F) * p.cols + base_at[b][0]];
-                        c[b][1] = c[b][3] = base[(q * (4 / F) + i / F) * p.cols + base_at[b][1]];
-                    }
+                        for (int i = 0; i < 2; ++i) {       // words 2, 3 of lanes 0, 1 for words 0, 1 of lanes 2, 3
+                            const uint32_t give = (t4 & 2) ? wh[h][i] : wh[h][i + 2];
+                            const uint32_t have = __shfl_xor_sync(0xFFFFFFFFu, give, 2);
+                            if (t4 & 2) wh[h][i] = have; else wh[h][i + 2] = have;
+                        }
                 }
-                const uint32_t av[4] = {w[0][i] & 0x0F0F0F0Fu, w[1][i] & 0x0F0F0F0Fu, (w[0][i] >> 4) & 0x0F0F0F0Fu,
-                                        (w[1][i] >> 4) & 0x0F0F0F0Fu};
+                if constexpr (F == 1) {
 #pragma unroll
-                for (int b = 0; b < NT; ++b) {
-                    if (i % 2 == 0) x[b] = lds128(act_at[b] + (q * 2 + i / 2) * (act_step / 2));
-                    mma_u8s8(c[b], av, i % 2 ? x[b].z : x[b].x, i % 2 ? x[b].w : x[b].y);
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 4; i += 2) {    // odd words of even lanes for even words of odd lanes
+                            const uint32_t give = (t4 & 1) ? wh[h][i] : wh[h][i + 1];
+                            const uint32_t have = __shfl_xor_sync(0xFFFFFFFFu, give, 1);
+                            if (t4 & 1) wh[h][i] = have; else wh[h][i + 1] = have;
+                        }
                 }
-                if ((i + 1) % F != 0) continue;
-                const int f = i / F;
-                float s0 = sc[0], s1 = sc[1], z0 = zr[0], z1 = zr[1];
-                if constexpr (F < 4) {
-                    const int from = (lane & 28) | (f * F);
-                    s0 = __shfl_sync(0xFFFFFFFFu, s0, from);
-                    s1 = __shfl_sync(0xFFFFFFFFu, s1, from);
-                    if (zeros) {
-                        z0 = __shfl_sync(0xFFFFFFFFu, z0, from);
-                        z1 = __shfl_sync(0xFFFFFFFFu, z1, from);
-                    }
-                }
+                float un[NB][2];
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float y;
-                        if constexpr (PACKED) {
-                            y = __uint_as_float(c[0][e]) - kMagic;
-                        } else {
-                            y = __uint_as_float(c[b * D + D - 1][e]) - kMagic;
+                    for (int e = 0; e < 2; ++e) un[b][e] = unit[qh * tcols + tab[b][e]];
+                uint4 x[NT];        // the operand columns of two words
+                uint32_t c[NT][4];
 #pragma unroll
-                            for (int d = D - 2; d >= 0; --d) y = fmaf(y, 256.0f, __uint_as_float(c[b * D + d][e]) - kMagic);
+                for (int i = 0; i < 4; ++i) {
+                    if (i % F == 0) {
+#pragma unroll
+                        for (int b = 0; b < NT; ++b) {
+                            c[b][0] = c[b][2] = base[(qh * (4 / F) + i / F) * p.cols + base_at[b][0]];
+                            c[b][1] = c[b][3] = base[(qh * (4 / F) + i / F) * p.cols + base_at[b][1]];
                         }
-                        if (zeros) y = fmaf(8.0f - (e < 2 ? z0 : z1), isum[(q * (4 / F) + f) * tcols + tab[b][e & 1]], y);
-                        tot[b][e] = fmaf((e < 2 ? s0 : s1) * un[b][e & 1], y, tot[b][e]);
                     }
+                    const uint32_t av[4] = {wh[0][i] & 0x0F0F0F0Fu, wh[1][i] & 0x0F0F0F0Fu, (wh[0][i] >> 4) & 0x0F0F0F0Fu,
+                                            (wh[1][i] >> 4) & 0x0F0F0F0Fu};
+#pragma unroll
+                    for (int b = 0; b < NT; ++b) {
+                        if (i % 2 == 0) x[b] = lds128(act_at[b] + (qh * 2 + i / 2) * act_half);
+                        mma_u8s8(c[b], av, i % 2 ? x[b].z : x[b].x, i % 2 ? x[b].w : x[b].y);
+                    }
+                    if ((i + 1) % F != 0) continue;
+                    const int f = i / F;
+                    float s0 = sc[half][0], s1 = sc[half][1], z0 = zr[half][0], z1 = zr[half][1];
+                    if constexpr (F < 4) {
+                        const int from = (lane & 28) | (f * F);
+                        s0 = __shfl_sync(0xFFFFFFFFu, s0, from);
+                        s1 = __shfl_sync(0xFFFFFFFFu, s1, from);
+                        if (zeros) {
+                            z0 = __shfl_sync(0xFFFFFFFFu, z0, from);
+                            z1 = __shfl_sync(0xFFFFFFFFu, z1, from);
+                        }
+                    }
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float y;
+                            if constexpr (PACKED) {
+                                y = __uint_as_float(c[0][e]) - kMagic;
+                            } else {
+                                y = __uint_as_float(c[b * D + D - 1][e]) - kMagic;
+#pragma unroll
+                                for (int d = D - 2; d >= 0; --d) y = fmaf(y, 256.0f, __uint_as_float(c[b * D + d][e]) - kMagic);
+                            }
+                            if (zeros) y = fmaf(e < 2 ? z0 : z1, isum[(qh * (4 / F) + f) * tcols + tab[b][e & 1]], y);
+                            tot[b][e] = fmaf((e < 2 ? s0 : s1) * un[b][e & 1], y, tot[b][e]);
+                        }
+                }
             }
         }
 
@@ -469,7 +494,7 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
             for (int e = 0; e < 4; ++e) sums[(warp * NB * 4 + b * 4 + e) * 32 + lane] = tot[b][e];
         sync();
         const bool whole = n == nq && gridDim.y == 1;
-        float* part_sums = whole ? nullptr : range_slots(blockIdx.y) + part_slot(shares, share, tile, nq, p.tiles) * (16 * ROWS);
+        float* part_sums = whole ? nullptr : range_slots(blockIdx.y) + static_cast<size_t>(lo <= tile * nq ? tile : p.tiles + share) * (16 * ROWS);
         for (int idx = tt; idx < 16 * mt; idx += kTeamThreads) {
             const int r = idx & 15, m = idx >> 4;
             const int64_t row = static_cast<int64_t>(tile) * 16 + r;
@@ -632,7 +657,7 @@ bool gemm_w4_plan(const W4Args& g, int num_sms, W4Plan* plan) {
     // what is left.
     const int warps = kTeams * kWarps;
     const int fixed = warps * (2 * k.blocks * 512 + kMaxSlots * 8) + 64;
-    const int per_step = plan->cols * (128 + 4 * (4 / k.flush)) + 4 * (k.packed ? plan->cols : plan->rows) * (1 + 4 / k.flush);
+    const int per_step = 2 * (plan->cols * (128 + 4 * (4 / k.flush)) + 4 * (k.packed ? plan->cols : plan->rows) * (1 + 4 / k.flush));
     const int64_t most = (kMaxSmem - fixed - warps * kMinSlots * kStepBytes) / per_step;
     const int64_t splits = (steps + most - 1) / most;
     plan->split_steps = static_cast<int>((steps + splits - 1) / splits);
