@@ -63,11 +63,11 @@ int dnnopt_cuda_gemm_w4(const dnnopt_w4_desc* d, const void* A, const uint8_t* W
     if (!gemm_w4_plan(g, ctx->num_sms, &plan)) return set_status(DNNOPT_STATUS_NOT_SUPPORTED);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     Workspace* w = nullptr;
-    st = ensure_workspace(ctx, s, plan.ws_floats, plan.tickets, plan.copy_bytes, &w);
+    st = ensure_workspace(ctx, s, plan.ws_floats, plan.tickets, plan.extra_bytes, &w);
     if (st != DNNOPT_STATUS_SUCCESS) return st;
     if ((st = inject_launch()) != DNNOPT_STATUS_SUCCESS) return st;
     cudaError_t e = launch_gemm_w4(g, plan, w->ws, w->counters, w->quant, w->err, s);
-    note_launch(plan.pitch ? 2 : 1);
+    note_launch(1 + (plan.pitch ? 1 : 0) + (plan.prepared ? 1 : 0));
     return cuda_status(e);
 }
 

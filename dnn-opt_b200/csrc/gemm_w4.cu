@@ -63,6 +63,8 @@ struct Params {
     int slots;                      // of a warp's ring
     int rows, cols;                 // rows of A at a time, and columns: a digit of each
     int bars_at;                    // of the barriers, in shared memory
+    uint32_t image_bytes;           // of a K-range's activations
+    unsigned char* images;          // made by the kernel before; nullptr: each CTA makes its own
     uint32_t gmul, gshift;          // chunk of 32 weights -> group
     float* ws;                      // partial tiles of a K-range: the part with a tile's first step by
                                     // tile, then the parts that begin a share by share
@@ -83,20 +85,22 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
 constexpr float kMagic = 12582912.0f;           // 1.5 * 2^23: whole numbers below 2^22 added to it keep their bits
 constexpr uint32_t kMagicBits = 0x4B400000u;
 
-// Equal shares of `total` steps, at least one for each warp of a team.
+// Equal shares of `total` steps but for one step, at least one step for each
+// warp of a team: the first `more` shares have one more than the others.
 struct Shares {
-    uint32_t total, n;
+    uint32_t n, each, more;
 
-    __device__ Shares(uint32_t steps, uint32_t most) : total(steps), n(steps / kWarps) {
+    __device__ Shares(uint32_t steps, uint32_t most) : n(steps / kWarps) {
         if (n > most) n = most;
         if (n < 1) n = 1;
+        each = steps / n;
+        more = steps - each * n;
     }
-    __device__ __forceinline__ uint32_t start(uint32_t s) const {
-        return static_cast<uint32_t>(static_cast<uint64_t>(s) * total / n);
-    }
+    __device__ __forceinline__ uint32_t start(uint32_t s) const { return s * each + min(s, more); }
     // The share that holds step t: the last one that starts at or before it.
     __device__ __forceinline__ uint32_t holder(uint32_t t) const {
-        return static_cast<uint32_t>((static_cast<uint64_t>(t + 1) * n - 1) / total);
+        const uint32_t big = more * (each + 1);
+        return t < big ? t / (each + 1) : more + (t - big) / each;
     }
 };
 
@@ -123,6 +127,155 @@ struct Cursor {
     }
 };
 
+// The activations of a K-range as the products read them.
+struct Image {
+    unsigned char* act;     // [128][2][col][t] 16 bytes: the digits of two words' activations
+    float* unit;            // [128][tcol]: what 1 stands for; negative where an infinity or NaN was left out
+    uint32_t* base;         // [128][flush][col]: -8 times the sum of the digits, as the bits of an FP32 number
+    float* isum;            // [128][flush][tcol]: the sum of the whole numbers (packed: of the digits)
+
+    __device__ Image(unsigned char* at, uint32_t steps, int cols, int tcols, int f) : act(at) {
+        unit = reinterpret_cast<float*>(act + static_cast<size_t>(steps) * cols * 256);
+        base = reinterpret_cast<uint32_t*>(unit + steps * 2 * tcols);
+        isum = reinterpret_cast<float*>(base + steps * 2 * (4 / f) * cols);
+    }
+};
+
+// 128 activations of row m0 + m, eight (a word's worth) to each lane of half a
+// warp: r is the lane's place, q the stretch within the K-range, `in` false for
+// a half that has nothing to do.  The whole warp takes part.
+template <DType IO, int MI, int F>
+__device__ __forceinline__ void stage(const Params& p, const Image& img, int m0, int k_step0, uint32_t m, uint32_t q, uint32_t r,
+                                      bool vec, bool in) {
+    using T = typename std::conditional<IO == DType::F32, float, __nv_bfloat16>::type;
+    constexpr bool PARTS = IO == DType::F32, PACKED = MI == 0;
+    constexpr int D = PARTS ? 4 : 3, BITS = PARTS ? 30 : 22;
+    const W4Args& g = p.g;
+    const int tcols = PACKED ? p.cols : p.rows;
+    // Which word of which lane these eight weights are, after the exchanges of the product's loop.
+    const uint32_t w = F == 4 ? (r & 3) : (F == 1 ? (r >> 2) : ((r >> 3) * 2 + (r & 1)));
+    const uint32_t t = F == 4 ? (r >> 2) : (F == 1 ? (r & 3) : (((r >> 2) & 1) + (r & 2)));
+    const int64_t k = static_cast<int64_t>(k_step0) * kStepK + q * 128 + r * 8;
+    const T* a = static_cast<const T*>(g.A) + static_cast<int64_t>(m0 + m) * g.lda + k;
+    float v[8] = {};
+    if (in) {
+        if (vec && k + 8 <= g.K) {
+            if constexpr (PARTS) {
+                const float4 x = __ldg(reinterpret_cast<const float4*>(a)), y = __ldg(reinterpret_cast<const float4*>(a) + 1);
+                v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+                v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+            } else {
+                const uint4 y = __ldg(reinterpret_cast<const uint4*>(a));
+                const uint32_t x[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[2 * i] = __uint_as_float(x[i] << 16);
+                    v[2 * i + 1] = __uint_as_float(x[i] & 0xFFFF0000u);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = k + i < g.K ? static_cast<float>(a[i]) : 0.0f;
+        }
+    }
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+    bool bad = top > 3.402823466e38f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bad = bad || v[i] != v[i];
+    if (bad) {
+        top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (!(fabsf(v[i]) <= 3.402823466e38f)) v[i] = 0.0f;
+            top = fmaxf(top, fabsf(v[i]));
+        }
+    }
+    const bool odd = (__ballot_sync(0xFFFFFFFFu, bad) >> (threadIdx.x & 16)) & 0xFFFFu;
+#pragma unroll
+    for (int s = 1; s < 16; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s));
+    // 2^e is above every |v|; the unit 2^(e - BITS) stays a normal number.
+    int e = static_cast<int>(__float_as_uint(top) >> 23) - 126;
+    e = max(e, BITS - 126);
+    const float scale = __uint_as_float(static_cast<uint32_t>(127 + BITS - e) << 23);
+    uint32_t x[8];
+    if constexpr (PARTS) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = static_cast<uint32_t>(__float2int_rn(v[i] * scale)) + 0x80808080u;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)     // every digit plus 128
+            x[i] = __float_as_uint(fmaf(v[i], scale, kMagic)) - kMagicBits + 0x00808080u;
+    }
+    // Even k are the low nibbles, the first operand register; odd k the second.
+    uint2 o[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t p0 = __byte_perm(x[h], x[h + 2], 0x5140), p1 = __byte_perm(x[h + 4], x[h + 6], 0x5140);
+        const uint32_t p2 = __byte_perm(x[h], x[h + 2], 0x7362), p3 = __byte_perm(x[h + 4], x[h + 6], 0x7362);
+        const uint32_t d0 = __byte_perm(p0, p1, 0x5410) ^ 0x80808080u, d1 = __byte_perm(p0, p1, 0x7632) ^ 0x80808080u;
+        const uint32_t d2 = __byte_perm(p2, p3, 0x5410) ^ 0x80808080u, d3 = __byte_perm(p2, p3, 0x7632) ^ 0x80808080u;
+        (h ? o[0].y : o[0].x) = d0;
+        (h ? o[1].y : o[1].x) = d1;
+        (h ? o[2].y : o[2].x) = d2;
+        (h ? o[3].y : o[3].x) = d3;
+    }
+    // Sums of the digits, two to a word: each stays within 16 bits.
+    int pair[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int lo = __dp4a(static_cast<int>(o[2 * h].x), 0x01010101, __dp4a(static_cast<int>(o[2 * h].y), 0x01010101, 0));
+        const int up = __dp4a(static_cast<int>(o[2 * h + 1].x), 0x01010101, __dp4a(static_cast<int>(o[2 * h + 1].y), 0x01010101, 0));
+        pair[h] = lo + up * 65536;
+        if (2 * h + 1 >= D) pair[h] = lo;
+#pragma unroll
+        for (int s = 1; s < 4 * F; s <<= 1) pair[h] += __shfl_xor_sync(0xFFFFFFFFu, pair[h], s);
+    }
+    if (in) {
+        unsigned char* dst = img.act + ((q * 2 + (w >> 1)) * p.cols + m) * 64 + t * 16 + (w & 1) * 8;
+#pragma unroll
+        for (int d = 0; d < D; ++d) *reinterpret_cast<uint2*>(dst + d * p.rows * 64) = o[d];
+        const float u1 = __uint_as_float((static_cast<uint32_t>(127 + e - BITS) << 23) | (odd ? 0x80000000u : 0u));
+        if (r == 0) {
+#pragma unroll
+            for (int d = 0; d < (PACKED ? D : 1); ++d)      // packed: digit d has a column of its own, worth 256^d
+                img.unit[q * tcols + d * p.rows + m] = u1 * static_cast<float>(1u << (8 * d));
+        }
+        if ((r & (4 * F - 1)) == 0) {
+            const uint32_t at = q * (4 / F) + r / (4 * F);
+            float sum = 0.0f;
+#pragma unroll
+            for (int d = D - 1; d >= 0; --d) {
+                const int lo = static_cast<int16_t>(pair[d / 2] & 0xFFFF);
+                const int digits = d % 2 ? (pair[d / 2] - lo) >> 16 : (d == 2 && D == 3 ? pair[1] : lo);
+                img.base[at * p.cols + d * p.rows + m] = kMagicBits - static_cast<uint32_t>(8 * digits);
+                if constexpr (PACKED) img.isum[at * tcols + d * p.rows + m] = static_cast<float>(digits);
+                sum = fmaf(sum, 256.0f, static_cast<float>(digits));
+            }
+            if constexpr (!PACKED) img.isum[at * tcols + m] = sum;
+        }
+    }
+}
+
+// Images of all K-ranges and blocks of rows, where making them in every CTA
+// takes longer than reading them back: a half-warp per 128 activations.
+template <DType IO, int MI, int F>
+__global__ void __launch_bounds__(128) gemm_w4_digits_kernel(const Params p) {
+    pdl_launch_dependents();
+    using T = typename std::conditional<IO == DType::F32, float, __nv_bfloat16>::type;
+    constexpr int D = IO == DType::F32 ? 4 : 3, ROWS = MI == 0 ? 8 / D : 8 * MI;
+    const W4Args& g = p.g;
+    const int m0 = blockIdx.z * ROWS, mt = g.M - m0 < ROWS ? g.M - m0 : ROWS;
+    const int k_step0 = blockIdx.y * p.split_steps;
+    const uint32_t nq = p.steps - k_step0 < p.split_steps ? p.steps - k_step0 : p.split_steps;
+    const Image img(p.images + (static_cast<size_t>(blockIdx.z) * gridDim.y + blockIdx.y) * p.image_bytes, p.split_steps, p.cols,
+                    MI == 0 ? p.cols : p.rows, F);
+    const bool vec = g.lda % (16 / sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(g.A) % 16 == 0;
+    const uint32_t u = blockIdx.x * 8 + (threadIdx.x >> 4), m = u / (nq * 2), q = u - m * nq * 2;
+    stage<IO, MI, F>(p, img, m0, k_step0, m, q, threadIdx.x & 15, vec, u < mt * nq * 2);
+}
+
 // D digits of an activation: three of bf16, four of FP32.  MI = 0: the digits of
 // up to 8 / D rows of A share one block of eight columns; else MI blocks of
 // eight rows for each digit.  F: chunks of 32 weights that share their scales
@@ -148,14 +301,15 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     const uint32_t per = static_cast<uint32_t>(p.split_steps);
 
     unsigned char* ring = smem + (team * kWarps + warp) * p.slots * kStepBytes;
-    unsigned char* act = smem + kTeams * kWarps * p.slots * kStepBytes;                      // [128][2][col][t] 16 bytes
-    float* unit = reinterpret_cast<float*>(act + static_cast<size_t>(per) * p.cols * 256);   // [128][tcol]
-    uint32_t* base = reinterpret_cast<uint32_t*>(unit + per * 2 * tcols);                    // [128][flush][col]
-    float* isum = reinterpret_cast<float*>(base + per * 2 * (4 / F) * p.cols);               // [128][flush][tcol]
-    float* red = isum + per * 2 * (4 / F) * tcols + team * 2 * kWarps * RED;                     // [2][warp][4 NB][lane]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(
-        smem + p.bars_at);
-    uint32_t* odd = reinterpret_cast<uint32_t*>(bars + kTeams * kWarps * kMaxSlots);    // rows of A with an infinity or NaN
+    unsigned char* act = smem + kTeams * kWarps * p.slots * kStepBytes;
+    const Image img(act, per, p.cols, tcols, F);
+    float* const unit = img.unit;
+    uint32_t* const base = img.base;
+    float* const isum = img.isum;
+    float* red = reinterpret_cast<float*>(act + p.image_bytes) + team * 2 * kWarps * RED;    // [2][warp][4 NB][lane]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + p.bars_at);
+    uint64_t* image_bar = bars + kTeams * kWarps * kMaxSlots;
+    uint32_t* odd = reinterpret_cast<uint32_t*>(image_bar + 1);                 // rows of A with an infinity or NaN
     bars += (team * kWarps + warp) * kMaxSlots;
     const bool zeros = g.zero != nullptr;
     const bool f32s = g.st == DType::F32;
@@ -168,7 +322,10 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     // --- producer: one step's weights, lane (g, t) two rows of the tile and 32 weights of each
     if (lane == 0)
         for (int i = 0; i < p.slots; ++i) mbar_init(bars + i, 1);
-    if (tid == 0) *odd = 0u;
+    if (tid == 0) {
+        *odd = 0u;
+        mbar_init(image_bar, 1);
+    }
     fence_mbar_init();
     __syncwarp();
     Cursor prod(lo, hi, nq, warp);
@@ -187,126 +344,34 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     };
     for (int s = 0; s < p.slots; ++s) request(s);
 
-    // --- the K-range's activations as digits in the operand's order, the unit of each 128, and the
-    // sums of whole numbers over each stretch of F chunks.  Half a warp takes 128 activations of a
-    // row, eight to a lane: a word's worth.
+    // --- the K-range's activations as digits: from the kernel before, or made here
     __syncthreads();
-    {
+    if (p.images) {
+        if (tid == 0) {
+            pdl_wait();
+            asm volatile("fence.proxy.async;" ::: "memory");
+            const size_t at = (static_cast<size_t>(blockIdx.z) * gridDim.y + blockIdx.y) * p.image_bytes;
+            mbar_arrive_expect_tx(image_bar, p.image_bytes);
+            bulk_load_1d(act, p.images + at, p.image_bytes, image_bar);
+        }
+        mbar_wait(image_bar, 0, nullptr, p.err);
+    } else {
         const bool vec = g.lda % (16 / sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(g.A) % 16 == 0;
         const uint32_t nh = nq * 2, units = mt * nh, r = tid & 15;
-        // Which word of which lane these eight weights are, after the exchanges below.
-        const uint32_t w = F == 4 ? (r & 3) : (F == 1 ? (r >> 2) : ((r >> 3) * 2 + (r & 1)));
-        const uint32_t t = F == 4 ? (r >> 2) : (F == 1 ? (r & 3) : (((r >> 2) & 1) + (r & 2)));
         uint32_t u = tid >> 4, m = u / nh, q = u - m * nh;       // q: stretch of 128
         const uint32_t dm = (kTeams * kTeamThreads / 16) / nh, dq = (kTeams * kTeamThreads / 16) - dm * nh;
         for (uint32_t u0 = u & ~1u; u0 < units; u0 += kTeams * kTeamThreads / 16) {     // the same count for a whole warp
-            const bool in = u < units;
-            const int64_t k = static_cast<int64_t>(k_step0) * kStepK + q * 128 + r * 8;
-            const T* a = static_cast<const T*>(g.A) + static_cast<int64_t>(m0 + m) * g.lda + k;
-            float v[8] = {};
-            if (in) {
-                if (vec && k + 8 <= g.K) {
-                    if constexpr (PARTS) {
-                        const float4 x = __ldg(reinterpret_cast<const float4*>(a)), y = __ldg(reinterpret_cast<const float4*>(a) + 1);
-                        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-                        v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
-                    } else {
-                        const uint4 y = __ldg(reinterpret_cast<const uint4*>(a));
-                        const uint32_t x[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            v[2 * i] = __uint_as_float(x[i] << 16);
-                            v[2 * i + 1] = __uint_as_float(x[i] & 0xFFFF0000u);
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = k + i < g.K ? static_cast<float>(a[i]) : 0.0f;
-                }
-            }
-            float top = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
-            bool bad = top > 3.402823466e38f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) bad = bad || v[i] != v[i];
-            if (bad) {
-                atomicOr(odd, 1u << m);
-                top = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (!(fabsf(v[i]) <= 3.402823466e38f)) v[i] = 0.0f;
-                    top = fmaxf(top, fabsf(v[i]));
-                }
-            }
-#pragma unroll
-            for (int s = 1; s < 16; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s));
-            // 2^e is above every |v|; the unit 2^(e - BITS) stays a normal number.
-            int e = static_cast<int>(__float_as_uint(top) >> 23) - 126;
-            e = max(e, BITS - 126);
-            const float scale = __uint_as_float(static_cast<uint32_t>(127 + BITS - e) << 23);
-            uint32_t x[8];
-            if constexpr (PARTS) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = static_cast<uint32_t>(__float2int_rn(v[i] * scale)) + 0x80808080u;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)     // every digit plus 128
-                    x[i] = __float_as_uint(fmaf(v[i], scale, kMagic)) - kMagicBits + 0x00808080u;
-            }
-            // Even k are the low nibbles, the first operand register; odd k the second.
-            uint2 o[4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t p0 = __byte_perm(x[h], x[h + 2], 0x5140), p1 = __byte_perm(x[h + 4], x[h + 6], 0x5140);
-                const uint32_t p2 = __byte_perm(x[h], x[h + 2], 0x7362), p3 = __byte_perm(x[h + 4], x[h + 6], 0x7362);
-                const uint32_t d0 = __byte_perm(p0, p1, 0x5410) ^ 0x80808080u, d1 = __byte_perm(p0, p1, 0x7632) ^ 0x80808080u;
-                const uint32_t d2 = __byte_perm(p2, p3, 0x5410) ^ 0x80808080u, d3 = __byte_perm(p2, p3, 0x7632) ^ 0x80808080u;
-                (h ? o[0].y : o[0].x) = d0;
-                (h ? o[1].y : o[1].x) = d1;
-                (h ? o[2].y : o[2].x) = d2;
-                (h ? o[3].y : o[3].x) = d3;
-            }
-            // Sums of the digits, two to a word: each stays within 16 bits.
-            int pair[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int lo = __dp4a(static_cast<int>(o[2 * h].x), 0x01010101, __dp4a(static_cast<int>(o[2 * h].y), 0x01010101, 0));
-                const int up = __dp4a(static_cast<int>(o[2 * h + 1].x), 0x01010101, __dp4a(static_cast<int>(o[2 * h + 1].y), 0x01010101, 0));
-                pair[h] = lo + up * 65536;
-                if (2 * h + 1 >= D) pair[h] = lo;
-#pragma unroll
-                for (int s = 1; s < 4 * F; s <<= 1) pair[h] += __shfl_xor_sync(0xFFFFFFFFu, pair[h], s);
-            }
-            if (in) {
-                unsigned char* dst = act + ((q * 2 + (w >> 1)) * p.cols + m) * 64 + t * 16 + (w & 1) * 8;
-#pragma unroll
-                for (int d = 0; d < D; ++d) *reinterpret_cast<uint2*>(dst + d * p.rows * 64) = o[d];
-                const float u1 = __uint_as_float(static_cast<uint32_t>(127 + e - BITS) << 23);
-                if (r == 0) {
-#pragma unroll
-                    for (int d = 0; d < (PACKED ? D : 1); ++d)      // packed: digit d has a column of its own, worth 256^d
-                        unit[q * tcols + d * p.rows + m] = u1 * static_cast<float>(1u << (8 * d));
-                }
-                if ((r & (4 * F - 1)) == 0) {
-                    const uint32_t at = q * (4 / F) + r / (4 * F);
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int d = D - 1; d >= 0; --d) {
-                        const int lo = static_cast<int16_t>(pair[d / 2] & 0xFFFF);
-                        const int digits = d % 2 ? (pair[d / 2] - lo) >> 16 : (d == 2 && D == 3 ? pair[1] : lo);
-                        base[at * p.cols + d * p.rows + m] = kMagicBits - static_cast<uint32_t>(8 * digits);
-                        if constexpr (PACKED) isum[at * tcols + d * p.rows + m] = static_cast<float>(digits);
-                        sum = fmaf(sum, 256.0f, static_cast<float>(digits));
-                    }
-                    if constexpr (!PACKED) isum[at * tcols + m] = sum;
-                }
-            }
+            stage<IO, MI, F>(p, img, m0, k_step0, m, q, r, vec, u < units);
             u += kTeams * kTeamThreads / 16;
             m += dm;
             q += dq;
             if (q >= nh) { q -= nh; ++m; }
         }
+        __syncthreads();
+    }
+    for (uint32_t i = tid; i < mt * nq * 2; i += kTeams * kTeamThreads) {
+        const uint32_t q = i / mt, m = i - q * mt;
+        if (unit[q * tcols + m] < 0.0f) atomicOr(odd, 1u << m);
     }
     __syncthreads();
     if (!busy) return;
@@ -434,7 +499,7 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) un[b][e] = unit[qh * tcols + tab[b][e]];
+                    for (int e = 0; e < 2; ++e) un[b][e] = fabsf(unit[qh * tcols + tab[b][e]]);
                 uint4 x[NT];        // the operand columns of two words
                 uint32_t c[NT][4];
 #pragma unroll
@@ -552,24 +617,34 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
             last[tt] = parts;
         }
         sync();
-        for (uint32_t i = 0; i < kTeamThreads && t0 + i <= tile; ++i) {
+        for (uint32_t i = warp; i < kTeamThreads && t0 + i <= tile; i += kWarps) {      // a warp to a tile
             if (last[i] == 0) continue;
             const uint32_t at = t0 + i;
-            for (int idx = tt; idx < 16 * mt; idx += kTeamThreads) {
-                const int r = idx & 15, m = idx >> 4;
-                const int64_t row = static_cast<int64_t>(at) * 16 + r;
-                if (row >= g.N) continue;
-                float sum = 0.0f;
+            for (int v = lane; v < 4 * mt; v += 32) {
+                const int r = (4 * v) & 15, m = v >> 2;
+                float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 for (uint32_t y = 0; y < gridDim.y; ++y) {
                     const uint32_t ny = p.steps - y * per < per ? p.steps - y * per : per;
                     const Shares sy(p.tiles * ny, gridDim.x * kTeams);
                     const uint32_t s0 = sy.holder(at * ny), s1 = sy.holder(at * ny + ny - 1);
-                    const float* base = range_slots(y) + idx;
+                    const float4* from = reinterpret_cast<const float4*>(range_slots(y)) + v;
 #pragma unroll 4
-                    for (uint32_t s = s0; s <= s1; ++s)
-                        sum += __ldcg(base + (s == s0 ? at : p.tiles + s) * static_cast<size_t>(16 * ROWS));
+                    for (uint32_t s = s0; s <= s1; ++s) {
+                        const float4 x = __ldcg(from + (s == s0 ? at : p.tiles + s) * static_cast<size_t>(4 * ROWS));
+                        sum.x += x.x;
+                        sum.y += x.y;
+                        sum.z += x.z;
+                        sum.w += x.w;
+                    }
                 }
-                static_cast<T*>(g.C)[static_cast<int64_t>(m0 + m) * g.ldc + row] = static_cast<T>(sum + (g.bias ? g.bias[row] : 0.0f));
+                const float x[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int64_t row = static_cast<int64_t>(at) * 16 + r + j;
+                    if (row < g.N)
+                        static_cast<T*>(g.C)[static_cast<int64_t>(m0 + m) * g.ldc + row] =
+                            static_cast<T>(x[j] + (g.bias ? g.bias[row] : 0.0f));
+                }
             }
         }
         sync();
@@ -594,7 +669,8 @@ __global__ void __launch_bounds__(256) repack_rows_kernel(const uint8_t* w, int6
 
 struct Kernel {
     const void* fn;
-    int rows, digits, blocks, flush, packed;
+    const void* digits;
+    int rows, n_digits, blocks, flush, packed;
 };
 
 template <DType IO, int MI>
@@ -603,7 +679,10 @@ Kernel kernel_for_flush(int f) {
     const void* fn = f == 4 ? reinterpret_cast<const void*>(&gemm_w4_kernel<IO, MI, 4>)
                      : f == 2 ? reinterpret_cast<const void*>(&gemm_w4_kernel<IO, MI, 2>)
                               : reinterpret_cast<const void*>(&gemm_w4_kernel<IO, MI, 1>);
-    return {fn, MI ? 8 * MI : 8 / D, D, MI ? MI : 1, f, MI == 0};
+    const void* digits = f == 4 ? reinterpret_cast<const void*>(&gemm_w4_digits_kernel<IO, MI, 4>)
+                         : f == 2 ? reinterpret_cast<const void*>(&gemm_w4_digits_kernel<IO, MI, 2>)
+                                  : reinterpret_cast<const void*>(&gemm_w4_digits_kernel<IO, MI, 1>);
+    return {fn, digits, MI ? 8 * MI : 8 / D, D, MI ? MI : 1, f, MI == 0};
 }
 
 Kernel select(const W4Args& g) {
@@ -652,11 +731,11 @@ bool gemm_w4_plan(const W4Args& g, int num_sms, W4Plan* plan) {
     const Kernel k = select(g);
     plan->rows = g.M < k.rows ? g.M : k.rows;
     const int64_t steps = (static_cast<int64_t>(g.K) + kStepK - 1) / kStepK, tiles = (static_cast<int64_t>(g.N) + 15) / 16;
-    plan->cols = k.digits * plan->rows;
+    plan->cols = k.n_digits * plan->rows;
     // As much of K at a time as the digits leave room for beside the smallest rings; the rings take
     // what is left.
     const int warps = kTeams * kWarps;
-    const int fixed = warps * (2 * k.blocks * 512 + kMaxSlots * 8) + 64;
+    const int fixed = warps * (2 * k.blocks * 512 + kMaxSlots * 8) + 64 + 16;
     const int per_step = 2 * (plan->cols * (128 + 4 * (4 / k.flush)) + 4 * (k.packed ? plan->cols : plan->rows) * (1 + 4 / k.flush));
     const int64_t most = (kMaxSmem - fixed - warps * kMinSlots * kStepBytes) / per_step;
     const int64_t splits = (steps + most - 1) / most;
@@ -666,9 +745,16 @@ bool gemm_w4_plan(const W4Args& g, int num_sms, W4Plan* plan) {
     plan->slots = rest < kMaxSlots ? rest : kMaxSlots;
     plan->smem = fixed + per_step * plan->split_steps + warps * plan->slots * kStepBytes;
     plan->bars_at = (plan->smem - warps * kMaxSlots * 8 - 16) & ~7;
+    plan->image_bytes = (per_step * plan->split_steps + 15) & ~15;
+    // 512 threads take a microsecond for every 32 stretches of 128 activations; a kernel before this
+    // one takes two and overlaps this one's start.
+    const int64_t stretches = static_cast<int64_t>(plan->rows) * plan->split_steps * 2;
+    plan->prepared = stretches > 64;
     plan->pitch = aligned_rows(g) ? 0 : (row_bytes_of(g) + 15) / 16 * 16;
     plan->copy_bytes = static_cast<size_t>(plan->pitch) * g.N;
     plan->blocks = (g.M + k.rows - 1) / k.rows;
+    plan->extra_bytes = plan->copy_bytes;
+    if (plan->prepared) plan->extra_bytes += static_cast<size_t>(plan->blocks) * plan->splits * plan->image_bytes;
     // Every SM a CTA, shared among the K-ranges; no more than there are shares of eight steps.
     int64_t ctas = (num_sms + plan->splits - 1) / plan->splits;
     const int64_t shares = (tiles * plan->split_steps + kWarps - 1) / kWarps;
@@ -681,7 +767,7 @@ bool gemm_w4_plan(const W4Args& g, int num_sms, W4Plan* plan) {
     return true;
 }
 
-cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint32_t* tickets, void* copy,
+cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint32_t* tickets, void* extra,
                            uint32_t* err, cudaStream_t s) {
     const Kernel k = select(g);
     static std::mutex mu;
@@ -719,17 +805,37 @@ cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint3
     const uint8_t* w = g.W;
     int64_t pitch = g.ldw;
     if (plan.pitch) {
-        w = static_cast<const uint8_t*>(copy);
+        w = static_cast<const uint8_t*>(extra);
         pitch = plan.pitch;
         repack_rows_kernel<<<(static_cast<unsigned>(g.N) + 7) / 8, 256, 0, s>>>(g.W, g.ldw, g.N, static_cast<int>(row_bytes_of(g)),
-                                                                              static_cast<uint8_t*>(copy), pitch);
+                                                                              static_cast<uint8_t*>(extra), pitch);
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
     }
     CUtensorMap map;
     if (!encode_weights(g, w, pitch, &map)) return cudaErrorNotSupported;
+    p.image_bytes = plan.image_bytes;
+    p.images = nullptr;
+    if (plan.prepared) {
+        p.images = static_cast<unsigned char*>(extra) + plan.copy_bytes;
+        const unsigned stretches = static_cast<unsigned>(plan.rows) * plan.split_steps * 2;
+        void* first[] = {&p};
+        e = cudaLaunchKernel(k.digits, dim3((stretches + 7) / 8, plan.splits, plan.blocks), dim3(128), first, 0, s);
+        if (e != cudaSuccess) return e;
+    }
+    // The kernel may start before the one that makes the digits is done: all that it reads or writes
+    // until it waits for that one is older, or its own.
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(plan.ctas, plan.splits, plan.blocks);
+    cfg.blockDim = dim3(kTeams * kTeamThreads);
+    cfg.dynamicSmemBytes = static_cast<size_t>(plan.smem);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = plan.prepared ? 1 : 0;
     void* args[] = {&p, &map};
-    return cudaLaunchKernel(k.fn, dim3(plan.ctas, plan.splits, plan.blocks), dim3(kTeams * kTeamThreads), args,
-                            static_cast<size_t>(plan.smem), s);
+    return cudaLaunchKernelExC(&cfg, k.fn, args);
 }
 
 }  // namespace dnnopt_b200

@@ -319,12 +319,15 @@ struct W4Plan {
     int ctas, splits, blocks;   // grid: shares of the steps, K-ranges, blocks of rows of A
     int split_steps, rows, cols, slots, smem, bars_at;
     int64_t pitch;              // rows of W are copied to this pitch first; 0: they are fine
-    size_t copy_bytes;
+    size_t copy_bytes;          // of that copy
+    bool prepared;              // a kernel of its own makes the activations' digits
+    int image_bytes;
+    size_t extra_bytes;         // copy and digits
     size_t ws_floats;           // partial tiles
     size_t tickets;             // zero on entry, left zero
 };
 bool gemm_w4_plan(const W4Args& g, int num_sms, W4Plan* plan);   // false: sizes past the kernel's counters
-cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint32_t* tickets, void* copy,
+cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint32_t* tickets, void* extra,
                            uint32_t* err, cudaStream_t s);
 
 // Attention of one new token per sequence over a paged cache (strides in elements).

@@ -244,17 +244,20 @@ struct Cursor {
     }
 };
 
-// Every CTA takes one share of the tiles, equal but for one tile.
+// Every CTA takes one share of the tiles, equal but for one tile: the first
+// `more` shares have one more than the others.
 struct Shares {
-    uint32_t total, ctas;
+    uint32_t ctas, each, more;
 
-    __device__ Shares(uint32_t tiles, uint32_t grid) : total(tiles), ctas(tiles < grid ? tiles : grid) {}
-    __device__ __forceinline__ uint32_t start(uint32_t c) const {
-        return static_cast<uint32_t>(static_cast<uint64_t>(c) * total / ctas);
+    __device__ Shares(uint32_t tiles, uint32_t grid) : ctas(tiles < grid ? tiles : grid) {
+        each = tiles / ctas;
+        more = tiles - each * ctas;
     }
+    __device__ __forceinline__ uint32_t start(uint32_t c) const { return c * each + min(c, more); }
     // The share that holds tile t: the last one that starts at or before it.
     __device__ __forceinline__ uint32_t holder(uint32_t t) const {
-        return static_cast<uint32_t>((static_cast<uint64_t>(t + 1) * ctas - 1) / total);
+        const uint32_t big = more * (each + 1);
+        return t < big ? t / (each + 1) : more + (t - big) / each;
     }
 };
 
