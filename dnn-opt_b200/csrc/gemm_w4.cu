@@ -73,13 +73,20 @@ struct Params {
 };
 
 __device__ __forceinline__ void mma_u8s8(uint32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+// A scale as it lies in memory: 32 bits, or 16 in the low half.
+__device__ __forceinline__ uint32_t ldg_scale(const char* p, bool f32) {
+    uint32_t v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %2, 0;\n\t@p ld.global.nc.u32 %0, [%1];\n\t@!p ld.global.nc.u16 %0, [%1];\n\t}"
+                 : "=r"(v) : "l"(p), "r"(static_cast<int>(f32)));
     return v;
 }
 constexpr float kMagic = 12582912.0f;           // 1.5 * 2^23: whole numbers below 2^22 added to it keep their bits
@@ -285,7 +292,7 @@ __global__ void __launch_bounds__(kTeams * kTeamThreads, 1)
 gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     using T = typename std::conditional<IO == DType::F32, float, __nv_bfloat16>::type;
     constexpr bool PARTS = IO == DType::F32, PACKED = MI == 0;
-    constexpr int D = PARTS ? 4 : 3, BITS = PARTS ? 30 : 22;
+    constexpr int D = PARTS ? 4 : 3;
     constexpr int NT = PACKED ? 1 : D * MI;                 // blocks of eight columns
     constexpr int NB = PACKED ? 1 : MI;                     // blocks of sums, after the digits are put together
     constexpr int ROWS = PACKED ? 8 / D : 8 * MI;           // rows of A per pass
@@ -383,23 +390,22 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
         return f32s ? __ldg(static_cast<const uint32_t*>(base) + e) : __ldg(static_cast<const uint16_t*>(base) + e);
     };
     auto value = [&](uint32_t raw) { return __uint_as_float(raw << up); };
-    auto group_of = [&](uint32_t chunk) {
-        const int gi = p.gmul ? static_cast<int>(__umulhi(chunk, p.gmul) >> p.gshift) : static_cast<int>(chunk);
-        return gi < g.groups ? gi : g.groups - 1;
-    };
+    auto group_of = [&](uint32_t chunk) { return min(static_cast<int>(__umulhi(2 * chunk, p.gmul) >> p.gshift), g.groups - 1); };
+    const int scale_bytes = f32s ? 4 : 2;
+    const int64_t to_zero = reinterpret_cast<intptr_t>(g.zero) - reinterpret_cast<intptr_t>(g.scale);
     // The slots of K-range y.
     auto range_slots = [&](uint32_t y) {
         return p.ws + (static_cast<size_t>(blockIdx.z) * gridDim.y + y) * (p.tiles + gridDim.x * kTeams) * (16 * ROWS);
     };
 
-    // Shared-memory addresses of the lane's operand columns (those that are not there repeat the last)
-    // and of its columns' tables.
-    uint32_t act_at[NT], base_at[NT][2], tab[NB][2];
+    // The lane's operand columns (those that are not there repeat the last) and its columns in the tables.
+    const unsigned char* act_at[NT];
+    uint32_t base_at[NT][2], tab[NB][2];
     const uint32_t ring_at = smem_u32(ring) + lane * 16, act_half = p.cols * 64;
 #pragma unroll
     for (int b = 0; b < NT; ++b) {
         const int col = PACKED ? min(gr, p.cols - 1) : (b % D) * p.rows + min(8 * (b / D) + gr, mt - 1);
-        act_at[b] = smem_u32(act) + col * 64 + t4 * 16;
+        act_at[b] = act + col * 64 + t4 * 16;
 #pragma unroll
         for (int e = 0; e < 2; ++e)
             base_at[b][e] = PACKED ? min(2 * t4 + e, p.cols - 1) : (b % D) * p.rows + min(8 * (b / D) + 2 * t4 + e, mt - 1);
@@ -410,13 +416,13 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
         for (int e = 0; e < 2; ++e) tab[b][e] = min(8 * b + 2 * t4 + e, tcols - 1);
     // Scales are read one step ahead of their products, across the ends of tiles.
     Cursor ahead(lo, hi, nq, warp);
-    int64_t srow[2];        // the lane's two rows' first scales
+    const char* srow[2];    // the lane's two rows' first scales
     uint32_t raw[2][2] = {}, rawz[2][2] = {};       // [half][row]
     auto open = [&](uint32_t t) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int64_t row = static_cast<int64_t>(t) * 16 + gr + 8 * h;
-            srow[h] = (row < g.N ? row : g.N - 1) * g.lds;
+            srow[h] = static_cast<const char*>(g.scale) + (row < g.N ? row : g.N - 1) * g.lds * scale_bytes;
         }
     };
     auto fetch_scales = [&]() {
@@ -426,8 +432,9 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
             const int gi = group_of((k_step0 + ahead.q) * 8 + half * 4 + t4);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                raw[half][h] = fetch(g.scale, srow[h] + gi);
-                if (zeros) rawz[half][h] = fetch(g.zero, srow[h] + gi);
+                const char* at = srow[h] + static_cast<int64_t>(gi) * scale_bytes;
+                raw[half][h] = ldg_scale(at, f32s);
+                if (zeros) rawz[half][h] = ldg_scale(at + to_zero, f32s);
             }
         }
         ahead.q += kWarps;
@@ -515,7 +522,7 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
                                             (wh[1][i] >> 4) & 0x0F0F0F0Fu};
 #pragma unroll
                     for (int b = 0; b < NT; ++b) {
-                        if (i % 2 == 0) x[b] = lds128(act_at[b] + (qh * 2 + i / 2) * act_half);
+                        if (i % 2 == 0) x[b] = *reinterpret_cast<const uint4*>(act_at[b] + (qh * 2 + i / 2) * act_half);
                         mma_u8s8(c[b], av, i % 2 ? x[b].z : x[b].x, i % 2 ? x[b].w : x[b].y);
                     }
                     if ((i + 1) % F != 0) continue;
@@ -749,7 +756,7 @@ bool gemm_w4_plan(const W4Args& g, int num_sms, W4Plan* plan) {
     // 512 threads take a microsecond for every 32 stretches of 128 activations; a kernel before this
     // one takes two and overlaps this one's start.
     const int64_t stretches = static_cast<int64_t>(plan->rows) * plan->split_steps * 2;
-    plan->prepared = stretches > 64;
+    plan->prepared = stretches > 32;
     plan->pitch = aligned_rows(g) ? 0 : (row_bytes_of(g) + 15) / 16 * 16;
     plan->copy_bytes = static_cast<size_t>(plan->pitch) * g.N;
     plan->blocks = (g.M + k.rows - 1) / k.rows;
@@ -793,12 +800,12 @@ cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint3
     p.cols = plan.cols;
     p.rows = plan.rows;
     p.bars_at = plan.bars_at;
-    // chunk / (group / 32) for chunks below 2^31: mul = ceil(2^(31 + ceil(log2 d)) / d).
+    // chunk / (group / 32) = mulhi(2 chunk, mul) >> log for chunks below 2^31: mul = ceil(2^(31 + ceil(log2 d)) / d).
     const int64_t d = g.groups > 1 ? g.group / 32 : int64_t(1) << 30;
     int log = 0;
     while ((int64_t(1) << log) < d) ++log;
-    p.gmul = d == 1 ? 0 : static_cast<uint32_t>(((uint64_t(1) << (31 + log)) + d - 1) / d);
-    p.gshift = log > 0 ? log - 1 : 0;
+    p.gmul = static_cast<uint32_t>(((uint64_t(1) << (31 + log)) + d - 1) / d);
+    p.gshift = log;
     p.ws = ws;
     p.tickets = tickets;
     p.err = err;
