@@ -1,30 +1,273 @@
 // The norms around a block with its gate and residual scale:
 //   h = rs * x + bs * gate * post(y),  z = pre(h).
 //
-// One CTA per row keeps the row's FP32 values in shared memory.
+// What bounds it: x, y (and gate) are read and h, z written once, a dozen
+// operations an element: HBM for many rows, the chain of load, sums over the
+// row and store for few.  So a row stays in registers from its first load to
+// its last store, and both norms, the gate and the residual take one kernel:
+//   * rows of up to 512 columns belong to a warp each (no barrier), longer ones
+//     to a CTA;
+//   * few rows: eight elements to a thread, so that many threads share a row;
+//   * many rows: 16 elements, and each warp or CTA takes row after row, the
+//     next one's loads under way while it works on this one;
+//   * rows past 16384 columns stay in shared memory.
+// Elements are read 16 bytes at a time where all rows and vectors allow, else
+// one by one, neighbouring threads neighbouring elements.  Means and mean
+// squares are sums over the values themselves (a layer norm's squares are
+// taken after its mean), in a fixed order.
+#include <mutex>
+#include <unordered_map>
+
 #include "common.cuh"
 #include "kernels.h"
 
 namespace dnnopt_b200 {
 namespace {
 
-constexpr int kThreads = 256;
-
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ void from_f32(float* p, float v) { *p = v; }
 __device__ __forceinline__ void from_f32(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
+// Eight consecutive elements, 16-byte aligned.
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+constexpr int kRowsPerCta = 8;      // of a warp each
+
+// Eight elements as they were read: 16-bit ones in pairs (VEC) or one to a word.
+template <typename T, bool VEC>
+struct Raw {
+    float w[8];
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = w[j];
+    }
+};
+template <bool VEC>
+struct Raw<__nv_bfloat16, VEC> {
+    uint32_t w[VEC ? 4 : 8];
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            v[j] = __uint_as_float(!VEC ? w[VEC ? 0 : j] << 16 : (j & 1) ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
+    }
+};
+
+// EPT elements of a row to each of `threads` threads: element j of block i is
+// column 8 * (me + i * threads) + j (VEC) or me + (8 i + j) * threads.
+template <bool VEC, int EPT>
+struct Row {
+    int me, threads, cols;
+
+    __device__ __forceinline__ int col(int i, int j) const {
+        return VEC ? 8 * (me + i * threads) + j : me + (8 * i + j) * threads;
+    }
+    // Block i of a row; columns that are not there give 0.
+    __device__ __forceinline__ void read(const float* p, int i, Raw<float, VEC>& r) const {
+        if (VEC && col(i, 0) + 8 <= cols) {
+            load8(p + col(i, 0), r.w);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r.w[j] = col(i, j) < cols ? p[col(i, j)] : 0.0f;
+        }
+    }
+    __device__ __forceinline__ void read(const __nv_bfloat16* p, int i, Raw<__nv_bfloat16, VEC>& r) const {
+        const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+        if constexpr (VEC) {
+            if (col(i, 0) + 8 <= cols) {
+                const uint4 x = *reinterpret_cast<const uint4*>(p + col(i, 0));
+                r.w[0] = x.x; r.w[1] = x.y; r.w[2] = x.z; r.w[3] = x.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    r.w[j] = col(i, 2 * j) < cols ? q[col(i, 2 * j)] : 0u;
+                    if (col(i, 2 * j + 1) < cols) r.w[j] |= static_cast<uint32_t>(q[col(i, 2 * j + 1)]) << 16;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r.w[j] = col(i, j) < cols ? q[col(i, j)] : 0u;
+        }
+    }
+    template <typename P>
+    __device__ __forceinline__ void load(const P* p, int i, float (&v)[8]) const {
+        Raw<P, VEC> r;
+        read(p, i, r);
+        r.get(v);
+    }
+    template <typename P>
+    __device__ __forceinline__ void store(P* p, int i, const float (&v)[8]) const {
+        if (VEC && col(i, 0) + 8 <= cols) {
+            store8(p + col(i, 0), v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (col(i, j) < cols) from_f32(p + col(i, j), v[j]);
+        }
+    }
+};
+
+// Sum over the row's threads, the same for all of them.  Two buffers in turn:
+// a barrier lies between a buffer's reading and its next writing.
+template <bool WARP>
+__device__ __forceinline__ float row_sum(float v, float (&part)[2][32], int& buffer) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    if (!WARP) {
+        const int lane = threadIdx.x & 31;
+        if (lane == 0) part[buffer][threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = lane < static_cast<int>(blockDim.x >> 5) ? part[buffer][lane] : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+        buffer ^= 1;
+    }
+    return v;
+}
+
+template <typename TW, bool WARP, bool VEC, int EPT>
+__device__ __forceinline__ void norm_row(const Row<VEC, EPT>& row, float (&v)[EPT / 8][8], int kind, const TW* w, const TW* b,
+                                         float eps, float offset, float inv, float (&part)[2][32], int& buffer) {
+    constexpr int NB = EPT / 8;
+    if (kind == 0) return;
+    if (kind == 2) {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s += v[i][j];
+        const float mean = row_sum<WARP>(s, part, buffer) * inv;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = row.col(i, j) < row.cols ? v[i][j] - mean : 0.0f;
+    }
+    float q = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q = fmaf(v[i][j], v[i][j], q);
+    const float rstd = rsqrtf(row_sum<WARP>(q, part, buffer) * inv + eps);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        float t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] *= rstd;
+        if (w) {
+            row.load(w, i, t);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] *= t[j] + offset;
+        }
+        if (b) {
+            row.load(b, i, t);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] += t[j];
+        }
+    }
+}
+
+// STREAM: row after row, gridDim rows (or blocks of them) apart.
+template <typename T, typename TW, bool VEC, int EPT, bool WARP, bool STREAM>
+__global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : (STREAM ? 512 : 1024)) block_norm_kernel(const BlockNormArgs a) {
+    constexpr int NB = EPT / 8;
+    __shared__ float part[2][32];
+    int buffer = 0;
+    int64_t r = WARP ? static_cast<int64_t>(blockIdx.x) * kRowsPerCta + (threadIdx.x >> 5) : blockIdx.x;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (WARP ? kRowsPerCta : 1);
+    if (r >= a.rows) return;
+    Row<VEC, EPT> row;
+    row.me = WARP ? threadIdx.x & 31 : threadIdx.x;
+    row.threads = WARP ? 32 : blockDim.x;
+    row.cols = a.cols;
+    const float inv = 1.0f / static_cast<float>(a.cols);
+
+    Raw<T, VEC> x[NB], y[NB], g[NB];
+    auto read = [&](int64_t at) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) row.read(static_cast<const T*>(a.x) + at * a.ldx, i, x[i]);
+        if (!a.y) return;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) row.read(static_cast<const T*>(a.y) + at * a.ldy, i, y[i]);
+        if (!a.gate) return;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) row.read(static_cast<const T*>(a.gate) + at / a.gate_rows * a.ldg, i, g[i]);
+    };
+    read(r);
+    for (;;) {
+        float v[NB][8];
+        if (a.y) {
+            float t[NB][8], u[8];
+#pragma unroll
+            for (int i = 0; i < NB; ++i) y[i].get(t[i]);
+            norm_row<TW, WARP, VEC, EPT>(row, t, a.post, static_cast<const TW*>(a.post_w), static_cast<const TW*>(a.post_b),
+                                         a.eps, a.offset, inv, part, buffer);
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                if (a.gate) {
+                    g[i].get(u);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) t[i][j] *= u[j];
+                }
+                x[i].get(v[i]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)     // a bias reaches columns that are not there
+                    v[i][j] = row.col(i, j) < a.cols ? fmaf(a.bs, t[i][j], a.rs * v[i][j]) : 0.0f;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                x[i].get(v[i]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] *= a.rs;
+            }
+        }
+        const int64_t now = r;
+        r += step;
+        if (STREAM && r < a.rows) read(r);      // in-place rows are this row's own
+        if (a.h) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i) row.store(static_cast<T*>(a.h) + now * a.ldh, i, v[i]);
+        }
+        if (a.z) {
+            norm_row<TW, WARP, VEC, EPT>(row, v, a.pre, static_cast<const TW*>(a.pre_w), static_cast<const TW*>(a.pre_b), a.eps,
+                                         a.offset, inv, part, buffer);
+#pragma unroll
+            for (int i = 0; i < NB; ++i) row.store(static_cast<T*>(a.z) + now * a.ldz, i, v[i]);
+        }
+        if (!STREAM || r >= a.rows) return;
+    }
+}
+
+// ---- rows that fill no CTA's registers: FP32 values in shared memory ----------
+constexpr int kLongThreads = 1024;
+
 __device__ __forceinline__ float block_sum(float v) {
-    __shared__ float part[kThreads / 32];
+    __shared__ float part[kLongThreads / 32];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = 0.0f;
+    v = part[threadIdx.x & 31];
 #pragma unroll
-    for (int i = 0; i < kThreads / 32; ++i) v += part[i];
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
     return v;
 }
 
@@ -36,11 +279,11 @@ __device__ __forceinline__ void row_stats(const float* v, int cols, int kind, fl
     const float inv = 1.0f / static_cast<float>(cols);
     if (kind == 2) {
         float s = 0.0f;
-        for (int c = threadIdx.x; c < cols; c += kThreads) s += v[c];
+        for (int c = threadIdx.x; c < cols; c += kLongThreads) s += v[c];
         *mean = block_sum(s) * inv;
     }
     float q = 0.0f;
-    for (int c = threadIdx.x; c < cols; c += kThreads) { const float t = v[c] - *mean; q = fmaf(t, t, q); }
+    for (int c = threadIdx.x; c < cols; c += kLongThreads) { const float t = v[c] - *mean; q = fmaf(t, t, q); }
     *rstd = rsqrtf(block_sum(q) * inv + eps);
 }
 
@@ -53,18 +296,18 @@ __device__ __forceinline__ float apply(float v, int c, float mean, float rstd, c
 }
 
 template <typename T, typename TW>
-__global__ void __launch_bounds__(kThreads) block_norm_row_kernel(BlockNormArgs a) {
+__global__ void __launch_bounds__(kLongThreads) block_norm_long_kernel(const BlockNormArgs a) {
     extern __shared__ float row[];
     const int64_t r = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + r * a.ldx;
     float mean, rstd;
     if (a.y) {
         const T* y = static_cast<const T*>(a.y) + r * a.ldy;
-        for (int c = threadIdx.x; c < a.cols; c += kThreads) row[c] = to_f32(y[c]);
+        for (int c = threadIdx.x; c < a.cols; c += kLongThreads) row[c] = to_f32(y[c]);
         row_stats(row, a.cols, a.post, a.eps, &mean, &rstd);
     }
     const T* gate = a.gate ? static_cast<const T*>(a.gate) + r / a.gate_rows * a.ldg : nullptr;
-    for (int c = threadIdx.x; c < a.cols; c += kThreads) {
+    for (int c = threadIdx.x; c < a.cols; c += kLongThreads) {
         float v = a.rs * to_f32(x[c]);
         if (a.y) {
             float t = row[c];
@@ -78,7 +321,7 @@ __global__ void __launch_bounds__(kThreads) block_norm_row_kernel(BlockNormArgs 
     }
     if (!a.z) return;
     row_stats(row, a.cols, a.pre, a.eps, &mean, &rstd);
-    for (int c = threadIdx.x; c < a.cols; c += kThreads) {
+    for (int c = threadIdx.x; c < a.cols; c += kLongThreads) {
         float v = row[c];
         if (a.pre != 0)
             v = apply(v, c, mean, rstd, static_cast<const TW*>(a.pre_w), static_cast<const TW*>(a.pre_b), a.offset);
@@ -86,22 +329,89 @@ __global__ void __launch_bounds__(kThreads) block_norm_row_kernel(BlockNormArgs 
     }
 }
 
-template <typename T, typename TW>
-cudaError_t launch_row(const BlockNormArgs& a, cudaStream_t s) {
-    const void* fn = reinterpret_cast<const void*>(&block_norm_row_kernel<T, TW>);
-    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kBlockNormMaxCols * 4);
+// Resident CTAs per SM, asked once per kernel, size of CTA and device.
+cudaError_t resident(const void* fn, int threads, int* ctas) {
+    static std::mutex mu;
+    static std::unordered_map<const void*, int> known[64][17];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    block_norm_row_kernel<T, TW><<<a.rows, kThreads, static_cast<size_t>(a.cols) * 4, s>>>(a);
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    std::lock_guard<std::mutex> lk(mu);
+    int& n = known[dev][threads / 32][fn];
+    if (n == 0) {
+        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, threads, 0);
+        if (e != cudaSuccess) return e;
+        if (n < 1) return cudaErrorLaunchOutOfResources;
+    }
+    *ctas = n;
+    return cudaSuccess;
+}
+
+template <typename T, typename TW, bool VEC, int EPT, bool WARP>
+cudaError_t launch_stream(const BlockNormArgs& a, int threads, int num_sms, cudaStream_t s) {
+    int ctas = 0;
+    cudaError_t e = resident(reinterpret_cast<const void*>(&block_norm_kernel<T, TW, VEC, EPT, WARP, true>), threads, &ctas);
+    if (e != cudaSuccess) return e;
+    const int64_t units = WARP ? (static_cast<int64_t>(a.rows) + kRowsPerCta - 1) / kRowsPerCta : a.rows;
+    const int64_t most = static_cast<int64_t>(ctas) * num_sms;
+    block_norm_kernel<T, TW, VEC, EPT, WARP, true><<<static_cast<unsigned>(units < most ? units : most), threads, 0, s>>>(a);
     return cudaGetLastError();
+}
+
+template <typename T, typename TW, bool VEC>
+cudaError_t launch_short(const BlockNormArgs& a, int num_sms, cudaStream_t s) {
+    if (a.cols <= 512) {
+        const int threads = 32 * kRowsPerCta;
+        if (a.rows > 4 * kRowsPerCta * num_sms)
+            return a.cols <= 256 ? launch_stream<T, TW, VEC, 8, true>(a, threads, num_sms, s)
+                                 : launch_stream<T, TW, VEC, 16, true>(a, threads, num_sms, s);
+        const unsigned grid = (static_cast<unsigned>(a.rows) + kRowsPerCta - 1) / kRowsPerCta;
+        if (a.cols <= 256) block_norm_kernel<T, TW, VEC, 8, true, false><<<grid, threads, 0, s>>>(a);
+        else block_norm_kernel<T, TW, VEC, 16, true, false><<<grid, threads, 0, s>>>(a);
+        return cudaGetLastError();
+    }
+    auto threads = [&](int ept) { return ((a.cols + ept - 1) / ept + 31) / 32 * 32; };
+    if (a.cols <= 8192) {
+        if (a.rows > 2 * num_sms) return launch_stream<T, TW, VEC, 16, false>(a, threads(16), num_sms, s);
+        block_norm_kernel<T, TW, VEC, 8, false, false><<<a.rows, threads(8), 0, s>>>(a);
+    } else {
+        block_norm_kernel<T, TW, VEC, 16, false, false><<<a.rows, threads(16), 0, s>>>(a);
+    }
+    return cudaGetLastError();
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+template <typename T, typename TW>
+cudaError_t launch(const BlockNormArgs& a, int num_sms, cudaStream_t s) {
+    if (a.cols > 16384) {
+        const void* fn = reinterpret_cast<const void*>(&block_norm_long_kernel<T, TW>);
+        cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kBlockNormMaxCols * 4);
+        if (e != cudaSuccess) return e;
+        block_norm_long_kernel<T, TW><<<a.rows, kLongThreads, static_cast<size_t>(a.cols) * 4, s>>>(a);
+        return cudaGetLastError();
+    }
+    bool vec = true;
+    for (const void* p : {a.x, a.y, a.gate, a.post_w, a.post_b, a.pre_w, a.pre_b, static_cast<const void*>(a.h),
+                          static_cast<const void*>(a.z)})
+        vec = vec && aligned16(p);
+    auto pitch = [&](const void* p, int64_t ld) { vec = vec && (!p || ld * static_cast<int64_t>(sizeof(T)) % 16 == 0); };
+    pitch(a.x, a.ldx);
+    pitch(a.y, a.ldy);
+    pitch(a.gate, a.ldg);
+    pitch(a.h, a.ldh);
+    pitch(a.z, a.ldz);
+    return vec ? launch_short<T, TW, true>(a, num_sms, s) : launch_short<T, TW, false>(a, num_sms, s);
 }
 
 }  // namespace
 
-cudaError_t launch_block_norm(const BlockNormArgs& a, cudaStream_t s) {
+cudaError_t launch_block_norm(const BlockNormArgs& a, int num_sms, cudaStream_t s) {
     if (a.io == DType::F32)
-        return a.wt == DType::F32 ? launch_row<float, float>(a, s) : launch_row<float, __nv_bfloat16>(a, s);
-    return a.wt == DType::F32 ? launch_row<__nv_bfloat16, float>(a, s)
-                              : launch_row<__nv_bfloat16, __nv_bfloat16>(a, s);
+        return a.wt == DType::F32 ? launch<float, float>(a, num_sms, s) : launch<float, __nv_bfloat16>(a, num_sms, s);
+    return a.wt == DType::F32 ? launch<__nv_bfloat16, float>(a, num_sms, s)
+                              : launch<__nv_bfloat16, __nv_bfloat16>(a, num_sms, s);
 }
 
 }  // namespace dnnopt_b200

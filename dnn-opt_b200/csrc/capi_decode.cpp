@@ -180,7 +180,7 @@ int dnnopt_cuda_block_norm(const dnnopt_block_norm_desc* d, const void* x, const
     a.h = h; a.z = z;
     a.ldx = d->ldx; a.ldy = d->ldy; a.ldh = d->ldh; a.ldz = d->ldz; a.ldg = d->ldg;
     a.gate_rows = d->gate_rows;
-    cudaError_t e = launch_block_norm(a, static_cast<cudaStream_t>(stream));
+    cudaError_t e = launch_block_norm(a, ctx->num_sms, static_cast<cudaStream_t>(stream));
     note_launch();
     return cuda_status(e);
 }

@@ -381,6 +381,6 @@ struct BlockNormArgs {
     int64_t ldx, ldy, ldh, ldz, ldg;
     int gate_rows;
 };
-cudaError_t launch_block_norm(const BlockNormArgs& a, cudaStream_t s);
+cudaError_t launch_block_norm(const BlockNormArgs& a, int num_sms, cudaStream_t s);
 
 }  // namespace dnnopt_b200
