@@ -70,19 +70,28 @@ struct Raw<__nv_bfloat16, VEC> {
     }
 };
 
-// EPT elements of a row to each of `threads` threads: element j of block i is
-// column 8 * (me + i * threads) + j (VEC) or me + (8 i + j) * threads.
-template <bool VEC, int EPT>
+// EPT elements of a row to each of TH threads (0: as many as the CTA has):
+// element j of block i is column 8 * (me + i * threads) + j (VEC) or
+// me + (8 i + j) * threads.  With TH known, columns are offsets from one address.
+template <bool VEC, int EPT, int TH>
 struct Row {
-    int me, threads, cols;
+    int me, cols;
 
+    __device__ __forceinline__ int threads() const { return TH ? TH : blockDim.x; }
     __device__ __forceinline__ int col(int i, int j) const {
-        return VEC ? 8 * (me + i * threads) + j : me + (8 * i + j) * threads;
+        return VEC ? 8 * (me + i * threads()) + j : me + (8 * i + j) * threads();
+    }
+    // Whether all of block i is there: for VEC this thread's, else every thread's.
+    __device__ __forceinline__ bool full(int i) const {
+        return VEC ? col(i, 0) + 8 <= cols : (8 * i + 8) * threads() <= cols;
     }
     // Block i of a row; columns that are not there give 0.
     __device__ __forceinline__ void read(const float* p, int i, Raw<float, VEC>& r) const {
-        if (VEC && col(i, 0) + 8 <= cols) {
+        if (VEC && full(i)) {
             load8(p + col(i, 0), r.w);
+        } else if (full(i)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r.w[j] = p[col(i, j)];
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) r.w[j] = col(i, j) < cols ? p[col(i, j)] : 0.0f;
@@ -91,7 +100,7 @@ struct Row {
     __device__ __forceinline__ void read(const __nv_bfloat16* p, int i, Raw<__nv_bfloat16, VEC>& r) const {
         const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
         if constexpr (VEC) {
-            if (col(i, 0) + 8 <= cols) {
+            if (full(i)) {
                 const uint4 x = *reinterpret_cast<const uint4*>(p + col(i, 0));
                 r.w[0] = x.x; r.w[1] = x.y; r.w[2] = x.z; r.w[3] = x.w;
             } else {
@@ -101,6 +110,9 @@ struct Row {
                     if (col(i, 2 * j + 1) < cols) r.w[j] |= static_cast<uint32_t>(q[col(i, 2 * j + 1)]) << 16;
                 }
             }
+        } else if (full(i)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r.w[j] = q[col(i, j)];
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) r.w[j] = col(i, j) < cols ? q[col(i, j)] : 0u;
@@ -114,8 +126,11 @@ struct Row {
     }
     template <typename P>
     __device__ __forceinline__ void store(P* p, int i, const float (&v)[8]) const {
-        if (VEC && col(i, 0) + 8 <= cols) {
+        if (VEC && full(i)) {
             store8(p + col(i, 0), v);
+        } else if (full(i)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) from_f32(p + col(i, j), v[j]);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -142,8 +157,8 @@ __device__ __forceinline__ float row_sum(float v, float (&part)[2][32], int& buf
     return v;
 }
 
-template <typename TW, bool WARP, bool VEC, int EPT>
-__device__ __forceinline__ void norm_row(const Row<VEC, EPT>& row, float (&v)[EPT / 8][8], int kind, const TW* w, const TW* b,
+template <typename TW, bool WARP, bool VEC, int EPT, int TH>
+__device__ __forceinline__ void norm_row(const Row<VEC, EPT, TH>& row, float (&v)[EPT / 8][8], int kind, const TW* w, const TW* b,
                                          float eps, float offset, float inv, float (&part)[2][32], int& buffer) {
     constexpr int NB = EPT / 8;
     if (kind == 0) return;
@@ -155,9 +170,15 @@ __device__ __forceinline__ void norm_row(const Row<VEC, EPT>& row, float (&v)[EP
             for (int j = 0; j < 8; ++j) s += v[i][j];
         const float mean = row_sum<WARP>(s, part, buffer) * inv;
 #pragma unroll
-        for (int i = 0; i < NB; ++i)
+        for (int i = 0; i < NB; ++i) {
+            if (row.full(i)) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = row.col(i, j) < row.cols ? v[i][j] - mean : 0.0f;
+                for (int j = 0; j < 8; ++j) v[i][j] -= mean;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] = row.col(i, j) < row.cols ? v[i][j] - mean : 0.0f;
+            }
+        }
     }
     float q = 0.0f;
 #pragma unroll
@@ -184,17 +205,16 @@ __device__ __forceinline__ void norm_row(const Row<VEC, EPT>& row, float (&v)[EP
 }
 
 // STREAM: row after row, gridDim rows (or blocks of them) apart.
-template <typename T, typename TW, bool VEC, int EPT, bool WARP, bool STREAM>
-__global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : (STREAM ? 512 : 1024)) block_norm_kernel(const BlockNormArgs a) {
+template <typename T, typename TW, bool VEC, int EPT, bool WARP, bool STREAM, int TH>
+__global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : (STREAM ? TH : 1024)) block_norm_kernel(const BlockNormArgs a) {
     constexpr int NB = EPT / 8;
     __shared__ float part[2][32];
     int buffer = 0;
     int64_t r = WARP ? static_cast<int64_t>(blockIdx.x) * kRowsPerCta + (threadIdx.x >> 5) : blockIdx.x;
     const int64_t step = static_cast<int64_t>(gridDim.x) * (WARP ? kRowsPerCta : 1);
     if (r >= a.rows) return;
-    Row<VEC, EPT> row;
+    Row<VEC, EPT, TH> row;
     row.me = WARP ? threadIdx.x & 31 : threadIdx.x;
-    row.threads = WARP ? 32 : blockDim.x;
     row.cols = a.cols;
     const float inv = 1.0f / static_cast<float>(a.cols);
 
@@ -216,7 +236,7 @@ __global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : (STREAM ? 512 : 1024
             float t[NB][8], u[8];
 #pragma unroll
             for (int i = 0; i < NB; ++i) y[i].get(t[i]);
-            norm_row<TW, WARP, VEC, EPT>(row, t, a.post, static_cast<const TW*>(a.post_w), static_cast<const TW*>(a.post_b),
+            norm_row<TW, WARP, VEC, EPT, TH>(row, t, a.post, static_cast<const TW*>(a.post_w), static_cast<const TW*>(a.post_b),
                                          a.eps, a.offset, inv, part, buffer);
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
@@ -227,8 +247,7 @@ __global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : (STREAM ? 512 : 1024
                 }
                 x[i].get(v[i]);
 #pragma unroll
-                for (int j = 0; j < 8; ++j)     // a bias reaches columns that are not there
-                    v[i][j] = row.col(i, j) < a.cols ? fmaf(a.bs, t[i][j], a.rs * v[i][j]) : 0.0f;
+                for (int j = 0; j < 8; ++j) v[i][j] = fmaf(a.bs, t[i][j], a.rs * v[i][j]);
             }
         } else {
 #pragma unroll
@@ -246,7 +265,7 @@ __global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : (STREAM ? 512 : 1024
             for (int i = 0; i < NB; ++i) row.store(static_cast<T*>(a.h) + now * a.ldh, i, v[i]);
         }
         if (a.z) {
-            norm_row<TW, WARP, VEC, EPT>(row, v, a.pre, static_cast<const TW*>(a.pre_w), static_cast<const TW*>(a.pre_b), a.eps,
+            norm_row<TW, WARP, VEC, EPT, TH>(row, v, a.pre, static_cast<const TW*>(a.pre_w), static_cast<const TW*>(a.pre_b), a.eps,
                                          a.offset, inv, part, buffer);
 #pragma unroll
             for (int i = 0; i < NB; ++i) row.store(static_cast<T*>(a.z) + now * a.ldz, i, v[i]);
@@ -348,35 +367,40 @@ cudaError_t resident(const void* fn, int threads, int* ctas) {
     return cudaSuccess;
 }
 
-template <typename T, typename TW, bool VEC, int EPT, bool WARP>
-cudaError_t launch_stream(const BlockNormArgs& a, int threads, int num_sms, cudaStream_t s) {
+template <typename T, typename TW, bool VEC, int EPT, bool WARP, int TH>
+cudaError_t launch_stream(const BlockNormArgs& a, int num_sms, cudaStream_t s) {
     int ctas = 0;
-    cudaError_t e = resident(reinterpret_cast<const void*>(&block_norm_kernel<T, TW, VEC, EPT, WARP, true>), threads, &ctas);
+    const int threads = WARP ? 32 * kRowsPerCta : TH;
+    cudaError_t e = resident(reinterpret_cast<const void*>(&block_norm_kernel<T, TW, VEC, EPT, WARP, true, TH>), threads, &ctas);
     if (e != cudaSuccess) return e;
     const int64_t units = WARP ? (static_cast<int64_t>(a.rows) + kRowsPerCta - 1) / kRowsPerCta : a.rows;
     const int64_t most = static_cast<int64_t>(ctas) * num_sms;
-    block_norm_kernel<T, TW, VEC, EPT, WARP, true><<<static_cast<unsigned>(units < most ? units : most), threads, 0, s>>>(a);
+    block_norm_kernel<T, TW, VEC, EPT, WARP, true, TH><<<static_cast<unsigned>(units < most ? units : most), threads, 0, s>>>(a);
     return cudaGetLastError();
 }
 
 template <typename T, typename TW, bool VEC>
 cudaError_t launch_short(const BlockNormArgs& a, int num_sms, cudaStream_t s) {
     if (a.cols <= 512) {
-        const int threads = 32 * kRowsPerCta;
         if (a.rows > 4 * kRowsPerCta * num_sms)
-            return a.cols <= 256 ? launch_stream<T, TW, VEC, 8, true>(a, threads, num_sms, s)
-                                 : launch_stream<T, TW, VEC, 16, true>(a, threads, num_sms, s);
+            return a.cols <= 256 ? launch_stream<T, TW, VEC, 8, true, 32>(a, num_sms, s)
+                                 : launch_stream<T, TW, VEC, 16, true, 32>(a, num_sms, s);
         const unsigned grid = (static_cast<unsigned>(a.rows) + kRowsPerCta - 1) / kRowsPerCta;
-        if (a.cols <= 256) block_norm_kernel<T, TW, VEC, 8, true, false><<<grid, threads, 0, s>>>(a);
-        else block_norm_kernel<T, TW, VEC, 16, true, false><<<grid, threads, 0, s>>>(a);
+        if (a.cols <= 256) block_norm_kernel<T, TW, VEC, 8, true, false, 32><<<grid, 32 * kRowsPerCta, 0, s>>>(a);
+        else block_norm_kernel<T, TW, VEC, 16, true, false, 32><<<grid, 32 * kRowsPerCta, 0, s>>>(a);
         return cudaGetLastError();
     }
     auto threads = [&](int ept) { return ((a.cols + ept - 1) / ept + 31) / 32 * 32; };
     if (a.cols <= 8192) {
-        if (a.rows > 2 * num_sms) return launch_stream<T, TW, VEC, 16, false>(a, threads(16), num_sms, s);
-        block_norm_kernel<T, TW, VEC, 8, false, false><<<a.rows, threads(8), 0, s>>>(a);
+        if (a.rows > 2 * num_sms) {
+            if (a.cols <= 1024) return launch_stream<T, TW, VEC, 16, false, 64>(a, num_sms, s);
+            if (a.cols <= 2048) return launch_stream<T, TW, VEC, 16, false, 128>(a, num_sms, s);
+            if (a.cols <= 4096) return launch_stream<T, TW, VEC, 16, false, 256>(a, num_sms, s);
+            return launch_stream<T, TW, VEC, 16, false, 512>(a, num_sms, s);
+        }
+        block_norm_kernel<T, TW, VEC, 8, false, false, 0><<<a.rows, threads(8), 0, s>>>(a);
     } else {
-        block_norm_kernel<T, TW, VEC, 16, false, false><<<a.rows, threads(16), 0, s>>>(a);
+        block_norm_kernel<T, TW, VEC, 16, false, false, 0><<<a.rows, threads(16), 0, s>>>(a);
     }
     return cudaGetLastError();
 }
