@@ -170,12 +170,14 @@ lib.dnnopt_stream_status.argtypes = [_P]
 
 def ptr(x) -> int | None:
     """Address of a numpy array, torch tensor, or raw integer (None -> NULL)."""
-    if x is None:
-        return None
+    if x is None or type(x) is int:
+        return x
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        pass
     if isinstance(x, int):
         return x
-    if hasattr(x, "data_ptr"):
-        return x.data_ptr()
     if hasattr(x, "ctypes"):
         return x.ctypes.data
     raise TypeError(f"cannot take the address of {type(x)!r}")
@@ -292,7 +294,12 @@ def cuda_conv3d(precision, params, inp, flt, bias, out, post_op=0, stream=None) 
 
 
 def _stream(stream):
-    return stream.cuda_stream if hasattr(stream, "cuda_stream") else ptr(stream)
+    if stream is None:
+        return None
+    try:
+        return stream.cuda_stream
+    except AttributeError:
+        return ptr(stream)
 
 
 # ---- decoder-step operators (device pointers, asynchronous on `stream`) ------
