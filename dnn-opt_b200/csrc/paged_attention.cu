@@ -158,7 +158,7 @@ struct Geo {
     static constexpr int EC = CT == DType::F32 ? 4 : (CT == DType::BF16 ? 2 : 1);
     static constexpr int HEADS = 8 * NT;                           // heads per item
     static constexpr int PITCH = DP * EC;                          // bytes of a cached row in shared memory
-    static constexpr int MT = CT == DType::E4M3 && DP <= 128 && NT == 1 ? 2 : 1;   // 16-token blocks per warp and tile
+    static constexpr int MT = CT == DType::E4M3 && DP <= 128 ? 2 : 1;   // 16-token blocks per warp and tile
     static constexpr int TOK = 16 * MT;
     static constexpr int KV = TOK * PITCH;                         // one warp's keys (or values) of a tile
     static constexpr int OUT = HEADS * DP * 4;                     // one warp's O at the end of an item
@@ -166,7 +166,7 @@ struct Geo {
     static constexpr int NW = WS >= 32768 ? 2 : 4;                 // warps
     static constexpr int TILE = NW * TOK;                          // tokens per tile
     // CTAs per SM: three where two stages fit three times and the registers (168 a thread) suffice.
-    static constexpr int CTAS = WS * NW <= 32768 && DP <= 128 && NT == 1 && !(CT == DType::E4M3) ? 3
+    static constexpr int CTAS = WS * NW <= 32768 && DP <= 128 && NT == 1 ? 3
                                 : (WS * NW <= 36 * 1024 ? 2 : 1);
     static constexpr int FIT = (CTAS == 3 ? 70 : (CTAS == 2 ? 108 : 216)) * 1024 / (WS * NW);
     static constexpr int STAGES = FIT > 4 ? 4 : FIT;
