@@ -210,6 +210,8 @@ __global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : (STREAM ? TH : 1024)
     constexpr int NB = EPT / 8;
     __shared__ float part[2][32];
     int buffer = 0;
+    pdl_wait();
+    pdl_launch_dependents();
     int64_t r = WARP ? static_cast<int64_t>(blockIdx.x) * kRowsPerCta + (threadIdx.x >> 5) : blockIdx.x;
     const int64_t step = static_cast<int64_t>(gridDim.x) * (WARP ? kRowsPerCta : 1);
     if (r >= a.rows) return;
@@ -317,6 +319,8 @@ __device__ __forceinline__ float apply(float v, int c, float mean, float rstd, c
 template <typename T, typename TW>
 __global__ void __launch_bounds__(kLongThreads) block_norm_long_kernel(const BlockNormArgs a) {
     extern __shared__ float row[];
+    pdl_wait();
+    pdl_launch_dependents();
     const int64_t r = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + r * a.ldx;
     float mean, rstd;
@@ -348,6 +352,21 @@ __global__ void __launch_bounds__(kLongThreads) block_norm_long_kernel(const Blo
     }
 }
 
+template <typename K>
+cudaError_t launch_pdl(K fn, int64_t grid, int threads, size_t smem, const BlockNormArgs& a, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, fn, a);
+}
+
 // Resident CTAs per SM, asked once per kernel, size of CTA and device.
 cudaError_t resident(const void* fn, int threads, int* ctas) {
     static std::mutex mu;
@@ -375,8 +394,7 @@ cudaError_t launch_stream(const BlockNormArgs& a, int num_sms, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     const int64_t units = WARP ? (static_cast<int64_t>(a.rows) + kRowsPerCta - 1) / kRowsPerCta : a.rows;
     const int64_t most = static_cast<int64_t>(ctas) * num_sms;
-    block_norm_kernel<T, TW, VEC, EPT, WARP, true, TH><<<static_cast<unsigned>(units < most ? units : most), threads, 0, s>>>(a);
-    return cudaGetLastError();
+    return launch_pdl(block_norm_kernel<T, TW, VEC, EPT, WARP, true, TH>, units < most ? units : most, threads, 0, a, s);
 }
 
 template <typename T, typename TW, bool VEC>
@@ -385,10 +403,9 @@ cudaError_t launch_short(const BlockNormArgs& a, int num_sms, cudaStream_t s) {
         if (a.rows > 4 * kRowsPerCta * num_sms)
             return a.cols <= 256 ? launch_stream<T, TW, VEC, 8, true, 32>(a, num_sms, s)
                                  : launch_stream<T, TW, VEC, 16, true, 32>(a, num_sms, s);
-        const unsigned grid = (static_cast<unsigned>(a.rows) + kRowsPerCta - 1) / kRowsPerCta;
-        if (a.cols <= 256) block_norm_kernel<T, TW, VEC, 8, true, false, 32><<<grid, 32 * kRowsPerCta, 0, s>>>(a);
-        else block_norm_kernel<T, TW, VEC, 16, true, false, 32><<<grid, 32 * kRowsPerCta, 0, s>>>(a);
-        return cudaGetLastError();
+        const int64_t grid = (static_cast<int64_t>(a.rows) + kRowsPerCta - 1) / kRowsPerCta;
+        return a.cols <= 256 ? launch_pdl(block_norm_kernel<T, TW, VEC, 8, true, false, 32>, grid, 32 * kRowsPerCta, 0, a, s)
+                             : launch_pdl(block_norm_kernel<T, TW, VEC, 16, true, false, 32>, grid, 32 * kRowsPerCta, 0, a, s);
     }
     auto threads = [&](int ept) { return ((a.cols + ept - 1) / ept + 31) / 32 * 32; };
     if (a.cols <= 8192) {
@@ -398,11 +415,9 @@ cudaError_t launch_short(const BlockNormArgs& a, int num_sms, cudaStream_t s) {
             if (a.cols <= 4096) return launch_stream<T, TW, VEC, 16, false, 256>(a, num_sms, s);
             return launch_stream<T, TW, VEC, 16, false, 512>(a, num_sms, s);
         }
-        block_norm_kernel<T, TW, VEC, 8, false, false, 0><<<a.rows, threads(8), 0, s>>>(a);
-    } else {
-        block_norm_kernel<T, TW, VEC, 16, false, false, 0><<<a.rows, threads(16), 0, s>>>(a);
+        return launch_pdl(block_norm_kernel<T, TW, VEC, 8, false, false, 0>, a.rows, threads(8), 0, a, s);
     }
-    return cudaGetLastError();
+    return launch_pdl(block_norm_kernel<T, TW, VEC, 16, false, false, 0>, a.rows, threads(16), 0, a, s);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -413,8 +428,7 @@ cudaError_t launch(const BlockNormArgs& a, int num_sms, cudaStream_t s) {
         const void* fn = reinterpret_cast<const void*>(&block_norm_long_kernel<T, TW>);
         cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kBlockNormMaxCols * 4);
         if (e != cudaSuccess) return e;
-        block_norm_long_kernel<T, TW><<<a.rows, kLongThreads, static_cast<size_t>(a.cols) * 4, s>>>(a);
-        return cudaGetLastError();
+        return launch_pdl(block_norm_long_kernel<T, TW>, a.rows, kLongThreads, static_cast<size_t>(a.cols) * 4, a, s);
     }
     bool vec = true;
     for (const void* p : {a.x, a.y, a.gate, a.post_w, a.post_b, a.pre_w, a.pre_b, static_cast<const void*>(a.h),

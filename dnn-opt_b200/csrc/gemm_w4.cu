@@ -269,7 +269,8 @@ __device__ __forceinline__ void stage(const Params& p, const Image& img, int m0,
 // takes longer than reading them back: a half-warp per 128 activations.
 template <DType IO, int MI, int F>
 __global__ void __launch_bounds__(128) gemm_w4_digits_kernel(const Params p) {
-    pdl_launch_dependents();
+    pdl_wait();
+    pdl_launch_dependents();    // what runs next finds everything older than this kernel done
     using T = typename std::conditional<IO == DType::F32, float, __nv_bfloat16>::type;
     constexpr int D = IO == DType::F32 ? 4 : 3, ROWS = MI == 0 ? 8 / D : 8 * MI;
     const W4Args& g = p.g;
@@ -321,6 +322,8 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     const bool zeros = g.zero != nullptr;
     const bool f32s = g.st == DType::F32;
 
+    if (!p.images) pdl_wait();
+    pdl_launch_dependents();
     const Shares shares(p.tiles * nq, gridDim.x * kTeams);
     const uint32_t share = team * gridDim.x + blockIdx.x;
     const bool busy = share < shares.n;
@@ -704,6 +707,20 @@ bool aligned_rows(const W4Args& g) { return g.ldw % 16 == 0 && reinterpret_cast<
 
 int64_t row_bytes_of(const W4Args& g) { return (static_cast<int64_t>(g.K) + 1) / 2; }
 
+cudaError_t launch_pdl(const void* fn, dim3 grid, int threads, void** args, int smem, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelExC(&cfg, fn, args);
+}
+
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -826,23 +843,13 @@ cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint3
         p.images = static_cast<unsigned char*>(extra) + plan.copy_bytes;
         const unsigned stretches = static_cast<unsigned>(plan.rows) * plan.split_steps * 2;
         void* first[] = {&p};
-        e = cudaLaunchKernel(k.digits, dim3((stretches + 7) / 8, plan.splits, plan.blocks), dim3(128), first, 0, s);
+        e = launch_pdl(k.digits, dim3((stretches + 7) / 8, plan.splits, plan.blocks), 128, first, 0, s);
         if (e != cudaSuccess) return e;
     }
-    // The kernel may start before the one that makes the digits is done: all that it reads or writes
-    // until it waits for that one is older, or its own.
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(plan.ctas, plan.splits, plan.blocks);
-    cfg.blockDim = dim3(kTeams * kTeamThreads);
-    cfg.dynamicSmemBytes = static_cast<size_t>(plan.smem);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = plan.prepared ? 1 : 0;
+    // With digits made before it, the kernel starts before they are done: all that it reads or writes
+    // until it waits for them is older than the kernel that makes them, or its own.
     void* args[] = {&p, &map};
-    return cudaLaunchKernelExC(&cfg, k.fn, args);
+    return launch_pdl(k.fn, dim3(plan.ctas, plan.splits, plan.blocks), kTeams * kTeamThreads, args, plan.smem, s);
 }
 
 }  // namespace dnnopt_b200

@@ -281,6 +281,8 @@ __global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTA
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     const int items = a.kv_heads * p.hblocks;
     const int dim = a.dim;
+    pdl_wait();
+    pdl_launch_dependents();
 
     // --- all tiles in (sequence, item, tile) order; a thread (a lane, for up to 32 sequences) knows
     // the tiles of its own sequences and of those before them
@@ -350,30 +352,36 @@ __global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTA
     uint32_t item0 = lo - cons.t;       // first tile of the current item
     Cursor prod = cons;
 
-    // --- producer: one warp's tokens of one tile, the page numbers one tile ahead
+    // --- producer: one warp's tokens of one tile
     constexpr int LPR = G::PITCH / 16 < 8 ? G::PITCH / 16 : 8;      // lanes per row
     constexpr int RPP = 32 / LPR;                                   // rows per pass
     const int nch = dim * G::EC / 16, lrow = lane / LPR, lch = lane % LPR;
-    int ent = -1, slot = 0;
-    bool want = false, fresh = false;
-    auto look = [&]() {
-        const int pos = prod.first + prod.t * TILE + warp * TOK + (lane & (TOK - 1));
-        want = pos < prod.len;
-        const int pg = a.page_size == 1 ? pos : static_cast<int>(__umulhi(pos, p.page_mul) >> p.page_shift);
-        slot = pos - pg * a.page_size;
-        ent = want ? __ldg(a.table + prod.b * a.table_stride + pg) : -1;
-        fresh = a.k_new != nullptr && pos == prod.len - 1;
+    struct Ask {            // where a tile's row `lane` is, asked two tiles ahead of its loads
+        int ent, slot, b, r;
+        bool want, fresh;
     };
-    auto issue = [&](int stage) {
-        const bool ok = want && ent >= 0 && ent < a.num_pages;
-        if (want && !ok) record_kernel_error(a.err, kKerrBadIndex);
+    auto look = [&]() {
+        Ask k;
+        const int pos = prod.first + prod.t * TILE + warp * TOK + (lane & (TOK - 1));
+        k.want = pos < prod.len;
+        const int pg = a.page_size == 1 ? pos : static_cast<int>(__umulhi(pos, p.page_mul) >> p.page_shift);
+        k.slot = pos - pg * a.page_size;
+        k.ent = k.want ? __ldg(a.table + prod.b * a.table_stride + pg) : -1;
+        k.fresh = a.k_new != nullptr && pos == prod.len - 1;
+        k.b = prod.b;
+        k.r = prod.r;
+        return k;
+    };
+    auto issue = [&](int stage, const Ask& k) {
+        const bool ok = k.want && k.ent >= 0 && k.ent < a.num_pages;
+        if (k.want && !ok) record_kernel_error(a.err, kKerrBadIndex);
         uint32_t valid = __ballot_sync(0xFFFFFFFFu, ok);
-        const uint32_t real = __ballot_sync(0xFFFFFFFFu, ok && !fresh);
+        const uint32_t real = __ballot_sync(0xFFFFFFFFu, ok && !k.fresh);
         if constexpr (TOK < 32) valid &= 0xFFFFu;
         if (lane == 0) s_mask[stage * NW + warp] = valid;
         if (valid) {
-            const int kvh = p.hblocks == 1 ? prod.r : prod.r / p.hblocks;
-            const long long off = ok ? (ent * a.page_stride + slot * a.token_stride + kvh * a.head_stride) * G::EC : 0;
+            const int kvh = p.hblocks == 1 ? k.r : k.r / p.hblocks;
+            const long long off = ok ? (k.ent * a.page_stride + k.slot * a.token_stride + kvh * a.head_stride) * G::EC : 0;
             const uint32_t base = smem_u32(ring + (stage * NW + warp) * G::WS) + lrow * G::PITCH;
 #pragma unroll
             for (int i = 0; i < TOK / RPP; ++i) {
@@ -396,7 +404,7 @@ __global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTA
                 if (valid & ~real) {
                     // The new token's row, from its own tensors.
                     const int row = __ffs(valid & ~real) - 1;
-                    const int64_t from = prod.b * a.new_batch + kvh * a.new_head;
+                    const int64_t from = k.b * a.new_batch + kvh * a.new_head;
                     const uint32_t dst = smem_u32(ring + (stage * NW + warp) * G::WS);
                     const char* kn = reinterpret_cast<const char*>(static_cast<const typename I::S*>(a.k_new) + from);
                     const char* vn = reinterpret_cast<const char*>(static_cast<const typename I::S*>(a.v_new) + from);
@@ -410,16 +418,27 @@ __global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTA
         }
     };
     const int count = static_cast<int>(hi - lo);
-    int issued = 0;
-    look();
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
+    int issued = 0, asked = 0;
+    Ask near_ask = {}, far_ask = {};
+    auto ask = [&]() {
+        near_ask = far_ask;
+        if (asked < count) {
+            far_ask = look();
+            if (++asked < count) prod.next(p, items, TILE);
+        }
+    };
+    auto request = [&](int stage) {     // the next tile's loads, into a stage that the warp is done with
         if (issued < count) {
-            issue(s);
-            if (++issued < count) { prod.next(p, items, TILE); look(); }
+            issue(stage, near_ask);
+            ++issued;
+            ask();
         }
         cp_async_commit();
-    }
+    };
+    ask();
+    ask();
+#pragma unroll
+    for (int s = 0; s < S; ++s) request(s);
 
     // Lane (g, t) holds heads 2t and 2t + 1 of each block of eight, and of the queries head g.
     float acc[KSTEPS][NT][4], m[NT][2], l[NT][2], rowscale[NT][2];
@@ -933,11 +952,7 @@ __global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTA
         }
         // The stage is free: every stage's loads but this one's are under way while the next is awaited.
         __syncwarp();
-        if (issued < count) {
-            issue(stage);
-            if (++issued < count) { prod.next(p, items, TILE); look(); }
-        }
-        cp_async_commit();
+        request(stage);
         stage = stage + 1 == S ? 0 : stage + 1;
     }
     cp_async_wait<0>();
@@ -1115,7 +1130,17 @@ cudaError_t launch_paged_attention(const PagedAttnArgs& a, const PagedAttnPlan& 
     p.page_mul = static_cast<uint32_t>(((uint64_t(1) << (31 + log)) + a.page_size - 1) / a.page_size);
     p.page_shift = log > 0 ? log - 1 : 0;
     void* args[] = {&p};
-    return cudaLaunchKernel(k.fn, dim3(plan.ctas), dim3(k.threads), args, static_cast<size_t>(k.smem), s);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(plan.ctas);
+    cfg.blockDim = dim3(k.threads);
+    cfg.dynamicSmemBytes = static_cast<size_t>(k.smem);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelExC(&cfg, k.fn, args);
 }
 
 }  // namespace dnnopt_b200
