@@ -23,10 +23,10 @@
 // Activations that are infinite or NaN stay out of the products and are added
 // for their own row at the end.
 //
-// Work.  256 weights of 16 rows (2 KB) are a step, two TMA boxes into the ring of the
+// Work.  128 weights of 32 rows (2 KB) are a step, a TMA box into the ring of the
 // warp that works on it (16-byte cp.async of the same rows cost 23 shared-memory
 // cycles an instruction and held the kernel at 1.6 TB/s).  All steps, tile after
-// tile of 16 rows, are cut into equal shares, one for each team of four warps, four
+// tile of 32 rows, are cut into equal shares, one for each team of four warps, four
 // teams to an SM; a team's warps take the steps of a tile in turn and add up
 // in shared memory.  A tile cut by a share's end, or by the ends of a K-range, is
 // finished by the last of its shares to arrive, adding the parts in order.  The
@@ -50,15 +50,15 @@ constexpr int kTeamThreads = 128;
 constexpr int kWarps = 4;           // per team
 constexpr int kMaxSlots = 4;        // steps under way per warp, where the activations leave room
 constexpr int kMinSlots = 2;
-constexpr int kStepK = 256;
-constexpr int kStepBytes = 2048;
-constexpr int kBoxBytes = 1024;     // 128 weights of 16 rows
+constexpr int kStepK = 128;
+constexpr int kRows = 32;           // of W in a tile: two blocks of 16
+constexpr int kStepBytes = kRows * kStepK / 2;
 constexpr int kMaxSmem = 227 * 1024;
 
 struct Params {
     W4Args g;
-    int tiles;                      // of 16 rows of W
-    int steps;                      // ceil(K / 256)
+    int tiles;                      // of 32 rows of W
+    int steps;                      // ceil(K / 128)
     int split_steps;                // steps of one K-range (gridDim.y of them)
     int slots;                      // of a warp's ring
     int rows, cols;                 // rows of A at a time, and columns: a digit of each
@@ -92,13 +92,16 @@ __device__ __forceinline__ uint32_t ldg_scale(const char* p, bool f32) {
 constexpr float kMagic = 12582912.0f;           // 1.5 * 2^23: whole numbers below 2^22 added to it keep their bits
 constexpr uint32_t kMagicBits = 0x4B400000u;
 
-// Equal shares of `total` steps but for one step, at least one step for each
-// warp of a team: the first `more` shares have one more than the others.
+// Equal shares of all steps but for one step, at least one step for each warp
+// of a team: the first `more` shares have one more than the others.  Where every
+// tile finds a team of its own and has at most four steps for each of its warps,
+// the shares are the tiles: adding up parts would take longer than two steps.
 struct Shares {
     uint32_t n, each, more;
 
-    __device__ Shares(uint32_t steps, uint32_t most) : n(steps / kWarps) {
-        if (n > most) n = most;
+    __device__ Shares(uint32_t tiles, uint32_t per_tile, uint32_t most) {
+        const uint32_t steps = tiles * per_tile;
+        n = tiles <= most && per_tile <= 4 * kWarps ? tiles : min(steps / kWarps, most);
         if (n < 1) n = 1;
         each = steps / n;
         more = steps - each * n;
@@ -136,26 +139,26 @@ struct Cursor {
 
 // The activations of a K-range as the products read them.
 struct Image {
-    unsigned char* act;     // [128][2][col][t] 16 bytes: the digits of two words' activations
-    float* unit;            // [128][tcol]: what 1 stands for; negative where an infinity or NaN was left out
-    uint32_t* base;         // [128][flush][col]: -8 times the sum of the digits, as the bits of an FP32 number
-    float* isum;            // [128][flush][tcol]: the sum of the whole numbers (packed: of the digits)
+    unsigned char* act;     // [step][2][col][t] 16 bytes: the digits of two words' activations
+    float* unit;            // [step][tcol]: what 1 stands for; negative where an infinity or NaN was left out
+    uint32_t* base;         // [step][flush][col]: -8 times the sum of the digits, as the bits of an FP32 number
+    float* isum;            // [step][flush][tcol]: the sum of the whole numbers (packed: of the digits)
 
     __device__ Image(unsigned char* at, uint32_t steps, int cols, int tcols, int f) : act(at) {
-        unit = reinterpret_cast<float*>(act + static_cast<size_t>(steps) * cols * 256);
-        base = reinterpret_cast<uint32_t*>(unit + steps * 2 * tcols);
-        isum = reinterpret_cast<float*>(base + steps * 2 * (4 / f) * cols);
+        unit = reinterpret_cast<float*>(act + static_cast<size_t>(steps) * cols * 128);
+        base = reinterpret_cast<uint32_t*>(unit + steps * tcols);
+        isum = reinterpret_cast<float*>(base + steps * (4 / f) * cols);
     }
 };
 
 // 128 activations of row m0 + m, eight (a word's worth) to each lane of half a
 // warp: r is the lane's place, q the stretch within the K-range, `in` false for
 // a half that has nothing to do.  The whole warp takes part.
-template <DType IO, int MI, int F>
+template <DType IO, bool PACKED, int F>
 __device__ __forceinline__ void stage(const Params& p, const Image& img, int m0, int k_step0, uint32_t m, uint32_t q, uint32_t r,
                                       bool vec, bool in) {
     using T = typename std::conditional<IO == DType::F32, float, __nv_bfloat16>::type;
-    constexpr bool PARTS = IO == DType::F32, PACKED = MI == 0;
+    constexpr bool PARTS = IO == DType::F32;
     constexpr int D = PARTS ? 4 : 3, BITS = PARTS ? 30 : 22;
     const W4Args& g = p.g;
     const int tcols = PACKED ? p.cols : p.rows;
@@ -267,37 +270,37 @@ __device__ __forceinline__ void stage(const Params& p, const Image& img, int m0,
 
 // Images of all K-ranges and blocks of rows, where making them in every CTA
 // takes longer than reading them back: a half-warp per 128 activations.
-template <DType IO, int MI, int F>
+template <DType IO, bool PACKED, int F>
 __global__ void __launch_bounds__(128) gemm_w4_digits_kernel(const Params p) {
     pdl_wait();
     pdl_launch_dependents();    // what runs next finds everything older than this kernel done
     using T = typename std::conditional<IO == DType::F32, float, __nv_bfloat16>::type;
-    constexpr int D = IO == DType::F32 ? 4 : 3, ROWS = MI == 0 ? 8 / D : 8 * MI;
+    constexpr int D = IO == DType::F32 ? 4 : 3, ROWS = PACKED ? 8 / D : 8;
     const W4Args& g = p.g;
     const int m0 = blockIdx.z * ROWS, mt = g.M - m0 < ROWS ? g.M - m0 : ROWS;
     const int k_step0 = blockIdx.y * p.split_steps;
     const uint32_t nq = p.steps - k_step0 < p.split_steps ? p.steps - k_step0 : p.split_steps;
     const Image img(p.images + (static_cast<size_t>(blockIdx.z) * gridDim.y + blockIdx.y) * p.image_bytes, p.split_steps, p.cols,
-                    MI == 0 ? p.cols : p.rows, F);
+                    PACKED ? p.cols : p.rows, F);
     const bool vec = g.lda % (16 / sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(g.A) % 16 == 0;
-    const uint32_t u = blockIdx.x * 8 + (threadIdx.x >> 4), m = u / (nq * 2), q = u - m * nq * 2;
-    stage<IO, MI, F>(p, img, m0, k_step0, m, q, threadIdx.x & 15, vec, u < mt * nq * 2);
+    const uint32_t u = blockIdx.x * 8 + (threadIdx.x >> 4), m = u / nq, q = u - m * nq;
+    stage<IO, PACKED, F>(p, img, m0, k_step0, m, q, threadIdx.x & 15, vec, u < mt * nq);
 }
 
-// D digits of an activation: three of bf16, four of FP32.  MI = 0: the digits of
-// up to 8 / D rows of A share one block of eight columns; else MI blocks of
-// eight rows for each digit.  F: chunks of 32 weights that share their scales
+// D digits of an activation: three of bf16, four of FP32.  PACKED: the digits of
+// up to 8 / D rows of A share one block of eight columns; else each digit has a
+// block for up to eight rows.  (16 rows at once took longer than eight twice: 105
+// against 86 us for 16x28672x8192, their sums spill.)  F: chunks of 32 weights that share their scales
 // for sure (4, 2 or 1); sums are scaled every F chunks.
-template <DType IO, int MI, int F>
+template <DType IO, bool PACKED, int F>
 __global__ void __launch_bounds__(kTeams * kTeamThreads, 1)
 gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     using T = typename std::conditional<IO == DType::F32, float, __nv_bfloat16>::type;
-    constexpr bool PARTS = IO == DType::F32, PACKED = MI == 0;
+    constexpr bool PARTS = IO == DType::F32;
     constexpr int D = PARTS ? 4 : 3;
-    constexpr int NT = PACKED ? 1 : D * MI;                 // blocks of eight columns
-    constexpr int NB = PACKED ? 1 : MI;                     // blocks of sums, after the digits are put together
-    constexpr int ROWS = PACKED ? 8 / D : 8 * MI;           // rows of A per pass
-    constexpr int RED = NB * 128;                           // floats of a warp's sums of a tile
+    constexpr int NT = PACKED ? 1 : D;              // blocks of eight columns
+    constexpr int ROWS = PACKED ? 8 / D : 8;        // rows of A per pass
+    constexpr int RED = 256;                        // floats of a warp's sums of a tile
     extern __shared__ __align__(128) unsigned char smem[];
     const W4Args& g = p.g;
     const int tid = threadIdx.x, lane = tid & 31, team = tid / kTeamThreads, tt = tid % kTeamThreads, warp = tt >> 5;
@@ -314,7 +317,7 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     float* const unit = img.unit;
     uint32_t* const base = img.base;
     float* const isum = img.isum;
-    float* red = reinterpret_cast<float*>(act + p.image_bytes) + team * 2 * kWarps * RED;    // [2][warp][4 NB][lane]
+    float* red = reinterpret_cast<float*>(act + p.image_bytes) + team * kWarps * RED;        // [warp][block of 16][4][lane]
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + p.bars_at);
     uint64_t* image_bar = bars + kTeams * kWarps * kMaxSlots;
     uint32_t* odd = reinterpret_cast<uint32_t*>(image_bar + 1);                 // rows of A with an infinity or NaN
@@ -324,12 +327,12 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
 
     if (!p.images) pdl_wait();
     pdl_launch_dependents();
-    const Shares shares(p.tiles * nq, gridDim.x * kTeams);
+    const Shares shares(p.tiles, nq, gridDim.x * kTeams);
     const uint32_t share = team * gridDim.x + blockIdx.x;
     const bool busy = share < shares.n;
     const uint32_t lo = busy ? shares.start(share) : 0, hi = busy ? shares.start(share + 1) : 0;
 
-    // --- producer: one step's weights, lane (g, t) two rows of the tile and 32 weights of each
+    // --- producer: one step's weights, lane (g, t) four rows of the tile and 32 weights of each
     if (lane == 0)
         for (int i = 0; i < p.slots; ++i) mbar_init(bars + i, 1);
     if (tid == 0) {
@@ -342,11 +345,9 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     auto request = [&](int slot) {      // the warp's next step, into a slot that it is done with
         if (prod.q < prod.end) {
             if (lane == 0) {
-                const int x = static_cast<int>((k_step0 + prod.q) * (kStepK / 2)), y = static_cast<int>(prod.tile * 16);
-                unsigned char* dst = ring + slot * kStepBytes;
                 mbar_arrive_expect_tx(bars + slot, kStepBytes);
-                tma_load_2d(dst, &map, bars + slot, x, y);
-                tma_load_2d(dst + kBoxBytes, &map, bars + slot, x + 64, y);
+                tma_load_2d(ring + slot * kStepBytes, &map, bars + slot, static_cast<int>((k_step0 + prod.q) * (kStepK / 2)),
+                            static_cast<int>(prod.tile * kRows));
             }
             prod.q += kWarps;
             if (prod.q >= prod.end) prod.settle(nq, warp);
@@ -367,19 +368,19 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
         mbar_wait(image_bar, 0, nullptr, p.err);
     } else {
         const bool vec = g.lda % (16 / sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(g.A) % 16 == 0;
-        const uint32_t nh = nq * 2, units = mt * nh, r = tid & 15;
-        uint32_t u = tid >> 4, m = u / nh, q = u - m * nh;       // q: stretch of 128
-        const uint32_t dm = (kTeams * kTeamThreads / 16) / nh, dq = (kTeams * kTeamThreads / 16) - dm * nh;
+        const uint32_t units = mt * nq, r = tid & 15;
+        uint32_t u = tid >> 4, m = u / nq, q = u - m * nq;
+        const uint32_t dm = (kTeams * kTeamThreads / 16) / nq, dq = (kTeams * kTeamThreads / 16) - dm * nq;
         for (uint32_t u0 = u & ~1u; u0 < units; u0 += kTeams * kTeamThreads / 16) {     // the same count for a whole warp
-            stage<IO, MI, F>(p, img, m0, k_step0, m, q, r, vec, u < units);
+            stage<IO, PACKED, F>(p, img, m0, k_step0, m, q, r, vec, u < units);
             u += kTeams * kTeamThreads / 16;
             m += dm;
             q += dq;
-            if (q >= nh) { q -= nh; ++m; }
+            if (q >= nq) { q -= nq; ++m; }
         }
         __syncthreads();
     }
-    for (uint32_t i = tid; i < mt * nq * 2; i += kTeams * kTeamThreads) {
+    for (uint32_t i = tid; i < mt * nq; i += kTeams * kTeamThreads) {
         const uint32_t q = i / mt, m = i - q * mt;
         if (unit[q * tcols + m] < 0.0f) atomicOr(odd, 1u << m);
     }
@@ -398,47 +399,41 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     const int64_t to_zero = reinterpret_cast<intptr_t>(g.zero) - reinterpret_cast<intptr_t>(g.scale);
     // The slots of K-range y.
     auto range_slots = [&](uint32_t y) {
-        return p.ws + (static_cast<size_t>(blockIdx.z) * gridDim.y + y) * (p.tiles + gridDim.x * kTeams) * (16 * ROWS);
+        return p.ws + (static_cast<size_t>(blockIdx.z) * gridDim.y + y) * (p.tiles + gridDim.x * kTeams) * (kRows * ROWS);
     };
 
     // The lane's operand columns (those that are not there repeat the last) and its columns in the tables.
     const unsigned char* act_at[NT];
-    uint32_t base_at[NT][2], tab[NB][2];
+    uint32_t base_at[NT][2], tab[2];
     const uint32_t ring_at = smem_u32(ring) + lane * 16, act_half = p.cols * 64;
 #pragma unroll
     for (int b = 0; b < NT; ++b) {
-        const int col = PACKED ? min(gr, p.cols - 1) : (b % D) * p.rows + min(8 * (b / D) + gr, mt - 1);
+        const int col = PACKED ? min(gr, p.cols - 1) : b * p.rows + min(gr, mt - 1);
         act_at[b] = act + col * 64 + t4 * 16;
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-            base_at[b][e] = PACKED ? min(2 * t4 + e, p.cols - 1) : (b % D) * p.rows + min(8 * (b / D) + 2 * t4 + e, mt - 1);
+            base_at[b][e] = PACKED ? min(2 * t4 + e, p.cols - 1) : b * p.rows + min(2 * t4 + e, mt - 1);
     }
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) tab[b][e] = min(8 * b + 2 * t4 + e, tcols - 1);
+    for (int e = 0; e < 2; ++e) tab[e] = min(2 * t4 + e, tcols - 1);
     // Scales are read one step ahead of their products, across the ends of tiles.
     Cursor ahead(lo, hi, nq, warp);
-    const char* srow[2];    // the lane's two rows' first scales
-    uint32_t raw[2][2] = {}, rawz[2][2] = {};       // [half][row]
+    const char* srow[4];    // the lane's four rows' first scales
+    uint32_t raw[4] = {}, rawz[4] = {};
     auto open = [&](uint32_t t) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int64_t row = static_cast<int64_t>(t) * 16 + gr + 8 * h;
+        for (int h = 0; h < 4; ++h) {
+            const int64_t row = static_cast<int64_t>(t) * kRows + gr + 8 * h;
             srow[h] = static_cast<const char*>(g.scale) + (row < g.N ? row : g.N - 1) * g.lds * scale_bytes;
         }
     };
     auto fetch_scales = [&]() {
         if (ahead.q >= ahead.end) return;
+        const int64_t gi = static_cast<int64_t>(group_of((k_step0 + ahead.q) * 4 + t4)) * scale_bytes;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int gi = group_of((k_step0 + ahead.q) * 8 + half * 4 + t4);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const char* at = srow[h] + static_cast<int64_t>(gi) * scale_bytes;
-                raw[half][h] = ldg_scale(at, f32s);
-                if (zeros) rawz[half][h] = ldg_scale(at + to_zero, f32s);
-            }
+        for (int h = 0; h < 4; ++h) {
+            raw[h] = ldg_scale(srow[h] + gi, f32s);
+            if (zeros) rawz[h] = ldg_scale(srow[h] + gi + to_zero, f32s);
         }
         ahead.q += kWarps;
         if (ahead.q >= ahead.end && ahead.left > 0) {
@@ -450,87 +445,92 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     fetch_scales();
 
     uint32_t tile = lo / nq, q0 = lo - tile * nq, done = lo;
-    uint32_t phase = 0, buffer = 0;
+    uint32_t phase = 0;
     int slot = 0;
     bool dead = false;
     while (done < hi) {
         const uint32_t n = hi - done < nq - q0 ? hi - done : nq - q0, q1 = q0 + n;
-        float tot[NB][4] = {};
+        float tot[2][4] = {};       // [block of 16 rows]
         for (uint32_t q = q0 + warp; q < q1; q += kWarps) {
-            float sc[2][2], zr[2][2];
+            float sc[4], zr[4];
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    sc[half][h] = value(raw[half][h]);
-                    zr[half][h] = 8.0f - (zeros ? value(rawz[half][h]) : 8.0f);
-                }
+            for (int h = 0; h < 4; ++h) {
+                sc[h] = value(raw[h]);
+                zr[h] = 8.0f - (zeros ? value(rawz[h]) : 8.0f);
+            }
             fetch_scales();
             if (!mbar_try_wait(bars + slot, phase) && !dead) dead = !mbar_wait(bars + slot, phase, nullptr, p.err);
-            uint32_t w[2][2][4];        // [half][row][word]
+            uint32_t w[4][4];           // [row][word]
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint4 v = lds128(ring_at + slot * kStepBytes + half * kBoxBytes + h * 512);
-                    w[half][h][0] = v.x; w[half][h][1] = v.y; w[half][h][2] = v.z; w[half][h][3] = v.w;
-                }
+            for (int h = 0; h < 4; ++h) {
+                const uint4 v = lds128(ring_at + slot * kStepBytes + h * 512);
+                w[h][0] = v.x; w[h][1] = v.y; w[h][2] = v.z; w[h][3] = v.w;
+            }
             __syncwarp();
             request(slot);      // every lane has read it
             if (++slot == p.slots) { slot = 0; phase ^= 1u; }
 
+            // A product takes a word from each lane of a quad.  Lane t holds the four words of chunk t:
+            // scales shared by fewer chunks want the words of one chunk (or two) on all four lanes.
+            if constexpr (F <= 2) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const uint32_t qh = q * 2 + half;
-                uint32_t (&wh)[2][4] = w[half];
-                // A product takes a word from each lane of a quad.  Lane t holds the four words of chunk t:
-                // scales shared by fewer chunks want the words of one chunk (or two) on all four lanes.
-                if constexpr (F <= 2) {
+                for (int h = 0; h < 4; ++h)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                    for (int i = 0; i < 2; ++i) {       // words 2, 3 of lanes 0, 1 for words 0, 1 of lanes 2, 3
+                        const uint32_t give = (t4 & 2) ? w[h][i] : w[h][i + 2];
+                        const uint32_t have = __shfl_xor_sync(0xFFFFFFFFu, give, 2);
+                        if (t4 & 2) w[h][i] = have; else w[h][i + 2] = have;
+                    }
+            }
+            if constexpr (F == 1) {
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {       // words 2, 3 of lanes 0, 1 for words 0, 1 of lanes 2, 3
-                            const uint32_t give = (t4 & 2) ? wh[h][i] : wh[h][i + 2];
-                            const uint32_t have = __shfl_xor_sync(0xFFFFFFFFu, give, 2);
-                            if (t4 & 2) wh[h][i] = have; else wh[h][i + 2] = have;
+                for (int h = 0; h < 4; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; i += 2) {    // odd words of even lanes for even words of odd lanes
+                        const uint32_t give = (t4 & 1) ? w[h][i] : w[h][i + 1];
+                        const uint32_t have = __shfl_xor_sync(0xFFFFFFFFu, give, 1);
+                        if (t4 & 1) w[h][i] = have; else w[h][i + 1] = have;
+                    }
+            }
+            float un[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) un[e] = fabsf(unit[q * tcols + tab[e]]);
+            uint4 x[NT];        // the operand columns of two words
+            uint32_t c[2][NT][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (i % F == 0) {
+#pragma unroll
+                    for (int b = 0; b < NT; ++b)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const uint32_t from = base[(q * (4 / F) + i / F) * p.cols + base_at[b][e]];
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) c[k][b][e] = c[k][b][e + 2] = from;
                         }
                 }
-                if constexpr (F == 1) {
+                if (i % 2 == 0) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int i = 0; i < 4; i += 2) {    // odd words of even lanes for even words of odd lanes
-                            const uint32_t give = (t4 & 1) ? wh[h][i] : wh[h][i + 1];
-                            const uint32_t have = __shfl_xor_sync(0xFFFFFFFFu, give, 1);
-                            if (t4 & 1) wh[h][i] = have; else wh[h][i + 1] = have;
-                        }
+                    for (int b = 0; b < NT; ++b) x[b] = *reinterpret_cast<const uint4*>(act_at[b] + (q * 2 + i / 2) * act_half);
                 }
-                float un[NB][2];
 #pragma unroll
-                for (int b = 0; b < NB; ++b)
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t (&w0)[4] = w[2 * k], (&w1)[4] = w[2 * k + 1];
+                    const uint32_t av[4] = {w0[i] & 0x0F0F0F0Fu, w1[i] & 0x0F0F0F0Fu, (w0[i] >> 4) & 0x0F0F0F0Fu,
+                                            (w1[i] >> 4) & 0x0F0F0F0Fu};
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) un[b][e] = fabsf(unit[qh * tcols + tab[b][e]]);
-                uint4 x[NT];        // the operand columns of two words
-                uint32_t c[NT][4];
+                    for (int b = 0; b < NT; ++b) mma_u8s8(c[k][b], av, i % 2 ? x[b].z : x[b].x, i % 2 ? x[b].w : x[b].y);
+                }
+                if ((i + 1) % F != 0) continue;
+                const int f = i / F;
+                float is[2] = {};
+                if (zeros) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (i % F == 0) {
+                    for (int e = 0; e < 2; ++e) is[e] = isum[(q * (4 / F) + f) * tcols + tab[e]];
+                }
 #pragma unroll
-                        for (int b = 0; b < NT; ++b) {
-                            c[b][0] = c[b][2] = base[(qh * (4 / F) + i / F) * p.cols + base_at[b][0]];
-                            c[b][1] = c[b][3] = base[(qh * (4 / F) + i / F) * p.cols + base_at[b][1]];
-                        }
-                    }
-                    const uint32_t av[4] = {wh[0][i] & 0x0F0F0F0Fu, wh[1][i] & 0x0F0F0F0Fu, (wh[0][i] >> 4) & 0x0F0F0F0Fu,
-                                            (wh[1][i] >> 4) & 0x0F0F0F0Fu};
-#pragma unroll
-                    for (int b = 0; b < NT; ++b) {
-                        if (i % 2 == 0) x[b] = *reinterpret_cast<const uint4*>(act_at[b] + (qh * 2 + i / 2) * act_half);
-                        mma_u8s8(c[b], av, i % 2 ? x[b].z : x[b].x, i % 2 ? x[b].w : x[b].y);
-                    }
-                    if ((i + 1) % F != 0) continue;
-                    const int f = i / F;
-                    float s0 = sc[half][0], s1 = sc[half][1], z0 = zr[half][0], z1 = zr[half][1];
+                for (int k = 0; k < 2; ++k) {
+                    float s0 = sc[2 * k], s1 = sc[2 * k + 1], z0 = zr[2 * k], z1 = zr[2 * k + 1];
                     if constexpr (F < 4) {
                         const int from = (lane & 28) | (f * F);
                         s0 = __shfl_sync(0xFFFFFFFFu, s0, from);
@@ -541,46 +541,35 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
                         }
                     }
 #pragma unroll
-                    for (int b = 0; b < NB; ++b)
+                    for (int e = 0; e < 4; ++e) {
+                        float y = __uint_as_float(c[k][NT - 1][e]) - kMagic;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float y;
-                            if constexpr (PACKED) {
-                                y = __uint_as_float(c[0][e]) - kMagic;
-                            } else {
-                                y = __uint_as_float(c[b * D + D - 1][e]) - kMagic;
-#pragma unroll
-                                for (int d = D - 2; d >= 0; --d) y = fmaf(y, 256.0f, __uint_as_float(c[b * D + d][e]) - kMagic);
-                            }
-                            if (zeros) y = fmaf(e < 2 ? z0 : z1, isum[(qh * (4 / F) + f) * tcols + tab[b][e & 1]], y);
-                            tot[b][e] = fmaf((e < 2 ? s0 : s1) * un[b][e & 1], y, tot[b][e]);
-                        }
+                        for (int d = NT - 2; d >= 0; --d) y = fmaf(y, 256.0f, __uint_as_float(c[k][d][e]) - kMagic);
+                        if (zeros) y = fmaf(e < 2 ? z0 : z1, is[e & 1], y);
+                        tot[k][e] = fmaf((e < 2 ? s0 : s1) * un[e & 1], y, tot[k][e]);
+                    }
                 }
             }
         }
 
-        // --- the tile's end in this share: add up the warps.  Two buffers in turn: whoever writes one
-        // again has passed the barrier that follows its last reading.
-        float* sums = red + buffer * kWarps * RED;
-        buffer ^= 1u;
+        // --- the tile's end in this share: add up the warps
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sums[(warp * NB * 4 + b * 4 + e) * 32 + lane] = tot[b][e];
+            for (int e = 0; e < 4; ++e) red[((warp * 2 + k) * 4 + e) * 32 + lane] = tot[k][e];
         sync();
         const bool whole = n == nq && gridDim.y == 1;
-        float* part_sums = whole ? nullptr : range_slots(blockIdx.y) + static_cast<size_t>(lo <= tile * nq ? tile : p.tiles + share) * (16 * ROWS);
-        for (int idx = tt; idx < 16 * mt; idx += kTeamThreads) {
-            const int r = idx & 15, m = idx >> 4;
-            const int64_t row = static_cast<int64_t>(tile) * 16 + r;
+        float* part_sums = whole ? nullptr : range_slots(blockIdx.y) + static_cast<size_t>(lo <= tile * nq ? tile : p.tiles + share) * (kRows * ROWS);
+        for (int idx = tt; idx < kRows * mt; idx += kTeamThreads) {
+            const int r = idx % kRows, m = idx / kRows;
+            const int64_t row = static_cast<int64_t>(tile) * kRows + r;
             if (row >= g.N) continue;
             float sum = 0.0f;
 #pragma unroll
             for (int d = 0; d < (PACKED ? D : 1); ++d) {
-                const int col = d * p.rows + m, b = col >> 3, e = (col & 1) + 2 * (r >> 3);
-                const int ln = (r & 7) * 4 + ((col & 7) >> 1);
+                const int col = d * p.rows + m, e = (col & 1) + 2 * ((r >> 3) & 1), ln = (r & 7) * 4 + (col >> 1);
 #pragma unroll
-                for (int wv = 0; wv < kWarps; ++wv) sum += sums[(wv * NB * 4 + b * 4 + e) * 32 + ln];
+                for (int wv = 0; wv < kWarps; ++wv) sum += red[((wv * 2 + (r >> 4)) * 4 + e) * 32 + ln];
             }
             if ((*odd >> m) & 1u) {
                 // The activations that stayed out.
@@ -601,10 +590,10 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
                 part_sums[idx] = sum;
             }
         }
+        sync();     // the sums have been read, and written where they go
         done += n;
         if (done < hi) { ++tile; q0 = 0; }
     }
-    sync();
 
     // --- tiles that other shares worked on too: the last to arrive adds the parts, K-range after
     // K-range and share after share, so that the sum does not depend on who that is
@@ -617,7 +606,7 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
             if (gridDim.y > 1 || t * nq < lo || (t + 1) * nq > hi) {
                 for (uint32_t y = 0; y < gridDim.y; ++y) {
                     const uint32_t ny = p.steps - y * per < per ? p.steps - y * per : per;
-                    const Shares sy(p.tiles * ny, gridDim.x * kTeams);
+                    const Shares sy(p.tiles, ny, gridDim.x * kTeams);
                     parts += sy.holder(t * ny + ny - 1) - sy.holder(t * ny) + 1;
                 }
                 uint32_t* ticket = p.tickets + static_cast<size_t>(blockIdx.z) * p.tiles + t;
@@ -630,17 +619,17 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
         for (uint32_t i = warp; i < kTeamThreads && t0 + i <= tile; i += kWarps) {      // a warp to a tile
             if (last[i] == 0) continue;
             const uint32_t at = t0 + i;
-            for (int v = lane; v < 4 * mt; v += 32) {
-                const int r = (4 * v) & 15, m = v >> 2;
+            for (int v = lane; v < kRows / 4 * mt; v += 32) {
+                const int r = 4 * v % kRows, m = 4 * v / kRows;
                 float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 for (uint32_t y = 0; y < gridDim.y; ++y) {
                     const uint32_t ny = p.steps - y * per < per ? p.steps - y * per : per;
-                    const Shares sy(p.tiles * ny, gridDim.x * kTeams);
+                    const Shares sy(p.tiles, ny, gridDim.x * kTeams);
                     const uint32_t s0 = sy.holder(at * ny), s1 = sy.holder(at * ny + ny - 1);
                     const float4* from = reinterpret_cast<const float4*>(range_slots(y)) + v;
 #pragma unroll 4
                     for (uint32_t s = s0; s <= s1; ++s) {
-                        const float4 x = __ldcg(from + (s == s0 ? at : p.tiles + s) * static_cast<size_t>(4 * ROWS));
+                        const float4 x = __ldcg(from + (s == s0 ? at : p.tiles + s) * static_cast<size_t>(kRows / 4 * ROWS));
                         sum.x += x.x;
                         sum.y += x.y;
                         sum.z += x.z;
@@ -650,7 +639,7 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
                 const float x[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int64_t row = static_cast<int64_t>(at) * 16 + r + j;
+                    const int64_t row = static_cast<int64_t>(at) * kRows + r + j;
                     if (row < g.N)
                         static_cast<T*>(g.C)[static_cast<int64_t>(m0 + m) * g.ldc + row] =
                             static_cast<T>(x[j] + (g.bias ? g.bias[row] : 0.0f));
@@ -680,27 +669,28 @@ __global__ void __launch_bounds__(256) repack_rows_kernel(const uint8_t* w, int6
 struct Kernel {
     const void* fn;
     const void* digits;
-    int rows, n_digits, blocks, flush, packed;
+    int rows, n_digits, flush;
+    bool packed;
 };
 
-template <DType IO, int MI>
+template <DType IO, bool PACKED>
 Kernel kernel_for_flush(int f) {
     constexpr int D = IO == DType::F32 ? 4 : 3;
-    const void* fn = f == 4 ? reinterpret_cast<const void*>(&gemm_w4_kernel<IO, MI, 4>)
-                     : f == 2 ? reinterpret_cast<const void*>(&gemm_w4_kernel<IO, MI, 2>)
-                              : reinterpret_cast<const void*>(&gemm_w4_kernel<IO, MI, 1>);
-    const void* digits = f == 4 ? reinterpret_cast<const void*>(&gemm_w4_digits_kernel<IO, MI, 4>)
-                         : f == 2 ? reinterpret_cast<const void*>(&gemm_w4_digits_kernel<IO, MI, 2>)
-                                  : reinterpret_cast<const void*>(&gemm_w4_digits_kernel<IO, MI, 1>);
-    return {fn, digits, MI ? 8 * MI : 8 / D, D, MI ? MI : 1, f, MI == 0};
+    const void* fn = f == 4 ? reinterpret_cast<const void*>(&gemm_w4_kernel<IO, PACKED, 4>)
+                     : f == 2 ? reinterpret_cast<const void*>(&gemm_w4_kernel<IO, PACKED, 2>)
+                              : reinterpret_cast<const void*>(&gemm_w4_kernel<IO, PACKED, 1>);
+    const void* digits = f == 4 ? reinterpret_cast<const void*>(&gemm_w4_digits_kernel<IO, PACKED, 4>)
+                         : f == 2 ? reinterpret_cast<const void*>(&gemm_w4_digits_kernel<IO, PACKED, 2>)
+                                  : reinterpret_cast<const void*>(&gemm_w4_digits_kernel<IO, PACKED, 1>);
+    return {fn, digits, PACKED ? 8 / D : 8, D, f, PACKED};
 }
 
 Kernel select(const W4Args& g) {
     // How many chunks of 32 weights share their scales for sure, up to the four of a step.
     const int f = g.groups == 1 || g.group % 128 == 0 ? 4 : (g.group % 64 == 0 ? 2 : 1);
-    if (g.io == DType::F32) return g.M <= 2 ? kernel_for_flush<DType::F32, 0>(f) : kernel_for_flush<DType::F32, 1>(f);
-    return g.M <= 2 ? kernel_for_flush<DType::BF16, 0>(f)
-           : g.M <= 8 ? kernel_for_flush<DType::BF16, 1>(f) : kernel_for_flush<DType::BF16, 2>(f);
+    // Two rows' digits fit one block of columns: a third (a quarter) of the products.
+    if (g.io == DType::F32) return g.M <= 2 ? kernel_for_flush<DType::F32, true>(f) : kernel_for_flush<DType::F32, false>(f);
+    return g.M <= 2 ? kernel_for_flush<DType::BF16, true>(f) : kernel_for_flush<DType::BF16, false>(f);
 }
 
 bool aligned_rows(const W4Args& g) { return g.ldw % 16 == 0 && reinterpret_cast<uintptr_t>(g.W) % 16 == 0; }
@@ -737,13 +727,13 @@ EncodeTiled encode_tiled() {
     return fn;
 }
 
-// W as bytes [N][(K+1)/2], read in boxes of 64 bytes x 16 rows; bytes and rows past the ends read as zeros.
+// W as bytes [N][(K+1)/2], read in boxes of 64 bytes x 32 rows; bytes and rows past the ends read as zeros.
 bool encode_weights(const W4Args& g, const uint8_t* w, int64_t pitch, CUtensorMap* map) {
     EncodeTiled fn = encode_tiled();
     if (!fn) return false;
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(row_bytes_of(g)), static_cast<cuuint64_t>(g.N)};
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
-    const cuuint32_t box[2] = {64, 16}, one[2] = {1, 1};
+    const cuuint32_t box[2] = {kStepK / 2, kRows}, one[2] = {1, 1};
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(w), dims, strides, box, one,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -754,13 +744,13 @@ bool encode_weights(const W4Args& g, const uint8_t* w, int64_t pitch, CUtensorMa
 bool gemm_w4_plan(const W4Args& g, int num_sms, W4Plan* plan) {
     const Kernel k = select(g);
     plan->rows = g.M < k.rows ? g.M : k.rows;
-    const int64_t steps = (static_cast<int64_t>(g.K) + kStepK - 1) / kStepK, tiles = (static_cast<int64_t>(g.N) + 15) / 16;
+    const int64_t steps = (static_cast<int64_t>(g.K) + kStepK - 1) / kStepK, tiles = (static_cast<int64_t>(g.N) + kRows - 1) / kRows;
     plan->cols = k.n_digits * plan->rows;
     // As much of K at a time as the digits leave room for beside the smallest rings; the rings take
     // what is left.
     const int warps = kTeams * kWarps;
-    const int fixed = warps * (2 * k.blocks * 512 + kMaxSlots * 8) + 64 + 16;
-    const int per_step = 2 * (plan->cols * (128 + 4 * (4 / k.flush)) + 4 * (k.packed ? plan->cols : plan->rows) * (1 + 4 / k.flush));
+    const int fixed = warps * (1024 + kMaxSlots * 8) + 64 + 16;
+    const int per_step = plan->cols * (128 + 4 * (4 / k.flush)) + 4 * (k.packed ? plan->cols : plan->rows) * (1 + 4 / k.flush);
     const int64_t most = (kMaxSmem - fixed - warps * kMinSlots * kStepBytes) / per_step;
     const int64_t splits = (steps + most - 1) / most;
     plan->split_steps = static_cast<int>((steps + splits - 1) / splits);
@@ -772,7 +762,7 @@ bool gemm_w4_plan(const W4Args& g, int num_sms, W4Plan* plan) {
     plan->image_bytes = (per_step * plan->split_steps + 15) & ~15;
     // 512 threads take a microsecond for every 32 stretches of 128 activations; a kernel before this
     // one takes two and overlaps this one's start.
-    const int64_t stretches = static_cast<int64_t>(plan->rows) * plan->split_steps * 2;
+    const int64_t stretches = static_cast<int64_t>(plan->rows) * plan->split_steps;
     plan->prepared = stretches > 32;
     plan->pitch = aligned_rows(g) ? 0 : (row_bytes_of(g) + 15) / 16 * 16;
     plan->copy_bytes = static_cast<size_t>(plan->pitch) * g.N;
@@ -786,7 +776,7 @@ bool gemm_w4_plan(const W4Args& g, int num_sms, W4Plan* plan) {
     plan->ctas = static_cast<int>(ctas);
     // Steps are counted in 32 bits; blocks and splits are grid dimensions.
     if (tiles * plan->split_steps > INT32_MAX || plan->splits > 65535 || plan->blocks > 65535) return false;
-    plan->ws_floats = static_cast<size_t>(plan->blocks) * plan->splits * (tiles + ctas * kTeams) * 16 * k.rows;
+    plan->ws_floats = static_cast<size_t>(plan->blocks) * plan->splits * (tiles + ctas * kTeams) * kRows * k.rows;
     plan->tickets = static_cast<size_t>(plan->blocks) * tiles;
     return true;
 }
@@ -810,7 +800,7 @@ cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint3
     }
     Params p;
     p.g = g;
-    p.tiles = (g.N + 15) / 16;
+    p.tiles = static_cast<int>((static_cast<int64_t>(g.N) + kRows - 1) / kRows);
     p.steps = static_cast<int>((static_cast<int64_t>(g.K) + kStepK - 1) / kStepK);
     p.split_steps = plan.split_steps;
     p.slots = plan.slots;
@@ -841,7 +831,7 @@ cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint3
     p.images = nullptr;
     if (plan.prepared) {
         p.images = static_cast<unsigned char*>(extra) + plan.copy_bytes;
-        const unsigned stretches = static_cast<unsigned>(plan.rows) * plan.split_steps * 2;
+        const unsigned stretches = static_cast<unsigned>(plan.rows) * plan.split_steps;
         void* first[] = {&p};
         e = launch_pdl(k.digits, dim3((stretches + 7) / 8, plan.splits, plan.blocks), 128, first, 0, s);
         if (e != cudaSuccess) return e;

@@ -394,10 +394,11 @@ __global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTA
                 const char* vs = static_cast<const char*>(a.v) + o;
 #pragma unroll
                 for (int u = 0; u < G::PITCH / 16 / LPR; ++u) {
-                    // Rows that are not there and dimensions past head_dim become zeros.
+                    // Rows that are not there and dimensions past head_dim become zeros: nothing of
+                    // their addresses is read.
                     const bool in = load && u * LPR + lch < nch;
-                    cp_async16(dst + u * LPR * 16, in ? ks + u * LPR * 16 : static_cast<const char*>(a.k), in);
-                    cp_async16(dst + u * LPR * 16 + G::KV, in ? vs + u * LPR * 16 : static_cast<const char*>(a.v), in);
+                    cp_async16(dst + u * LPR * 16, ks + u * LPR * 16, in);
+                    cp_async16(dst + u * LPR * 16 + G::KV, vs + u * LPR * 16, in);
                 }
             }
             if constexpr (CT != DType::E4M3) {
