@@ -232,15 +232,17 @@ struct Cursor {
             len = 0;
         }
         first = p.a.window > 0 && len > p.a.window ? len - p.a.window : 0;
-        const int n = (len - first + tile_tokens - 1) / tile_tokens;
-        tiles = n > 0 ? n : 1;      // an empty sequence still has outputs to write
+        tiles = (len - first + tile_tokens - 1) / tile_tokens;
     }
     __device__ __forceinline__ void next(const Params& p, int items, int tile_tokens) {
         if (++t < tiles) return;
         t = 0;
         if (++r < items) return;
         r = 0;
-        if (++b < p.a.batch) load(p, tile_tokens);
+        do {
+            if (++b >= p.a.batch) return;
+            load(p, tile_tokens);
+        } while (tiles == 0);
     }
 };
 
@@ -275,7 +277,8 @@ __global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTA
     float* s_l = s_m + NW * 16;
     float* s_f = s_l + NW * 16;                                                  // [16] query scale per head
     uint32_t* s_mask = reinterpret_cast<uint32_t*>(s_f + 16);                    // [S][NW]
-    int* s_find = reinterpret_cast<int*>(s_mask + S * NW);                       // [NW], words passed between threads
+    int* s_find = reinterpret_cast<int*>(s_mask + S * NW);                       // [4], words passed between threads
+    uint32_t* s_own = reinterpret_cast<uint32_t*>(s_find + 4);                   // [3]
 
     const PagedAttnArgs& a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
@@ -317,35 +320,97 @@ __global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTA
         __syncthreads();
     }
     total *= items;
-    const Shares shares(total, gridDim.x);
-    const uint32_t share = blockIdx.x;
-    if (share >= shares.ctas) return;
-    const uint32_t lo = shares.start(share), hi = shares.start(share + 1);
-    const uint32_t end = incl * items, start = (incl - mine) * items;
-    Cursor cons;
-    uint32_t off0;
-    if (few) {
-        const int owner = __ffs(__ballot_sync(0xFFFFFFFFu, lane < a.batch && lo < end)) - 1;
-        cons.b = owner;
-        off0 = __shfl_sync(0xFFFFFFFFu, start, owner);
-    } else {
-        if (lo >= start && lo < end) {
-            uint32_t at = start;
+
+    // --- sequences without a token: zeros
+    for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+        uint32_t tiles = 0;
+        if (few) {
+            tiles = __shfl_sync(0xFFFFFFFFu, mine, b);
+        } else {
             Cursor c;
-            c.b = b0;
-            for (;; ++c.b) {
-                c.load(p, TILE);
-                if (lo < at + c.tiles * items) break;
-                at += c.tiles * items;
-            }
-            s_find[0] = c.b;
-            s_find[1] = static_cast<int>(at);
+            c.b = b;
+            c.load(p, TILE);
+            tiles = c.tiles;
         }
-        __syncthreads();
-        cons.b = s_find[0];
-        off0 = s_find[1];
-        __syncthreads();
+        if (tiles != 0) continue;
+        constexpr int N = 16 / sizeof(typename I::S);
+        typename I::S* out = static_cast<typename I::S*>(a.out) + b * a.out_batch;
+        for (int i = tid; i < a.heads * (dim / N); i += NW * 32) {
+            const int h = i / (dim / N), d = (i - h * (dim / N)) * N;
+            *reinterpret_cast<uint4*>(out + h * a.out_head + d) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        if (a.lse)
+            for (int h = tid; h < a.heads; h += NW * 32) a.lse[static_cast<int64_t>(b) * a.heads + h] = -INFINITY;
     }
+    if (total == 0) return;
+
+    const Shares shares(total, gridDim.x);
+    const uint32_t share = blockIdx.x, end = incl * items, start = (incl - mine) * items;
+    uint32_t lo, hi, off0;
+    Cursor cons;
+    // Ending an item and beginning the next within a share costs about as much as two tiles.  So
+    // with few items each gets CTAs of its own, if these then have at most two tiles more.
+    bool own = false;
+    if (few) {
+        uint32_t most = (total + gridDim.x - 1) / gridDim.x, k = 0, sum = 0;
+        for (int tries = 0; tries < 3 && !own; ++tries, ++most) {
+            k = (mine + most - 1) / most;       // CTAs to each item of the lane's sequence
+            sum = k * items;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+                if (lane >= o) sum += v;
+            }
+            own = __shfl_sync(0xFFFFFFFFu, sum, 31) <= gridDim.x;
+        }
+        if (own) {
+            const uint32_t owners = __ballot_sync(0xFFFFFFFFu, share < sum);
+            if (owners == 0) return;
+            const int owner = __ffs(owners) - 1;
+            cons.b = owner;
+            k = __shfl_sync(0xFFFFFFFFu, k, owner);
+            const uint32_t at = share - (__shfl_sync(0xFFFFFFFFu, sum, owner) - k * items);
+            const uint32_t r = at / k, part = at - r * k;
+            const uint32_t tiles = __shfl_sync(0xFFFFFFFFu, mine, owner), each = tiles / k, more = tiles - each * k;
+            off0 = __shfl_sync(0xFFFFFFFFu, start, owner);
+            lo = off0 + r * tiles + part * each + min(part, more);
+            hi = lo + each + (part < more ? 1 : 0);
+            if (tid == 0) {
+                s_own[1] = share - part;
+                s_own[2] = share - part + k - 1;
+            }
+        }
+        if (tid == 0) s_own[0] = own;
+    } else if (tid == 0) {
+        s_own[0] = 0;
+    }
+    if (!own) {
+        if (share >= shares.ctas) return;
+        lo = shares.start(share);
+        hi = shares.start(share + 1);
+        if (few) {
+            const int owner = __ffs(__ballot_sync(0xFFFFFFFFu, lane < a.batch && lo < end)) - 1;
+            cons.b = owner;
+            off0 = __shfl_sync(0xFFFFFFFFu, start, owner);
+        } else {
+            if (lo >= start && lo < end) {
+                uint32_t at = start;
+                Cursor c;
+                c.b = b0;
+                for (;; ++c.b) {
+                    c.load(p, TILE);
+                    if (lo < at + c.tiles * items) break;
+                    at += c.tiles * items;
+                }
+                s_find[0] = c.b;
+                s_find[1] = static_cast<int>(at);
+            }
+            __syncthreads();
+            cons.b = s_find[0];
+            off0 = s_find[1];
+        }
+    }
+    __syncthreads();
     cons.load(p, TILE);
     cons.r = static_cast<int>((lo - off0) / cons.tiles);
     cons.t = static_cast<int>((lo - off0) % cons.tiles);
@@ -561,6 +626,12 @@ __global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTA
     };
     auto parts_of = [&](uint32_t item0, int tiles) {
         Parts r;
+        if (s_own[0]) {
+            r.first = s_own[1];
+            r.last = s_own[2];
+            r.tail = 0;
+            return r;
+        }
         r.first = shares.holder(item0);
         r.last = shares.holder(item0 + tiles - 1);
         r.tail = shares.start(r.first) < item0 ? 1 : 0;
