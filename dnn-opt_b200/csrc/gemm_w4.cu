@@ -355,6 +355,45 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     };
     for (int s = 0; s < p.slots; ++s) request(s);
 
+    // A scale or zero point as it lies in memory (bf16: in the low half), and its value.
+    const int up = f32s ? 0 : 16;
+    auto fetch = [&](const void* base, int64_t e) -> uint32_t {
+        return f32s ? __ldg(static_cast<const uint32_t*>(base) + e) : __ldg(static_cast<const uint16_t*>(base) + e);
+    };
+    auto value = [&](uint32_t raw) { return __uint_as_float(raw << up); };
+    auto group_of = [&](uint32_t chunk) { return min(static_cast<int>(__umulhi(2 * chunk, p.gmul) >> p.gshift), g.groups - 1); };
+    const int scale_bytes = f32s ? 4 : 2;
+    const int64_t to_zero = reinterpret_cast<intptr_t>(g.zero) - reinterpret_cast<intptr_t>(g.scale);
+    // Scales are read one step ahead of their products, across the ends of tiles.
+    Cursor ahead(lo, hi, nq, warp);
+    const char* srow[4];    // the lane's four rows' first scales
+    uint32_t raw[4] = {}, rawz[4] = {};
+    auto open = [&](uint32_t t) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            const int64_t row = static_cast<int64_t>(t) * kRows + gr + 8 * h;
+            srow[h] = static_cast<const char*>(g.scale) + (row < g.N ? row : g.N - 1) * g.lds * scale_bytes;
+        }
+    };
+    auto fetch_scales = [&]() {
+        if (ahead.q >= ahead.end) return;
+        const int64_t gi = static_cast<int64_t>(group_of((k_step0 + ahead.q) * 4 + t4)) * scale_bytes;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            raw[h] = ldg_scale(srow[h] + gi, f32s);
+            if (zeros) rawz[h] = ldg_scale(srow[h] + gi + to_zero, f32s);
+        }
+        ahead.q += kWarps;
+        if (ahead.q >= ahead.end && ahead.left > 0) {
+            ahead.settle(nq, warp);
+            open(ahead.tile);
+        }
+    };
+    if (busy) {
+        open(ahead.tile);
+        fetch_scales();
+    }
+
     // --- the K-range's activations as digits: from the kernel before, or made here
     __syncthreads();
     if (p.images) {
@@ -388,15 +427,6 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     if (!busy) return;
 
     auto sync = [&]() { named_barrier_sync(1 + team, kTeamThreads); };
-    // A scale or zero point as it lies in memory (bf16: in the low half), and its value.
-    const int up = f32s ? 0 : 16;
-    auto fetch = [&](const void* base, int64_t e) -> uint32_t {
-        return f32s ? __ldg(static_cast<const uint32_t*>(base) + e) : __ldg(static_cast<const uint16_t*>(base) + e);
-    };
-    auto value = [&](uint32_t raw) { return __uint_as_float(raw << up); };
-    auto group_of = [&](uint32_t chunk) { return min(static_cast<int>(__umulhi(2 * chunk, p.gmul) >> p.gshift), g.groups - 1); };
-    const int scale_bytes = f32s ? 4 : 2;
-    const int64_t to_zero = reinterpret_cast<intptr_t>(g.zero) - reinterpret_cast<intptr_t>(g.scale);
     // The slots of K-range y.
     auto range_slots = [&](uint32_t y) {
         return p.ws + (static_cast<size_t>(blockIdx.z) * gridDim.y + y) * (p.tiles + gridDim.x * kTeams) * (kRows * ROWS);
@@ -416,34 +446,6 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) tab[e] = min(2 * t4 + e, tcols - 1);
-    // Scales are read one step ahead of their products, across the ends of tiles.
-    Cursor ahead(lo, hi, nq, warp);
-    const char* srow[4];    // the lane's four rows' first scales
-    uint32_t raw[4] = {}, rawz[4] = {};
-    auto open = [&](uint32_t t) {
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            const int64_t row = static_cast<int64_t>(t) * kRows + gr + 8 * h;
-            srow[h] = static_cast<const char*>(g.scale) + (row < g.N ? row : g.N - 1) * g.lds * scale_bytes;
-        }
-    };
-    auto fetch_scales = [&]() {
-        if (ahead.q >= ahead.end) return;
-        const int64_t gi = static_cast<int64_t>(group_of((k_step0 + ahead.q) * 4 + t4)) * scale_bytes;
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            raw[h] = ldg_scale(srow[h] + gi, f32s);
-            if (zeros) rawz[h] = ldg_scale(srow[h] + gi + to_zero, f32s);
-        }
-        ahead.q += kWarps;
-        if (ahead.q >= ahead.end && ahead.left > 0) {
-            ahead.settle(nq, warp);
-            open(ahead.tile);
-        }
-    };
-    open(ahead.tile);
-    fetch_scales();
-
     uint32_t tile = lo / nq, q0 = lo - tile * nq, done = lo;
     uint32_t phase = 0;
     int slot = 0;
