@@ -89,6 +89,33 @@ __device__ __forceinline__ uint32_t ldg_scale(const char* p, bool f32) {
                  : "=r"(v) : "l"(p), "r"(static_cast<int>(f32)));
     return v;
 }
+// Two FP32 operations in one instruction.
+__device__ __forceinline__ unsigned long long as64(float2 v) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1,%2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+    return r;
+}
+__device__ __forceinline__ float2 as_pair(unsigned long long r) {
+    float2 v;
+    asm("mov.b64 {%0,%1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
+    return v;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(as64(a)), "l"(as64(b)), "l"(as64(c)));
+    return as_pair(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(as64(a)), "l"(as64(b)));
+    return as_pair(r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(as64(a)), "l"(as64(b)));
+    return as_pair(r);
+}
+__device__ __forceinline__ float2 bits2(const uint32_t* c) { return make_float2(__uint_as_float(c[0]), __uint_as_float(c[1])); }
 constexpr float kMagic = 12582912.0f;           // 1.5 * 2^23: whole numbers below 2^22 added to it keep their bits
 constexpr uint32_t kMagicBits = 0x4B400000u;
 
@@ -452,7 +479,7 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     bool dead = false;
     while (done < hi) {
         const uint32_t n = hi - done < nq - q0 ? hi - done : nq - q0, q1 = q0 + n;
-        float tot[2][4] = {};       // [block of 16 rows]
+        float2 tot[2][2] = {};      // [block of 16 rows][its half]
         for (uint32_t q = q0 + warp; q < q1; q += kWarps) {
             float sc[4], zr[4];
 #pragma unroll
@@ -543,12 +570,14 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
                         }
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float y = __uint_as_float(c[k][NT - 1][e]) - kMagic;
+                    for (int h = 0; h < 2; ++h) {       // a row's two columns at once
+                        const float sh = h ? s1 : s0, zh = h ? z1 : z0;
+                        float2 y = add2(bits2(&c[k][NT - 1][2 * h]), make_float2(-kMagic, -kMagic));
 #pragma unroll
-                        for (int d = NT - 2; d >= 0; --d) y = fmaf(y, 256.0f, __uint_as_float(c[k][d][e]) - kMagic);
-                        if (zeros) y = fmaf(e < 2 ? z0 : z1, is[e & 1], y);
-                        tot[k][e] = fmaf((e < 2 ? s0 : s1) * un[e & 1], y, tot[k][e]);
+                        for (int d = NT - 2; d >= 0; --d)
+                            y = fma2(y, make_float2(256.0f, 256.0f), add2(bits2(&c[k][d][2 * h]), make_float2(-kMagic, -kMagic)));
+                        if (zeros) y = fma2(make_float2(zh, zh), make_float2(is[0], is[1]), y);
+                        tot[k][h] = fma2(mul2(make_float2(sh, sh), make_float2(un[0], un[1])), y, tot[k][h]);
                     }
                 }
             }
@@ -558,7 +587,7 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) red[((warp * 2 + k) * 4 + e) * 32 + lane] = tot[k][e];
+            for (int e = 0; e < 4; ++e) red[((warp * 2 + k) * 4 + e) * 32 + lane] = e % 2 ? tot[k][e / 2].y : tot[k][e / 2].x;
         sync();
         const bool whole = n == nq && gridDim.y == 1;
         float* part_sums = whole ? nullptr : range_slots(blockIdx.y) + static_cast<size_t>(lo <= tile * nq ? tile : p.tiles + share) * (kRows * ROWS);
