@@ -81,17 +81,19 @@ struct Row {
     __device__ __forceinline__ int col(int i, int j) const {
         return VEC ? 8 * (me + i * threads()) + j : me + (8 * i + j) * threads();
     }
-    // Whether all of block i is there: for VEC this thread's, else every thread's.
+    // Whether all of block i is there: for VEC this thread's, else every thread's but for its last element.
     __device__ __forceinline__ bool full(int i) const {
-        return VEC ? col(i, 0) + 8 <= cols : (8 * i + 8) * threads() <= cols;
+        return VEC ? col(i, 0) + 8 <= cols : (8 * i + 7) * threads() <= cols;
     }
+    // Whether element j of such a block is there.
+    __device__ __forceinline__ bool in(int i, int j) const { return VEC || j < 7 || col(i, j) < cols; }
     // Block i of a row; columns that are not there give 0.
     __device__ __forceinline__ void read(const float* p, int i, Raw<float, VEC>& r) const {
         if (VEC && full(i)) {
             load8(p + col(i, 0), r.w);
         } else if (full(i)) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) r.w[j] = p[col(i, j)];
+            for (int j = 0; j < 8; ++j) r.w[j] = in(i, j) ? p[col(i, j)] : 0.0f;
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) r.w[j] = col(i, j) < cols ? p[col(i, j)] : 0.0f;
@@ -112,7 +114,7 @@ struct Row {
             }
         } else if (full(i)) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) r.w[j] = q[col(i, j)];
+            for (int j = 0; j < 8; ++j) r.w[j] = in(i, j) ? q[col(i, j)] : 0u;
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) r.w[j] = col(i, j) < cols ? q[col(i, j)] : 0u;
@@ -130,7 +132,8 @@ struct Row {
             store8(p + col(i, 0), v);
         } else if (full(i)) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) from_f32(p + col(i, j), v[j]);
+            for (int j = 0; j < 8; ++j)
+                if (in(i, j)) from_f32(p + col(i, j), v[j]);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -173,7 +176,7 @@ __device__ __forceinline__ void norm_row(const Row<VEC, EPT, TH>& row, float (&v
         for (int i = 0; i < NB; ++i) {
             if (row.full(i)) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] -= mean;
+                for (int j = 0; j < 8; ++j) v[i][j] = row.in(i, j) ? v[i][j] - mean : 0.0f;
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[i][j] = row.col(i, j) < row.cols ? v[i][j] - mean : 0.0f;
