@@ -445,6 +445,21 @@ def test_attention_split_over_length(gpu, dn, cache, batch, longest):
     Paged(gpu, dn, lens, 4, 2, 64, 64, cache, append=True, layout="head").check()
 
 
+@pytest.mark.parametrize("cache", ["bf16", "e4m3", "f32"])
+@pytest.mark.parametrize("batch", [1, 2, 31, 32, 33, 400])
+@pytest.mark.parametrize("heads,kv", [(4, 4), (16, 1)])
+def test_attention_among_empty_sequences(gpu, dn, cache, batch, heads, kv):
+    """Sequences without a token first, last, in runs and everywhere; the others of one to many tiles."""
+    rng = np.random.default_rng(batch)
+    lens = rng.choice([1, 15, 64, 65, 200, 1000 if batch <= 33 else 129], batch)
+    lens[rng.random(batch) < 0.6] = 0
+    lens[:batch // 4] = 0
+    lens[batch - batch // 8:] = 0
+    Paged(gpu, dn, lens.tolist(), heads, kv, 64, 32, cache).check()
+    Paged(gpu, dn, lens[::-1].tolist(), heads, kv, 64, 32, cache, window=70).check()
+    Paged(gpu, dn, [0] * batch, heads, kv, 64, 32, cache).check()
+
+
 def test_attention_same_bits_each_time(gpu, dn):
     for cache in ("bf16", "e4m3", "f32"):
         p = Paged(gpu, dn, [9000, 10, 0, 777], 8, 2, 128, 16, cache, append=True)
