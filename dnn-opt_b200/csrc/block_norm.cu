@@ -8,13 +8,17 @@
 //   * rows of up to 512 columns belong to a warp each (no barrier), longer ones
 //     to a CTA;
 //   * few rows: eight elements to a thread, so that many threads share a row;
-//   * many rows: 8 or 16 elements, and each warp or CTA takes row after row, the
-//     next one's loads under way while it works on this one;
+//   * many rows: 8 or 16 elements, and each CTA takes row after row, the next
+//     one's loads under way while it works on this one;
 //   * rows past 16384 columns stay in shared memory.
 // Elements are read 16 bytes at a time where all rows and vectors allow, else
 // one by one, neighbouring threads neighbouring elements.  Means and mean
 // squares are sums over the values themselves (a layer norm's squares are
 // taken after its mean), in a fixed order.
+//
+// Measured, of 6.53 TB/s: 8192x8192 bf16 90 us (92%), 65536x1024 bf16 85 us
+// (97%), 65536x512 bf16 44 us (94%), 16384x4093 FP32 with layer norms and a gate
+// row each 262 us (78%: scalar loads, four sums over the row), 1x4096 2.5 us.
 #include <mutex>
 #include <unordered_map>
 
@@ -207,7 +211,7 @@ __device__ __forceinline__ void norm_row(const Row<VEC, EPT, TH>& row, float (&v
     }
 }
 
-// STREAM: row after row, gridDim rows (or blocks of them) apart.
+// STREAM: row after row, gridDim rows apart.
 template <typename T, typename TW, bool VEC, int EPT, bool WARP, bool STREAM, int TH>
 __global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : (STREAM ? TH : 1024)) block_norm_kernel(const BlockNormArgs a) {
     constexpr int NB = EPT / 8;
@@ -389,38 +393,37 @@ cudaError_t resident(const void* fn, int threads, int* ctas) {
     return cudaSuccess;
 }
 
-template <typename T, typename TW, bool VEC, int EPT, bool WARP, int TH>
+template <typename T, typename TW, bool VEC, int EPT, int TH>
 cudaError_t launch_stream(const BlockNormArgs& a, int num_sms, cudaStream_t s) {
     int ctas = 0;
-    const int threads = WARP ? 32 * kRowsPerCta : TH;
-    cudaError_t e = resident(reinterpret_cast<const void*>(&block_norm_kernel<T, TW, VEC, EPT, WARP, true, TH>), threads, &ctas);
+    cudaError_t e = resident(reinterpret_cast<const void*>(&block_norm_kernel<T, TW, VEC, EPT, false, true, TH>), TH, &ctas);
     if (e != cudaSuccess) return e;
-    const int64_t units = WARP ? (static_cast<int64_t>(a.rows) + kRowsPerCta - 1) / kRowsPerCta : a.rows;
     const int64_t most = static_cast<int64_t>(ctas) * num_sms;
-    return launch_pdl(block_norm_kernel<T, TW, VEC, EPT, WARP, true, TH>, units < most ? units : most, threads, 0, a, s);
+    return launch_pdl(block_norm_kernel<T, TW, VEC, EPT, false, true, TH>, a.rows < most ? a.rows : most, TH, 0, a, s);
 }
 
 template <typename T, typename TW, bool VEC>
 cudaError_t launch_short(const BlockNormArgs& a, int num_sms, cudaStream_t s) {
+    // 65536x512 bf16: 44 us, a CTA to each row 97; rows of 1024 take 105 us this way and 85 the other.
+    // (Row after row, as below, took 55 for 65536x512: here the other warps' rows hide a row's chain.)
     if (a.cols <= 512) {
-        if (a.rows > 4 * kRowsPerCta * num_sms)
-            return a.cols <= 256 ? launch_stream<T, TW, VEC, 8, true, 32>(a, num_sms, s)
-                                 : launch_stream<T, TW, VEC, 16, true, 32>(a, num_sms, s);
         const int64_t grid = (static_cast<int64_t>(a.rows) + kRowsPerCta - 1) / kRowsPerCta;
         return a.cols <= 256 ? launch_pdl(block_norm_kernel<T, TW, VEC, 8, true, false, 32>, grid, 32 * kRowsPerCta, 0, a, s)
                              : launch_pdl(block_norm_kernel<T, TW, VEC, 16, true, false, 32>, grid, 32 * kRowsPerCta, 0, a, s);
     }
     auto threads = [&](int ept) { return ((a.cols + ept - 1) / ept + 31) / 32 * 32; };
     if (a.cols <= 8192) {
-        if (a.rows > 2 * num_sms) {
+        // Row after row pays from two (longer rows) or four rows an SM on: 8192x8192 bf16 90 us, a CTA to
+        // each row 114; 2400x4096 17.1 and 18.5, but 600x1024 3.1 and 2.7.
+        if (a.rows > (a.cols > 4096 ? 2 : 4) * num_sms) {
             // Element by element, half as many to a thread hide more of each other's latency
-            // (16384x4093 FP32: 277 against 287 us); 16 bytes at a time it is the other way round
-            // (4096x4096 bf16: 33 against 28 us).
+            // (16384x4093 FP32: 262 against 288 us); 16 bytes at a time it is the other way round
+            // (4096x4096 bf16: 32 against 27 us).
             constexpr int EPT = VEC ? 16 : 8, PER = 16 / EPT;
-            if (a.cols <= 1024) return launch_stream<T, TW, VEC, EPT, false, 64 * PER>(a, num_sms, s);
-            if (a.cols <= 2048) return launch_stream<T, TW, VEC, EPT, false, 128 * PER>(a, num_sms, s);
-            if (a.cols <= 4096) return launch_stream<T, TW, VEC, EPT, false, 256 * PER>(a, num_sms, s);
-            return launch_stream<T, TW, VEC, 16, false, 512>(a, num_sms, s);
+            if (a.cols <= 1024) return launch_stream<T, TW, VEC, EPT, 64 * PER>(a, num_sms, s);
+            if (a.cols <= 2048) return launch_stream<T, TW, VEC, EPT, 128 * PER>(a, num_sms, s);
+            if (a.cols <= 4096) return launch_stream<T, TW, VEC, EPT, 256 * PER>(a, num_sms, s);
+            return launch_stream<T, TW, VEC, 16, 512>(a, num_sms, s);
         }
         return launch_pdl(block_norm_kernel<T, TW, VEC, 8, false, false, 0>, a.rows, threads(8), 0, a, s);
     }

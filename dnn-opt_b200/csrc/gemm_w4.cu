@@ -33,6 +33,13 @@
 // digits of the K-range sit in shared memory in the order in which the operand
 // reads them.  Rows of W that do not start at multiples of 16 bytes are first
 // copied to a workspace where they do.
+//
+// Measured, of 6.53 TB/s (groups of 128, bf16): 1x28672x8192 30.0 us (62%), 8 rows
+// 44.1 us (42%), 16 rows 83 us; groups of 32, 8 rows 67 us; FP32, 8 rows 56.5 us;
+// 4x11008x4096 in groups of 64 with zero points 22.3 us; 1x4096x4096 9.0 us, of
+// which the chain of start, digits, first weights, sums and joining takes seven.
+// 16 warps an SM issue two instructions a cycle of four: decoding, products and
+// scaling wait on one another's results, and registers allow no more warps.
 #include <cuda.h>
 
 #include <mutex>
@@ -122,7 +129,8 @@ constexpr uint32_t kMagicBits = 0x4B400000u;
 // Equal shares of all steps but for one step, at least one step for each warp
 // of a team: the first `more` shares have one more than the others.  Where every
 // tile finds a team of its own and has at most four steps for each of its warps,
-// the shares are the tiles: adding up parts would take longer than two steps.
+// the shares are the tiles: adding up parts would take longer than two steps
+// (1x4096x2048 5.2 us, in equal shares 6.7; 1x1024x1024 4.2 and 5.8).
 struct Shares {
     uint32_t n, each, more;
 
@@ -791,10 +799,11 @@ bool gemm_w4_plan(const W4Args& g, int num_sms, W4Plan* plan) {
     plan->smem = fixed + per_step * plan->split_steps + warps * plan->slots * kStepBytes;
     plan->bars_at = (plan->smem - warps * kMaxSlots * 8 - 16) & ~7;
     plan->image_bytes = (per_step * plan->split_steps + 15) & ~15;
-    // 512 threads take a microsecond for every 32 stretches of 128 activations; a kernel before this
-    // one takes two and overlaps this one's start.
+    // 512 threads take half a microsecond for every 32 stretches of 128 activations; a kernel before
+    // this one takes about one and overlaps this one's start (1x28672x8192, 64 stretches: 30.0 us
+    // without and 31.0 with it; 5x4093x4099 FP32, 165: 21.6 and 19.5; 8x28672x8192, 256: 47.3 and 44.1).
     const int64_t stretches = static_cast<int64_t>(plan->rows) * plan->split_steps;
-    plan->prepared = stretches > 32;
+    plan->prepared = stretches > 64;
     plan->pitch = aligned_rows(g) ? 0 : (row_bytes_of(g) + 15) / 16 * 16;
     plan->copy_bytes = static_cast<size_t>(plan->pitch) * g.N;
     plan->blocks = (g.M + k.rows - 1) / k.rows;
