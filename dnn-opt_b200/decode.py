@@ -8,7 +8,7 @@ What a caller of the small-M products runs to generate a token, end to end:
     u       = W_up z ; g = W_gate z        4-bit weights      dnnopt_cuda_gemm_w4
     h, z    = norms(h, W_down (silu(g) u)) post, gate, pre    dnnopt_cuda_block_norm
 
-Six launches of the library and one elementwise torch operation a layer, all on
+Eight calls of the library and two elementwise torch operations a layer, all on
 the caller's stream, nothing synchronised: a step can be captured in a CUDA
 graph once the cache's pages are assigned.
 

@@ -249,11 +249,15 @@ enum { DNNOPT_TYPE_F32 = 0, DNNOPT_TYPE_BF16 = 1, DNNOPT_TYPE_E4M3 = 2 /* OCP E4
  * zero == NULL stands for 8 (codes of signed values -8..7).  group is a
  * multiple of 32, or 0 for one group per row; the last group may be short.
  * A (M x K, lda) and C (M x N, ldc) are row-major in io_type, bias is FP32 [N]
- * or NULL.  Products and sums are FP32 or better (bf16 operands are multiplied
- * exactly, FP32 activations are split into three bf16 parts without loss), C
- * is rounded once, and results do not depend on the order of execution.
- * M, N or K == 0 is a no-op.  Fastest with W 16-byte aligned and ldw a
- * multiple of 16, and M <= 8. */
+ * or NULL.  Within each 128 consecutive k, the activations of a row are held
+ * as whole multiples of a power of two, 22 bits (BF16) or 30 bits (FP32) below
+ * the largest of the 128: exact down to 2^-14 (2^-6) of it, smaller ones
+ * rounded by at most 2^-23 (2^-31) of it.  Their products with the codes are
+ * summed exactly in integers, scaled and added in FP32, and C is rounded once.
+ * Infinite or NaN activations give what the formula gives.  Results do not
+ * depend on the order of execution.  M, N or K == 0 is a no-op.  Fastest with
+ * M <= 8, W 16-byte aligned and ldw a multiple of 16: rows of W that start
+ * elsewhere are copied to the stream's workspace in every call. */
 typedef struct dnnopt_w4_desc {
     int M, N, K;
     int lda, ldw, ldc;
@@ -293,7 +297,9 @@ int dnnopt_cuda_gemm_w4(const dnnopt_w4_desc* d, const void* A, const uint8_t* W
  * or above max_pages * page_size makes its sequence count as empty, a needed
  * page number outside [0, num_pages) leaves out that page's tokens (nothing is
  * stored there), and dnnopt_stream_status() then returns
- * DNNOPT_STATUS_INVALID_VALUE. */
+ * DNNOPT_STATUS_INVALID_VALUE.  Attended keys and values are expected to be
+ * finite: others may make their sequence's output NaN.  Results do not depend
+ * on the order of execution. */
 typedef struct dnnopt_paged_attn_desc {
     int batch, heads, kv_heads, head_dim;
     int page_size;                 /* tokens per page, >= 1 */
