@@ -52,6 +52,9 @@
 namespace dnnopt_b200 {
 namespace {
 
+#ifndef TCMODE
+#define TCMODE 1
+#endif
 constexpr int kTeams = 4;           // per CTA
 constexpr int kTeamThreads = 128;
 constexpr int kWarps = 4;           // per team
@@ -61,6 +64,10 @@ constexpr int kStepK = 128;
 constexpr int kRows = 32;           // of W in a tile: two blocks of 16
 constexpr int kStepBytes = kRows * kStepK / 2;
 constexpr int kMaxSmem = 227 * 1024;
+constexpr int kTcRows = 128;        // of W in a tile of the tensor-memory kernel
+constexpr int kTcStepBytes = kTcRows * kStepK / 2;
+constexpr int kTcColumns = 128;     // of tensor memory for each of its teams
+constexpr int kTcThreads = kTeams * kTeamThreads + kTeams * 32;
 
 struct Params {
     W4Args g;
@@ -134,9 +141,9 @@ constexpr uint32_t kMagicBits = 0x4B400000u;
 struct Shares {
     uint32_t n, each, more;
 
-    __device__ Shares(uint32_t tiles, uint32_t per_tile, uint32_t most) {
+    __device__ Shares(uint32_t tiles, uint32_t per_tile, uint32_t most, uint32_t warps) {
         const uint32_t steps = tiles * per_tile;
-        n = tiles <= most && per_tile <= 4 * kWarps ? tiles : min(steps / kWarps, most);
+        n = tiles <= most && per_tile <= 4 * warps ? tiles : min(steps / warps, most);
         if (n < 1) n = 1;
         each = steps / n;
         more = steps - each * n;
@@ -175,21 +182,21 @@ struct Cursor {
 // The activations of a K-range as the products read them.
 struct Image {
     unsigned char* act;     // [step][2][col][t] 16 bytes: the digits of two words' activations
-    float* unit;            // [step][tcol]: what 1 stands for; negative where an infinity or NaN was left out
     uint32_t* base;         // [step][flush][col]: -8 times the sum of the digits, as the bits of an FP32 number
+    float* unit;            // [step][tcol]: what 1 stands for; negative where an infinity or NaN was left out
     float* isum;            // [step][flush][tcol]: the sum of the whole numbers (packed: of the digits)
 
     __device__ Image(unsigned char* at, uint32_t steps, int cols, int tcols, int f) : act(at) {
-        unit = reinterpret_cast<float*>(act + static_cast<size_t>(steps) * cols * 128);
-        base = reinterpret_cast<uint32_t*>(unit + steps * tcols);
-        isum = reinterpret_cast<float*>(base + steps * (4 / f) * cols);
+        base = reinterpret_cast<uint32_t*>(act + static_cast<size_t>(steps) * cols * 128);
+        unit = reinterpret_cast<float*>(base + steps * (4 / f) * cols);
+        isum = unit + steps * tcols;
     }
 };
 
 // 128 activations of row m0 + m, eight (a word's worth) to each lane of half a
 // warp: r is the lane's place, q the stretch within the K-range, `in` false for
 // a half that has nothing to do.  The whole warp takes part.
-template <DType IO, bool PACKED, int F>
+template <DType IO, bool PACKED, int F, bool TC>
 __device__ __forceinline__ void stage(const Params& p, const Image& img, int m0, int k_step0, uint32_t m, uint32_t q, uint32_t r,
                                       bool vec, bool in) {
     using T = typename std::conditional<IO == DType::F32, float, __nv_bfloat16>::type;
@@ -278,9 +285,17 @@ __device__ __forceinline__ void stage(const Params& p, const Image& img, int m0,
         for (int s = 1; s < 4 * F; s <<= 1) pair[h] += __shfl_xor_sync(0xFFFFFFFFu, pair[h], s);
     }
     if (in) {
-        unsigned char* dst = img.act + ((q * 2 + (w >> 1)) * p.cols + m) * 64 + t * 16 + (w & 1) * 8;
+        if constexpr (TC) {     // a digit's column is a row of 128 bytes, even k before odd k within each eight
 #pragma unroll
-        for (int d = 0; d < D; ++d) *reinterpret_cast<uint2*>(dst + d * p.rows * 64) = o[d];
+            for (int d = 0; d < D; ++d) {
+                const uint32_t n = d * p.rows + m;
+                *reinterpret_cast<uint2*>(img.act + q * (p.cols * 128) + n * 128 + (((r >> 1) ^ (n & 7)) << 4) + (r & 1) * 8) = o[d];
+            }
+        } else {
+            unsigned char* dst = img.act + ((q * 2 + (w >> 1)) * p.cols + m) * 64 + t * 16 + (w & 1) * 8;
+#pragma unroll
+            for (int d = 0; d < D; ++d) *reinterpret_cast<uint2*>(dst + d * p.rows * 64) = o[d];
+        }
         const float u1 = __uint_as_float((static_cast<uint32_t>(127 + e - BITS) << 23) | (odd ? 0x80000000u : 0u));
         if (r == 0) {
 #pragma unroll
@@ -305,12 +320,13 @@ __device__ __forceinline__ void stage(const Params& p, const Image& img, int m0,
 
 // Images of all K-ranges and blocks of rows, where making them in every CTA
 // takes longer than reading them back: a half-warp per 128 activations.
-template <DType IO, bool PACKED, int F>
+template <DType IO, bool PACKED, int F, bool TC>
 __global__ void __launch_bounds__(128) gemm_w4_digits_kernel(const Params p) {
     pdl_wait();
     pdl_launch_dependents();    // what runs next finds everything older than this kernel done
     using T = typename std::conditional<IO == DType::F32, float, __nv_bfloat16>::type;
-    constexpr int D = IO == DType::F32 ? 4 : 3, ROWS = PACKED ? 8 / D : 8;
+    constexpr int D = IO == DType::F32 ? 4 : 3;
+    const int ROWS = TC ? p.rows : (PACKED ? 8 / D : 8);
     const W4Args& g = p.g;
     const int m0 = blockIdx.z * ROWS, mt = g.M - m0 < ROWS ? g.M - m0 : ROWS;
     const int k_step0 = blockIdx.y * p.split_steps;
@@ -319,7 +335,86 @@ __global__ void __launch_bounds__(128) gemm_w4_digits_kernel(const Params p) {
                     PACKED ? p.cols : p.rows, F);
     const bool vec = g.lda % (16 / sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(g.A) % 16 == 0;
     const uint32_t u = blockIdx.x * 8 + (threadIdx.x >> 4), m = u / nq, q = u - m * nq;
-    stage<IO, PACKED, F>(p, img, m0, k_step0, m, q, threadIdx.x & 15, vec, u < mt * nq);
+    stage<IO, PACKED, F, TC>(p, img, m0, k_step0, m, q, threadIdx.x & 15, vec, u < mt * nq);
+}
+
+// Tiles that other shares worked on too: the last to arrive adds the parts, K-range after K-range and
+// share after share, so that the sum does not depend on who that is.  R: rows of a tile; WARPS: of
+// which each takes steps of its own; `last` has a word for each thread of the team.
+template <typename T, int R, int ROWS, int WARPS, typename Slots, typename Sync>
+__device__ __forceinline__ void join_tiles(const Params& p, const Shares& shares, uint32_t share, uint32_t nq, int m0, int mt,
+                                           uint32_t tile, uint32_t* last, Slots range_slots, Sync sync) {
+    const W4Args& g = p.g;
+    const int tt = threadIdx.x % kTeamThreads;
+    const uint32_t per = static_cast<uint32_t>(p.split_steps);
+    const uint32_t lo = shares.start(share), hi = shares.start(share + 1), tile0 = lo / nq;
+    for (uint32_t t0 = tile0; t0 <= tile; t0 += kTeamThreads) {
+        const uint32_t t = t0 + tt;
+        if (t <= tile) {
+            uint32_t parts = 0;
+            if (gridDim.y > 1 || t * nq < lo || (t + 1) * nq > hi) {
+                for (uint32_t y = 0; y < gridDim.y; ++y) {
+                    const uint32_t ny = p.steps - y * per < per ? p.steps - y * per : per;
+                    const Shares sy(p.tiles, ny, gridDim.x * kTeams, WARPS);
+                    parts += sy.holder(t * ny + ny - 1) - sy.holder(t * ny) + 1;
+                }
+                uint32_t* ticket = p.tickets + static_cast<size_t>(blockIdx.z) * p.tiles + t;
+                if (atom_add_acq_rel_gpu_u32(ticket, 1u) == parts - 1) *ticket = 0u;
+                else parts = 0;
+            }
+            last[tt] = parts;
+        }
+        sync();
+        constexpr int EACH = R > 32 ? kTeamThreads : 32;        // threads to a tile
+        constexpr int NV = (R / 4 * ROWS + EACH - 1) / EACH;    // four rows of W and one of A each
+        for (uint32_t i = tt / EACH; i < kTeamThreads && t0 + i <= tile; i += kTeamThreads / EACH) {
+            if (last[i] == 0) continue;
+            const uint32_t at = t0 + i;
+            float4 sum[NV];
+#pragma unroll
+            for (int j = 0; j < NV; ++j) sum[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (uint32_t y = 0; y < gridDim.y; ++y) {
+                const uint32_t ny = p.steps - y * per < per ? p.steps - y * per : per;
+                const Shares sy(p.tiles, ny, gridDim.x * kTeams, WARPS);
+                const uint32_t s0 = sy.holder(at * ny), s1 = sy.holder(at * ny + ny - 1);
+                const float4* from = reinterpret_cast<const float4*>(range_slots(y)) + tt % EACH;
+                for (uint32_t s = s0; s <= s1; s += 4) {        // four parts asked for at once
+                    float4 x[4][NV];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int j = 0; j < NV; ++j)
+                            x[k][j] = s + k <= s1 && tt % EACH + j * EACH < R / 4 * mt
+                                          ? __ldcg(from + (s + k == s0 ? at : p.tiles + s + k) * static_cast<size_t>(R / 4 * ROWS) + j * EACH)
+                                          : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int j = 0; j < NV; ++j) {
+                            sum[j].x += x[k][j].x;
+                            sum[j].y += x[k][j].y;
+                            sum[j].z += x[k][j].z;
+                            sum[j].w += x[k][j].w;
+                        }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int v = tt % EACH + j * EACH;
+                if (v >= R / 4 * mt) continue;
+                const int r = 4 * v % R, m = 4 * v / R;
+                const float x[4] = {sum[j].x, sum[j].y, sum[j].z, sum[j].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int64_t row = static_cast<int64_t>(at) * R + r + e;
+                    if (row < g.N)
+                        static_cast<T*>(g.C)[static_cast<int64_t>(m0 + m) * g.ldc + row] =
+                            static_cast<T>(x[e] + (g.bias ? g.bias[row] : 0.0f));
+                }
+            }
+        }
+        sync();
+    }
 }
 
 // D digits of an activation: three of bf16, four of FP32.  PACKED: the digits of
@@ -336,7 +431,7 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     constexpr int NT = PACKED ? 1 : D;              // blocks of eight columns
     constexpr int ROWS = PACKED ? 8 / D : 8;        // rows of A per pass
     constexpr int RED = 256;                        // floats of a warp's sums of a tile
-    extern __shared__ __align__(128) unsigned char smem[];
+    extern __shared__ __align__(1024) unsigned char smem[];
     const W4Args& g = p.g;
     const int tid = threadIdx.x, lane = tid & 31, team = tid / kTeamThreads, tt = tid % kTeamThreads, warp = tt >> 5;
     const int gr = lane >> 2, t4 = lane & 3;
@@ -362,7 +457,7 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
 
     if (!p.images) pdl_wait();
     pdl_launch_dependents();
-    const Shares shares(p.tiles, nq, gridDim.x * kTeams);
+    const Shares shares(p.tiles, nq, gridDim.x * kTeams, kWarps);
     const uint32_t share = team * gridDim.x + blockIdx.x;
     const bool busy = share < shares.n;
     const uint32_t lo = busy ? shares.start(share) : 0, hi = busy ? shares.start(share + 1) : 0;
@@ -446,7 +541,7 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
         uint32_t u = tid >> 4, m = u / nq, q = u - m * nq;
         const uint32_t dm = (kTeams * kTeamThreads / 16) / nq, dq = (kTeams * kTeamThreads / 16) - dm * nq;
         for (uint32_t u0 = u & ~1u; u0 < units; u0 += kTeams * kTeamThreads / 16) {     // the same count for a whole warp
-            stage<IO, PACKED, F>(p, img, m0, k_step0, m, q, r, vec, u < units);
+            stage<IO, PACKED, F, false>(p, img, m0, k_step0, m, q, r, vec, u < units);
             u += kTeams * kTeamThreads / 16;
             m += dm;
             q += dq;
@@ -634,59 +729,335 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
         if (done < hi) { ++tile; q0 = 0; }
     }
 
-    // --- tiles that other shares worked on too: the last to arrive adds the parts, K-range after
-    // K-range and share after share, so that the sum does not depend on who that is
-    const uint32_t tile0 = lo / nq;
-    uint32_t* last = reinterpret_cast<uint32_t*>(red);
-    for (uint32_t t0 = tile0; t0 <= tile; t0 += kTeamThreads) {
-        const uint32_t t = t0 + tt;
-        if (t <= tile) {
-            uint32_t parts = 0;
-            if (gridDim.y > 1 || t * nq < lo || (t + 1) * nq > hi) {
-                for (uint32_t y = 0; y < gridDim.y; ++y) {
-                    const uint32_t ny = p.steps - y * per < per ? p.steps - y * per : per;
-                    const Shares sy(p.tiles, ny, gridDim.x * kTeams);
-                    parts += sy.holder(t * ny + ny - 1) - sy.holder(t * ny) + 1;
-                }
-                uint32_t* ticket = p.tickets + static_cast<size_t>(blockIdx.z) * p.tiles + t;
-                if (atom_add_acq_rel_gpu_u32(ticket, 1u) == parts - 1) *ticket = 0u;
-                else parts = 0;
-            }
-            last[tt] = parts;
+    join_tiles<T, kRows, ROWS, kWarps>(p, shares, share, nq, m0, mt, tile, reinterpret_cast<uint32_t*>(red), range_slots, sync);
+}
+
+// ---- the same products by tcgen05, the codes as bytes in tensor memory -------
+__device__ __forceinline__ void umma_i8_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+                 "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+                 "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+                 "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+                 "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+                 "r"(r[31])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_x4(uint32_t taddr, uint32_t (&r)[4]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr));
+}
+
+// ROWS: of A per pass (2, 4 or 8); F as above.
+template <DType IO, int ROWS, int F>
+__global__ void __launch_bounds__(kTcThreads, 1)
+gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
+    using T = typename std::conditional<IO == DType::F32, float, __nv_bfloat16>::type;
+    constexpr int D = IO == DType::F32 ? 4 : 3, NF = 4 / F;
+    constexpr int NC = (D * ROWS + 7) / 8 * 8;      // digits' columns in shared memory
+    constexpr int NM = (NC + 15) / 16 * 16;         // of a product: of 128 rows it has multiples of 16, the last 8 are not read
+    static_assert(NM * NF <= 32, "two products of a step and two operands in a team's tensor memory");
+    constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(NM >> 3) << 17) | ((128u >> 4) << 24);
+    extern __shared__ __align__(1024) unsigned char smem[];
+    const W4Args& g = p.g;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const bool issuer = tid >= kTeams * kTeamThreads;   // a warp for each team asks for weights and issues products
+    const int team = issuer ? (tid - kTeams * kTeamThreads) >> 5 : tid / kTeamThreads, tt = tid % kTeamThreads, warp = tt >> 5;
+    const int m0 = blockIdx.z * ROWS, mt = g.M - m0 < ROWS ? g.M - m0 : ROWS;
+    const int k_step0 = blockIdx.y * p.split_steps;
+    const uint32_t nq = p.steps - k_step0 < p.split_steps ? p.steps - k_step0 : p.split_steps;
+    const uint32_t per = static_cast<uint32_t>(p.split_steps);
+
+    unsigned char* ring = smem + team * p.slots * kTcStepBytes;
+    unsigned char* act = smem + kTeams * p.slots * kTcStepBytes;
+    const Image img(act, per, NC, ROWS, F);
+    uint32_t* last = reinterpret_cast<uint32_t*>(act + p.image_bytes) + team * kTeamThreads;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + p.bars_at);
+    uint64_t* image_bar = bars + kTeams * (kMaxSlots + 4);
+    uint32_t* odd = reinterpret_cast<uint32_t*>(image_bar + 1);                 // rows of A with an infinity or NaN
+    uint32_t* tmem_at = odd + 1;
+    bars += team * (kMaxSlots + 4);
+    uint64_t* code_bars = bars + kMaxSlots;         // a step's codes are in tensor memory
+    uint64_t* done_bars = code_bars + 2;            // and its products
+    const bool zeros = g.zero != nullptr;
+    const bool f32s = g.st == DType::F32;
+
+    if (!p.images) pdl_wait();
+    pdl_launch_dependents();
+    const Shares shares(p.tiles, nq, gridDim.x * kTeams, 1);
+    const uint32_t share = team * gridDim.x + blockIdx.x;
+    const bool busy = share < shares.n;
+    const uint32_t lo = busy ? shares.start(share) : 0, hi = busy ? shares.start(share + 1) : 0;
+
+    // --- weights, a step at a time
+    uint32_t ptile = lo / nq, pq = lo - ptile * nq, pleft = hi - lo;
+    auto request = [&](int slot) {
+        if (pleft == 0) return;
+        mbar_arrive_expect_tx(bars + slot, kTcStepBytes);
+        tma_load_2d(ring + slot * kTcStepBytes, &map, bars + slot, static_cast<int>((k_step0 + pq) * (kStepK / 2)),
+                    static_cast<int>(ptile * kTcRows));
+        --pleft;
+        if (++pq == nq) { pq = 0; ++ptile; }
+    };
+    if (issuer && lane == 0) {
+        for (int i = 0; i < p.slots; ++i) mbar_init(bars + i, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(code_bars + i, kWarps);
+            mbar_init(done_bars + i, 1);
         }
-        sync();
-        for (uint32_t i = warp; i < kTeamThreads && t0 + i <= tile; i += kWarps) {      // a warp to a tile
-            if (last[i] == 0) continue;
-            const uint32_t at = t0 + i;
-            for (int v = lane; v < kRows / 4 * mt; v += 32) {
-                const int r = 4 * v % kRows, m = 4 * v / kRows;
-                float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                for (uint32_t y = 0; y < gridDim.y; ++y) {
-                    const uint32_t ny = p.steps - y * per < per ? p.steps - y * per : per;
-                    const Shares sy(p.tiles, ny, gridDim.x * kTeams);
-                    const uint32_t s0 = sy.holder(at * ny), s1 = sy.holder(at * ny + ny - 1);
-                    const float4* from = reinterpret_cast<const float4*>(range_slots(y)) + v;
-#pragma unroll 4
-                    for (uint32_t s = s0; s <= s1; ++s) {
-                        const float4 x = __ldcg(from + (s == s0 ? at : p.tiles + s) * static_cast<size_t>(kRows / 4 * ROWS));
-                        sum.x += x.x;
-                        sum.y += x.y;
-                        sum.z += x.z;
-                        sum.w += x.w;
+        if (team == 0) {
+            *odd = 0u;
+            mbar_init(image_bar, 1);
+        }
+        fence_mbar_init();
+        for (int s = 0; s < p.slots; ++s) request(s);
+    }
+    __syncwarp();
+    if (tid < 32) {
+        tmem_alloc(tmem_at, kTeams * kTcColumns);
+        tmem_relinquish();
+    }
+
+    // --- scales are read one step ahead, across the ends of tiles
+    const int up = f32s ? 0 : 16;
+    auto fetch = [&](const void* base, int64_t e) -> uint32_t {
+        return f32s ? __ldg(static_cast<const uint32_t*>(base) + e) : __ldg(static_cast<const uint16_t*>(base) + e);
+    };
+    auto value = [&](uint32_t raw) { return __uint_as_float(raw << up); };
+    auto group_of = [&](uint32_t chunk) { return min(static_cast<int>(__umulhi(2 * chunk, p.gmul) >> p.gshift), g.groups - 1); };
+    const int scale_bytes = f32s ? 4 : 2;
+    const int64_t to_zero = reinterpret_cast<intptr_t>(g.zero) - reinterpret_cast<intptr_t>(g.scale);
+    uint32_t atile = lo / nq, aq = lo - atile * nq, aleft = hi - lo;
+    const char* srow = nullptr;
+    uint32_t raw[NF] = {}, rawz[NF] = {};
+    auto open = [&]() {
+        const int64_t row = static_cast<int64_t>(atile) * kTcRows + tt;
+        srow = static_cast<const char*>(g.scale) + (row < g.N ? row : g.N - 1) * g.lds * scale_bytes;
+    };
+    auto fetch_scales = [&]() {
+        if (aleft == 0) return;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            const int64_t gi = static_cast<int64_t>(group_of((k_step0 + aq) * 4 + f * F)) * scale_bytes;
+            raw[f] = ldg_scale(srow + gi, f32s);
+            if (zeros) rawz[f] = ldg_scale(srow + gi + to_zero, f32s);
+        }
+        --aleft;
+        if (++aq == nq) {
+            aq = 0;
+            ++atile;
+            open();
+        }
+    };
+    if (busy && !issuer) {
+        open();
+        fetch_scales();
+    }
+
+    // --- the K-range's activations as digits: from the kernel before, or made here
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_at;
+    if (p.images) {
+        if (tid == 0) {
+            pdl_wait();
+            asm volatile("fence.proxy.async;" ::: "memory");
+            const size_t at = (static_cast<size_t>(blockIdx.z) * gridDim.y + blockIdx.y) * p.image_bytes;
+            mbar_arrive_expect_tx(image_bar, p.image_bytes);
+            bulk_load_1d(act, p.images + at, p.image_bytes, image_bar);
+        }
+        mbar_wait(image_bar, 0, nullptr, p.err);
+    } else {
+        const bool vec = g.lda % (16 / sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(g.A) % 16 == 0;
+        const uint32_t units = mt * nq, r = tid & 15;
+        uint32_t u0 = (tid >> 4) & ~1u;
+        if (issuer) u0 = units;
+        for (; u0 < units; u0 += kTeams * kTeamThreads / 16) {    // the same count for a whole warp
+            const uint32_t u = u0 + ((tid >> 4) & 1), m = u / nq, q = u - m * nq;
+            stage<IO, false, F, true>(p, img, m0, k_step0, m, q, r, vec, u < units);
+        }
+        fence_proxy_async_smem();
+        __syncthreads();
+    }
+    for (uint32_t i = tid; i < mt * nq; i += kTcThreads) {
+        const uint32_t q = i / mt, m = i - q * mt;
+        const float u = img.unit[q * ROWS + m];
+        if (u < 0.0f) {
+            atomicOr(odd, 1u << m);
+            img.unit[q * ROWS + m] = -u;
+        }
+    }
+    __syncthreads();
+
+    auto sync = [&]() { named_barrier_sync(1 + team, kTeamThreads); };
+    // The slots of K-range y.
+    auto range_slots = [&](uint32_t y) {
+        return p.ws + (static_cast<size_t>(blockIdx.z) * gridDim.y + y) * (p.tiles + gridDim.x * kTeams) * (kTcRows * ROWS);
+    };
+    const uint32_t own = tmem + team * kTcColumns, lanes = static_cast<uint32_t>(warp) << 21;  // 32 lanes a warp, in bits 16 up
+    const uint32_t ring_at = smem_u32(ring) + tt * 64, swz = (tt >> 1) & 3, act_at = smem_u32(act);
+    const uint32_t base_at = smem_u32(img.base), unit_at = smem_u32(img.unit), isum_at = smem_u32(img.isum);
+    uint32_t step = 0, phase = 0;
+    int slot = 0;
+    bool dead = false;
+    if (issuer) {
+        if (lane == 0) {
+            uint32_t q = lo - lo / nq * nq;
+            for (uint32_t left = hi - lo; left > 0; --left, ++step) {
+                const uint32_t i = step & 1;
+                if (!mbar_try_wait(code_bars + i, (step >> 1) & 1) && !dead) dead = !mbar_wait(code_bars + i, (step >> 1) & 1, nullptr, p.err);
+                tc_fence_after();
+                const uint64_t b = umma_desc_k_sw128(act_at + q * (NC * 128));
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    umma_i8_ts(own + 64 + i * 32 + (k / F) * NM, own + i * 32 + k * 8, b + k * 2, IDESC, k % F != 0);
+                umma_commit(done_bars + i);
+                request(slot);      // every thread has read it
+                if (++slot == p.slots) slot = 0;
+                if (++q == nq) q = 0;
+            }
+        }
+        __syncwarp();
+    }
+    float2 tot[ROWS / 2];
+    // Scales the products of the step before: i counts steps, q is its place in the K-range.
+    auto scale_step = [&](uint32_t i, uint32_t q, const float (&sc)[NF], const float (&zr)[NF]) {
+        if (!mbar_try_wait(done_bars + (i & 1), (i >> 1) & 1) && !dead) dead = !mbar_wait(done_bars + (i & 1), (i >> 1) & 1, nullptr, p.err);
+        __syncwarp();
+        tc_fence_after();
+        const uint32_t from = own + lanes + 64 + (i & 1) * 32;
+        constexpr int MB = ROWS < 4 ? ROWS : 4;     // rows of A at a time
+#pragma unroll
+        for (int m0 = 0; m0 < ROWS; m0 += MB) {
+            float un[MB];
+            if constexpr (MB == 4) {
+                const uint4 v = lds128(unit_at + (q * ROWS + m0) * 4);
+                un[0] = __uint_as_float(v.x); un[1] = __uint_as_float(v.y);
+                un[2] = __uint_as_float(v.z); un[3] = __uint_as_float(v.w);
+            } else {
+                un[0] = img.unit[q * ROWS];
+                un[1] = img.unit[q * ROWS + 1];
+            }
+#pragma unroll
+            for (int f = 0; f < NF; ++f) {
+                uint32_t c[MB == 4 ? D : 2][4];         // digit after digit, MB columns of each
+                if constexpr (MB == 4) {
+#pragma unroll
+                    for (int d = 0; d < D; ++d) tmem_ld_x4(from + f * NM + d * ROWS + m0, c[d]);
+                } else {
+                    tmem_ld_x8(from + f * NM, &c[0][0]);
+                }
+                tmem_ld_wait();
+#pragma unroll
+                for (int d = 0; d < (MB == 4 ? D : 2); ++d) {
+                    const uint4 v = lds128(base_at + ((q * NF + f) * NC + (MB == 4 ? d * ROWS + m0 : 4 * d)) * 4);
+                    c[d][0] += v.x; c[d][1] += v.y; c[d][2] += v.z; c[d][3] += v.w;
+                }
+#pragma unroll
+                for (int m = 0; m < MB; m += 2) {
+                    auto digit = [&](int d) {
+                        const uint32_t* at = &c[0][0] + d * MB + m;
+                        return add2(bits2(at), make_float2(-kMagic, -kMagic));
+                    };
+                    float2 y = digit(D - 1);
+#pragma unroll
+                    for (int d = D - 2; d >= 0; --d) y = fma2(y, make_float2(256.0f, 256.0f), digit(d));
+                    if (zeros) {
+                        const float2 is = *reinterpret_cast<const float2*>(img.isum + (q * NF + f) * ROWS + m0 + m);
+                        y = fma2(make_float2(zr[f], zr[f]), is, y);
+                    }
+                    tot[(m0 + m) / 2] = fma2(mul2(make_float2(sc[f], sc[f]), make_float2(un[m], un[m + 1])), y, tot[(m0 + m) / 2]);
+                }
+            }
+        }
+    };
+
+    if (busy && !issuer) {
+        uint32_t tile = lo / nq, q0 = lo - tile * nq, done = lo;
+        while (done < hi) {
+            const uint32_t n = hi - done < nq - q0 ? hi - done : nq - q0, q1 = q0 + n;
+#pragma unroll
+            for (int m = 0; m < ROWS / 2; ++m) tot[m] = make_float2(0.0f, 0.0f);
+            float sc[NF], zr[NF];
+            for (uint32_t q = q0; q < q1; ++q) {
+                if (!mbar_try_wait(bars + slot, phase) && !dead) dead = !mbar_wait(bars + slot, phase, nullptr, p.err);
+                uint32_t a[32];     // byte b of word 2j + h is code 8j + 2b + h
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const uint4 v = lds128(ring_at + slot * kTcStepBytes + ((c ^ swz) << 4));
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        a[8 * c + 2 * j] = w[j] & 0x0F0F0F0Fu;
+                        a[8 * c + 2 * j + 1] = (w[j] >> 4) & 0x0F0F0F0Fu;
                     }
                 }
-                const float x[4] = {sum.x, sum.y, sum.z, sum.w};
+                __syncwarp();
+                tmem_st_x32(own + lanes + (step & 1) * 32, a);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(code_bars + (step & 1));
+                if (++slot == p.slots) { slot = 0; phase ^= 1u; }
+                if (q > q0) scale_step(step - 1, q - 1, sc, zr);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int64_t row = static_cast<int64_t>(at) * kRows + r + j;
-                    if (row < g.N)
-                        static_cast<T*>(g.C)[static_cast<int64_t>(m0 + m) * g.ldc + row] =
-                            static_cast<T>(x[j] + (g.bias ? g.bias[row] : 0.0f));
+                for (int f = 0; f < NF; ++f) {
+                    sc[f] = value(raw[f]);
+                    zr[f] = 8.0f - (zeros ? value(rawz[f]) : 8.0f);
+                }
+                fetch_scales();
+                ++step;
+            }
+            scale_step(step - 1, q1 - 1, sc, zr);
+
+            // --- the tile's end in this share
+            const bool whole = n == nq && gridDim.y == 1;
+            float* part_sums = whole ? nullptr : range_slots(blockIdx.y) + static_cast<size_t>(lo <= tile * nq ? tile : p.tiles + share) * (kTcRows * ROWS);
+            const int64_t row = static_cast<int64_t>(tile) * kTcRows + tt;
+            if (row < g.N) {
+#pragma unroll
+                for (int m = 0; m < ROWS; ++m) {
+                    if (m >= mt) continue;
+                    float sum = m % 2 ? tot[m / 2].y : tot[m / 2].x;
+                    if ((*odd >> m) & 1u) {
+                        // The activations that stayed out.
+                        const T* x = static_cast<const T*>(g.A) + static_cast<int64_t>(m0 + m) * g.lda;
+                        const int64_t k1 = static_cast<int64_t>(k_step0 + q1) * kStepK < g.K ? static_cast<int64_t>(k_step0 + q1) * kStepK : g.K;
+                        for (int64_t k = static_cast<int64_t>(k_step0 + q0) * kStepK; k < k1; ++k) {
+                            const float v = static_cast<float>(x[k]);
+                            if (fabsf(v) <= 3.402823466e38f) continue;
+                            const uint32_t code = (g.W[row * g.ldw + k / 2] >> (4 * (k & 1))) & 15u;
+                            const int64_t e = row * g.lds + k / g.group;
+                            sum += v * (value(fetch(g.scale, e)) * (static_cast<float>(code) - (zeros ? value(fetch(g.zero, e)) : 8.0f)));
+                        }
+                    }
+                    if (whole) {
+                        const float out = sum + (g.bias ? g.bias[row] : 0.0f);
+                        static_cast<T*>(g.C)[static_cast<int64_t>(m0 + m) * g.ldc + row] = static_cast<T>(out);
+                    } else {
+                        part_sums[m * kTcRows + tt] = sum;
+                    }
                 }
             }
+            done += n;
+            if (done < hi) { ++tile; q0 = 0; }
         }
-        sync();
+        sync();     // the team's sums are written
+        join_tiles<T, kTcRows, ROWS, 1>(p, shares, share, nq, m0, mt, tile, last, range_slots, sync);
     }
+    tc_fence_before();
+    __syncthreads();
+    if (tid < 32) tmem_dealloc(tmem, kTeams * kTcColumns);
 }
 
 // Rows of W at multiples of 16 bytes: a warp copies a row's words of four bytes, each cut from the two
@@ -709,8 +1080,21 @@ struct Kernel {
     const void* fn;
     const void* digits;
     int rows, n_digits, flush;
-    bool packed;
+    bool packed, tc;
 };
+
+template <DType IO, int ROWS, int F>
+Kernel tc_kernel() {
+    return {reinterpret_cast<const void*>(&gemm_w4_tc_kernel<IO, ROWS, F>),
+            reinterpret_cast<const void*>(&gemm_w4_digits_kernel<IO, false, F, true>), ROWS, IO == DType::F32 ? 4 : 3, F, false, true};
+}
+
+template <DType IO>
+Kernel tc_kernel_for(int M, int f) {
+    if (M <= 2) return f == 4 ? tc_kernel<IO, 2, 4>() : tc_kernel<IO, 2, 2>();
+    if (M <= 4) return f == 4 ? tc_kernel<IO, 4, 4>() : tc_kernel<IO, 4, 2>();
+    return tc_kernel<IO, 8, 4>();
+}
 
 template <DType IO, bool PACKED>
 Kernel kernel_for_flush(int f) {
@@ -718,15 +1102,17 @@ Kernel kernel_for_flush(int f) {
     const void* fn = f == 4 ? reinterpret_cast<const void*>(&gemm_w4_kernel<IO, PACKED, 4>)
                      : f == 2 ? reinterpret_cast<const void*>(&gemm_w4_kernel<IO, PACKED, 2>)
                               : reinterpret_cast<const void*>(&gemm_w4_kernel<IO, PACKED, 1>);
-    const void* digits = f == 4 ? reinterpret_cast<const void*>(&gemm_w4_digits_kernel<IO, PACKED, 4>)
-                         : f == 2 ? reinterpret_cast<const void*>(&gemm_w4_digits_kernel<IO, PACKED, 2>)
-                                  : reinterpret_cast<const void*>(&gemm_w4_digits_kernel<IO, PACKED, 1>);
-    return {fn, digits, PACKED ? 8 / D : 8, D, f, PACKED};
+    const void* digits = f == 4 ? reinterpret_cast<const void*>(&gemm_w4_digits_kernel<IO, PACKED, 4, false>)
+                         : f == 2 ? reinterpret_cast<const void*>(&gemm_w4_digits_kernel<IO, PACKED, 2, false>)
+                                  : reinterpret_cast<const void*>(&gemm_w4_digits_kernel<IO, PACKED, 1, false>);
+    return {fn, digits, PACKED ? 8 / D : 8, D, f, PACKED, false};
 }
 
 Kernel select(const W4Args& g) {
     // How many chunks of 32 weights share their scales for sure, up to the four of a step.
     const int f = g.groups == 1 || g.group % 128 == 0 ? 4 : (g.group % 64 == 0 ? 2 : 1);
+    if (TCMODE && (f == 4 || (g.M <= 4 && f == 2)))
+        return g.io == DType::F32 ? tc_kernel_for<DType::F32>(g.M, f) : tc_kernel_for<DType::BF16>(g.M, f);
     // Two rows' digits fit one block of columns: a third (a quarter) of the products.
     if (g.io == DType::F32) return g.M <= 2 ? kernel_for_flush<DType::F32, true>(f) : kernel_for_flush<DType::F32, false>(f);
     return g.M <= 2 ? kernel_for_flush<DType::BF16, true>(f) : kernel_for_flush<DType::BF16, false>(f);
@@ -767,14 +1153,14 @@ EncodeTiled encode_tiled() {
 }
 
 // W as bytes [N][(K+1)/2], read in boxes of 64 bytes x 32 rows; bytes and rows past the ends read as zeros.
-bool encode_weights(const W4Args& g, const uint8_t* w, int64_t pitch, CUtensorMap* map) {
+bool encode_weights(const W4Args& g, const uint8_t* w, int64_t pitch, bool tc, CUtensorMap* map) {
     EncodeTiled fn = encode_tiled();
     if (!fn) return false;
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(row_bytes_of(g)), static_cast<cuuint64_t>(g.N)};
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
-    const cuuint32_t box[2] = {kStepK / 2, kRows}, one[2] = {1, 1};
+    const cuuint32_t box[2] = {kStepK / 2, static_cast<cuuint32_t>(tc ? kTcRows : kRows)}, one[2] = {1, 1};
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(w), dims, strides, box, one,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, tc ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -782,27 +1168,28 @@ bool encode_weights(const W4Args& g, const uint8_t* w, int64_t pitch, CUtensorMa
 
 bool gemm_w4_plan(const W4Args& g, int num_sms, W4Plan* plan) {
     const Kernel k = select(g);
-    plan->rows = g.M < k.rows ? g.M : k.rows;
-    const int64_t steps = (static_cast<int64_t>(g.K) + kStepK - 1) / kStepK, tiles = (static_cast<int64_t>(g.N) + kRows - 1) / kRows;
-    plan->cols = k.n_digits * plan->rows;
+    const int tile_rows = k.tc ? kTcRows : kRows, step_bytes = k.tc ? kTcStepBytes : kStepBytes;
+    plan->rows = !k.tc && g.M < k.rows ? g.M : k.rows;
+    const int64_t steps = (static_cast<int64_t>(g.K) + kStepK - 1) / kStepK, tiles = (static_cast<int64_t>(g.N) + tile_rows - 1) / tile_rows;
+    plan->cols = k.tc ? (k.n_digits * plan->rows + 7) / 8 * 8 : k.n_digits * plan->rows;
     // As much of K at a time as the digits leave room for beside the smallest rings; the rings take
     // what is left.
-    const int warps = kTeams * kWarps;
-    const int fixed = warps * (1024 + kMaxSlots * 8) + 64 + 16;
+    const int rings = k.tc ? kTeams : kTeams * kWarps, bars = k.tc ? kTeams * (kMaxSlots + 4) * 8 : kTeams * kWarps * kMaxSlots * 8;
+    const int fixed = kTeams * (k.tc ? kTeamThreads * 4 : kWarps * 1024) + bars + 64 + 16;
     const int per_step = plan->cols * (128 + 4 * (4 / k.flush)) + 4 * (k.packed ? plan->cols : plan->rows) * (1 + 4 / k.flush);
-    const int64_t most = (kMaxSmem - fixed - warps * kMinSlots * kStepBytes) / per_step;
+    const int64_t most = (kMaxSmem - fixed - rings * kMinSlots * step_bytes) / per_step;
     const int64_t splits = (steps + most - 1) / most;
     plan->split_steps = static_cast<int>((steps + splits - 1) / splits);
     plan->splits = static_cast<int>((steps + plan->split_steps - 1) / plan->split_steps);
-    const int rest = (kMaxSmem - fixed - per_step * plan->split_steps) / (warps * kStepBytes);
+    const int rest = (kMaxSmem - fixed - per_step * plan->split_steps) / (rings * step_bytes);
     plan->slots = rest < kMaxSlots ? rest : kMaxSlots;
-    plan->smem = fixed + per_step * plan->split_steps + warps * plan->slots * kStepBytes;
-    plan->bars_at = (plan->smem - warps * kMaxSlots * 8 - 16) & ~7;
+    plan->smem = fixed + per_step * plan->split_steps + rings * plan->slots * step_bytes;
+    plan->bars_at = (plan->smem - bars - 16) & ~7;
     plan->image_bytes = (per_step * plan->split_steps + 15) & ~15;
     // 512 threads take half a microsecond for every 32 stretches of 128 activations; a kernel before
     // this one takes about one and overlaps this one's start (1x28672x8192, 64 stretches: 30.0 us
     // without and 31.0 with it; 5x4093x4099 FP32, 165: 21.6 and 19.5; 8x28672x8192, 256: 47.3 and 44.1).
-    const int64_t stretches = static_cast<int64_t>(plan->rows) * plan->split_steps;
+    const int64_t stretches = static_cast<int64_t>(g.M < k.rows ? g.M : k.rows) * plan->split_steps;
     plan->prepared = stretches > 64;
     plan->pitch = aligned_rows(g) ? 0 : (row_bytes_of(g) + 15) / 16 * 16;
     plan->copy_bytes = static_cast<size_t>(plan->pitch) * g.N;
@@ -811,12 +1198,12 @@ bool gemm_w4_plan(const W4Args& g, int num_sms, W4Plan* plan) {
     if (plan->prepared) plan->extra_bytes += static_cast<size_t>(plan->blocks) * plan->splits * plan->image_bytes;
     // Every SM a CTA, shared among the K-ranges; no more than there are shares of eight steps.
     int64_t ctas = (num_sms + plan->splits - 1) / plan->splits;
-    const int64_t shares = (tiles * plan->split_steps + kWarps - 1) / kWarps;
+    const int64_t shares = (tiles * plan->split_steps + (k.tc ? kTeams : kWarps) - 1) / (k.tc ? kTeams : kWarps);
     if (ctas > shares) ctas = shares;
     plan->ctas = static_cast<int>(ctas);
     // Steps are counted in 32 bits; blocks and splits are grid dimensions.
     if (tiles * plan->split_steps > INT32_MAX || plan->splits > 65535 || plan->blocks > 65535) return false;
-    plan->ws_floats = static_cast<size_t>(plan->blocks) * plan->splits * (tiles + ctas * kTeams) * kRows * k.rows;
+    plan->ws_floats = static_cast<size_t>(plan->blocks) * plan->splits * (tiles + ctas * kTeams) * tile_rows * k.rows;
     plan->tickets = static_cast<size_t>(plan->blocks) * tiles;
     return true;
 }
@@ -840,7 +1227,8 @@ cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint3
     }
     Params p;
     p.g = g;
-    p.tiles = static_cast<int>((static_cast<int64_t>(g.N) + kRows - 1) / kRows);
+    const int tile_rows = k.tc ? kTcRows : kRows;
+    p.tiles = static_cast<int>((static_cast<int64_t>(g.N) + tile_rows - 1) / tile_rows);
     p.steps = static_cast<int>((static_cast<int64_t>(g.K) + kStepK - 1) / kStepK);
     p.split_steps = plan.split_steps;
     p.slots = plan.slots;
@@ -866,12 +1254,12 @@ cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint3
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
     }
     CUtensorMap map;
-    if (!encode_weights(g, w, pitch, &map)) return cudaErrorNotSupported;
+    if (!encode_weights(g, w, pitch, k.tc, &map)) return cudaErrorNotSupported;
     p.image_bytes = plan.image_bytes;
     p.images = nullptr;
     if (plan.prepared) {
         p.images = static_cast<unsigned char*>(extra) + plan.copy_bytes;
-        const unsigned stretches = static_cast<unsigned>(plan.rows) * plan.split_steps;
+        const unsigned stretches = static_cast<unsigned>(g.M < plan.rows ? g.M : plan.rows) * plan.split_steps;
         void* first[] = {&p};
         e = launch_pdl(k.digits, dim3((stretches + 7) / 8, plan.splits, plan.blocks), 128, first, 0, s);
         if (e != cudaSuccess) return e;
@@ -879,7 +1267,7 @@ cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint3
     // With digits made before it, the kernel starts before they are done: all that it reads or writes
     // until it waits for them is older than the kernel that makes them, or its own.
     void* args[] = {&p, &map};
-    return launch_pdl(k.fn, dim3(plan.ctas, plan.splits, plan.blocks), kTeams * kTeamThreads, args, plan.smem, s);
+    return launch_pdl(k.fn, dim3(plan.ctas, plan.splits, plan.blocks), k.tc ? kTcThreads : kTeams * kTeamThreads, args, plan.smem, s);
 }
 
 }  // namespace dnnopt_b200
