@@ -753,12 +753,8 @@ __device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t* r) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_ld_x4(uint32_t taddr, uint32_t (&r)[4]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr));
-}
-
 // ROWS: of A per pass (2, 4 or 8); F as above.
-template <DType IO, int ROWS, int F>
+template <DType IO, int ROWS, int F, bool ZEROS>
 __global__ void __launch_bounds__(kTcThreads, 1)
 gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     using T = typename std::conditional<IO == DType::F32, float, __nv_bfloat16>::type;
@@ -788,7 +784,6 @@ gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     bars += team * (kMaxSlots + 4);
     uint64_t* code_bars = bars + kMaxSlots;         // a step's codes are in tensor memory
     uint64_t* done_bars = code_bars + 2;            // and its products
-    const bool zeros = g.zero != nullptr;
     const bool f32s = g.st == DType::F32;
 
     if (!p.images) pdl_wait();
@@ -833,25 +828,35 @@ gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
         return f32s ? __ldg(static_cast<const uint32_t*>(base) + e) : __ldg(static_cast<const uint16_t*>(base) + e);
     };
     auto value = [&](uint32_t raw) { return __uint_as_float(raw << up); };
-    auto group_of = [&](uint32_t chunk) { return min(static_cast<int>(__umulhi(2 * chunk, p.gmul) >> p.gshift), g.groups - 1); };
     const int scale_bytes = f32s ? 4 : 2;
     const int64_t to_zero = reinterpret_cast<intptr_t>(g.zero) - reinterpret_cast<intptr_t>(g.scale);
     uint32_t atile = lo / nq, aq = lo - atile * nq, aleft = hi - lo;
-    const char* srow = nullptr;
-    uint32_t raw[NF] = {}, rawz[NF] = {};
+    const char* sat = nullptr;      // the scale of the row's group
+    int within = 0;                 // weights of that group before
+    uint32_t raw[NF] = {}, rawz[ZEROS ? NF : 1] = {};
     auto open = [&]() {
-        const int64_t row = static_cast<int64_t>(atile) * kTcRows + tt;
-        srow = static_cast<const char*>(g.scale) + (row < g.N ? row : g.N - 1) * g.lds * scale_bytes;
+        const int64_t row = static_cast<int64_t>(atile) * kTcRows + tt, k = static_cast<int64_t>(k_step0 + aq) * kStepK;
+        const int group = static_cast<int>(g.groups > 1 ? k / g.group : 0);
+        within = static_cast<int>(k - static_cast<int64_t>(group) * g.group);
+        sat = static_cast<const char*>(g.scale) + ((row < g.N ? row : g.N - 1) * g.lds + group) * scale_bytes;
     };
     auto fetch_scales = [&]() {
         if (aleft == 0) return;
+        --aleft;
 #pragma unroll
         for (int f = 0; f < NF; ++f) {
-            const int64_t gi = static_cast<int64_t>(group_of((k_step0 + aq) * 4 + f * F)) * scale_bytes;
-            raw[f] = ldg_scale(srow + gi, f32s);
-            if (zeros) rawz[f] = ldg_scale(srow + gi + to_zero, f32s);
+            if (f == 0 || (k_step0 + aq) * kStepK + f * F * 32 < static_cast<uint32_t>(g.K)) {
+                raw[f] = ldg_scale(sat, f32s);
+                if constexpr (ZEROS) rawz[f] = ldg_scale(sat + to_zero, f32s);
+            } else {
+                raw[f] = 0u;        // past the last weight
+            }
+            within += F * 32;
+            if (within >= g.group) {
+                within = 0;
+                sat += scale_bytes;
+            }
         }
-        --aleft;
         if (++aq == nq) {
             aq = 0;
             ++atile;
@@ -936,48 +941,40 @@ gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
         __syncwarp();
         tc_fence_after();
         const uint32_t from = own + lanes + 64 + (i & 1) * 32;
-        constexpr int MB = ROWS < 4 ? ROWS : 4;     // rows of A at a time
 #pragma unroll
-        for (int m0 = 0; m0 < ROWS; m0 += MB) {
-            float un[MB];
-            if constexpr (MB == 4) {
-                const uint4 v = lds128(unit_at + (q * ROWS + m0) * 4);
-                un[0] = __uint_as_float(v.x); un[1] = __uint_as_float(v.y);
-                un[2] = __uint_as_float(v.z); un[3] = __uint_as_float(v.w);
-            } else {
-                un[0] = img.unit[q * ROWS];
-                un[1] = img.unit[q * ROWS + 1];
+        for (int f = 0; f < NF; ++f) {
+            uint32_t c[NC];
+#pragma unroll
+            for (int b = 0; b < NC; b += 8) tmem_ld_x8(from + f * NM + b, c + b);
+            float un[ROWS];
+#pragma unroll
+            for (int m = 0; m < ROWS; m += 4) {
+                if constexpr (ROWS >= 4) {
+                    const uint4 v = lds128(unit_at + (q * ROWS + m) * 4);
+                    un[m] = __uint_as_float(v.x); un[m + 1] = __uint_as_float(v.y);
+                    un[m + 2] = __uint_as_float(v.z); un[m + 3] = __uint_as_float(v.w);
+                } else {
+                    un[0] = img.unit[q * ROWS];
+                    un[1] = img.unit[q * ROWS + 1];
+                }
+            }
+            tmem_ld_wait();
+#pragma unroll
+            for (int b = 0; b < NC; b += 4) {
+                const uint4 v = lds128(base_at + ((q * NF + f) * NC + b) * 4);
+                c[b] += v.x; c[b + 1] += v.y; c[b + 2] += v.z; c[b + 3] += v.w;
             }
 #pragma unroll
-            for (int f = 0; f < NF; ++f) {
-                uint32_t c[MB == 4 ? D : 2][4];         // digit after digit, MB columns of each
-                if constexpr (MB == 4) {
+            for (int m = 0; m < ROWS; m += 2) {
+                auto digit = [&](int d) { return add2(bits2(c + d * ROWS + m), make_float2(-kMagic, -kMagic)); };
+                float2 y = digit(D - 1);
 #pragma unroll
-                    for (int d = 0; d < D; ++d) tmem_ld_x4(from + f * NM + d * ROWS + m0, c[d]);
-                } else {
-                    tmem_ld_x8(from + f * NM, &c[0][0]);
+                for (int d = D - 2; d >= 0; --d) y = fma2(y, make_float2(256.0f, 256.0f), digit(d));
+                if constexpr (ZEROS) {
+                    const float2 is = *reinterpret_cast<const float2*>(img.isum + (q * NF + f) * ROWS + m);
+                    y = fma2(make_float2(zr[f], zr[f]), is, y);
                 }
-                tmem_ld_wait();
-#pragma unroll
-                for (int d = 0; d < (MB == 4 ? D : 2); ++d) {
-                    const uint4 v = lds128(base_at + ((q * NF + f) * NC + (MB == 4 ? d * ROWS + m0 : 4 * d)) * 4);
-                    c[d][0] += v.x; c[d][1] += v.y; c[d][2] += v.z; c[d][3] += v.w;
-                }
-#pragma unroll
-                for (int m = 0; m < MB; m += 2) {
-                    auto digit = [&](int d) {
-                        const uint32_t* at = &c[0][0] + d * MB + m;
-                        return add2(bits2(at), make_float2(-kMagic, -kMagic));
-                    };
-                    float2 y = digit(D - 1);
-#pragma unroll
-                    for (int d = D - 2; d >= 0; --d) y = fma2(y, make_float2(256.0f, 256.0f), digit(d));
-                    if (zeros) {
-                        const float2 is = *reinterpret_cast<const float2*>(img.isum + (q * NF + f) * ROWS + m0 + m);
-                        y = fma2(make_float2(zr[f], zr[f]), is, y);
-                    }
-                    tot[(m0 + m) / 2] = fma2(mul2(make_float2(sc[f], sc[f]), make_float2(un[m], un[m + 1])), y, tot[(m0 + m) / 2]);
-                }
+                tot[m / 2] = fma2(mul2(make_float2(sc[f], sc[f]), make_float2(un[m], un[m + 1])), y, tot[m / 2]);
             }
         }
     };
@@ -1013,7 +1010,7 @@ gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
 #pragma unroll
                 for (int f = 0; f < NF; ++f) {
                     sc[f] = value(raw[f]);
-                    zr[f] = 8.0f - (zeros ? value(rawz[f]) : 8.0f);
+                    zr[f] = ZEROS ? 8.0f - value(rawz[f]) : 0.0f;
                 }
                 fetch_scales();
                 ++step;
@@ -1038,7 +1035,7 @@ gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
                             if (fabsf(v) <= 3.402823466e38f) continue;
                             const uint32_t code = (g.W[row * g.ldw + k / 2] >> (4 * (k & 1))) & 15u;
                             const int64_t e = row * g.lds + k / g.group;
-                            sum += v * (value(fetch(g.scale, e)) * (static_cast<float>(code) - (zeros ? value(fetch(g.zero, e)) : 8.0f)));
+                            sum += v * (value(fetch(g.scale, e)) * (static_cast<float>(code) - (ZEROS ? value(fetch(g.zero, e)) : 8.0f)));
                         }
                     }
                     if (whole) {
@@ -1084,16 +1081,17 @@ struct Kernel {
 };
 
 template <DType IO, int ROWS, int F>
-Kernel tc_kernel() {
-    return {reinterpret_cast<const void*>(&gemm_w4_tc_kernel<IO, ROWS, F>),
+Kernel tc_kernel(bool zeros) {
+    return {zeros ? reinterpret_cast<const void*>(&gemm_w4_tc_kernel<IO, ROWS, F, true>)
+                  : reinterpret_cast<const void*>(&gemm_w4_tc_kernel<IO, ROWS, F, false>),
             reinterpret_cast<const void*>(&gemm_w4_digits_kernel<IO, false, F, true>), ROWS, IO == DType::F32 ? 4 : 3, F, false, true};
 }
 
 template <DType IO>
-Kernel tc_kernel_for(int M, int f) {
-    if (M <= 2) return f == 4 ? tc_kernel<IO, 2, 4>() : tc_kernel<IO, 2, 2>();
-    if (M <= 4) return f == 4 ? tc_kernel<IO, 4, 4>() : tc_kernel<IO, 4, 2>();
-    return tc_kernel<IO, 8, 4>();
+Kernel tc_kernel_for(int M, int f, bool zeros) {
+    if (M <= 2) return f == 4 ? tc_kernel<IO, 2, 4>(zeros) : tc_kernel<IO, 2, 2>(zeros);
+    if (M <= 4) return f == 4 ? tc_kernel<IO, 4, 4>(zeros) : tc_kernel<IO, 4, 2>(zeros);
+    return tc_kernel<IO, 8, 4>(zeros);
 }
 
 template <DType IO, bool PACKED>
@@ -1112,7 +1110,7 @@ Kernel select(const W4Args& g) {
     // How many chunks of 32 weights share their scales for sure, up to the four of a step.
     const int f = g.groups == 1 || g.group % 128 == 0 ? 4 : (g.group % 64 == 0 ? 2 : 1);
     if (TCMODE && (f == 4 || (g.M <= 4 && f == 2)))
-        return g.io == DType::F32 ? tc_kernel_for<DType::F32>(g.M, f) : tc_kernel_for<DType::BF16>(g.M, f);
+        return g.io == DType::F32 ? tc_kernel_for<DType::F32>(g.M, f, g.zero != nullptr) : tc_kernel_for<DType::BF16>(g.M, f, g.zero != nullptr);
     // Two rows' digits fit one block of columns: a third (a quarter) of the products.
     if (g.io == DType::F32) return g.M <= 2 ? kernel_for_flush<DType::F32, true>(f) : kernel_for_flush<DType::F32, false>(f);
     return g.M <= 2 ? kernel_for_flush<DType::BF16, true>(f) : kernel_for_flush<DType::BF16, false>(f);
