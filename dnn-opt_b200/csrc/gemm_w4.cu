@@ -52,9 +52,6 @@
 namespace dnnopt_b200 {
 namespace {
 
-#ifndef TCMODE
-#define TCMODE 1
-#endif
 constexpr int kTeams = 4;           // per CTA
 constexpr int kTeamThreads = 128;
 constexpr int kWarps = 4;           // per team
@@ -373,20 +370,30 @@ __device__ __forceinline__ void join_tiles(const Params& p, const Shares& shares
             float4 sum[NV];
 #pragma unroll
             for (int j = 0; j < NV; ++j) sum[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (uint32_t y = 0; y < gridDim.y; ++y) {
-                const uint32_t ny = p.steps - y * per < per ? p.steps - y * per : per;
-                const Shares sy(p.tiles, ny, gridDim.x * kTeams, WARPS);
-                const uint32_t s0 = sy.holder(at * ny), s1 = sy.holder(at * ny + ny - 1);
-                const float4* from = reinterpret_cast<const float4*>(range_slots(y)) + tt % EACH;
-                for (uint32_t s = s0; s <= s1; s += 4) {        // four parts asked for at once
+            for (uint32_t y = 0; y < gridDim.y; y += 2) {       // two K-ranges' parts, four asked for at once
+                const float4* from[2] = {};
+                uint32_t s0[2], n[2] = {};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (y + h >= gridDim.y) continue;
+                    const uint32_t ny = p.steps - (y + h) * per < per ? p.steps - (y + h) * per : per;
+                    const Shares sy(p.tiles, ny, gridDim.x * kTeams, WARPS);
+                    s0[h] = sy.holder(at * ny);
+                    n[h] = sy.holder(at * ny + ny - 1) - s0[h] + 1;
+                    from[h] = reinterpret_cast<const float4*>(range_slots(y + h)) + tt % EACH;
+                }
+                for (uint32_t i0 = 0; i0 < n[0] + n[1]; i0 += 4) {
                     float4 x[4][NV];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t i = i0 + k;
+                        const bool h = i >= n[0];
+                        const uint32_t s = h ? i - n[0] : i;
+                        const float4* part = (h ? from[1] : from[0]) + (s == 0 ? at : p.tiles + (h ? s0[1] : s0[0]) + s) * static_cast<size_t>(R / 4 * ROWS);
 #pragma unroll
                         for (int j = 0; j < NV; ++j)
-                            x[k][j] = s + k <= s1 && tt % EACH + j * EACH < R / 4 * mt
-                                          ? __ldcg(from + (s + k == s0 ? at : p.tiles + s + k) * static_cast<size_t>(R / 4 * ROWS) + j * EACH)
-                                          : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            x[k][j] = i < n[0] + n[1] && tt % EACH + j * EACH < R / 4 * mt ? __ldcg(part + j * EACH) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    }
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -753,15 +760,15 @@ __device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t* r) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "r"(taddr));
 }
-// ROWS: of A per pass (2, 4 or 8); F as above.
-template <DType IO, int ROWS, int F, bool ZEROS>
+// ROWS: of A per pass, 4 or 8.
+template <DType IO, int ROWS, bool ZEROS>
 __global__ void __launch_bounds__(kTcThreads, 1)
 gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     using T = typename std::conditional<IO == DType::F32, float, __nv_bfloat16>::type;
-    constexpr int D = IO == DType::F32 ? 4 : 3, NF = 4 / F;
+    constexpr int D = IO == DType::F32 ? 4 : 3;
     constexpr int NC = (D * ROWS + 7) / 8 * 8;      // digits' columns in shared memory
     constexpr int NM = (NC + 15) / 16 * 16;         // of a product: of 128 rows it has multiples of 16, the last 8 are not read
-    static_assert(NM * NF <= 32, "two products of a step and two operands in a team's tensor memory");
+    static_assert(NM <= 32, "two steps' products and codes in a team's tensor memory");
     constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(NM >> 3) << 17) | ((128u >> 4) << 24);
     extern __shared__ __align__(1024) unsigned char smem[];
     const W4Args& g = p.g;
@@ -775,7 +782,7 @@ gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
 
     unsigned char* ring = smem + team * p.slots * kTcStepBytes;
     unsigned char* act = smem + kTeams * p.slots * kTcStepBytes;
-    const Image img(act, per, NC, ROWS, F);
+    const Image img(act, per, NC, ROWS, 4);
     uint32_t* last = reinterpret_cast<uint32_t*>(act + p.image_bytes) + team * kTeamThreads;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + p.bars_at);
     uint64_t* image_bar = bars + kTeams * (kMaxSlots + 4);
@@ -833,7 +840,7 @@ gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     uint32_t atile = lo / nq, aq = lo - atile * nq, aleft = hi - lo;
     const char* sat = nullptr;      // the scale of the row's group
     int within = 0;                 // weights of that group before
-    uint32_t raw[NF] = {}, rawz[ZEROS ? NF : 1] = {};
+    uint32_t raw = 0u, rawz = 0u;
     auto open = [&]() {
         const int64_t row = static_cast<int64_t>(atile) * kTcRows + tt, k = static_cast<int64_t>(k_step0 + aq) * kStepK;
         const int group = static_cast<int>(g.groups > 1 ? k / g.group : 0);
@@ -843,19 +850,12 @@ gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     auto fetch_scales = [&]() {
         if (aleft == 0) return;
         --aleft;
-#pragma unroll
-        for (int f = 0; f < NF; ++f) {
-            if (f == 0 || (k_step0 + aq) * kStepK + f * F * 32 < static_cast<uint32_t>(g.K)) {
-                raw[f] = ldg_scale(sat, f32s);
-                if constexpr (ZEROS) rawz[f] = ldg_scale(sat + to_zero, f32s);
-            } else {
-                raw[f] = 0u;        // past the last weight
-            }
-            within += F * 32;
-            if (within >= g.group) {
-                within = 0;
-                sat += scale_bytes;
-            }
+        raw = ldg_scale(sat, f32s);
+        if constexpr (ZEROS) rawz = ldg_scale(sat + to_zero, f32s);
+        within += kStepK;
+        if (within >= g.group) {
+            within = 0;
+            sat += scale_bytes;
         }
         if (++aq == nq) {
             aq = 0;
@@ -889,7 +889,7 @@ gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
         if (issuer) u0 = units;
         for (; u0 < units; u0 += kTeams * kTeamThreads / 16) {    // the same count for a whole warp
             const uint32_t u = u0 + ((tid >> 4) & 1), m = u / nq, q = u - m * nq;
-            stage<IO, false, F, true>(p, img, m0, k_step0, m, q, r, vec, u < units);
+            stage<IO, false, 4, true>(p, img, m0, k_step0, m, q, r, vec, u < units);
         }
         fence_proxy_async_smem();
         __syncthreads();
@@ -911,7 +911,7 @@ gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     };
     const uint32_t own = tmem + team * kTcColumns, lanes = static_cast<uint32_t>(warp) << 21;  // 32 lanes a warp, in bits 16 up
     const uint32_t ring_at = smem_u32(ring) + tt * 64, swz = (tt >> 1) & 3, act_at = smem_u32(act);
-    const uint32_t base_at = smem_u32(img.base), unit_at = smem_u32(img.unit), isum_at = smem_u32(img.isum);
+    const uint32_t base_at = smem_u32(img.base), unit_at = smem_u32(img.unit);
     uint32_t step = 0, phase = 0;
     int slot = 0;
     bool dead = false;
@@ -925,7 +925,7 @@ gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
                 const uint64_t b = umma_desc_k_sw128(act_at + q * (NC * 128));
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    umma_i8_ts(own + 64 + i * 32 + (k / F) * NM, own + i * 32 + k * 8, b + k * 2, IDESC, k % F != 0);
+                    umma_i8_ts(own + 64 + i * 32, own + i * 32 + k * 8, b + k * 2, IDESC, k != 0);
                 umma_commit(done_bars + i);
                 request(slot);      // every thread has read it
                 if (++slot == p.slots) slot = 0;
@@ -936,46 +936,35 @@ gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     }
     float2 tot[ROWS / 2];
     // Scales the products of the step before: i counts steps, q is its place in the K-range.
-    auto scale_step = [&](uint32_t i, uint32_t q, const float (&sc)[NF], const float (&zr)[NF]) {
+    auto scale_step = [&](uint32_t i, uint32_t q, float sc, float zr) {
         if (!mbar_try_wait(done_bars + (i & 1), (i >> 1) & 1) && !dead) dead = !mbar_wait(done_bars + (i & 1), (i >> 1) & 1, nullptr, p.err);
         __syncwarp();
         tc_fence_after();
         const uint32_t from = own + lanes + 64 + (i & 1) * 32;
+        uint32_t c[NC];
 #pragma unroll
-        for (int f = 0; f < NF; ++f) {
-            uint32_t c[NC];
+        for (int b = 0; b < NC; b += 8) tmem_ld_x8(from + b, c + b);
+        float un[ROWS];
 #pragma unroll
-            for (int b = 0; b < NC; b += 8) tmem_ld_x8(from + f * NM + b, c + b);
-            float un[ROWS];
+        for (int m = 0; m < ROWS; m += 4) {
+            const uint4 v = lds128(unit_at + (q * ROWS + m) * 4);
+            un[m] = __uint_as_float(v.x); un[m + 1] = __uint_as_float(v.y);
+            un[m + 2] = __uint_as_float(v.z); un[m + 3] = __uint_as_float(v.w);
+        }
+        tmem_ld_wait();
 #pragma unroll
-            for (int m = 0; m < ROWS; m += 4) {
-                if constexpr (ROWS >= 4) {
-                    const uint4 v = lds128(unit_at + (q * ROWS + m) * 4);
-                    un[m] = __uint_as_float(v.x); un[m + 1] = __uint_as_float(v.y);
-                    un[m + 2] = __uint_as_float(v.z); un[m + 3] = __uint_as_float(v.w);
-                } else {
-                    un[0] = img.unit[q * ROWS];
-                    un[1] = img.unit[q * ROWS + 1];
-                }
-            }
-            tmem_ld_wait();
+        for (int b = 0; b < NC; b += 4) {
+            const uint4 v = lds128(base_at + (q * NC + b) * 4);
+            c[b] += v.x; c[b + 1] += v.y; c[b + 2] += v.z; c[b + 3] += v.w;
+        }
 #pragma unroll
-            for (int b = 0; b < NC; b += 4) {
-                const uint4 v = lds128(base_at + ((q * NF + f) * NC + b) * 4);
-                c[b] += v.x; c[b + 1] += v.y; c[b + 2] += v.z; c[b + 3] += v.w;
-            }
+        for (int m = 0; m < ROWS; m += 2) {
+            auto digit = [&](int d) { return add2(bits2(c + d * ROWS + m), make_float2(-kMagic, -kMagic)); };
+            float2 y = digit(D - 1);
 #pragma unroll
-            for (int m = 0; m < ROWS; m += 2) {
-                auto digit = [&](int d) { return add2(bits2(c + d * ROWS + m), make_float2(-kMagic, -kMagic)); };
-                float2 y = digit(D - 1);
-#pragma unroll
-                for (int d = D - 2; d >= 0; --d) y = fma2(y, make_float2(256.0f, 256.0f), digit(d));
-                if constexpr (ZEROS) {
-                    const float2 is = *reinterpret_cast<const float2*>(img.isum + (q * NF + f) * ROWS + m);
-                    y = fma2(make_float2(zr[f], zr[f]), is, y);
-                }
-                tot[m / 2] = fma2(mul2(make_float2(sc[f], sc[f]), make_float2(un[m], un[m + 1])), y, tot[m / 2]);
-            }
+            for (int d = D - 2; d >= 0; --d) y = fma2(y, make_float2(256.0f, 256.0f), digit(d));
+            if constexpr (ZEROS) y = fma2(make_float2(zr, zr), *reinterpret_cast<const float2*>(img.isum + q * ROWS + m), y);
+            tot[m / 2] = fma2(mul2(make_float2(sc, sc), make_float2(un[m], un[m + 1])), y, tot[m / 2]);
         }
     };
 
@@ -985,7 +974,7 @@ gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
             const uint32_t n = hi - done < nq - q0 ? hi - done : nq - q0, q1 = q0 + n;
 #pragma unroll
             for (int m = 0; m < ROWS / 2; ++m) tot[m] = make_float2(0.0f, 0.0f);
-            float sc[NF], zr[NF];
+            float sc = 0.0f, zr = 0.0f;
             for (uint32_t q = q0; q < q1; ++q) {
                 if (!mbar_try_wait(bars + slot, phase) && !dead) dead = !mbar_wait(bars + slot, phase, nullptr, p.err);
                 uint32_t a[32];     // byte b of word 2j + h is code 8j + 2b + h
@@ -1007,11 +996,8 @@ gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
                 if (lane == 0) mbar_arrive(code_bars + (step & 1));
                 if (++slot == p.slots) { slot = 0; phase ^= 1u; }
                 if (q > q0) scale_step(step - 1, q - 1, sc, zr);
-#pragma unroll
-                for (int f = 0; f < NF; ++f) {
-                    sc[f] = value(raw[f]);
-                    zr[f] = ZEROS ? 8.0f - value(rawz[f]) : 0.0f;
-                }
+                sc = value(raw);
+                if constexpr (ZEROS) zr = 8.0f - value(rawz);
                 fetch_scales();
                 ++step;
             }
@@ -1080,18 +1066,10 @@ struct Kernel {
     bool packed, tc;
 };
 
-template <DType IO, int ROWS, int F>
+template <DType IO, int ROWS>
 Kernel tc_kernel(bool zeros) {
-    return {zeros ? reinterpret_cast<const void*>(&gemm_w4_tc_kernel<IO, ROWS, F, true>)
-                  : reinterpret_cast<const void*>(&gemm_w4_tc_kernel<IO, ROWS, F, false>),
-            reinterpret_cast<const void*>(&gemm_w4_digits_kernel<IO, false, F, true>), ROWS, IO == DType::F32 ? 4 : 3, F, false, true};
-}
-
-template <DType IO>
-Kernel tc_kernel_for(int M, int f, bool zeros) {
-    if (M <= 2) return f == 4 ? tc_kernel<IO, 2, 4>(zeros) : tc_kernel<IO, 2, 2>(zeros);
-    if (M <= 4) return f == 4 ? tc_kernel<IO, 4, 4>(zeros) : tc_kernel<IO, 4, 2>(zeros);
-    return tc_kernel<IO, 8, 4>(zeros);
+    return {zeros ? reinterpret_cast<const void*>(&gemm_w4_tc_kernel<IO, ROWS, true>) : reinterpret_cast<const void*>(&gemm_w4_tc_kernel<IO, ROWS, false>),
+            reinterpret_cast<const void*>(&gemm_w4_digits_kernel<IO, false, 4, true>), ROWS, IO == DType::F32 ? 4 : 3, 4, false, true};
 }
 
 template <DType IO, bool PACKED>
@@ -1109,8 +1087,14 @@ Kernel kernel_for_flush(int f) {
 Kernel select(const W4Args& g) {
     // How many chunks of 32 weights share their scales for sure, up to the four of a step.
     const int f = g.groups == 1 || g.group % 128 == 0 ? 4 : (g.group % 64 == 0 ? 2 : 1);
-    if (TCMODE && (f == 4 || (g.M <= 4 && f == 2)))
-        return g.io == DType::F32 ? tc_kernel_for<DType::F32>(g.M, f, g.zero != nullptr) : tc_kernel_for<DType::BF16>(g.M, f, g.zero != nullptr);
+    // Codes in tensor memory: 8x28672x8192 37.7 us (products of registers 42.9), 4 rows 33.7 (40.2),
+    // 8x28672x4096 23.8 (26.4), 8x8192x4096 16.5 (16.0).  Its tiles of 128 rows are too few of too many
+    // parts for less: 8x11008x2048 14.4 (10.6), 8x4096x11008 21.5 (18.8).
+    if (f == 4 && g.M > 2 && g.N >= 8192 && static_cast<int64_t>(g.N) * g.K >= int64_t(1) << 25) {
+        const bool zeros = g.zero != nullptr;
+        if (g.io == DType::F32) return g.M <= 4 ? tc_kernel<DType::F32, 4>(zeros) : tc_kernel<DType::F32, 8>(zeros);
+        return g.M <= 4 ? tc_kernel<DType::BF16, 4>(zeros) : tc_kernel<DType::BF16, 8>(zeros);
+    }
     // Two rows' digits fit one block of columns: a third (a quarter) of the products.
     if (g.io == DType::F32) return g.M <= 2 ? kernel_for_flush<DType::F32, true>(f) : kernel_for_flush<DType::F32, false>(f);
     return g.M <= 2 ? kernel_for_flush<DType::BF16, true>(f) : kernel_for_flush<DType::BF16, false>(f);
@@ -1194,8 +1178,10 @@ bool gemm_w4_plan(const W4Args& g, int num_sms, W4Plan* plan) {
     plan->blocks = (g.M + k.rows - 1) / k.rows;
     plan->extra_bytes = plan->copy_bytes;
     if (plan->prepared) plan->extra_bytes += static_cast<size_t>(plan->blocks) * plan->splits * plan->image_bytes;
-    // Every SM a CTA, shared among the K-ranges; no more than there are shares of eight steps.
-    int64_t ctas = (num_sms + plan->splits - 1) / plan->splits;
+    // Every SM a CTA, shared among the K-ranges (one more would wait for a second round); no more than
+    // there are shares.
+    int64_t ctas = num_sms / plan->splits;
+    if (ctas < 1) ctas = 1;
     const int64_t shares = (tiles * plan->split_steps + (k.tc ? kTeams : kWarps) - 1) / (k.tc ? kTeams : kWarps);
     if (ctas > shares) ctas = shares;
     plan->ctas = static_cast<int>(ctas);
