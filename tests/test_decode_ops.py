@@ -140,6 +140,38 @@ def test_w4_pitches(gpu, dn, K, pitch, pad, io):
     w4_check(gpu, dn, 5, 77, K, 32, io, "f32", zeros=True, bias=True, pad=pad, pitch=pitch)
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("M,N,K,group,io,pitch", [(3, 8195, 4099, 128, "bf16", 16), (4, 8192, 4096, 256, "f32", 16),
+                                                  (5, 9000, 4000, 0, "bf16", 1), (8, 8321, 4225, 128, "f32", 16),
+                                                  (9, 8192, 12289, 128, "bf16", 64), (8, 8200, 20000, 1024, "f32", 16),
+                                                  (17, 65600, 513, 128, "bf16", 16), (4, 33000, 1025, 384, "f32", 1)])
+def test_w4_long_products(gpu, dn, M, N, K, group, io, pitch, zeros):
+    """Products of 2^25 weights and more: the first and last rows of W and some between."""
+    torch = gpu
+    t = types(torch, dn)
+    A, W, scale, zero, bias = w4_inputs(torch, M, N, K, group, t[io][0], torch.float32 if zeros else torch.bfloat16,
+                                        zeros, True, pitch=pitch)
+    C = w4_run(torch, dn, M, N, K, group, A, W, scale, zero, bias, pad_c=3)
+    rows = torch.cat((torch.arange(140), torch.randint(0, N, (200,), generator=torch.Generator().manual_seed(1)),
+                      torch.arange(N - 140, N))).cuda()
+    want, mag = w4_exact(torch, A, W[rows], scale[rows], None if zero is None else zero[rows], bias[rows], K, group)
+    within(C[:, rows], want, r_of(torch, t[io][0]) * want.abs() + sum_tol(K) * mag, f"{M}x{N}x{K}")
+    assert bool(C[:, N:].isnan().all())
+    assert bool(C[:, :N].isfinite().all())
+    assert torch.equal(C[:, :N], w4_run(torch, dn, M, N, K, group, A, W, scale, zero, bias))
+    # An infinity and a NaN reach their own rows.
+    clean = C[:, :N].clone()
+    A[1, K - 1], A[2, 700 % K] = float("inf"), float("nan")
+    C = w4_run(torch, dn, M, N, K, group, A, W, scale, zero, bias)
+    keep = [m for m in range(M) if m not in (1, 2)]
+    assert torch.equal(C[keep], clean[keep])
+    last = (W[:, (K - 1) // 2] >> (4 * ((K - 1) % 2))) & 15
+    sign = last.float() - (8.0 if zero is None else zero[:, (K - 1) // group if group else 0].float())
+    some = sign != 0
+    assert torch.equal(C[1, some].float(), torch.where(sign > 0, float("inf"), -float("inf"))[some])
+    assert bool(C[1, ~some].isnan().all()) and bool(C[2].isnan().all())
+
+
 def test_w4_unaligned_bases(gpu, dn):
     """Operands that start one element into their allocation."""
     torch = gpu
