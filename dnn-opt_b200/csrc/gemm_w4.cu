@@ -4,12 +4,11 @@
 // What bounds it: a weight is half a byte and used M times, so HBM up to
 // M of about 64; below that, turning codes into operands is the work, on the
 // pipe that shifts and masks 16 lanes a cycle.  The products are therefore
-// integer ones, mma.sync m16n8k32 of unsigned by signed bytes: the eight codes
-// of a word become two operand registers in three operations (a code to bf16
-// takes one for each and held this kernel at 2.1 TB/s).  16 rows of W are the
-// rows, digits of the activations the columns; a tcgen05 tile would need the
-// decoded weights in shared memory first, four times the bytes that arrive,
-// for at most 24 of its at least 64 columns.
+// integer ones of bytes: the eight codes of a word become two operand words in
+// three operations (a code to bf16 takes one for each and held this kernel at
+// 2.1 TB/s).  Rows of W are the rows, digits of the activations the columns.
+// Two kernels: mma.sync m16n8k32 out of registers, and for long products with
+// three rows of A or more tcgen05 out of tensor memory (further down).
 //
 // Mathematics.  Within 128 consecutive k, a row of A is a power of two times
 // whole numbers |i| < 2^22 (bf16) or 2^30 (FP32), the power chosen by the
@@ -34,12 +33,12 @@
 // reads them.  Rows of W that do not start at multiples of 16 bytes are first
 // copied to a workspace where they do.
 //
-// Measured, of 6.53 TB/s (groups of 128, bf16): 1x28672x8192 30.0 us (62%), 8 rows
-// 44.1 us (42%), 16 rows 83 us; groups of 32, 8 rows 67 us; FP32, 8 rows 56.5 us;
-// 4x11008x4096 in groups of 64 with zero points 22.3 us; 1x4096x4096 9.0 us, of
-// which the chain of start, digits, first weights, sums and joining takes seven.
-// 16 warps an SM issue two instructions a cycle of four: decoding, products and
-// scaling wait on one another's results, and registers allow no more warps.
+// Measured, of 6.53 TB/s (bf16, groups of 128): 1x28672x8192 30.0 us (62%); groups
+// of 32, 8 rows 63 us; 4x11008x4096 in groups of 64 with zero points 23.0 us;
+// 1x4096x4096 9.0 us, of which the chain of start, digits, first weights, sums
+// and joining takes seven.  16 warps an SM issue two instructions a cycle of
+// four: decoding, products and scaling wait on one another's results, and
+// registers allow no more warps.
 #include <cuda.h>
 
 #include <mutex>
@@ -740,6 +739,17 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
 }
 
 // ---- the same products by tcgen05, the codes as bytes in tensor memory -------
+// A step is 128 weights of 128 rows (8 KB), a team's thread has a row: it decodes
+// the row's 64 bytes into 32 columns of its lane, where a warp of its own for
+// each team multiplies them (four products of K = 32, 128 rows and 16 or 32
+// columns) by the digits in shared memory, and it scales its row's sums of the
+// step before out of tensor memory.  So no operand of W passes through shared
+// memory again, no instruction is spent on operands of A, and a row's scale is
+// read once, not by four lanes.  Codes and sums are double: 128 columns a team.
+// Even k come before odd k within eight, in the digits as in the decoded codes.
+// Measured: 8x28672x8192 37.9 us (49%; by registers 42.9), 4 rows 33.7 (40.2), FP32
+// 39.6, 16 rows 69.  345 instructions a warp and step became 290; half of the issue
+// slots go by, two thirds of them on tensor memory, barriers and fixed latencies.
 __device__ __forceinline__ void umma_i8_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
                  "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
@@ -760,6 +770,7 @@ __device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t* r) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "r"(taddr));
 }
+
 // ROWS: of A per pass, 4 or 8.
 template <DType IO, int ROWS, bool ZEROS>
 __global__ void __launch_bounds__(kTcThreads, 1)
