@@ -748,8 +748,9 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
 // read once, not by four lanes.  Codes and sums are double: 128 columns a team.
 // Even k come before odd k within eight, in the digits as in the decoded codes.
 // Measured: 8x28672x8192 37.9 us (49%; by registers 42.9), 4 rows 33.7 (40.2), FP32
-// 39.6, 16 rows 69.  345 instructions a warp and step became 290; half of the issue
-// slots go by, two thirds of them on tensor memory, barriers and fixed latencies.
+// 39.6, 16 rows 69.  A warp issues 299 instructions a step, half of the issue slots
+// go by: on tensor memory, barriers and fixed latencies.  Waiting for a quarter
+// of the digits at a time instead of all took longer (39.2).
 __device__ __forceinline__ void umma_i8_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
                  "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
