@@ -67,7 +67,7 @@ int dnnopt_cuda_gemm_w4(const dnnopt_w4_desc* d, const void* A, const uint8_t* W
     if (st != DNNOPT_STATUS_SUCCESS) return st;
     if ((st = inject_launch()) != DNNOPT_STATUS_SUCCESS) return st;
     cudaError_t e = launch_gemm_w4(g, plan, w->ws, w->counters, w->quant, w->err, s);
-    note_launch(1 + (plan.pitch ? 1 : 0) + (plan.prepared ? 1 : 0));
+    note_launch(plan.pitch || plan.prepared ? 2 : 1);
     return cuda_status(e);
 }
 

@@ -75,6 +75,9 @@ struct Params {
     int bars_at;                    // of the barriers, in shared memory
     uint32_t image_bytes;           // of a K-range's activations
     unsigned char* images;          // made by the kernel before; nullptr: each CTA makes its own
+    uint8_t* copy;                  // of W, made by the kernel before; nullptr: W is read as it is
+    int64_t copy_pitch;
+    uint32_t digit_ctas;            // of that kernel's grid in x; the rest copy
     uint32_t gmul, gshift;          // chunk of 32 weights -> group
     float* ws;                      // partial tiles of a K-range: the part with a tile's first step by
                                     // tile, then the parts that begin a share by share
@@ -314,12 +317,33 @@ __device__ __forceinline__ void stage(const Params& p, const Image& img, int m0,
     }
 }
 
-// Images of all K-ranges and blocks of rows, where making them in every CTA
-// takes longer than reading them back: a half-warp per 128 activations.
+// A row of W at a multiple of 16 bytes: a warp copies its words of four bytes, each cut from the two
+// aligned words that hold it.
+__device__ __forceinline__ void copy_row(const Params& p, int64_t n) {
+    const W4Args& g = p.g;
+    if (n >= g.N) return;
+    const int bytes = (g.K >> 1) + (g.K & 1);
+    const uintptr_t row = reinterpret_cast<uintptr_t>(g.W) + n * g.ldw, end = row + bytes;
+    const uint32_t* from = reinterpret_cast<const uint32_t*>(row & ~uintptr_t(3));
+    const uint32_t shift = static_cast<uint32_t>(row & 3) * 8;
+    for (int i = threadIdx.x & 31; i < (bytes + 3) / 4; i += 32) {
+        const uint32_t lo = __ldg(from + i);
+        const uint32_t hi = shift && reinterpret_cast<uintptr_t>(from + i + 1) < end ? __ldg(from + i + 1) : 0u;
+        *reinterpret_cast<uint32_t*>(p.copy + n * p.copy_pitch + i * 4) = __funnelshift_r(lo, hi, shift);
+    }
+}
+
+// What a product wants made before it.  Images of all K-ranges and blocks of rows, where making them in
+// every CTA takes longer than reading them back: a half-warp per 128 activations.  And the rows of W at
+// multiples of 16 bytes, if they are not there: a warp to a row.
 template <DType IO, bool PACKED, int F, bool TC>
 __global__ void __launch_bounds__(128) gemm_w4_digits_kernel(const Params p) {
     pdl_wait();
     pdl_launch_dependents();    // what runs next finds everything older than this kernel done
+    if (blockIdx.x >= p.digit_ctas) {
+        if (blockIdx.y == 0 && blockIdx.z == 0) copy_row(p, static_cast<int64_t>(blockIdx.x - p.digit_ctas) * 4 + (threadIdx.x >> 5));
+        return;
+    }
     using T = typename std::conditional<IO == DType::F32, float, __nv_bfloat16>::type;
     constexpr int D = IO == DType::F32 ? 4 : 3;
     const int ROWS = TC ? p.rows : (PACKED ? 8 / D : 8);
@@ -461,7 +485,7 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     const bool zeros = g.zero != nullptr;
     const bool f32s = g.st == DType::F32;
 
-    if (!p.images) pdl_wait();
+    if (!p.images || p.copy) pdl_wait();
     pdl_launch_dependents();
     const Shares shares(p.tiles, nq, gridDim.x * kTeams, kWarps);
     const uint32_t share = team * gridDim.x + blockIdx.x;
@@ -805,7 +829,7 @@ gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     uint64_t* done_bars = code_bars + 2;            // and its products
     const bool f32s = g.st == DType::F32;
 
-    if (!p.images) pdl_wait();
+    if (!p.images || p.copy) pdl_wait();
     pdl_launch_dependents();
     const Shares shares(p.tiles, nq, gridDim.x * kTeams, 1);
     const uint32_t share = team * gridDim.x + blockIdx.x;
@@ -1055,22 +1079,6 @@ gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     if (tid < 32) tmem_dealloc(tmem, kTeams * kTcColumns);
 }
 
-// Rows of W at multiples of 16 bytes: a warp copies a row's words of four bytes, each cut from the two
-// aligned words that hold it.
-__global__ void __launch_bounds__(256) repack_rows_kernel(const uint8_t* w, int64_t ldw, int rows, int row_bytes, uint8_t* out,
-                                                          int64_t pitch) {
-    const int64_t n = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    if (n >= rows) return;
-    const uintptr_t row = reinterpret_cast<uintptr_t>(w) + n * ldw, end = row + row_bytes;
-    const uint32_t* from = reinterpret_cast<const uint32_t*>(row & ~uintptr_t(3));
-    const uint32_t shift = static_cast<uint32_t>(row & 3) * 8;
-    for (int i = threadIdx.x & 31; i < (row_bytes + 3) / 4; i += 32) {
-        const uint32_t lo = __ldg(from + i);
-        const uint32_t hi = shift && reinterpret_cast<uintptr_t>(from + i + 1) < end ? __ldg(from + i + 1) : 0u;
-        *reinterpret_cast<uint32_t*>(out + n * pitch + i * 4) = __funnelshift_r(lo, hi, shift);
-    }
-}
-
 struct Kernel {
     const void* fn;
     const void* digits;
@@ -1240,28 +1248,23 @@ cudaError_t launch_gemm_w4(const W4Args& g, const W4Plan& plan, float* ws, uint3
     p.ws = ws;
     p.tickets = tickets;
     p.err = err;
-    const uint8_t* w = g.W;
-    int64_t pitch = g.ldw;
-    if (plan.pitch) {
-        w = static_cast<const uint8_t*>(extra);
-        pitch = plan.pitch;
-        repack_rows_kernel<<<(static_cast<unsigned>(g.N) + 7) / 8, 256, 0, s>>>(g.W, g.ldw, g.N, static_cast<int>(row_bytes_of(g)),
-                                                                              static_cast<uint8_t*>(extra), pitch);
-        if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    }
+    p.copy = plan.pitch ? static_cast<uint8_t*>(extra) : nullptr;
+    p.copy_pitch = plan.pitch;
     CUtensorMap map;
-    if (!encode_weights(g, w, pitch, k.tc, &map)) return cudaErrorNotSupported;
+    if (!encode_weights(g, plan.pitch ? p.copy : g.W, plan.pitch ? plan.pitch : g.ldw, k.tc, &map)) return cudaErrorNotSupported;
     p.image_bytes = plan.image_bytes;
-    p.images = nullptr;
-    if (plan.prepared) {
-        p.images = static_cast<unsigned char*>(extra) + plan.copy_bytes;
+    p.images = plan.prepared ? static_cast<unsigned char*>(extra) + plan.copy_bytes : nullptr;
+    p.digit_ctas = 0;
+    if (plan.prepared || plan.pitch) {
         const unsigned stretches = static_cast<unsigned>(g.M < plan.rows ? g.M : plan.rows) * plan.split_steps;
+        if (plan.prepared) p.digit_ctas = (stretches + 7) / 8;
+        const unsigned copies = plan.pitch ? (static_cast<unsigned>(g.N) + 3) / 4 : 0;
         void* first[] = {&p};
-        e = launch_pdl(k.digits, dim3((stretches + 7) / 8, plan.splits, plan.blocks), 128, first, 0, s);
+        e = launch_pdl(k.digits, plan.prepared ? dim3(p.digit_ctas + copies, plan.splits, plan.blocks) : dim3(copies), 128, first, 0, s);
         if (e != cudaSuccess) return e;
     }
-    // With digits made before it, the kernel starts before they are done: all that it reads or writes
-    // until it waits for them is older than the kernel that makes them, or its own.
+    // With only digits made before it, the kernel starts before they are done: all that it reads or
+    // writes until it waits for them is older than the kernel that makes them, or its own.
     void* args[] = {&p, &map};
     return launch_pdl(k.fn, dim3(plan.ctas, plan.splits, plan.blocks), k.tc ? kTcThreads : kTeams * kTeamThreads, args, plan.smem, s);
 }
