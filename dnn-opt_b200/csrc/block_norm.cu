@@ -148,7 +148,7 @@ struct Row {
 
 // Sum over the row's threads, the same for all of them.  Two buffers in turn:
 // a barrier lies between a buffer's reading and its next writing.
-template <bool WARP>
+template <bool WARP, int TH>
 __device__ __forceinline__ float row_sum(float v, float (&part)[2][32], int& buffer) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
@@ -156,9 +156,18 @@ __device__ __forceinline__ float row_sum(float v, float (&part)[2][32], int& buf
         const int lane = threadIdx.x & 31;
         if (lane == 0) part[buffer][threadIdx.x >> 5] = v;
         __syncthreads();
-        v = lane < static_cast<int>(blockDim.x >> 5) ? part[buffer][lane] : 0.0f;
+        if constexpr (TH >= 128) {      // every thread adds them all: less to wait for than five shuffles
+            v = 0.0f;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+            for (int i = 0; i < TH / 128; ++i) {
+                const float4 x = reinterpret_cast<const float4*>(part[buffer])[i];
+                v += (x.x + x.y) + (x.z + x.w);
+            }
+        } else {
+            v = lane < static_cast<int>(blockDim.x >> 5) ? part[buffer][lane] : 0.0f;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+        }
         buffer ^= 1;
     }
     return v;
@@ -175,7 +184,7 @@ __device__ __forceinline__ void norm_row(const Row<VEC, EPT, TH>& row, float (&v
         for (int i = 0; i < NB; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) s += v[i][j];
-        const float mean = row_sum<WARP>(s, part, buffer) * inv;
+        const float mean = row_sum<WARP, TH>(s, part, buffer) * inv;
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
             if (row.full(i)) {
@@ -192,7 +201,7 @@ __device__ __forceinline__ void norm_row(const Row<VEC, EPT, TH>& row, float (&v
     for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) q = fmaf(v[i][j], v[i][j], q);
-    const float rstd = rsqrtf(row_sum<WARP>(q, part, buffer) * inv + eps);
+    const float rstd = rsqrtf(row_sum<WARP, TH>(q, part, buffer) * inv + eps);
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
         float t[8];
@@ -211,11 +220,16 @@ __device__ __forceinline__ void norm_row(const Row<VEC, EPT, TH>& row, float (&v
     }
 }
 
+// Whether 1024 threads an SM (64 registers each) beat fewer with more: not for 16 FP32 elements, which
+// would spill (4096x8192 with gate rows: 109 us as it is, 140 so; 8192x8192 bf16 119 and 91).
+template <typename T>
+constexpr bool tight(int ept) { return ept == 8 || sizeof(T) == 2; }
+
 // STREAM: row after row, gridDim rows apart.
 template <typename T, typename TW, bool VEC, int EPT, bool WARP, bool STREAM, int TH>
-__global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : (STREAM ? TH : 1024)) block_norm_kernel(const BlockNormArgs a) {
+__global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : (STREAM ? TH : 1024), STREAM && tight<T>(EPT) ? 1024 / (TH ? TH : 1024) : 1) block_norm_kernel(const BlockNormArgs a) {
     constexpr int NB = EPT / 8;
-    __shared__ float part[2][32];
+    __shared__ __align__(16) float part[2][32];
     int buffer = 0;
     pdl_wait();
     pdl_launch_dependents();
