@@ -156,7 +156,7 @@ __device__ __forceinline__ float row_sum(float v, float (&part)[2][32], int& buf
         const int lane = threadIdx.x & 31;
         if (lane == 0) part[buffer][threadIdx.x >> 5] = v;
         __syncthreads();
-        if constexpr (TH >= 128) {      // every thread adds them all: less to wait for than five shuffles
+        if constexpr (TH > 0 && TH % 128 == 0) {    // every thread adds them all: less to wait for than five shuffles
             v = 0.0f;
 #pragma unroll
             for (int i = 0; i < TH / 128; ++i) {
@@ -433,11 +433,17 @@ cudaError_t launch_short(const BlockNormArgs& a, int num_sms, cudaStream_t s) {
             // Element by element, half as many to a thread hide more of each other's latency
             // (16384x4093 FP32: 262 against 288 us); 16 bytes at a time it is the other way round
             // (4096x4096 bf16: 32 against 27 us).
-            constexpr int EPT = VEC ? 16 : 8, PER = 16 / EPT;
-            if (a.cols <= 1024) return launch_stream<T, TW, VEC, EPT, 64 * PER>(a, num_sms, s);
-            if (a.cols <= 2048) return launch_stream<T, TW, VEC, EPT, 128 * PER>(a, num_sms, s);
-            if (a.cols <= 4096) return launch_stream<T, TW, VEC, EPT, 256 * PER>(a, num_sms, s);
-            return launch_stream<T, TW, VEC, 16, 512>(a, num_sms, s);
+            constexpr int EPT = VEC ? 16 : 8;
+            const int need = (a.cols + EPT - 1) / EPT;
+            if (a.cols > 4096)
+                return a.cols <= 6144 ? launch_stream<T, TW, VEC, 16, 384>(a, num_sms, s) : launch_stream<T, TW, VEC, 16, 512>(a, num_sms, s);
+            if (need <= 64) return launch_stream<T, TW, VEC, EPT, 64>(a, num_sms, s);
+            if (need <= 96) return launch_stream<T, TW, VEC, EPT, 96>(a, num_sms, s);
+            if (need <= 128) return launch_stream<T, TW, VEC, EPT, 128>(a, num_sms, s);
+            if (need <= 192) return launch_stream<T, TW, VEC, EPT, 192>(a, num_sms, s);
+            if (VEC || need <= 256) return launch_stream<T, TW, VEC, EPT, 256>(a, num_sms, s);
+            if (need <= 384) return launch_stream<T, TW, VEC, EPT, VEC ? 256 : 384>(a, num_sms, s);
+            return launch_stream<T, TW, VEC, EPT, VEC ? 256 : 512>(a, num_sms, s);
         }
         return launch_pdl(block_norm_kernel<T, TW, VEC, 8, false, false, 0>, a.rows, threads(8), 0, a, s);
     }
