@@ -12,13 +12,16 @@
 //     one's loads under way while it works on this one;
 //   * rows past 16384 columns stay in shared memory.
 // Elements are read 16 bytes at a time where all rows and vectors allow, else
-// one by one, neighbouring threads neighbouring elements.  Means and mean
+// in pairs (16384x1100 bf16: 49 us, one by one 71) or one by one, neighbouring
+// threads neighbouring elements.  Means and mean
 // squares are sums over the values themselves (a layer norm's squares are
 // taken after its mean), in a fixed order.
 //
 // Measured, of 6.53 TB/s: 8192x8192 bf16 90 us (92%), 65536x1024 bf16 85 us
-// (97%), 65536x512 bf16 44 us (94%), 16384x4093 FP32 with layer norms and a gate
-// row each 262 us (78%: scalar loads, four sums over the row), 1x4096 2.5 us.
+// (97%), 65536x512 bf16 44 us (94%), 4096x8192 FP32 with gate rows 110 us (93%),
+// 16384x4093 FP32 with layer norms and a gate row each 259 us (79%: scalar loads,
+// four sums over the row), 8192x2999 bf16 83 us (37%: two bytes an access),
+// 1x4096 2.5 us.
 #include <mutex>
 #include <unordered_map>
 
@@ -53,10 +56,20 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
     *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Two, at a multiple of their size.
+__device__ __forceinline__ void store2(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
+__device__ __forceinline__ void store2(__nv_bfloat16* p, float a, float b) {
+    *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b);
+}
+
 constexpr int kRowsPerCta = 8;      // of a warp each
 
-// Eight elements as they were read: 16-bit ones in pairs (VEC) or one to a word.
-template <typename T, bool VEC>
+// How rows lie, as far as it holds for all of them and the vectors: elements anywhere, pairs of elements
+// at multiples of their size, or eight elements at multiples of 16 bytes.
+enum { kAny = 0, kPairs = 1, kEights = 2 };
+
+// Eight elements as they were read: 16-bit ones in pairs or one to a word (kAny).
+template <typename T, int V>
 struct Raw {
     float w[8];
     __device__ __forceinline__ void get(float (&v)[8]) const {
@@ -64,85 +77,109 @@ struct Raw {
         for (int j = 0; j < 8; ++j) v[j] = w[j];
     }
 };
-template <bool VEC>
-struct Raw<__nv_bfloat16, VEC> {
-    uint32_t w[VEC ? 4 : 8];
+template <int V>
+struct Raw<__nv_bfloat16, V> {
+    uint32_t w[V == kAny ? 8 : 4];
     __device__ __forceinline__ void get(float (&v)[8]) const {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            v[j] = __uint_as_float(!VEC ? w[VEC ? 0 : j] << 16 : (j & 1) ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
+            v[j] = __uint_as_float(V == kAny ? w[V == kAny ? j : 0] << 16 : (j & 1) ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
     }
 };
 
-// EPT elements of a row to each of TH threads (0: as many as the CTA has):
-// element j of block i is column 8 * (me + i * threads) + j (VEC) or
-// me + (8 i + j) * threads.  With TH known, columns are offsets from one address.
-template <bool VEC, int EPT, int TH>
+// EPT elements of a row to each of TH threads (0: as many as the CTA has), eight
+// to a block: eight columns in a row (kEights), or pairs or single columns that
+// neighbouring threads have next to each other.  With TH known, columns are
+// offsets from one address.
+template <int V, int EPT, int TH>
 struct Row {
     int me, cols;
 
     __device__ __forceinline__ int threads() const { return TH ? TH : blockDim.x; }
     __device__ __forceinline__ int col(int i, int j) const {
-        return VEC ? 8 * (me + i * threads()) + j : me + (8 * i + j) * threads();
+        return V == kEights ? 8 * (me + i * threads()) + j
+               : V == kPairs ? 2 * (me + (4 * i + (j >> 1)) * threads()) + (j & 1) : me + (8 * i + j) * threads();
     }
-    // Whether all of block i is there: for VEC this thread's, else every thread's but for its last element.
+    // Whether all of block i is there: for kEights this thread's, else every thread's but for its last
+    // element or pair.
     __device__ __forceinline__ bool full(int i) const {
-        return VEC ? col(i, 0) + 8 <= cols : (8 * i + 7) * threads() <= cols;
+        return V == kEights ? col(i, 0) + 8 <= cols : V == kPairs ? (8 * i + 6) * threads() <= cols : (8 * i + 7) * threads() <= cols;
     }
     // Whether element j of such a block is there.
-    __device__ __forceinline__ bool in(int i, int j) const { return VEC || j < 7 || col(i, j) < cols; }
-    // Block i of a row; columns that are not there give 0.
-    __device__ __forceinline__ void read(const float* p, int i, Raw<float, VEC>& r) const {
-        if (VEC && full(i)) {
-            load8(p + col(i, 0), r.w);
-        } else if (full(i)) {
+    __device__ __forceinline__ bool in(int i, int j) const {
+        return V == kEights || j < (V == kPairs ? 6 : 7) || col(i, j) < cols;
+    }
+    // Block i of a row; columns that are not there give 0.  ALL: but for in().
+    template <bool ALL>
+    __device__ __forceinline__ bool there(int i, int j) const { return ALL ? in(i, j) : col(i, j) < cols; }
+    template <bool ALL>
+    __device__ __forceinline__ void read_some(const float* p, int i, Raw<float, V>& r) const {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) r.w[j] = in(i, j) ? p[col(i, j)] : 0.0f;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) r.w[j] = col(i, j) < cols ? p[col(i, j)] : 0.0f;
+        for (int j = 0; j < 8; j += 2) {
+            if (V == kPairs && there<ALL>(i, j + 1)) {
+                const float2 x = *reinterpret_cast<const float2*>(p + col(i, j));
+                r.w[j] = x.x;
+                r.w[j + 1] = x.y;
+            } else {
+                r.w[j] = there<ALL>(i, j) ? p[col(i, j)] : 0.0f;
+                r.w[j + 1] = V != kPairs && there<ALL>(i, j + 1) ? p[col(i, j + 1)] : 0.0f;
+            }
         }
     }
-    __device__ __forceinline__ void read(const __nv_bfloat16* p, int i, Raw<__nv_bfloat16, VEC>& r) const {
+    template <bool ALL>
+    __device__ __forceinline__ void read_some(const __nv_bfloat16* p, int i, Raw<__nv_bfloat16, V>& r) const {
         const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
-        if constexpr (VEC) {
-            if (full(i)) {
-                const uint4 x = *reinterpret_cast<const uint4*>(p + col(i, 0));
-                r.w[0] = x.x; r.w[1] = x.y; r.w[2] = x.z; r.w[3] = x.w;
-            } else {
+        if constexpr (V == kAny) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    r.w[j] = col(i, 2 * j) < cols ? q[col(i, 2 * j)] : 0u;
-                    if (col(i, 2 * j + 1) < cols) r.w[j] |= static_cast<uint32_t>(q[col(i, 2 * j + 1)]) << 16;
-                }
-            }
-        } else if (full(i)) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) r.w[j] = in(i, j) ? q[col(i, j)] : 0u;
+            for (int j = 0; j < 8; ++j) r.w[j] = there<ALL>(i, j) ? q[col(i, j)] : 0u;
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) r.w[j] = col(i, j) < cols ? q[col(i, j)] : 0u;
+            for (int j = 0; j < 4; ++j) {
+                if (V == kPairs && there<ALL>(i, 2 * j + 1)) {
+                    r.w[j] = *reinterpret_cast<const uint32_t*>(q + col(i, 2 * j));
+                } else {
+                    r.w[j] = there<ALL>(i, 2 * j) ? q[col(i, 2 * j)] : 0u;
+                    if (V != kPairs && there<ALL>(i, 2 * j + 1)) r.w[j] |= static_cast<uint32_t>(q[col(i, 2 * j + 1)]) << 16;
+                }
+            }
         }
+    }
+    __device__ __forceinline__ void read_eight(const float* p, Raw<float, V>& r) const { load8(p, r.w); }
+    __device__ __forceinline__ void read_eight(const __nv_bfloat16* p, Raw<__nv_bfloat16, V>& r) const {
+        if constexpr (V != kAny) {
+            const uint4 x = *reinterpret_cast<const uint4*>(p);
+            r.w[0] = x.x; r.w[1] = x.y; r.w[2] = x.z; r.w[3] = x.w;
+        }
+    }
+    template <typename P>
+    __device__ __forceinline__ void read(const P* p, int i, Raw<P, V>& r) const {
+        if (!full(i)) read_some<false>(p, i, r);
+        else if (V == kEights) read_eight(p + col(i, 0), r);
+        else read_some<true>(p, i, r);
     }
     template <typename P>
     __device__ __forceinline__ void load(const P* p, int i, float (&v)[8]) const {
-        Raw<P, VEC> r;
+        Raw<P, V> r;
         read(p, i, r);
         r.get(v);
     }
+    template <bool ALL, typename P>
+    __device__ __forceinline__ void store_some(P* p, int i, const float (&v)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            if (V == kPairs && there<ALL>(i, j + 1)) {
+                store2(p + col(i, j), v[j], v[j + 1]);
+            } else {
+                if (there<ALL>(i, j)) from_f32(p + col(i, j), v[j]);
+                if (V != kPairs && there<ALL>(i, j + 1)) from_f32(p + col(i, j + 1), v[j + 1]);
+            }
+        }
+    }
     template <typename P>
     __device__ __forceinline__ void store(P* p, int i, const float (&v)[8]) const {
-        if (VEC && full(i)) {
-            store8(p + col(i, 0), v);
-        } else if (full(i)) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (in(i, j)) from_f32(p + col(i, j), v[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (col(i, j) < cols) from_f32(p + col(i, j), v[j]);
-        }
+        if (!full(i)) store_some<false>(p, i, v);
+        else if (V == kEights) store8(p + col(i, 0), v);
+        else store_some<true>(p, i, v);
     }
 };
 
@@ -173,8 +210,8 @@ __device__ __forceinline__ float row_sum(float v, float (&part)[2][32], int& buf
     return v;
 }
 
-template <typename TW, bool WARP, bool VEC, int EPT, int TH>
-__device__ __forceinline__ void norm_row(const Row<VEC, EPT, TH>& row, float (&v)[EPT / 8][8], int kind, const TW* w, const TW* b,
+template <typename TW, bool WARP, int V, int EPT, int TH>
+__device__ __forceinline__ void norm_row(const Row<V, EPT, TH>& row, float (&v)[EPT / 8][8], int kind, const TW* w, const TW* b,
                                          float eps, float offset, float inv, float (&part)[2][32], int& buffer) {
     constexpr int NB = EPT / 8;
     if (kind == 0) return;
@@ -226,7 +263,7 @@ template <typename T>
 constexpr bool tight(int ept) { return ept == 8 || sizeof(T) == 2; }
 
 // STREAM: row after row, gridDim rows apart.
-template <typename T, typename TW, bool VEC, int EPT, bool WARP, bool STREAM, int TH>
+template <typename T, typename TW, int V, int EPT, bool WARP, bool STREAM, int TH>
 __global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : (STREAM ? TH : 1024), STREAM && tight<T>(EPT) ? 1024 / (TH ? TH : 1024) : 1) block_norm_kernel(const BlockNormArgs a) {
     constexpr int NB = EPT / 8;
     __shared__ __align__(16) float part[2][32];
@@ -236,12 +273,12 @@ __global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : (STREAM ? TH : 1024)
     int64_t r = WARP ? static_cast<int64_t>(blockIdx.x) * kRowsPerCta + (threadIdx.x >> 5) : blockIdx.x;
     const int64_t step = static_cast<int64_t>(gridDim.x) * (WARP ? kRowsPerCta : 1);
     if (r >= a.rows) return;
-    Row<VEC, EPT, TH> row;
+    Row<V, EPT, TH> row;
     row.me = WARP ? threadIdx.x & 31 : threadIdx.x;
     row.cols = a.cols;
     const float inv = 1.0f / static_cast<float>(a.cols);
 
-    Raw<T, VEC> x[NB], y[NB], g[NB];
+    Raw<T, V> x[NB], y[NB], g[NB];
     auto read = [&](int64_t at) {
 #pragma unroll
         for (int i = 0; i < NB; ++i) row.read(static_cast<const T*>(a.x) + at * a.ldx, i, x[i]);
@@ -259,7 +296,7 @@ __global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : (STREAM ? TH : 1024)
             float t[NB][8], u[8];
 #pragma unroll
             for (int i = 0; i < NB; ++i) y[i].get(t[i]);
-            norm_row<TW, WARP, VEC, EPT, TH>(row, t, a.post, static_cast<const TW*>(a.post_w), static_cast<const TW*>(a.post_b),
+            norm_row<TW, WARP, V, EPT, TH>(row, t, a.post, static_cast<const TW*>(a.post_w), static_cast<const TW*>(a.post_b),
                                          a.eps, a.offset, inv, part, buffer);
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
@@ -288,7 +325,7 @@ __global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : (STREAM ? TH : 1024)
             for (int i = 0; i < NB; ++i) row.store(static_cast<T*>(a.h) + now * a.ldh, i, v[i]);
         }
         if (a.z) {
-            norm_row<TW, WARP, VEC, EPT, TH>(row, v, a.pre, static_cast<const TW*>(a.pre_w), static_cast<const TW*>(a.pre_b), a.eps,
+            norm_row<TW, WARP, V, EPT, TH>(row, v, a.pre, static_cast<const TW*>(a.pre_w), static_cast<const TW*>(a.pre_b), a.eps,
                                          a.offset, inv, part, buffer);
 #pragma unroll
             for (int i = 0; i < NB; ++i) row.store(static_cast<T*>(a.z) + now * a.ldz, i, v[i]);
@@ -407,23 +444,23 @@ cudaError_t resident(const void* fn, int threads, int* ctas) {
     return cudaSuccess;
 }
 
-template <typename T, typename TW, bool VEC, int EPT, int TH>
+template <typename T, typename TW, int V, int EPT, int TH>
 cudaError_t launch_stream(const BlockNormArgs& a, int num_sms, cudaStream_t s) {
     int ctas = 0;
-    cudaError_t e = resident(reinterpret_cast<const void*>(&block_norm_kernel<T, TW, VEC, EPT, false, true, TH>), TH, &ctas);
+    cudaError_t e = resident(reinterpret_cast<const void*>(&block_norm_kernel<T, TW, V, EPT, false, true, TH>), TH, &ctas);
     if (e != cudaSuccess) return e;
     const int64_t most = static_cast<int64_t>(ctas) * num_sms;
-    return launch_pdl(block_norm_kernel<T, TW, VEC, EPT, false, true, TH>, a.rows < most ? a.rows : most, TH, 0, a, s);
+    return launch_pdl(block_norm_kernel<T, TW, V, EPT, false, true, TH>, a.rows < most ? a.rows : most, TH, 0, a, s);
 }
 
-template <typename T, typename TW, bool VEC>
+template <typename T, typename TW, int V>
 cudaError_t launch_short(const BlockNormArgs& a, int num_sms, cudaStream_t s) {
     // 65536x512 bf16: 44 us, a CTA to each row 97; rows of 1024 take 105 us this way and 85 the other.
     // (Row after row, as below, took 55 for 65536x512: here the other warps' rows hide a row's chain.)
     if (a.cols <= 512) {
         const int64_t grid = (static_cast<int64_t>(a.rows) + kRowsPerCta - 1) / kRowsPerCta;
-        return a.cols <= 256 ? launch_pdl(block_norm_kernel<T, TW, VEC, 8, true, false, 32>, grid, 32 * kRowsPerCta, 0, a, s)
-                             : launch_pdl(block_norm_kernel<T, TW, VEC, 16, true, false, 32>, grid, 32 * kRowsPerCta, 0, a, s);
+        return a.cols <= 256 ? launch_pdl(block_norm_kernel<T, TW, V, 8, true, false, 32>, grid, 32 * kRowsPerCta, 0, a, s)
+                             : launch_pdl(block_norm_kernel<T, TW, V, 16, true, false, 32>, grid, 32 * kRowsPerCta, 0, a, s);
     }
     auto threads = [&](int ept) { return ((a.cols + ept - 1) / ept + 31) / 32 * 32; };
     if (a.cols <= 8192) {
@@ -432,25 +469,25 @@ cudaError_t launch_short(const BlockNormArgs& a, int num_sms, cudaStream_t s) {
         if (a.rows > (a.cols > 4096 ? 2 : 4) * num_sms) {
             // Element by element, half as many to a thread hide more of each other's latency
             // (16384x4093 FP32: 262 against 288 us); 16 bytes at a time it is the other way round
-            // (4096x4096 bf16: 32 against 27 us).
-            constexpr int EPT = VEC ? 16 : 8;
+            // (4096x4096 bf16: 32 against 27 us) but for short rows (16384x600 FP32: 30 against 36).
+            // As few threads as hold a row: 8192x5120 bf16 71 us, with 512 threads 96.
+            constexpr int EPT = V == kEights ? 16 : 8;
             const int need = (a.cols + EPT - 1) / EPT;
             if (a.cols > 4096)
-                return a.cols <= 6144 ? launch_stream<T, TW, VEC, 16, 384>(a, num_sms, s) : launch_stream<T, TW, VEC, 16, 512>(a, num_sms, s);
-            if (need <= 64) return launch_stream<T, TW, VEC, EPT, 64>(a, num_sms, s);
-            if (need <= 96) return launch_stream<T, TW, VEC, EPT, 96>(a, num_sms, s);
-            if (need <= 128) return launch_stream<T, TW, VEC, EPT, 128>(a, num_sms, s);
-            if (need <= 192) return launch_stream<T, TW, VEC, EPT, 192>(a, num_sms, s);
-            if (VEC || need <= 256) return launch_stream<T, TW, VEC, EPT, 256>(a, num_sms, s);
-            if (need <= 384) return launch_stream<T, TW, VEC, EPT, VEC ? 256 : 384>(a, num_sms, s);
-            return launch_stream<T, TW, VEC, EPT, VEC ? 256 : 512>(a, num_sms, s);
+                return a.cols <= 6144 ? launch_stream<T, TW, V, 16, 384>(a, num_sms, s) : launch_stream<T, TW, V, 16, 512>(a, num_sms, s);
+            if (a.cols <= 768) return launch_stream<T, TW, V, 8, 96>(a, num_sms, s);
+            if (need <= 64) return launch_stream<T, TW, V, EPT, 64>(a, num_sms, s);
+            if (need <= 96) return launch_stream<T, TW, V, EPT, 96>(a, num_sms, s);
+            if (need <= 128) return launch_stream<T, TW, V, EPT, 128>(a, num_sms, s);
+            if (need <= 192) return launch_stream<T, TW, V, EPT, 192>(a, num_sms, s);
+            if (EPT == 16 || need <= 256) return launch_stream<T, TW, V, EPT, 256>(a, num_sms, s);
+            if (need <= 384) return launch_stream<T, TW, V, EPT, EPT == 16 ? 256 : 384>(a, num_sms, s);
+            return launch_stream<T, TW, V, EPT, EPT == 16 ? 256 : 512>(a, num_sms, s);
         }
-        return launch_pdl(block_norm_kernel<T, TW, VEC, 8, false, false, 0>, a.rows, threads(8), 0, a, s);
+        return launch_pdl(block_norm_kernel<T, TW, V, 8, false, false, 0>, a.rows, threads(8), 0, a, s);
     }
-    return launch_pdl(block_norm_kernel<T, TW, VEC, 16, false, false, 0>, a.rows, threads(16), 0, a, s);
+    return launch_pdl(block_norm_kernel<T, TW, V, 16, false, false, 0>, a.rows, threads(16), 0, a, s);
 }
-
-bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 template <typename T, typename TW>
 cudaError_t launch(const BlockNormArgs& a, int num_sms, cudaStream_t s) {
@@ -460,17 +497,16 @@ cudaError_t launch(const BlockNormArgs& a, int num_sms, cudaStream_t s) {
         if (e != cudaSuccess) return e;
         return launch_pdl(block_norm_long_kernel<T, TW>, a.rows, kLongThreads, static_cast<size_t>(a.cols) * 4, a, s);
     }
-    bool vec = true;
-    for (const void* p : {a.x, a.y, a.gate, a.post_w, a.post_b, a.pre_w, a.pre_b, static_cast<const void*>(a.h),
-                          static_cast<const void*>(a.z)})
-        vec = vec && aligned16(p);
-    auto pitch = [&](const void* p, int64_t ld) { vec = vec && (!p || ld * static_cast<int64_t>(sizeof(T)) % 16 == 0); };
-    pitch(a.x, a.ldx);
-    pitch(a.y, a.ldy);
-    pitch(a.gate, a.ldg);
-    pitch(a.h, a.ldh);
-    pitch(a.z, a.ldz);
-    return vec ? launch_short<T, TW, true>(a, num_sms, s) : launch_short<T, TW, false>(a, num_sms, s);
+    // The elements that all addresses and pitches are a multiple of.
+    const uintptr_t ptrs = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.gate) |
+                           reinterpret_cast<uintptr_t>(a.h) | reinterpret_cast<uintptr_t>(a.z);
+    const uintptr_t vectors = reinterpret_cast<uintptr_t>(a.post_w) | reinterpret_cast<uintptr_t>(a.post_b) |
+                              reinterpret_cast<uintptr_t>(a.pre_w) | reinterpret_cast<uintptr_t>(a.pre_b);
+    const int64_t pitch = a.ldx | (a.y ? a.ldy : 0) | (a.gate ? a.ldg : 0) | (a.h ? a.ldh : 0) | (a.z ? a.ldz : 0);
+    const uintptr_t bytes = ptrs | static_cast<uintptr_t>(pitch * static_cast<int64_t>(sizeof(T)));
+    if (bytes % 16 == 0 && vectors % 16 == 0) return launch_short<T, TW, kEights>(a, num_sms, s);
+    if (bytes % (2 * sizeof(T)) == 0 && vectors % (2 * sizeof(TW)) == 0) return launch_short<T, TW, kPairs>(a, num_sms, s);
+    return launch_short<T, TW, kAny>(a, num_sms, s);
 }
 
 }  // namespace

@@ -744,6 +744,15 @@ def test_norm_pitches(gpu, dn, cols, pad, io):
     norm_check(gpu, dn, 7, cols, io, "f32", gate="row", pad=pad)
 
 
+@pytest.mark.parametrize("io,wt", [("bf16", "bf16"), ("f32", "f32"), ("bf16", "f32")])
+@pytest.mark.parametrize("rows,cols,pad", [(700, 1100, 0), (700, 1099, 1), (700, 1099, 0), (700, 5001, 1), (700, 2999, 3),
+                                           (3, 334, 0), (3, 333, 1), (2, 12002, 0), (700, 602, 0), (700, 601, 1),
+                                           (700, 768, 0), (650, 1536, 0), (650, 3071, 1), (5, 20002, 0), (700, 6146, 0)])
+def test_norm_pairs_and_sizes(gpu, dn, rows, cols, pad, io, wt):
+    """Rows at multiples of one, two and eight elements, whose last pair may have one."""
+    norm_check(gpu, dn, rows, cols, io, wt, post="layer", gate="row", pad=pad, biases=True)
+
+
 @pytest.mark.parametrize("io", ["bf16", "f32"])
 @pytest.mark.parametrize("cols", [96, 4096, 20000])
 @pytest.mark.parametrize("alias", ["x-", "y-", "-x", "-y", "xy", "yx"])
