@@ -15,10 +15,10 @@
 // most 16 of its rows or columns filled.
 //
 // Exactness.  bf16 products are exact and summed in FP32; weights exp(s - m)
-// enter the second product as two bf16 parts (16 bits), so that the output
-// carries one rounding, its own.  E4M3 keys and values are exact in f16: they
-// are multiplied there, the query normalised by a power of two per head and
-// the weights scaled by 2^7 so that neither leaves f16's range.  FP32 operands
+// enter the second product as three bf16 parts, which hold all 24 bits.  E4M3
+// keys and values are exact in f16: they are multiplied there, the query
+// normalised by a power of two per head and the weights scaled by 2^7 so that
+// neither leaves f16's range, and cut into two f16 parts (22 bits).  FP32 operands
 // are cut into three bf16 parts each (24 bits, no loss); products below 2^-24
 // of the largest are left out, and each step's sum starts from zero, because
 // the matrix units truncate what they add to.
@@ -138,19 +138,11 @@ __device__ __forceinline__ uint32_t pack_rn(float x, float y) {
     else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
     return r;
 }
-// x and y as a rounded part and what it leaves.
-template <bool F16>
+// x and y as a rounded f16 part and what it leaves.
 __device__ __forceinline__ void cut2(float x, float y, uint32_t& h, uint32_t& l) {
-    h = pack_rn<F16>(x, y);
-    float hx, hy;
-    if constexpr (F16) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-        hx = f.x; hy = f.y;
-    } else {
-        hx = __uint_as_float(h << 16);
-        hy = __uint_as_float(h & 0xFFFF0000u);
-    }
-    l = pack_rn<F16>(x - hx, y - hy);
+    h = pack_rn<true>(x, y);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    l = pack_rn<true>(x - f.x, y - f.y);
 }
 // The power of two that brings `top` to [1, 2); 1 for zero, denormal and infinite values.
 __device__ __forceinline__ float to_unit(float top) {
@@ -853,7 +845,7 @@ __global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTA
             }
 
             // --- weights, transposed into the second product's operand: tokens by pairs, a head to each g
-            constexpr int PP = CT == DType::F32 ? 3 : 2;        // parts of a weight
+            constexpr int PP = F16 ? 2 : 3;     // parts of a weight
             uint32_t w[MT][NT][PP][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -869,12 +861,12 @@ __global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTA
                         l[n][e & 1] += x[e];
                     }
                     uint32_t c[PP][2];
-                    if constexpr (CT == DType::F32) {
+                    if constexpr (F16) {
+                        cut2(x[0], x[1], c[0][0], c[1][0]);
+                        cut2(x[2], x[3], c[0][1], c[1][1]);
+                    } else {
                         cut3(x[0], x[1], c[0][0], c[1][0], c[PP - 1][0]);
                         cut3(x[2], x[3], c[0][1], c[1][1], c[PP - 1][1]);
-                    } else {
-                        cut2<F16>(x[0], x[1], c[0][0], c[1][0]);
-                        cut2<F16>(x[2], x[3], c[0][1], c[1][1]);
                     }
 #pragma unroll
                     for (int q = 0; q < PP; ++q) {
@@ -895,10 +887,9 @@ __global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTA
                         uint32_t v[4];
                         ldsm_x4_t(k32 + G::KV + b * 16 * G::PITCH + chunk_at<CT, G::PITCH>(row, 2 * j + ((lane >> 3) & 1)), v);
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            mma<false>(acc[j][n], v, w[b][n][1][0], w[b][n][1][1]);
-                            mma<false>(acc[j][n], v, w[b][n][0][0], w[b][n][0][1]);
-                        }
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int q = PP - 1; q >= 0; --q) mma<false>(acc[j][n], v, w[b][n][q][0], w[b][n][q][1]);
                     }
             } else if constexpr (CT == DType::E4M3) {
 #pragma unroll

@@ -289,7 +289,11 @@ int dnnopt_cuda_gemm_w4(const dnnopt_w4_desc* d, const void* A, const uint8_t* W
  * written so must belong to one sequence.
  * Types: FP32 q / out with an FP32 cache, or BF16 q / out with a BF16 or E4M3
  * cache; k_scale and v_scale must be 1 unless the cache is E4M3.  Scores,
- * softmax and sums are FP32.  lse ([b][heads], may be NULL) is FP32 and serves
+ * softmax and sums are FP32, and so are the products with a BF16 cache.  With an
+ * FP32 cache, partial products below 2^-24 of an element's are left out.  With an
+ * E4M3 cache the queries of a head are held as f16 next to the largest of them
+ * (exact down to 2^-17 of it, smaller ones to 2^-24 of it) and the softmax
+ * weights to 22 bits.  lse ([b][heads], may be NULL) is FP32 and serves
  * to join this result with attention over other keys.
  * head_dim is a multiple of 16 up to 256; cache pointers 16-byte aligned and
  * strides in multiples of 16 bytes (else DNNOPT_STATUS_NOT_SUPPORTED).  Lengths
