@@ -830,7 +830,6 @@ gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     const bool f32s = g.st == DType::F32;
 
     if (!p.images || p.copy) pdl_wait();
-    pdl_launch_dependents();
     const Shares shares(p.tiles, nq, gridDim.x * kTeams, 1);
     const uint32_t share = team * gridDim.x + blockIdx.x;
     const bool busy = share < shares.n;
@@ -909,6 +908,9 @@ gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_at;
+    // Dependent kernels may start once every CTA holds its tensor memory: one that allocated first would
+    // wait for this grid to end, and this grid for its columns.
+    pdl_launch_dependents();
     if (p.images) {
         if (tid == 0) {
             pdl_wait();
