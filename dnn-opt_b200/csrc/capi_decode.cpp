@@ -114,7 +114,9 @@ int dnnopt_cuda_paged_attention(const dnnopt_paged_attn_desc* d, const void* q, 
     if (!ctx) return st;
     PagedAttnArgs a;
     a.batch = d->batch; a.heads = d->heads; a.kv_heads = d->kv_heads; a.dim = d->head_dim;
-    a.page_size = d->page_size; a.num_pages = d->num_pages; a.max_pages = d->max_pages;
+    a.page_size = d->page_size; a.num_pages = d->num_pages;
+    // Without pages every length above 0 is out of range: a table, which may then be NULL, is not read.
+    a.max_pages = d->num_pages > 0 ? d->max_pages : 0;
     a.window = d->window;
     a.io = static_cast<DType>(d->io_type); a.ct = static_cast<DType>(d->cache_type);
     a.scale = d->scale; a.softcap = d->softcap; a.k_scale = d->k_scale; a.v_scale = d->v_scale;

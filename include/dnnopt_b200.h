@@ -298,7 +298,8 @@ int dnnopt_cuda_gemm_w4(const dnnopt_w4_desc* d, const void* A, const uint8_t* W
  * head_dim is a multiple of 16 up to 256; cache pointers 16-byte aligned and
  * strides in multiples of 16 bytes (else DNNOPT_STATUS_NOT_SUPPORTED).  Lengths
  * and page numbers are read on the device and checked there: a length below 0
- * or above max_pages * page_size makes its sequence count as empty, a needed
+ * or above max_pages * page_size (0 for a cache without pages, whose pointers and
+ * table may be NULL) makes its sequence count as empty, a needed
  * page number outside [0, num_pages) leaves out that page's tokens (nothing is
  * stored there), and dnnopt_stream_status() then returns
  * DNNOPT_STATUS_INVALID_VALUE.  Attended keys and values are expected to be
