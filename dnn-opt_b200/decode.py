@@ -72,7 +72,8 @@ def dequantize_w4(packed: torch.Tensor, scale: torch.Tensor, zero, K: int, group
 
 
 class W4Linear:
-    """y = x W^T with a 4-bit weight; x and y bf16, any number of rows (few are fast)."""
+    """y = x W^T with a 4-bit weight; x and y bf16, any number of rows (few are fast).  x has its
+    rows' elements side by side, rows any pitch apart."""
 
     def __init__(self, w: torch.Tensor, group: int = 128, symmetric: bool = True):
         self.N, self.K = w.shape
@@ -81,8 +82,12 @@ class W4Linear:
 
     def __call__(self, x: torch.Tensor, stream=None) -> torch.Tensor:
         dn = _package()
+        if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != self.K:
+            raise ValueError(f"rows of {self.K} bf16 elements are wanted: got {x.dtype} {tuple(x.shape)}")
+        if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < self.K:
+            raise ValueError(f"rows' elements have to lie side by side: got strides {x.stride()}")
         y = torch.empty(x.shape[0], self.N, device=x.device, dtype=x.dtype)
-        d = dn.w4_desc(x.shape[0], self.N, self.K, x.stride(0), self.packed.stride(0), self.N, self.group,
+        d = dn.w4_desc(x.shape[0], self.N, self.K, max(x.stride(0), self.K), self.packed.stride(0), self.N, self.group,
                        self.scale.stride(0))
         dn.check(dn.cuda_gemm_w4(d, x, self.packed, self.scale, self.zero, None, y,
                                  stream or torch.cuda.current_stream()), "cuda_gemm_w4")
@@ -95,13 +100,15 @@ class W4Linear:
 
 # ---- paged cache --------------------------------------------------------------
 class PagedCache:
-    """Key and value pages of one layer, and the pages that sequences share out.
+    """Key and value pages of the layers, bf16 or E4M3, and the pages that sequences share out.
 
     Pages are assigned on the host (`grow`), one page table for all layers; the
     step reads lengths and table on the device."""
 
     def __init__(self, batch: int, kv_heads: int, head_dim: int, pages: int, page_size: int, max_pages: int,
                  layers: int = 1, dtype=torch.bfloat16, device="cuda"):
+        if dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+            raise ValueError(f"the cache of a bf16 layer holds bfloat16 or float8_e4m3fn, not {dtype}")
         self.page_size, self.max_pages = page_size, max_pages
         shape = (pages, page_size, kv_heads, head_dim)
         self.k = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(layers)]
@@ -178,14 +185,20 @@ class DecoderLayer:
         """h: residual stream [B, hidden], updated in place; z: its norm, this layer's input.
         Returns the next layer's input.  cache.lens counts the new token."""
         dn, c = _package(), self.c
-        B, D = h.shape[0], c.head_dim
+        B, D = cache.lens.shape[0], c.head_dim
+        for name, t in (("h", h), ("z", z)):
+            if t.dtype != torch.bfloat16 or tuple(t.shape) != (B, c.hidden) or not t.is_contiguous():
+                raise ValueError(f"{name} has to be contiguous bf16 [{B}, {c.hidden}]: got {t.dtype} {tuple(t.shape)}")
+        if cache.k[layer].shape[2:] != (c.kv_heads, D):
+            raise ValueError(f"the cache has rows of {tuple(cache.k[layer].shape[2:])}, the layer {(c.kv_heads, D)}")
         qkv = self.qkv(z)
         row = qkv.stride(0)
         q, k, v = qkv, qkv[:, c.heads * D:], qkv[:, (c.heads + c.kv_heads) * D:]
         a = torch.empty(B, c.heads * D, device=h.device, dtype=h.dtype)
         keys, values = cache.k[layer], cache.v[layer]
+        kind = dn.TYPE_BF16 if keys.dtype == torch.bfloat16 else dn.TYPE_E4M3
         d = dn.paged_attn_desc(B, c.heads, c.kv_heads, D, cache.page_size, keys.shape[0], cache.max_pages,
-                               q_strides=(row, D), new_strides=(row, D))
+                               cache_type=kind, q_strides=(row, D), new_strides=(row, D))
         dn.check(dn.cuda_paged_attention(d, q, keys, values, cache.table, cache.lens, a, k_new=k, v_new=v,
                                          stream=torch.cuda.current_stream()), "cuda_paged_attention")
         z = self._norms(0, h, self.o(a))
