@@ -46,6 +46,29 @@ cudaError_t grow(T** p, size_t* have, size_t need) {
     return cudaSuccess;
 }
 
+// The same for a stream's workspace, whose outgrown blocks stay: a graph that
+// was captured on the stream has their addresses in its launches.  A block is
+// at least twice the one before, so that all of them together are no larger
+// than the last; where memory is short, as large as the call needs.
+template <typename T>
+cudaError_t grow_kept(T** p, size_t* have, size_t need, std::vector<void*>* outgrown) {
+    if (need <= *have) return cudaSuccess;
+    size_t alloc = need + need / 4 > 2 * *have ? need + need / 4 : 2 * *have;
+    if (*p) outgrown->reserve(outgrown->size() + 1);
+    void* block = nullptr;
+    cudaError_t e = cudaMalloc(&block, alloc * sizeof(T));
+    if (e == cudaErrorMemoryAllocation) {
+        cudaGetLastError();
+        alloc = need;
+        e = cudaMalloc(&block, alloc * sizeof(T));
+    }
+    if (e != cudaSuccess) return e;
+    if (*p) outgrown->push_back(*p);
+    *p = static_cast<T*>(block);
+    *have = alloc;
+    return cudaSuccess;
+}
+
 }  // namespace
 
 int set_status(int st) {
@@ -121,18 +144,16 @@ int ensure_workspace(DeviceContext* ctx, cudaStream_t stream, size_t ws_floats, 
         w.absmax = w.err + 4;
         w.scales = reinterpret_cast<float*>(w.err + 8);
     }
-    if ((e = grow(&w.ws, &w.ws_floats, ws_floats)) != cudaSuccess) return cuda_status(e);
+    if ((e = grow_kept(&w.ws, &w.ws_floats, ws_floats, &w.outgrown)) != cudaSuccess) return cuda_status(e);
     if (counters > w.n_counters) {
-        size_t old = w.n_counters;
-        (void)old;
-        if ((e = grow(&w.counters, &w.n_counters, counters)) != cudaSuccess) return cuda_status(e);
+        if ((e = grow_kept(&w.counters, &w.n_counters, counters, &w.outgrown)) != cudaSuccess) return cuda_status(e);
         // Tickets must start at zero; kernels leave them at zero.
         e = cudaMemsetAsync(w.counters, 0, w.n_counters * sizeof(uint32_t), stream);
         if (e != cudaSuccess) return cuda_status(e);
     }
     if (quant_bytes > w.quant_bytes) {
         unsigned char* q = static_cast<unsigned char*>(w.quant);
-        if ((e = grow(&q, &w.quant_bytes, quant_bytes)) != cudaSuccess) return cuda_status(e);
+        if ((e = grow_kept(&q, &w.quant_bytes, quant_bytes, &w.outgrown)) != cudaSuccess) return cuda_status(e);
         w.quant = q;
     }
     *out = &w;

@@ -17,7 +17,7 @@
 namespace dnnopt_b200 {
 
 // Scratch owned by one (device, stream) pair.  Everything grows on demand and
-// is freed at process exit.
+// is freed at process exit, outgrown blocks too: captured graphs use them.
 struct Workspace {
     float* ws = nullptr;            // split-K partial strips
     size_t ws_floats = 0;
@@ -28,6 +28,7 @@ struct Workspace {
     float* scales = nullptr;        // [2] sA, sB
     void* quant = nullptr;          // quantised copies of A and B
     size_t quant_bytes = 0;
+    std::vector<void*> outgrown;
 };
 
 struct DeviceContext {

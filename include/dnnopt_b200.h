@@ -236,7 +236,10 @@ int dnnopt_cuda_gemm_f32_noalloc(const dnnopt_gemm_desc* d, const float* A, cons
  * pointers only, asynchronous on `stream`, nothing is copied or synchronised.
  * Inference only (no gradients).  Calls on one stream share its workspace;
  * a first call with a larger problem may allocate, so make it before a stream
- * capture.
+ * capture.  A captured graph stays usable when later calls outgrow the
+ * workspace that it was captured with; it may be launched on any stream, but
+ * not run at the same time as other calls on the stream of its capture or
+ * graphs captured there, with which it shares that workspace.
  * ---------------------------------------------------------------------- */
 enum { DNNOPT_TYPE_F32 = 0, DNNOPT_TYPE_BF16 = 1, DNNOPT_TYPE_E4M3 = 2 /* OCP E4M3FN */ };
 

@@ -37,3 +37,50 @@ def test_lengths_without_pages(gpu, dn, cache, max_pages, lens):
         assert dn.stream_status(s) == dn.INVALID_VALUE
         assert bool((out == 0).all()) and bool((lse == -math.inf).all())
         assert dn.stream_status(s) == dn.SUCCESS
+
+
+def test_graphs_outlive_a_grown_workspace(gpu, dn):
+    """A step captured for few rows replays after larger calls on its stream, whose workspace has grown,
+    and after other memory was taken and written."""
+    from test_decode_ops import Paged, w4_inputs
+    torch = gpu
+    side = torch.cuda.Stream()
+    M, N, K = 2, 1009, 20000        # digits made before the product, tiles in several parts
+    A, W, scale, _, _ = w4_inputs(torch, M, N, K, 128, torch.bfloat16, torch.bfloat16, False, False)
+    C = torch.empty(M, N, device="cuda", dtype=torch.bfloat16)
+    d = dn.w4_desc(M, N, K, K, W.stride(0), N, 128, scale.stride(0))
+    p = Paged(torch, dn, [3000, 40], 8, 2, 64, 16, "bf16")
+    q, out = p.q.cuda(), torch.empty_like(p.q, device="cuda")
+    torch.cuda.synchronize()
+
+    def step():
+        dn.check(dn.cuda_gemm_w4(d, A, W, scale, None, None, C, side))
+        dn.check(dn.cuda_paged_attention(p.desc(), q, p.k, p.v, p.table, p.lens_t, out, stream=side))
+
+    step()
+    side.synchronize()
+    want = C.clone(), out.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step()
+    kept = []
+    for rows in (9, 40, 200):
+        big = w4_inputs(torch, rows, 9000, K, 128, torch.bfloat16, torch.bfloat16, False, False)
+        Cb = torch.empty(rows, 9000, device="cuda", dtype=torch.bfloat16)
+        db = dn.w4_desc(rows, 9000, K, K, big[1].stride(0), 9000, 128, big[2].stride(0))
+        pb = Paged(torch, dn, [70] * (4 * rows), 16, 4, 64, 16, "bf16")
+        torch.cuda.synchronize()
+        dn.check(dn.cuda_gemm_w4(db, big[0], big[1], big[2], None, None, Cb, side))
+        with torch.cuda.stream(side):
+            pb.run(stream=side)
+        side.synchronize()
+        torch.cuda.empty_cache()
+        kept.append(torch.full((1 << 28,), 0xFF, device="cuda", dtype=torch.uint8))
+        for t in (C, out):
+            t.zero_()
+        torch.cuda.synchronize()
+        for _ in range(2):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(C, want[0]) and torch.equal(out, want[1]), rows
+    assert dn.stream_status(side) == dn.SUCCESS
