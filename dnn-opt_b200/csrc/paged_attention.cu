@@ -237,7 +237,7 @@ struct Cursor {
     __device__ __forceinline__ void load(const Params& p, int tile_tokens) {
         len = __ldg(p.a.lens + b);
         if (len < 0 || len > static_cast<int64_t>(p.a.max_pages) * p.a.page_size) {
-            if (threadIdx.x == 0) record_kernel_error(p.a.err, kKerrBadIndex);
+            record_kernel_error(p.a.err, kKerrBadIndex);    // a sequence may be one thread's alone
             len = 0;
         }
         first = p.a.window > 0 && len > p.a.window ? len - p.a.window : 0;

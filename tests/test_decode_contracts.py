@@ -16,7 +16,7 @@ def gpu(torch_cuda, dn):
 
 @pytest.mark.parametrize("cache", ["bf16", "e4m3", "f32"])
 @pytest.mark.parametrize("max_pages", [0, 4])
-@pytest.mark.parametrize("lens", [[5], [5, 0, 0], [0] * 40 + [64, 1]])
+@pytest.mark.parametrize("lens", [[5], [5, 0, 0], [0, 5, 0], [0] * 40 + [64, 1]])
 def test_lengths_without_pages(gpu, dn, cache, max_pages, lens):
     """A cache without pages has no table to read: lengths above 0 are reported, all outputs are those
     of empty sequences."""
@@ -84,3 +84,24 @@ def test_graphs_outlive_a_grown_workspace(gpu, dn):
         torch.cuda.synchronize()
         assert torch.equal(C, want[0]) and torch.equal(out, want[1]), rows
     assert dn.stream_status(side) == dn.SUCCESS
+
+
+@pytest.mark.parametrize("cache", ["bf16", "e4m3", "f32"])
+@pytest.mark.parametrize("lens", [[0, -1, 40], [0, -1, 0], [0, 0, 10 ** 6, 5], [-1], [40, 0, 0, -5], [0] * 31 + [-1],
+                                  [0] * 32 + [-1], [0] * 200 + [-1] + [0] * 100, [7] * 31 + [1 << 30]])
+def test_bad_lengths_after_empty_sequences(gpu, dn, cache, lens):
+    """A length out of range is reported wherever it stands, and only its sequence counts as empty."""
+    from test_decode_ops import Paged, within
+    torch = gpu
+    s = torch.cuda.current_stream()
+    assert dn.stream_status(s) == dn.SUCCESS
+    p = Paged(torch, dn, [n if 0 <= n < 1000 else 0 for n in lens], 4, 2, 64, 16, cache)
+    want, want_lse, tol, tol_lse = p.exact()
+    p.lens_t.copy_(torch.tensor(lens, dtype=torch.int32))
+    for window in (0, 16):
+        out, lse = p.run(window=window)
+        assert dn.stream_status(s) == dn.INVALID_VALUE
+        assert dn.stream_status(s) == dn.SUCCESS
+        if not window:
+            within(out, want, tol)
+            within(lse, want_lse, tol_lse)
