@@ -16,7 +16,9 @@
 // sum_k (code - 8) i_d are exact in 32-bit integers: they start from -8 sum i_d
 // and the bits of 1.5 * 2^23, so that they come out as FP32 numbers.  Then, in
 // FP32, once for every group or 128 weights:
-//   sum (code - zero) a = 2^e (sum_d 256^d sum (code - 8) i_d - (zero - 8) sum i).
+//   scale sum (code - zero) a = 2^e (scale (sum_d 256^d sum (code - 8) i_d - (zero - 8) sum i)),
+// multiplied in this order: nothing on the way is below FP32's normal numbers
+// where the result is not.
 // What is rounded are activations below 2^-14 (bf16; 2^-6, FP32) of the largest
 // of their 128, to 2^-23 (2^-31) of it: less than FP32 sums round.
 // Activations that are infinite or NaN stay out of the products and are added
@@ -710,7 +712,8 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
                         for (int d = NT - 2; d >= 0; --d)
                             y = fma2(y, make_float2(256.0f, 256.0f), add2(bits2(&c[k][d][2 * h]), make_float2(-kMagic, -kMagic)));
                         if (zeros) y = fma2(make_float2(zh, zh), make_float2(is[0], is[1]), y);
-                        tot[k][h] = fma2(mul2(make_float2(sh, sh), make_float2(un[0], un[1])), y, tot[k][h]);
+                        // The unit comes last: it and the scale alone may multiply to less than FP32's normal numbers.
+                        tot[k][h] = fma2(mul2(make_float2(sh, sh), y), make_float2(un[0], un[1]), tot[k][h]);
                     }
                 }
             }
@@ -1002,7 +1005,8 @@ gemm_w4_tc_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
 #pragma unroll
             for (int d = D - 2; d >= 0; --d) y = fma2(y, make_float2(256.0f, 256.0f), digit(d));
             if constexpr (ZEROS) y = fma2(make_float2(zr, zr), *reinterpret_cast<const float2*>(img.isum + q * ROWS + m), y);
-            tot[m / 2] = fma2(mul2(make_float2(sc, sc), make_float2(un[m], un[m + 1])), y, tot[m / 2]);
+            // The unit comes last: it and the scale alone may multiply to less than FP32's normal numbers.
+            tot[m / 2] = fma2(mul2(make_float2(sc, sc), y), make_float2(un[m], un[m + 1]), tot[m / 2]);
         }
     };
 

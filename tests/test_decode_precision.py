@@ -10,7 +10,7 @@ import math
 
 import pytest
 
-from test_decode_ops import Paged, U, r_of, types
+from test_decode_ops import Paged, U, r_of, types, w4_inputs, w4_run
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,28 @@ def test_attention_weights_keep_their_bits(gpu, dn, cache, heads, dim, second):
     off = float((out.double() - want).abs().max())
     assert off <= r_of(torch, p.q.dtype) * abs(want) + 2.0 ** -20 * size, off / size * 2.0 ** 20
     assert float((lse.double() - math.log1p(w)).abs().max()) <= 2.0 ** -20
+
+
+# ------------------------------------------------------------------ gemm_w4
+# Rows and groups that take each form of the kernels: digits of one or two rows side by side, digits apart
+# with scales for 32, 64 and 128 weights, and codes in tensor memory for up to four and eight rows.
+W4_FORMS = [(2, 70, 700, 32), (2, 70, 700, 64), (2, 70, 700, 128), (5, 70, 700, 32), (5, 70, 700, 64), (5, 70, 700, 128),
+            (4, 8193, 4097, 128), (8, 8193, 4097, 128)]
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("M,N,K,group", W4_FORMS)
+def test_w4_scales_with_its_operands(gpu, dn, M, N, K, group, io, zeros):
+    """Activations and scales times powers of two give the product times these, to the bit: every step
+    is exact under them while nothing leaves FP32's normal numbers, as no result here does.
+
+    The largest of 128 normal activations is between 1 and 8, so that its unit, 2^-30 (FP32) or 2^-22 of
+    it, is a normal number down to activations of 2^-97 and 2^-104; results are above 2^-124 but where
+    their terms cancel to 2^-24 of themselves."""
+    torch = gpu
+    A, W, scale, zero, _ = w4_inputs(torch, M, N, K, group, types(torch, dn)[io][0], torch.float32, zeros, False)
+    want = w4_run(torch, dn, M, N, K, group, A, W, scale, zero, None)
+    for a, s in ((-85, 0), (-60, -30), (-85, -10), (0, -60), (60, -30), (80, 20)):
+        C = w4_run(torch, dn, M, N, K, group, A * 2.0 ** a, W, scale * 2.0 ** s, zero, None)
+        assert torch.equal(C.double(), want.double() * 2.0 ** (a + s)), (a, s)
