@@ -20,7 +20,8 @@
 // multiplied in this order: nothing on the way is below FP32's normal numbers
 // where the result is not.
 // What is rounded are activations below 2^-14 (bf16; 2^-6, FP32) of the largest
-// of their 128, to 2^-23 (2^-31) of it: less than FP32 sums round.
+// of their 128, by up to 2^-22 (2^-30) of it.  That is below what an FP32 sum of
+// the 128 rounds, unless scales differ within them by as much as the activations.
 // Activations that are infinite or NaN stay out of the products and are added
 // for their own row at the end.
 //

@@ -255,7 +255,8 @@ enum { DNNOPT_TYPE_F32 = 0, DNNOPT_TYPE_BF16 = 1, DNNOPT_TYPE_E4M3 = 2 /* OCP E4
  * or NULL.  Within each 128 consecutive k, the activations of a row are held
  * as whole multiples of a power of two, 22 bits (BF16) or 30 bits (FP32) below
  * the largest of the 128: exact down to 2^-14 (2^-6) of it, smaller ones
- * rounded by at most 2^-23 (2^-31) of it.  Their products with the codes are
+ * rounded by at most 2^-22 (2^-30) of it, or by 2^-127 where that is more (a
+ * largest below 2^-105 or 2^-97).  Their products with the codes are
  * summed exactly in integers, scaled and added in FP32, and C is rounded once.
  * Infinite or NaN activations give what the formula gives.  Results do not
  * depend on the order of execution.  M, N or K == 0 is a no-op.  Fastest with

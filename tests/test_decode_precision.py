@@ -52,7 +52,39 @@ def test_attention_weights_keep_their_bits(gpu, dn, cache, heads, dim, second):
     assert float((lse.double() - math.log1p(w)).abs().max()) <= 2.0 ** -20
 
 
+
 # ------------------------------------------------------------------ gemm_w4
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("M,N,K", [(2, 127, 128), (8, 127, 128), (4, 8192, 4096), (8, 8192, 4096)])
+def test_w4_activations_next_to_large_ones(gpu, dn, M, N, K, io):
+    """Each column of C is one activation as it is held next to the largest of its 128: exact from 2^-14
+    (BF16; 2^-6, FP32) of that, else within 2^-22 (2^-30) of it, or 2^-127.  What is held fits C's type.
+
+    Row m's largest is a power of two, where the bound is sharp; it stands alone, so that nothing is summed."""
+    torch = gpu
+    f32 = io == "f32"
+    tops = [0, 5, -90, 60, -20, 1, -97, 100] if f32 else [0, 5, -90, 60, -20, 1, -105, 100]
+    T = types(torch, dn)[io][0]
+    g = torch.Generator().manual_seed(M)
+    A = torch.zeros(M, K, dtype=torch.float64)
+    for m in range(M):
+        down = torch.rand(127, generator=g, dtype=torch.float64) * 40 if f32 else torch.rand(127, generator=g, dtype=torch.float64) * 30
+        A[m, 1:128] = 2.0 ** (tops[m] - down) * torch.where(torch.rand(127, generator=g) < 0.5, -1.0, 1.0)
+        A[m, 0] = 2.0 ** tops[m]
+    A = A.to(T).cuda()
+    at = 1 + torch.arange(N) % 127
+    codes = torch.full((N, K), 8, dtype=torch.uint8)
+    codes[torch.arange(N), at] = 9
+    W = (codes[:, 0::2] | codes[:, 1::2] << 4).cuda()
+    C = w4_run(torch, dn, M, N, K, 128, A, W, torch.ones(N, -(-K // 128), device="cuda"), None, None)
+    want = A.double().cpu()[:, at]
+    top = A.double().cpu()[:, :1]
+    held, low = (2.0 ** -30, 2.0 ** -6) if f32 else (2.0 ** -22, 2.0 ** -14)
+    tol = torch.where(want.abs() >= low * top, torch.zeros(1, dtype=torch.float64), torch.clamp(held * top, min=2.0 ** -127))
+    off = (C.double().cpu() - want).abs()
+    assert bool((off <= tol).all()), float((off / top).max())
+
+
 # Rows and groups that take each form of the kernels: digits of one or two rows side by side, digits apart
 # with scales for 32, 64 and 128 weights, and codes in tensor memory for up to four and eight rows.
 W4_FORMS = [(2, 70, 700, 32), (2, 70, 700, 64), (2, 70, 700, 128), (5, 70, 700, 32), (5, 70, 700, 64), (5, 70, 700, 128),
