@@ -1,6 +1,7 @@
 // C ABI of the decoder-step operators: products with 4-bit weights, attention
 // over a paged key-value cache, and the norms around a block.  Argument checks,
 // workspace and launch; see include/dnnopt_b200.h for each entry's contract.
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -59,16 +60,32 @@ int dnnopt_cuda_gemm_w4(const dnnopt_w4_desc* d, const void* A, const uint8_t* W
     g.scale = scale; g.zero = zero; g.lds = d->lds;
     g.bias = bias;
     g.C = C; g.ldc = d->ldc;
-    W4Plan plan;
-    if (!gemm_w4_plan(g, ctx->num_sms, &plan)) return set_status(DNNOPT_STATUS_NOT_SUPPORTED);
+    // kW4RowsAtOnce rows of A at a time, and what is left: the workspace grows with the rows of a launch.
+    W4Plan plan, rest = {};
+    W4Args part = g;
+    part.M = g.M < kW4RowsAtOnce ? g.M : kW4RowsAtOnce;
+    if (!gemm_w4_plan(part, ctx->num_sms, &plan)) return set_status(DNNOPT_STATUS_NOT_SUPPORTED);
+    const int left = g.M > kW4RowsAtOnce ? g.M % kW4RowsAtOnce : 0;
+    part.M = left;
+    if (left > 0 && !gemm_w4_plan(part, ctx->num_sms, &rest)) return set_status(DNNOPT_STATUS_NOT_SUPPORTED);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     Workspace* w = nullptr;
-    st = ensure_workspace(ctx, s, plan.ws_floats, plan.tickets, plan.extra_bytes, &w);
+    st = ensure_workspace(ctx, s, std::max(plan.ws_floats, rest.ws_floats), std::max(plan.tickets, rest.tickets),
+                          std::max(plan.extra_bytes, rest.extra_bytes), &w);
     if (st != DNNOPT_STATUS_SUCCESS) return st;
     if ((st = inject_launch()) != DNNOPT_STATUS_SUCCESS) return st;
-    cudaError_t e = launch_gemm_w4(g, plan, w->ws, w->counters, w->quant, w->err, s);
-    note_launch(plan.pitch || plan.prepared ? 2 : 1);
-    return cuda_status(e);
+    const int64_t a_row = static_cast<int64_t>(d->lda) * type_bytes(d->io_type), c_row = static_cast<int64_t>(d->ldc) * type_bytes(d->io_type);
+    for (int64_t m = 0; m < g.M; m += kW4RowsAtOnce) {
+        const bool last = g.M - m < kW4RowsAtOnce && left > 0;
+        const W4Plan& now = last ? rest : plan;
+        part.M = last ? left : (g.M < kW4RowsAtOnce ? g.M : kW4RowsAtOnce);
+        part.A = static_cast<const char*>(A) + m * a_row;
+        part.C = static_cast<char*>(C) + m * c_row;
+        const cudaError_t e = launch_gemm_w4(part, now, w->ws, w->counters, w->quant, w->err, s);
+        if (e != cudaSuccess) return cuda_status(e);
+        note_launch(now.pitch || now.prepared ? 2 : 1);
+    }
+    return set_status(DNNOPT_STATUS_SUCCESS);
 }
 
 int dnnopt_cuda_paged_attention(const dnnopt_paged_attn_desc* d, const void* q, void* k_cache,

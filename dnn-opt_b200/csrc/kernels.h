@@ -315,6 +315,9 @@ struct W4Args {
     void* C;
     int64_t ldc;
 };
+// Rows of A in one launch at most: 64 blocks of eight, whose partial tiles are some 0.3 GB for 28672 rows
+// of W, and the blocks' grid dimension stays small for any number of rows.
+constexpr int kW4RowsAtOnce = 512;
 struct W4Plan {
     int ctas, splits, blocks;   // grid: shares of the steps, K-ranges, blocks of rows of A
     int split_steps, rows, cols, slots, smem, bars_at;

@@ -86,6 +86,38 @@ def test_graphs_outlive_a_grown_workspace(gpu, dn):
     assert dn.stream_status(side) == dn.SUCCESS
 
 
+@pytest.mark.parametrize("M,N,K,pitch,pad", [(511, 70, 300, 16, 0), (512, 70, 300, 16, 0), (513, 70, 300, 1, 5), (1100, 33, 129, 16, 1),
+                                             (1538, 8192, 4096, 16, 0)])
+def test_w4_many_rows(gpu, dn, M, N, K, pitch, pad):
+    """Rows past those of one launch, the last launch of one, two or more of them."""
+    from test_decode_ops import sum_tol, w4_exact, w4_inputs, w4_run, within
+    torch = gpu
+    ins = w4_inputs(torch, M, N, K, 128, torch.bfloat16, torch.bfloat16, True, True, pad, pitch=pitch)
+    C = w4_run(torch, dn, M, N, K, 128, *ins, pad_c=pad)
+    rows = sorted({*range(0, M, 37), *range(505, min(M, 520)), *range(M - 4, M)})
+    want, mag = w4_exact(torch, ins[0][rows], *ins[1:], K, 128)
+    within(C[rows][:, :N], want, 2.0 ** -8 * want.abs() + sum_tol(K) * mag)
+    assert bool(C[:, N:].isnan().all()) and bool(C[:, :N].isfinite().all())
+
+
+def test_w4_rows_without_end(gpu, dn):
+    """More rows than a grid has blocks; a workspace that does not grow with them."""
+    torch = gpu
+    M, N, K = 530000, 32, 32
+    A = torch.randint(-8, 9, (M, K), device="cuda").bfloat16()
+    W = torch.randint(0, 256, (N, 16), device="cuda", dtype=torch.uint8)
+    scale = torch.ones(N, 1, device="cuda").bfloat16()
+    codes = torch.stack((W & 15, W >> 4), 2).view(N, K).float() - 8
+    C = torch.empty(M, N, device="cuda", dtype=torch.bfloat16)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    dn.check(dn.cuda_gemm_w4(dn.w4_desc(M, N, K, K, 16, N, 0, 1), A, W, scale, None, None, C, side))
+    side.synchronize()
+    assert free - torch.cuda.mem_get_info()[0] < 1 << 28
+    assert torch.equal(C, (A.float() @ codes.t()).bfloat16())      # whole numbers below 2^24
+
+
 @pytest.mark.parametrize("cache", ["bf16", "e4m3", "f32"])
 @pytest.mark.parametrize("lens", [[0, -1, 40], [0, -1, 0], [0, 0, 10 ** 6, 5], [-1], [40, 0, 0, -5], [0] * 31 + [-1],
                                   [0] * 32 + [-1], [0] * 200 + [-1] + [0] * 100, [7] * 31 + [1 << 30]])
