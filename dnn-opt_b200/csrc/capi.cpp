@@ -515,10 +515,8 @@ int host_entry(Kind kind, const dnnopt_gemm_desc* d, const void* A, const void* 
             if (e != cudaSuccess) return cuda_status(e);
         }
         if (code != 0) {
-            // Clears the error word and the conv prep's grid-barrier and
-            // absmax words (a timed-out barrier may have left them set).
-            cudaMemset(it->second.err, 0, 16 * sizeof(uint32_t));
-            return set_status(kernel_error_status(code));
+            clear_kernel_error(it->second);
+            return set_status(DNNOPT_STATUS_KERNEL_TIMEOUT);
         }
     }
     return set_status(DNNOPT_STATUS_SUCCESS);
@@ -1200,14 +1198,16 @@ int dnnopt_stream_status(void* stream) {
     if (e != cudaSuccess) return cuda_status(e);
     auto it = ctx->ws.find(s);
     if (it != ctx->ws.end() && it->second.err) {
-        uint32_t code = 0;
-        e = cudaMemcpy(&code, it->second.err, sizeof(code), cudaMemcpyDeviceToHost);
+        uint32_t code[2] = {0, 0};      // the error word and the bad index
+        e = cudaMemcpy(code, it->second.err, sizeof(code), cudaMemcpyDeviceToHost);
         if (e != cudaSuccess) return cuda_status(e);
-        if (code != 0) {
-            // Clears the error word and the conv prep's grid-barrier and
-            // absmax words (a timed-out barrier may have left them set).
-            cudaMemset(it->second.err, 0, 16 * sizeof(uint32_t));
-            return set_status(kernel_error_status(code));
+        if (code[0] != 0) {
+            clear_kernel_error(it->second);
+            return set_status(DNNOPT_STATUS_KERNEL_TIMEOUT);
+        }
+        if (code[1] != 0) {
+            cudaMemset(it->second.bad_index, 0, sizeof(uint32_t));
+            return set_status(DNNOPT_STATUS_INVALID_VALUE);
         }
     }
     return set_status(DNNOPT_STATUS_SUCCESS);

@@ -153,7 +153,7 @@ int dnnopt_cuda_paged_attention(const dnnopt_paged_attn_desc* d, const void* q, 
     st = ensure_workspace(ctx, s, plan.ws_floats, plan.tickets, 0, &w);
     if (st != DNNOPT_STATUS_SUCCESS) return st;
     if ((st = inject_launch()) != DNNOPT_STATUS_SUCCESS) return st;
-    a.err = w->err;
+    a.err = w->bad_index;
     e = launch_paged_attention(a, plan, w->ws, w->counters, s);
     note_launch();
     return cuda_status(e);

@@ -84,9 +84,10 @@ int cuda_status(cudaError_t e) {
     return set_status(DNNOPT_STATUS_CUDA_ERROR);
 }
 
-int kernel_error_status(uint32_t code) {
-    constexpr uint32_t kBadIndex = 4;   // kKerrBadIndex
-    return code == kBadIndex ? DNNOPT_STATUS_INVALID_VALUE : DNNOPT_STATUS_KERNEL_TIMEOUT;
+cudaError_t clear_kernel_error(const Workspace& w) {
+    cudaError_t e = cudaMemset(w.err, 0, sizeof(uint32_t));
+    if (e != cudaSuccess) return e;
+    return cudaMemset(w.absmax, 0, 12 * sizeof(uint32_t));
 }
 
 void note_launch(int n) { g_launches.fetch_add(static_cast<uint64_t>(n), std::memory_order_relaxed); }
@@ -131,7 +132,7 @@ int ensure_workspace(DeviceContext* ctx, cudaStream_t stream, size_t ws_floats, 
     Workspace& w = ctx->ws[stream];
     cudaError_t e;
     if (!w.err) {
-        // err (word 0), absmax (words 4-5), the conv prep's grid-barrier
+        // err (word 0), bad index (word 1), absmax (words 4-5), the conv prep's grid-barrier
         // count and generation (words 6-7), scales (words 8-11) and the conv
         // prep's two absmax slots (words 12-15) share one small
         // zero-initialised allocation.
@@ -141,6 +142,7 @@ int ensure_workspace(DeviceContext* ctx, cudaStream_t stream, size_t ws_floats, 
         e = cudaMemsetAsync(small, 0, 64, stream);
         if (e != cudaSuccess) { cudaFree(small); return cuda_status(e); }
         w.err = static_cast<uint32_t*>(small);
+        w.bad_index = w.err + 1;
         w.absmax = w.err + 4;
         w.scales = reinterpret_cast<float*>(w.err + 8);
     }

@@ -24,6 +24,7 @@ struct Workspace {
     uint32_t* counters = nullptr;   // split-K tickets (kept zero between launches)
     size_t n_counters = 0;
     uint32_t* err = nullptr;        // bounded-wait error word
+    uint32_t* bad_index = nullptr;  // set by a kernel that met an index out of range in device memory
     uint32_t* absmax = nullptr;     // [2] absmax bit patterns (FP32-API int8), [2..3] grid-barrier words
     float* scales = nullptr;        // [2] sA, sB
     void* quant = nullptr;          // quantised copies of A and B
@@ -62,7 +63,9 @@ int set_status(int st);                 // records as the thread's last status
 int cuda_status(cudaError_t e);         // maps a CUDA error to a status (and records it)
 void note_launch(int n = 1);            // library kernel launch counter
 
-int kernel_error_status(uint32_t code); // status of a kernel's error word (nonzero KernelErrorCode)
+// Clears the error word and the conv prep's grid-barrier and absmax words (a
+// timed-out barrier may have left them set); a bad index stays to be reported.
+cudaError_t clear_kernel_error(const Workspace& w);
 
 // Host-side fault injection (tests): returns DNNOPT_STATUS_INJECTED_FAULT
 // while an injected fault of `site` is pending.

@@ -407,7 +407,7 @@ int dnnopt_cuda_peer_wait(const unsigned int* flags, int world, unsigned int epo
 /* Synchronises `stream` and reports (then clears) a bounded wait that gave up
  * in a kernel this library queued on it, or an index in device memory (a
  * sequence length, a page number) that a kernel refused to follow
- * (DNNOPT_STATUS_INVALID_VALUE). */
+ * (DNNOPT_STATUS_INVALID_VALUE; no other call reports or clears that). */
 int dnnopt_stream_status(void* stream);
 
 /* ------------------------------------------------------------------------

@@ -86,6 +86,28 @@ def test_graphs_outlive_a_grown_workspace(gpu, dn):
     assert dn.stream_status(side) == dn.SUCCESS
 
 
+def test_bad_lengths_are_not_another_calls(gpu, dn):
+    """A product of host operands on the same stream succeeds, and leaves the report where it is."""
+    import numpy as np
+    from test_decode_ops import Paged
+    torch = gpu
+    side = torch.cuda.Stream()
+    p = Paged(torch, dn, [40, 40], 4, 2, 64, 16, "bf16")
+    p.lens_t.copy_(torch.tensor([40, -1], dtype=torch.int32))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        p.run(stream=side)
+    a, b, c = np.ones((4, 8), np.float32), np.ones((8, 16), np.float32), np.zeros((4, 16), np.float32)
+    dn.set_stream(side)
+    try:
+        assert dn.gemm_f32_desc(dn.desc(4, 16, 8, 8, 16, 16), a, b, c) == dn.SUCCESS
+    finally:
+        dn.set_stream(None)
+    assert (c == 8).all()
+    assert dn.stream_status(side) == dn.INVALID_VALUE
+    assert dn.stream_status(side) == dn.SUCCESS
+
+
 @pytest.mark.parametrize("M,N,K,pitch,pad", [(511, 70, 300, 16, 0), (512, 70, 300, 16, 0), (513, 70, 300, 1, 5), (1100, 33, 129, 16, 1),
                                              (1538, 8192, 4096, 16, 0)])
 def test_w4_many_rows(gpu, dn, M, N, K, pitch, pad):
