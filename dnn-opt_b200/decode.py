@@ -118,17 +118,26 @@ class PagedCache:
         self.free = list(range(pages - 1, -1, -1))
         self.held = [[] for _ in range(batch)]
 
-    def grow(self, tokens: int = 1) -> None:
-        """Makes every sequence `tokens` longer, assigning the pages that this takes."""
+    def grow(self, tokens: int = 1, slots=None) -> None:
+        """Makes every sequence, or those of `slots` alone, `tokens` longer, assigning the pages that
+        this takes.  Where they are not there nothing changes.  A slot that is left out keeps its
+        length: an ended one (`release`) stays empty, and the step answers zeros for its attention."""
         lens = self.lens.tolist()
-        for b, n in enumerate(lens):
-            while len(self.held[b]) * self.page_size < n + tokens:
-                if len(self.held[b]) == self.max_pages or not self.free:
-                    raise RuntimeError("the cache has no page left for a longer sequence")
+        grown = range(len(lens)) if slots is None else sorted(set(slots))
+        if any(not 0 <= b < len(lens) for b in grown):
+            raise IndexError(f"slots are 0 to {len(lens) - 1}: got {list(grown)}")
+        want = {b: max(0, -(-(lens[b] + tokens) // self.page_size) - len(self.held[b])) for b in grown}
+        if sum(want.values()) > len(self.free) or any(len(self.held[b]) + n > self.max_pages for b, n in want.items()):
+            raise RuntimeError("the cache has no page left for a longer sequence")
+        for b, n in want.items():
+            for _ in range(n):
                 page = self.free.pop()
                 self.table[b, len(self.held[b])] = page
                 self.held[b].append(page)
-        self.lens += tokens
+        if slots is None:
+            self.lens += tokens
+        elif want:
+            self.lens[list(want)] += tokens
 
     def release(self, b: int) -> None:
         """Ends sequence b: its pages are free again."""

@@ -40,6 +40,35 @@ def test_step_inputs(decode):
             layer.step(x, x, other, 0)
 
 
+def test_ended_slots_stay_empty(decode):
+    c = decode.PagedCache(3, 1, 16, pages=5, page_size=4, max_pages=2, device="cpu")
+    c.grow(4)
+    c.release(1)
+    free = list(c.free)
+    c.grow(1, slots=[0, 2, 2])
+    assert c.lens.tolist() == [5, 0, 5] and c.held[1] == [] and len(c.free) == len(free) - 2
+    assert c.table[1].tolist() == [-1, -1] and sorted(c.table[[0, 2]].flatten().tolist()) == sorted(c.held[0] + c.held[2])
+    c.grow(1, slots=[])
+    assert c.lens.tolist() == [5, 0, 5]
+    c.grow(4, slots=(1,))
+    assert c.lens.tolist() == [5, 4, 5] and len(c.held[1]) == 1
+    for slots in ([3], [-1]):
+        with pytest.raises(IndexError):
+            c.grow(1, slots=slots)
+
+
+def test_growing_without_pages_changes_nothing(decode):
+    c = decode.PagedCache(3, 1, 16, pages=5, page_size=4, max_pages=2, device="cpu")
+    c.grow(4)
+    before = c.lens.tolist(), c.table.tolist(), list(c.free), [list(h) for h in c.held]
+    for tokens, slots in ((1, None), (5, [0]), (9, [1])):     # three pages of two; past max_pages
+        with pytest.raises(RuntimeError):
+            c.grow(tokens, slots=slots)
+        assert before == (c.lens.tolist(), c.table.tolist(), list(c.free), [list(h) for h in c.held])
+    c.grow(1, slots=[0, 1])
+    assert c.lens.tolist() == [5, 5, 4] and c.free == []
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 64), (4, 4, 128)])
 def test_steps_over_an_e4m3_cache(torch_cuda, decode, heads, kv_heads, dim):
