@@ -107,3 +107,74 @@ def test_w4_scales_with_its_operands(gpu, dn, M, N, K, group, io, zeros):
     for a, s in ((-85, 0), (-60, -30), (-85, -10), (0, -60), (60, -30), (80, 20)):
         C = w4_run(torch, dn, M, N, K, group, A * 2.0 ** a, W, scale * 2.0 ** s, zero, None)
         assert torch.equal(C.double(), want.double() * 2.0 ** (a + s)), (a, s)
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("M,N,K,group", W4_FORMS + [(2, 70, 28700, 128), (8, 70, 9000, 32), (7, 1009, 28700, 256), (9, 8192, 20000, 128)])
+def test_w4_whole_numbers_are_exact(gpu, dn, M, N, K, group, io, zeros):
+    """Every digit of an activation counts, at its worth: no rounding but C's own.
+
+    A row of A is whole numbers |v| < 32 times 2^s, next to one 2^29 (BF16: 2^21) in each 128 whose weight
+    is 0: so 1 is the unit in which the row is held, and v lies s bits above it, s going through all digits.
+    Sums of (code - zero) v 2^s are below 2^(5 + 4 + 15 - 1) 2^s, scales 1, 2 or 4: multiples of 2^s with 24 bits
+    for K <= 8192 and less for the random signs of longer rows.  With zero points the sums of all
+    activations of 128, 2^29 among them, are also multiples of 2^s, with 24 bits from s = 12 (4) on."""
+    torch = gpu
+    f32 = io == "f32"
+    T = types(torch, dn)[io][0]
+    top = 29 if f32 else 21
+    lowest = (12 if f32 else 4) if zeros else 0
+    g = torch.Generator().manual_seed(K + M)
+    G = -(-K // group)
+    at = torch.arange(K) // group
+    z = torch.randint(0, 16, (N, G), generator=g) if zeros else torch.full((N, G), 8)
+    codes = torch.randint(0, 16, (N, K), generator=g)
+    tops = torch.arange(0, K, 128) + torch.randint(0, 128, (-(-K // 128),), generator=g)
+    tops = tops[tops < K]
+    codes[:, tops] = z[:, at[tops]]
+    padded = torch.zeros(N, -(-K // 32) * 32, dtype=torch.uint8)
+    padded[:, :K] = codes.to(torch.uint8)
+    W = (padded[:, 0::2] | padded[:, 1::2] << 4).cuda()
+    scale = 2.0 ** torch.randint(0, 3, (N, G), generator=g)
+    weight = ((codes - z[:, at]) * scale[:, at]).double()
+    v = torch.randint(-31, 32, (M, K), generator=g).double()
+    v[:, tops] = 0.0
+    sums = v @ weight.t()
+    assert float(sums.abs().max()) < 2.0 ** 24
+    zt = z.float().cuda() if zeros else None
+    for first in range(lowest, top - 5, M):
+        s = torch.tensor([lowest + (first - lowest + m) % (top - 5 - lowest) for m in range(M)], dtype=torch.float64)[:, None]
+        A = v * 2.0 ** s
+        A[:, tops] = 2.0 ** top
+        C = w4_run(torch, dn, M, N, K, group, A.to(T).cuda(), W, scale.cuda(), zt, None)
+        want = (sums * 2.0 ** s).to(torch.float32).to(T)
+        assert torch.equal(C.cpu(), want), first
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("M,N,K,group", [(2, 1009, 8192, 128), (5, 1009, 8192, 64), (4, 100, 28672, 32), (8, 4096, 4096, 128),
+                                         (1, 33, 65000, 0), (9, 700, 20000, 96)])
+def test_w4_infinities_across_parts(gpu, dn, M, N, K, group, io, zeros):
+    """Infinities and NaN anywhere in K, where rows of W are cut into parts and K into ranges: they reach
+    their own rows of C as the formula says, and no other."""
+    torch = gpu
+    A, W, scale, zero, _ = w4_inputs(torch, M, N, K, group, types(torch, dn)[io][0], torch.float32, zeros, False)
+    clean = w4_run(torch, dn, M, N, K, group, A, W, scale, zero, None)
+    codes = torch.stack((W & 15, W >> 4), 2).view(N, -1)[:, :K].double().cpu()
+    at = torch.arange(K) // (group or K)
+    sign = (codes - (zero.double().cpu()[:, at] if zeros else 8.0)) * scale.double().cpu()[:, at]
+    inf, nan = float("inf"), float("nan")
+    spots = [0, 1, 31, 127, 128, K // 2 - 1, K // 2, K // 2 + 1, K - 129, K - 2, K - 1] + list(range(500, K, 4097))
+    for i, k in enumerate(spots):
+        m, value = i % M, (inf, -inf, nan)[i % 3 if i % 7 == 2 else i % 2]
+        B = A.clone()
+        B[m, k] = value
+        want = clean.clone()
+        want[m] = (value * sign[:, k]).to(clean.dtype).cuda()      # inf * 0 is NaN
+        if i % 5 == 4:      # two of them
+            B[m, (k + 777) % K] = inf
+            want[m] = (value * sign[:, k] + inf * sign[:, (k + 777) % K]).to(clean.dtype).cuda()
+        C = w4_run(torch, dn, M, N, K, group, B, W, scale, zero, None)
+        assert bool(((C == want) | (C.isnan() & want.isnan())).all()), (m, k, value)
