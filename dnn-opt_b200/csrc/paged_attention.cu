@@ -20,8 +20,8 @@
 // normalised by a power of two per head and the weights scaled by 2^7 so that
 // neither leaves f16's range, and cut into two f16 parts (22 bits).  FP32 operands
 // are cut into three bf16 parts each (24 bits, no loss); products below 2^-24
-// of the largest are left out, and each step's sum starts from zero, because
-// the matrix units truncate what they add to.
+// of the largest are left out.  The matrix units truncate what they add to, so
+// sums start from zero at every step, or now and then where that is dearer.
 //
 // The reference m of exp(s - m) moves only when a score exceeds it by 2^8:
 // finding a tile's maximum takes six shuffles, asking whether any score
@@ -59,6 +59,7 @@ constexpr float kUp = 7.0f;         // log2 of the scale of f16 weights: 2^(7 + 
 struct Params {
     PagedAttnArgs a;
     float* ws;                      // partial results: two slots per share
+    float* aside;                   // sums that warps have put aside
     uint32_t* tickets;              // one per item, then two per share
     int group, hpb, hblocks;        // heads per kv head; per item; items per kv head
     uint32_t page_mul, page_shift;  // pos / page_size = mulhi(pos, page_mul) >> page_shift (page_size > 1)
@@ -103,6 +104,14 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// c += x, two at a time.
+__device__ __forceinline__ void add4(float (&c)[4], const float (&x)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; i += 2)
+        asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0,%1};\n\tmov.b64 b, {%2,%3};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0,%1}, a;\n\t}"
+            : "+f"(c[i]), "+f"(c[i + 1]) : "f"(x[i]), "f"(x[i + 1]));
 }
 
 // Transposes an 8 x 8 matrix of 16-bit elements over the warp's lanes.
@@ -186,6 +195,9 @@ struct Geo {
     static constexpr int SMALL = 2 * NW * 16 * 4 + 16 * 4 + STAGES * NW * 4 + 64;
     static constexpr int SMEM = STAGES * NW * WS + QBYTES + SMALL;
     static constexpr int PART = HEADS * (DP + 2);                  // floats of one partial result
+    // Each step's products start from zero, or all sums of a CTA's warps are put aside now and then.
+    static constexpr bool FRESH = CT == DType::F32 || (CT == DType::BF16 && DP <= 128);
+    static constexpr int ASIDE = FRESH ? 0 : NW * HEADS * DP;
     static_assert(STAGES >= 2, "a pipeline needs two stages");
 };
 
@@ -518,6 +530,44 @@ __global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTA
 
     // Lane (g, t) holds heads 2t and 2t + 1 of each block of eight, and of the queries head g.
     float acc[KSTEPS][NT][4], m[NT][2], l[NT][2], rowscale[NT][2];
+    // The matrix units truncate what they add to, two or three times for every 16 tokens: together 2^-13 of
+    // the sum of one CTA's 65536 tokens.  So each step's products start from zero and are added (FRESH), or,
+    // where that takes longer, sums are put aside every 1024 tokens of a warp and start anew: one sequence
+    // of 65536 tokens, heads of 256, 99 us (from zero 113, neither 96); 32 x 8192 e4m3 107 (109, 105); but
+    // bf16, 16 heads of 128 to a key, 32 x 8192, 115 (112, 104).
+    constexpr bool FRESH = G::FRESH;
+    constexpr int RUN = 64 / MT;
+    float* const aside = FRESH ? nullptr : p.aside + static_cast<size_t>(blockIdx.x * NW + warp) * (HEADS * DP) + lane * 4;
+    float kept[NT][2];          // what the sums put aside are multiplied by: the reference has moved since
+    bool held = false;          // there are some
+    int run = 0;
+    auto take_back = [&]() {
+#pragma unroll
+        for (int j = 0; j < KSTEPS; ++j)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float4 x = *reinterpret_cast<const float4*>(aside + (j * NT + n) * 128);
+                acc[j][n][0] = fmaf(x.x, kept[n][0], acc[j][n][0]);
+                acc[j][n][1] = fmaf(x.y, kept[n][1], acc[j][n][1]);
+                acc[j][n][2] = fmaf(x.z, kept[n][0], acc[j][n][2]);
+                acc[j][n][3] = fmaf(x.w, kept[n][1], acc[j][n][3]);
+            }
+    };
+    auto put_aside = [&]() {
+        if (held) take_back();
+#pragma unroll
+        for (int j = 0; j < KSTEPS; ++j)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float (&c)[4] = acc[j][n];
+                *reinterpret_cast<float4*>(aside + (j * NT + n) * 128) = make_float4(c[0], c[1], c[2], c[3]);
+                c[0] = c[1] = c[2] = c[3] = 0.0f;
+            }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) kept[n][0] = kept[n][1] = 1.0f;
+        held = true;
+        run = 0;
+    };
     uint32_t qreg[G::QREG ? KSTEPS : 1][QW];
     const float cap2 = a.softcap * kLog2e;
     auto heads_of = [&](const Cursor& c, int64_t& head0) {
@@ -621,6 +671,7 @@ __global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTA
             for (int e = 0; e < 2; ++e) {
                 m[n][e] = -INFINITY;
                 l[n][e] = 0.0f;
+                kept[n][e] = 0.0f;
                 float f = a.scale * a.k_scale;
                 if constexpr (CT == DType::E4M3) f /= __shfl_sync(0xFFFFFFFFu, f8[n], 4 * (2 * t4 + e));    // exact
                 rowscale[n][e] = a.softcap > 0.0f ? f / a.softcap : f * kLog2e;
@@ -836,6 +887,7 @@ __global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTA
                         const float alpha = m[n][e] == -INFINITY ? 0.0f : ex2(m[n][e] - top);
                         m[n][e] = top;
                         l[n][e] *= alpha;
+                        if constexpr (!FRESH) kept[n][e] *= alpha;
 #pragma unroll
                         for (int j = 0; j < KSTEPS; ++j) {
                             acc[j][n][e] *= alpha;
@@ -880,16 +932,29 @@ __global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTA
             const unsigned char* vt = kt + G::KV;
             if constexpr (CT == DType::BF16) {
                 const int row = (lane & 7) + ((lane >> 4) << 3);    // lanes 8-15, 24-31 the block's second half
+                constexpr int JB = FRESH && NT == 1 ? 4 : 1;        // blocks at a time (64 ragged sequences, heads of 64: 105 us, one 109)
 #pragma unroll
-                for (int j = 0; j < KSTEPS; ++j)
+                for (int j = 0; j < KSTEPS; j += JB)
 #pragma unroll
                     for (int b = 0; b < MT; ++b) {
-                        uint32_t v[4];
-                        ldsm_x4_t(k32 + G::KV + b * 16 * G::PITCH + chunk_at<CT, G::PITCH>(row, 2 * j + ((lane >> 3) & 1)), v);
+                        uint32_t v[JB][4];
+                        float o[JB][NT][4] = {};
 #pragma unroll
-                        for (int n = 0; n < NT; ++n)
+                        for (int u = 0; u < JB; ++u)
+                            ldsm_x4_t(k32 + G::KV + b * 16 * G::PITCH + chunk_at<CT, G::PITCH>(row, 2 * (j + u) + ((lane >> 3) & 1)), v[u]);
 #pragma unroll
-                            for (int q = PP - 1; q >= 0; --q) mma<false>(acc[j][n], v, w[b][n][q][0], w[b][n][q][1]);
+                        for (int q = PP - 1; q >= 0; --q)
+#pragma unroll
+                            for (int u = 0; u < JB; ++u)
+#pragma unroll
+                                for (int n = 0; n < NT; ++n)
+                                    mma<false>(FRESH ? o[u][n] : acc[j + u][n], v[u], w[b][n][q][0], w[b][n][q][1]);
+                        if constexpr (FRESH) {
+#pragma unroll
+                            for (int u = 0; u < JB; ++u)
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) add4(acc[j + u][n], o[u][n]);
+                        }
                     }
             } else if constexpr (CT == DType::E4M3) {
 #pragma unroll
@@ -956,6 +1021,14 @@ __global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTA
         }
 
         const bool ends = cons.t == cons.tiles - 1 || i + 1 == count;
+        if constexpr (!FRESH) {
+            if (++run == RUN && !ends) put_aside();
+            if (ends) {
+                if (held) take_back();
+                held = false;
+                run = 0;
+            }
+        }
         if (ends) {
             // --- the item's end in this share: join the warps; the stage just used holds their sums
             __syncwarp();
@@ -1122,13 +1195,13 @@ __global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTA
 
 struct Kernel {
     const void* fn;
-    int threads, smem, rows, part_floats, tile;
+    int threads, smem, rows, part_floats, tile, aside_floats;
 };
 
 template <DType IO, DType CT, int DP, int NT>
 Kernel kernel_of() {
     using G = Geo<CT, DP, NT>;
-    return {reinterpret_cast<const void*>(&paged_attention_kernel<IO, CT, DP, NT>), G::NW * 32, G::SMEM, G::HEADS, G::PART, G::TILE};
+    return {reinterpret_cast<const void*>(&paged_attention_kernel<IO, CT, DP, NT>), G::NW * 32, G::SMEM, G::HEADS, G::PART, G::TILE, G::ASIDE};
 }
 
 template <DType IO, DType CT, int NT>
@@ -1191,7 +1264,7 @@ cudaError_t paged_attention_plan(const PagedAttnArgs& a, int num_sms, PagedAttnP
     plan->ctas = static_cast<int>(ctas);
     // Tiles are counted in 32 bits.
     if (tiles * items > INT32_MAX) return cudaErrorNotSupported;
-    plan->ws_floats = static_cast<size_t>(2 * ctas) * k.part_floats;
+    plan->ws_floats = static_cast<size_t>(ctas) * (2 * k.part_floats + k.aside_floats);
     plan->tickets = static_cast<size_t>(items + 2 * ctas);
     return cudaSuccess;
 }
@@ -1202,6 +1275,7 @@ cudaError_t launch_paged_attention(const PagedAttnArgs& a, const PagedAttnPlan& 
     Params p;
     p.a = a;
     p.ws = ws;
+    p.aside = ws + static_cast<size_t>(2 * plan.ctas) * k.part_floats;
     p.tickets = tickets;
     p.group = a.heads / a.kv_heads;
     p.hpb = k.rows;

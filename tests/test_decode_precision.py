@@ -53,6 +53,48 @@ def test_attention_weights_keep_their_bits(gpu, dn, cache, heads, dim, second):
 
 
 
+@pytest.mark.parametrize("cache", ["bf16", "e4m3", "f32"])
+@pytest.mark.parametrize("heads,dim", [(1, 64), (8, 64), (8, 128), (8, 256), (16, 64), (16, 128), (16, 256)])
+def test_attention_sums_do_not_drift(gpu, dn, cache, heads, dim):
+    """One CTA's sum of 65536 values 1/4, and of 64 values that take it back to about zero.
+
+    Their weights are of all sizes, next to 64 tokens of value 0 that come first and weigh most.  Each of
+    the four warps adds 1025 numbers, each sum rounded within u of its part of half the sum of p |v| and
+    of random sign: 6 sqrt(1025) u is beyond six standard deviations.  Where matrix units add to what they
+    truncate, they do so for 1024 tokens, 64 times up to three parts: 192 times up to 2u of sums that are
+    half of their last on average.  Over all tokens the truncations would take ten times that."""
+    torch = gpu
+    t = types(torch, dn)
+    pages, page, batch = 1026, 64, 450      # enough sequences that each has a CTA; all of them read the same pages
+    io, kind = t["f32" if cache == "f32" else "bf16"], t[cache]
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    k = torch.zeros(pages, page, 1, dim, device="cuda")
+    k[..., 0] = -torch.randn(pages, page, 1, device="cuda", generator=g).abs()
+    k[0, ..., 0] = 0.5
+    k, L = k.to(kind[0]), pages * page
+    w = torch.exp(k[..., 0, 0].double()).cpu()
+    x = torch.full((pages, page), 0.25, dtype=torch.float64)
+    x[0] = 0.0
+    left = float((w[1:-1] * x[1:-1]).sum())
+    for i in range(page):
+        x[-1, i] = float(torch.tensor(-left / float(w[-1, i:].sum())).to(kind[0]))
+        left += float(w[-1, i] * x[-1, i])
+    want, size = left / float(w.sum()), float((w * x.abs()).sum() / w.sum())
+    assert abs(want) < 2.0 ** -9 and 0.45 < size < 0.55
+    v = x.float().cuda()[:, :, None, None].expand(-1, -1, 1, dim).contiguous().to(kind[0])
+    q = torch.zeros(batch, heads, dim, device="cuda", dtype=io[0])
+    q[..., 0] = 1.0
+    table = torch.arange(pages, device="cuda", dtype=torch.int32).expand(batch, -1).contiguous()
+    lens = torch.full((batch,), L, device="cuda", dtype=torch.int32)
+    out = torch.empty_like(q)
+    d = dn.paged_attn_desc(batch, heads, 1, dim, page, pages, pages, io_type=io[1], cache_type=kind[1], scale=1.0)
+    dn.check(dn.cuda_paged_attention(d, q, k, v, table, lens, out, stream=torch.cuda.current_stream()))
+    off = float((out.double() - want).abs().max())
+    drift = 192 if cache == "e4m3" or cache == "bf16" and dim > 128 else 0
+    tol = r_of(torch, io[0]) * abs(want) + (6 * math.sqrt(L / 64) + drift) * U * size / 2
+    assert off <= tol, (off / (U * size / 2), tol / (U * size / 2))
+
+
 # ------------------------------------------------------------------ gemm_w4
 @pytest.mark.parametrize("io", ["f32", "bf16"])
 @pytest.mark.parametrize("M,N,K", [(2, 127, 128), (8, 127, 128), (4, 8192, 4096), (8, 8192, 4096)])
