@@ -34,10 +34,11 @@
 // finished by the last of its shares to arrive, adding the parts in order.  The
 // digits of the K-range sit in shared memory in the order in which the operand
 // reads them.  Rows of W that do not start at multiples of 16 bytes are first
-// copied to a workspace where they do.
+// copied to a workspace where they do: 8x28672x8189 with dense rows 78 us, with
+// rows at 16 bytes 38; one row 69 and 30.
 //
 // Measured, of 6.53 TB/s (bf16, groups of 128): 1x28672x8192 30.0 us (62%); groups
-// of 32, 8 rows 63 us; 4x11008x4096 in groups of 64 with zero points 23.0 us;
+// of 32, 8 rows 63 us; 4x11008x4096 in groups of 64 with zero points 22.5 us;
 // 1x4096x4096 9.0 us, of which the chain of start, digits, first weights, sums
 // and joining takes seven.  16 warps an SM issue two instructions a cycle of
 // four: decoding, products and scaling wait on one another's results, and
@@ -452,8 +453,8 @@ __device__ __forceinline__ void join_tiles(const Params& p, const Shares& shares
 
 // D digits of an activation: three of bf16, four of FP32.  PACKED: the digits of
 // up to 8 / D rows of A share one block of eight columns; else each digit has a
-// block for up to eight rows.  (16 rows at once took longer than eight twice: 105
-// against 86 us for 16x28672x8192, their sums spill.)  F: chunks of 32 weights that share their scales
+// block for up to eight rows.  (16 rows at once took longer than eight twice, 105
+// against 86 us for 16x28672x8192 by this kernel: their sums spill.)  F: chunks of 32 weights that share their scales
 // for sure (4, 2 or 1); sums are scaled every F chunks.
 template <DType IO, bool PACKED, int F>
 __global__ void __launch_bounds__(kTeams * kTeamThreads, 1)
@@ -775,8 +776,8 @@ gemm_w4_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
 // memory again, no instruction is spent on operands of A, and a row's scale is
 // read once, not by four lanes.  Codes and sums are double: 128 columns a team.
 // Even k come before odd k within eight, in the digits as in the decoded codes.
-// Measured: 8x28672x8192 37.9 us (49%; by registers 42.9), 4 rows 33.7 (40.2), FP32
-// 39.6, 16 rows 69.  A warp issues 299 instructions a step, half of the issue slots
+// Measured: 8x28672x8192 38.1 us (49%; by registers 42.3), 4 rows 34.1 (40.5), FP32
+// 40.8, 16 rows 69.  A warp issues 299 instructions a step, half of the issue slots
 // go by: on tensor memory, barriers and fixed latencies.  Waiting for a quarter
 // of the digits at a time instead of all took longer (39.2).
 __device__ __forceinline__ void umma_i8_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -1114,9 +1115,11 @@ Kernel kernel_for_flush(int f) {
 Kernel select(const W4Args& g) {
     // How many chunks of 32 weights share their scales for sure, up to the four of a step.
     const int f = g.groups == 1 || g.group % 128 == 0 ? 4 : (g.group % 64 == 0 ? 2 : 1);
-    // Codes in tensor memory: 8x28672x8192 37.7 us (products of registers 42.9), 4 rows 33.7 (40.2),
-    // 8x28672x4096 23.8 (26.4), 8x8192x4096 16.5 (16.0).  Its tiles of 128 rows are too few of too many
-    // parts for less: 8x11008x2048 14.4 (10.6), 8x4096x11008 21.5 (18.8).
+    // Codes in tensor memory: 8x28672x8192 38.1 us (products of registers 42.3), 4 rows 34.2 (40.5), 3 rows
+    // 34.0 (41.4), 8x28672x4096 23.3 (26.4), 8x65536x512 10.4 (15.3), 8x11008x4096 17.1 (18.1), 3x8192x4096
+    // 14.3 (15.1).  At the rule's edge it can lose: 8x8192x4096 16.4 (15.7), 8x8192x8192 22.4 (21.0),
+    // 8x16384x2048 15.0 (12.4), whose tiles of 32 rows the registers' teams take whole.  Below it, its
+    // tiles of 128 rows are too few of too many parts: 8x8192x2048 11.6 (9.1), 8x4096x11008 21.9 (19.0).
     if (f == 4 && g.M > 2 && g.N >= 8192 && static_cast<int64_t>(g.N) * g.K >= int64_t(1) << 25) {
         const bool zeros = g.zero != nullptr;
         if (g.io == DType::F32) return g.M <= 4 ? tc_kernel<DType::F32, 4>(zeros) : tc_kernel<DType::F32, 8>(zeros);
@@ -1196,8 +1199,9 @@ bool gemm_w4_plan(const W4Args& g, int num_sms, W4Plan* plan) {
     plan->bars_at = (plan->smem - bars - 16) & ~7;
     plan->image_bytes = (per_step * plan->split_steps + 15) & ~15;
     // 512 threads take half a microsecond for every 32 stretches of 128 activations; a kernel before
-    // this one takes about one and overlaps this one's start (1x28672x8192, 64 stretches: 30.0 us
-    // without and 31.0 with it; 5x4093x4099 FP32, 165: 21.6 and 19.5; 8x28672x8192, 256: 47.3 and 44.1).
+    // this one takes about one and overlaps this one's start (products of registers: 1x28672x8192, 64
+    // stretches, 30.0 us without and 31.0 with it; 5x4093x4099 FP32, 165, 21.6 and 19.5; 8x28672x8192,
+    // 256, 47.3 and 44.1).
     const int64_t stretches = static_cast<int64_t>(g.M < k.rows ? g.M : k.rows) * plan->split_steps;
     plan->prepared = stretches > 64;
     plan->pitch = aligned_rows(g) ? 0 : (row_bytes_of(g) + 15) / 16 * 16;

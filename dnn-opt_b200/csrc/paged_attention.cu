@@ -35,10 +35,11 @@
 // the parts' order, so that results do not depend on who that is.
 //
 // Measured, of 6.53 TB/s (bf16, 32 heads on 8 keys of 128 unless said): 1 x 131072
-// tokens 91 us (90%), 64 ragged sequences up to 8192 160 us (95%), 32 x 8192 e4m3
-// 106 us (78%: products, decoding and softmax of one-byte elements), FP32 16 heads
-// of 64, 16 x 4096 105 us (78%); 8 x 1024 14.2 us, 1 x 17 5.3 us: start, first page
-// number, first keys, join.
+// tokens 89 us (92%), 64 ragged sequences up to 8192 159 us (96%), 16 heads to a
+// key, 32 x 8192 112 us (73%), heads of 256, 1 x 65536 99 us (83%), 32 x 4096 183 us
+// (90%); 32 x 8192 e4m3 104 us (79%: products, decoding and softmax of one-byte
+// elements), FP32 16 heads of 64, 16 x 4096 106 us (78%); 8 x 1024 14.9 us, 1 x 17
+// 5.5 us: start, first page number, first keys, join.
 #include <cuda_fp8.h>
 
 #include <mutex>
@@ -371,7 +372,7 @@ __global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTA
     Cursor cons;
     // Ending an item and beginning the next within a share costs about as much as two tiles.  So
     // with few items each gets CTAs of its own, if these then have at most two tiles more (8 x 1024
-    // tokens 14.2 us, in equal shares 16.6; 16 ragged windowed e4m3 sequences 31.9 and 35.7).
+    // tokens 14.9 us, in equal shares some 2.4 more; 16 ragged windowed e4m3 sequences 31.9 and 35.7).
     bool own = false;
     if (few) {
         uint32_t most = (total + gridDim.x - 1) / gridDim.x, k = 0, sum = 0;
@@ -700,7 +701,7 @@ __global__ void __launch_bounds__(Geo<CT, DP, NT>::NW * 32, Geo<CT, DP, NT>::CTA
     };
     auto slot_of = [&](const Parts& r, uint32_t c) { return 2 * c + (c == r.first ? r.tail : 0); };
     // The parts that one CTA joins at a time, and the ticket that says who is the last of them: with
-    // up to 32 parts all (1 x 2048 tokens, 32 parts: 11.2 us, in two steps 12.2), else groups of
+    // up to 32 parts all (1 x 2048 tokens, 32 parts: 11.5 us, in two steps a microsecond more), else groups of
     // neighbours, and then the groups (131072 tokens, 56 parts: 91 us, in one step 93).
     auto near_of = [](uint32_t n) { return n <= 32 ? n : (n <= 256 ? 16u : 32u); };
     auto first_ticket = [&](const Parts& r, const Cursor& c) {
