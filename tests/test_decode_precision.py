@@ -95,6 +95,46 @@ def test_attention_sums_do_not_drift(gpu, dn, cache, heads, dim):
     assert off <= tol, (off / (U * size / 2), tol / (U * size / 2))
 
 
+@pytest.mark.parametrize("cache", ["bf16", "e4m3", "f32"])
+@pytest.mark.parametrize("heads,kv,dim", [(2, 2, 64), (8, 1, 128), (8, 1, 256), (32, 2, 128), (16, 1, 256)])
+@pytest.mark.parametrize("rise", [60.0, -60.0])
+def test_attention_over_long_sequences_of_one_cta(gpu, dn, cache, heads, kv, dim, rise):
+    """Scores that rise (or fall) by far more than the reference of exp tolerates while a CTA works on one
+    sequence of ten runs of sums: what was put aside is brought to the new reference, item after item.
+
+    Sums as in the tests of other lengths; the scores' products are exact but for their scaling."""
+    torch = gpu
+    t = types(torch, dn)
+    pages, page, batch = 640, 64, 240
+    io, kind = t["f32" if cache == "f32" else "bf16"], t[cache]
+    g = torch.Generator(device="cuda").manual_seed(dim + heads)
+    L = pages * page - 5
+    k = torch.zeros(pages, page, kv, dim, device="cuda")
+    k[..., 0] = torch.linspace(0, 1, pages * page, device="cuda").view(pages, page, 1) + 0.05 * torch.randn(
+        pages, page, kv, device="cuda", generator=g)
+    k = k.to(kind[0])
+    v = torch.randn(pages, page, kv, dim, device="cuda", generator=g).to(kind[0])
+    q = torch.zeros(batch, heads, dim, device="cuda", dtype=io[0])
+    q[..., 0] = 1.0
+    q[:, 1::2, 0] = 0.5
+    table = torch.arange(pages, device="cuda", dtype=torch.int32).expand(batch, -1).contiguous()
+    lens = torch.full((batch,), L, device="cuda", dtype=torch.int32)
+    out, lse = torch.empty_like(q), torch.empty(batch, heads, device="cuda")
+    d = dn.paged_attn_desc(batch, heads, kv, dim, page, pages, pages, io_type=io[1], cache_type=kind[1], scale=rise)
+    dn.check(dn.cuda_paged_attention(d, q, k, v, table, lens, out, lse=lse, stream=torch.cuda.current_stream()))
+    k64, v64 = k.view(-1, kv, dim)[:L].double(), v.view(-1, kv, dim)[:L].double()
+    for h in range(heads):
+        s = rise * float(q[0, h, 0]) * k64[:, h // (heads // kv), 0]
+        total = torch.logsumexp(s, 0)
+        p = torch.exp(s - total)
+        values = v64[:, h // (heads // kv)]
+        want, size = p @ values, p @ values.abs()
+        score = 8 * U * float(s.abs().max())
+        tol = r_of(torch, io[0]) * want.abs() + (2.2 * score + 2.0 ** -16) * size
+        assert bool(((out[:, h].double() - want).abs() <= tol).all()), h
+        assert bool(((lse[:, h].double() - total).abs() <= score + 2.0 ** -16).all()), h
+
+
 # ------------------------------------------------------------------ gemm_w4
 @pytest.mark.parametrize("io", ["f32", "bf16"])
 @pytest.mark.parametrize("M,N,K", [(2, 127, 128), (8, 127, 128), (4, 8192, 4096), (8, 8192, 4096)])
